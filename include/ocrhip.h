@@ -192,7 +192,8 @@ int ocr_recognize_device(ocr_recognizer *rec, const ocr_batch *d_batches, uint32
 /* Kernel timing for measurement (the role of the reference's OPPROFILE, src/gpu.rs:1247-1368,
  * without its waits): between start and stop, every launch of the kernel family (process-wide:
  * "conv_mfma", "gru", "conv_transpose", "conv_direct", "conv_generic", "maxpool", "mask_up",
- * "grey_resize", "line_crop", "avgpool_t", "argmax", "copy") is bracketed by HIP events on its
+ * "grey_resize", "line_crop", "avgpool_t", "argmax", "copy", "text_append", "text_read",
+ * "text_attention", "text_decode", "text_fork", "beam_select") is bracketed by HIP events on its
  * own stream. stop waits for them and returns the launches, their summed duration in ms and
  * their summed algorithmic FLOPs and bytes. Where a family has several kernels that a rule on
  * sizes picks from, each is a name of its own as well ("gemm_thin" of "gemm_dma"). */
@@ -405,6 +406,172 @@ int ocr_line_images(ocr_ctx *ctx, const uint8_t *rgb, uint32_t page_w, uint32_t 
  * [count][3][48][wb] (host), zero past each line's width. */
 int ocr_pp_line_images(ocr_ctx *ctx, const uint8_t *rgb, uint32_t page_w, uint32_t page_h, const int32_t *lines,
                        uint32_t count, uint32_t wb, float *out);
+
+/* ---- A text decoder's operators ----------------------------------------------------------------
+ * The reference's recognisers end in CTC (a class a step, src/bin/ocr-bench.rs:61-75); it has no
+ * counterpart of these. They are what a decoder that writes text token by token adds: a paged
+ * cache of keys and values, quantised as it is written, attention over prompts and of single
+ * tokens over the cache, beam search. All buffers are in device memory; the work is queued on the
+ * context's stream (ocr_stream_acquire and ocr_stream_release order it with the caller's own
+ * streams). Sizes and pointers are checked by the call. Lengths, positions and page numbers live in device memory
+ * and are checked by the kernels: what lies outside the buffers is neither read nor written. */
+
+/* Everything queued on `stream` (a hipStream_t of the context's device; NULL: the default stream)
+ * so far comes before what is queued on the context from now on; and the other way round. */
+int ocr_stream_acquire(ocr_ctx *ctx, void *stream);
+int ocr_stream_release(ocr_ctx *ctx, void *stream);
+
+/* Element types. */
+#define OCR_F32 0
+#define OCR_F16 1
+#define OCR_BF16 2
+#define OCR_I8 3   /* whole numbers from -127 to 127 */
+#define OCR_E4M3 4 /* OCP e4m3: 1 sign, 4 exponent, 3 mantissa bits, at most 448 */
+
+/* A pool of pages of `page` positions (at most 1024): keys and values [pages][heads][page][dim]
+ * (dim at most 256) of type OCR_F16, OCR_BF16, OCR_I8 or OCR_E4M3; for the 8-bit types a float
+ * scale a vector, [pages][heads][page]: a value is its code times its vector's scale. */
+typedef struct ocr_kv_cache {
+    void *k;
+    void *v;
+    float *k_scale;
+    float *v_scale;
+    uint32_t pages;
+    uint32_t heads;
+    uint32_t page;
+    uint32_t dim;
+    int32_t type;
+} ocr_kv_cache;
+
+/* Which pages every sequence has: rows (sequences) of width entries, position p of a sequence in
+ * the page that entry p / page names. An entry that is negative or names no page holds nothing:
+ * writes there are dropped, reads give zeros. */
+typedef struct ocr_page_table {
+    const int32_t *table;
+    uint32_t rows;
+    uint32_t width;
+} ocr_page_table;
+
+/* n tokens' projections qkv (OCR_F32, OCR_F16 or OCR_BF16; token t at qkv + t * stride values:
+ * q_heads query vectors, then cache.heads key and as many value vectors of cache.dim values).
+ * Queries and keys are divided by sqrt(mean of squares + eps) and multiplied by q_norm / k_norm
+ * (dim floats; NULL: no norm), then their first rot values (even, 0: none) rotated by the token's
+ * position: pair i by pos * theta^(-2 i / rot), a pair being values (i, i + rot / 2), or
+ * (2 i, 2 i + 1) with adjacent != 0. Queries go to q [n][q_heads][dim] (out_type OCR_F16 or
+ * OCR_BF16), keys and values into the cache at position pos[t] of sequence seq[t], and, if k is not
+ * NULL, keys to k [n][heads][dim] too (out_type). The 8-bit types hold round(x / scale), scale =
+ * the vector's largest magnitude / 127 (OCR_I8) or / 448 (OCR_E4M3); a vector under 1e-30 is held
+ * as zeros, one with a value that is not finite reads as NaN. Two tokens of one call must not
+ * share a position of a sequence. */
+typedef struct ocr_kv_append_args {
+    const int32_t *seq;
+    const int32_t *pos;
+    const void *qkv;
+    int32_t type;
+    uint32_t n;
+    uint32_t q_heads;
+    int64_t stride;
+    const float *q_norm;
+    const float *k_norm;
+    float eps;
+    uint32_t rot;
+    double theta;
+    int32_t adjacent;
+    void *q;
+    void *k;
+    int32_t out_type;
+} ocr_kv_append_args;
+int ocr_kv_append_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_table *pages, const ocr_kv_append_args *args);
+
+/* The cached vectors of every sequence's first `most` positions, as type (OCR_F16 or OCR_BF16):
+ * k and v [rows][most][heads][dim], zeros past a sequence's length (lens, one a row). */
+int ocr_kv_read_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_table *pages, const int32_t *lens,
+                       uint32_t most, int32_t type, void *k, void *v);
+
+/* Attention over n tokens that hold documents one after another: docs[d] .. docs[d + 1] - 1 are
+ * document d's (ndocs + 1 rising offsets; NULL: one document of n tokens). A token sees the tokens
+ * before it in its document, itself, and its document's first prefix[d] tokens (NULL: none; a
+ * prefix of the document's length: all see all). Tokens outside every document see nothing and
+ * give zeros. Scores: scale q.k, then cap tanh(s / cap) where cap > 0, less slopes[head] (q_heads
+ * floats; NULL: none) times the distance. q, out: q_heads vectors of dim values every q_stride /
+ * out_stride values, k, v: kv_heads (q_heads a multiple) every k_stride / v_stride; type OCR_F16 or
+ * OCR_BF16, dim at most 256. out must not overlap an input. Values a token does not see do not
+ * reach its output, whatever they are. */
+typedef struct ocr_attention_args {
+    const void *q;
+    const void *k;
+    const void *v;
+    void *out;
+    int32_t type;
+    uint32_t n;
+    uint32_t q_heads;
+    uint32_t kv_heads;
+    uint32_t dim;
+    int64_t q_stride;
+    int64_t k_stride;
+    int64_t v_stride;
+    int64_t out_stride;
+    const int32_t *docs;
+    uint32_t ndocs;
+    const int32_t *prefix;
+    float scale;
+    float cap;
+    const float *slopes;
+} ocr_attention_args;
+int ocr_attention_device(ocr_ctx *ctx, const ocr_attention_args *args);
+
+/* The same for the last token of every sequence of a cache (its length, lens[row], counts it; 0: it
+ * sees nothing and gives zeros): q and out a row a sequence, type OCR_F16 or OCR_BF16 (a 16-bit
+ * cache's own type). */
+typedef struct ocr_decode_args {
+    const int32_t *lens;
+    const void *q;
+    void *out;
+    int32_t type;
+    uint32_t q_heads;
+    int64_t q_stride;
+    int64_t out_stride;
+    float scale;
+    float cap;
+    const float *slopes;
+} ocr_decode_args;
+int ocr_decode_attention_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_table *pages,
+                                const ocr_decode_args *args);
+
+/* A step of beam search: logits [groups * beams] rows of vocab values (type OCR_F32, OCR_F16 or
+ * OCR_BF16) every stride values, scores [groups][beams]. A continuation (beam w, token t) of a
+ * group scores scores[w] + log-softmax(logits of w)[t]; a beam whose finished flag is set keeps its
+ * score with token eos and has no other. The best `beams` (at most 32) of each group in order, ties
+ * to the lower w * vocab + t: out_scores, parents (w), tokens (t), out_finished (finished, or t ==
+ * eos; may be NULL), each [groups][beams]. NaN logits weigh nothing, scores that are not numbers
+ * count as minus infinity. finished may be NULL, eos negative (none) then. out_scores and
+ * out_finished may be scores and finished. */
+typedef struct ocr_beam_args {
+    const void *logits;
+    int32_t type;
+    uint32_t groups;
+    uint32_t beams;
+    uint32_t vocab;
+    int64_t stride;
+    const float *scores;
+    const int32_t *finished;
+    int32_t eos;
+    float *out_scores;
+    int32_t *parents;
+    int32_t *tokens;
+    int32_t *out_finished;
+} ocr_beam_args;
+int ocr_beam_select_device(ocr_ctx *ctx, const ocr_beam_args *args);
+
+/* The beams' pages after a step: row (group, w) of table_out and lens_out is that of its parent
+ * (parents, one a row, within the group). Whole pages are shared; a part-filled last page stays
+ * with the lowest w that continues the parent, the others get its contents in their own page
+ * spare[row] (used[row] = 1, else 0). Entries past the last page are -1. A parent outside the
+ * group gives an empty sequence. Spare pages must be in no row of the table and all different;
+ * table_out and lens_out must not overlap the old ones. */
+int ocr_kv_fork_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_table *pages, const int32_t *lens,
+                       const int32_t *parents, uint32_t beams, const int32_t *spare, int32_t *table_out,
+                       int32_t *lens_out, int32_t *used);
 
 #ifdef __cplusplus
 }

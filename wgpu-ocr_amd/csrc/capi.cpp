@@ -1,6 +1,7 @@
 // The C ABI (include/ocrhip.h): status codes and a thread-local message, nothing thrown across.
 #include "../../include/ocrhip.h"
 
+#include <cmath>
 #include <cstring>
 #include <memory>
 #include <string>
@@ -13,6 +14,7 @@
 #include "png.h"
 #include "crop.h"
 #include "pp_pipeline.h"
+#include "text.h"
 
 using namespace ocr;
 
@@ -1157,6 +1159,115 @@ int ocr_pp_line_images(ocr_ctx *ctx, const uint8_t *rgb, uint32_t page_w, uint32
         c.h2d(dc.get(), crops.data(), crops.size() * sizeof(PpCropLine));
         pp_line_crop(dc.as<PpCropLine>(), int(count), int(wb), c.stream());
         c.d2h(out, dout.get(), size_t(count) * slot * sizeof(float));
+    });
+}
+
+int ocr_stream_acquire(ocr_ctx *ctx, void *stream) {
+    return guard([&] {
+        need(ctx, "ctx");
+        ctx->ctx->bind();
+        ctx->ctx->order(static_cast<hipStream_t>(stream), ctx->ctx->stream());
+    });
+}
+
+int ocr_stream_release(ocr_ctx *ctx, void *stream) {
+    return guard([&] {
+        need(ctx, "ctx");
+        ctx->ctx->bind();
+        ctx->ctx->order(ctx->ctx->stream(), static_cast<hipStream_t>(stream));
+    });
+}
+
+}  // extern "C"
+
+namespace {
+
+KvCache cache_of(const ocr_kv_cache *c) {
+    need(c, "cache");
+    return {c->k, c->v, c->k_scale, c->v_scale, c->pages, c->heads, c->page, c->dim, c->type};
+}
+PageTable table_of(const ocr_page_table *t) {
+    need(t, "page table");
+    return {t->table, t->rows, t->width};
+}
+
+}  // namespace
+
+extern "C" {
+
+int ocr_kv_append_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_table *pages, const ocr_kv_append_args *args) {
+    return guard([&] {
+        need(ctx, "ctx");
+        need(args, "args");
+        const ocr_kv_append_args &x = *args;
+        const AppendArgs a{cache_of(cache), table_of(pages), x.seq, x.pos, x.qkv, x.type, x.n, x.q_heads, x.stride, x.q_norm, x.k_norm,
+                           x.eps, x.rot, std::log2(x.theta), x.adjacent, x.q, x.k, x.out_type};
+        if (!check_append(a)) return;
+        ctx->ctx->bind();
+        launch_append(a, ctx->ctx->stream());
+    });
+}
+
+int ocr_kv_read_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_table *pages, const int32_t *lens,
+                       uint32_t most, int32_t type, void *k, void *v) {
+    return guard([&] {
+        need(ctx, "ctx");
+        const ReadArgs a{cache_of(cache), table_of(pages), lens, most, type, k, v};
+        if (!check_read(a)) return;
+        ctx->ctx->bind();
+        launch_read(a, ctx->ctx->stream());
+    });
+}
+
+int ocr_attention_device(ocr_ctx *ctx, const ocr_attention_args *args) {
+    return guard([&] {
+        need(ctx, "ctx");
+        need(args, "args");
+        const ocr_attention_args &x = *args;
+        const AttentionArgs a{x.q, x.k, x.v, x.out, x.type, x.n, x.q_heads, x.kv_heads, x.dim, x.q_stride, x.k_stride, x.v_stride,
+                              x.out_stride, x.docs, x.ndocs, x.prefix, x.scale, x.cap, x.slopes};
+        if (!check_attention(a)) return;
+        ctx->ctx->bind();
+        launch_attention(a, ctx->ctx->stream());
+    });
+}
+
+int ocr_decode_attention_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_table *pages,
+                                const ocr_decode_args *args) {
+    return guard([&] {
+        need(ctx, "ctx");
+        need(args, "args");
+        const ocr_decode_args &x = *args;
+        const DecodeArgs a{cache_of(cache), table_of(pages), x.lens, x.q, x.out, x.type, x.q_heads, x.q_stride, x.out_stride, x.scale,
+                           x.cap, x.slopes};
+        if (!check_decode(a)) return;
+        ctx->ctx->bind();
+        launch_decode(*ctx->ctx, a, ctx->ctx->stream());
+    });
+}
+
+int ocr_beam_select_device(ocr_ctx *ctx, const ocr_beam_args *args) {
+    return guard([&] {
+        need(ctx, "ctx");
+        need(args, "args");
+        const ocr_beam_args &x = *args;
+        const BeamArgs a{x.logits, x.type, x.groups, x.beams, x.vocab, x.stride, x.scores, x.finished, x.eos, x.out_scores, x.parents,
+                         x.tokens, x.out_finished};
+        if (!check_beam(a)) return;
+        ctx->ctx->bind();
+        launch_beam(*ctx->ctx, a, ctx->ctx->stream());
+    });
+}
+
+int ocr_kv_fork_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_table *pages, const int32_t *lens,
+                       const int32_t *parents, uint32_t beams, const int32_t *spare, int32_t *table_out,
+                       int32_t *lens_out, int32_t *used) {
+    return guard([&] {
+        need(ctx, "ctx");
+        const ForkArgs a{cache_of(cache), table_of(pages), lens, parents, beams, spare, table_out, lens_out, used};
+        if (!check_fork(a)) return;
+        ctx->ctx->bind();
+        launch_fork(a, ctx->ctx->stream());
     });
 }
 

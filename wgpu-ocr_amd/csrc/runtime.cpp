@@ -337,6 +337,10 @@ Ctx::Ctx(int device, uint32_t lines, size_t pool_mb) : device_(device), lines_(l
     if (std::string(prop.gcnArchName).rfind("gfx950", 0) != 0)
         fail(std::string("this library is built for gfx950; device is ") + prop.gcnArchName);
     OCR_HIP(hipStreamCreateWithFlags(&stream_, hipStreamNonBlocking));
+    if (hipEventCreateWithFlags(&order_, hipEventDisableTiming) != hipSuccess) {
+        (void)hipStreamDestroy(stream_);
+        fail("no event for the context");
+    }
 }
 
 Ctx::~Ctx() {
@@ -347,7 +351,14 @@ Ctx::~Ctx() {
     if (ring_) (void)hipHostFree(ring_);
     pool_.trim();
     for (void *p : weights_) (void)hipFree(p);
+    if (order_) (void)hipEventDestroy(order_);
     if (stream_) (void)hipStreamDestroy(stream_);
+}
+
+void Ctx::order(hipStream_t first, hipStream_t then) {
+    if (first == then) return;
+    OCR_HIP(hipEventRecord(order_, first));
+    OCR_HIP(hipStreamWaitEvent(then, order_, 0));
 }
 
 namespace {

@@ -185,6 +185,7 @@ class Ctx {
     Pool &pool() { return pool_; }
     void bind() const;  // make this context's device current on the calling thread
     void sync();        // waits for stream()
+    void order(hipStream_t first, hipStream_t then);  // work queued on `then` from now on waits for first's so far
 
     // Weights live until the context is destroyed.
     template <class T> const T *upload_weights(const T *data, size_t count) {
@@ -200,6 +201,7 @@ class Ctx {
     int device_;
     uint32_t lines_;
     hipStream_t stream_ = nullptr;
+    hipEvent_t order_ = nullptr;
     Pool pool_;
     std::vector<void *> weights_;
     // Pinned staging ring of h2d: regions still read by a copy on the stream, oldest first.

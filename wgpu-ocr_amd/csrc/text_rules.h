@@ -1,0 +1,86 @@
+// The rules of the text decoder's operators that kernels and host share, free of HIP calls so that
+// they run on the CPU too: where a cached vector lies, which keys a prompt's token sees, what a
+// fork of a beam's pages does, how a launch is cut.
+#pragma once
+
+#include <cstdint>
+
+#ifdef __HIPCC__
+#define OCR_HD __host__ __device__ inline
+#else
+#define OCR_HD inline
+#endif
+
+namespace ocr {
+
+// The page that holds position pos of a sequence (its row of the table, width entries), or -1 where
+// there is none: a position outside the table, an entry that names no page of the pool.
+OCR_HD int32_t page_of(const int32_t *row, uint32_t width, uint32_t page, uint32_t pages, int64_t pos) {
+    if (pos < 0 || pos >= int64_t(width) * page) return -1;
+    const int32_t p = row[pos / page];
+    return p >= 0 && uint32_t(p) < pages ? p : -1;
+}
+
+// Vector index of (page p, head, slot) in a pool laid out [pages][heads][page].
+OCR_HD int64_t slot_of(int32_t p, uint32_t heads, uint32_t page, uint32_t head, uint32_t slot) {
+    return (int64_t(p) * heads + head) * page + slot;
+}
+
+// Positions of a sequence that there are: its length within its table.
+OCR_HD int32_t clamp_len(int32_t len, uint32_t width, uint32_t page) {
+    const int64_t most = int64_t(width) * page;
+    return len < 0 ? 0 : int64_t(len) > most ? int32_t(most) : len;
+}
+
+// Keys [lo, hi) that token i of a packed row sees. docs: ndocs + 1 rising offsets, prefix: each document's tokens that
+// all of it sees (null: none). Every token of a document sees those before it, itself and the
+// document's prefix; tokens outside every document see nothing. Offsets that do not rise give some
+// range inside [0, n).
+struct KeyRange {
+    int lo, hi;
+};
+OCR_HD KeyRange key_range(int i, int n, const int32_t *docs, int ndocs, const int32_t *prefix) {
+    if (i < 0 || i >= n) return {0, 0};
+    int a = 0, b = n, pre = 0;
+    if (docs) {
+        // The last document that starts at or before i.
+        int lo = 0, hi = ndocs;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (docs[mid] <= i) lo = mid + 1;
+            else hi = mid;
+        }
+        if (lo == 0 || docs[lo] <= i) return {0, 0};
+        a = docs[lo - 1] < 0 ? 0 : docs[lo - 1];
+        b = docs[lo] > n ? n : docs[lo];
+        if (prefix) pre = prefix[lo - 1];
+    } else if (prefix) {
+        pre = prefix[0];
+    }
+    int top = i + 1;
+    if (pre > 0 && pre > top - a) top = pre < b - a ? a + pre : b;
+    return {a, top < b ? top : b};
+}
+
+// A row of a reordered table: what beam w of a group takes from its parent. len: the parent's
+// length; full pages are shared, a part-filled last page goes to the first child and is copied for
+// the others.
+struct Fork {
+    int32_t len;
+    uint32_t full, tail;  // whole pages, slots of the last one
+    bool copy;
+};
+OCR_HD Fork fork_of(const int32_t *parents, uint32_t beams, uint32_t w, const int32_t *lens, uint32_t width, uint32_t page) {
+    Fork f{0, 0, 0, false};
+    const int32_t p = parents[w];
+    if (p < 0 || uint32_t(p) >= beams) return f;
+    f.len = clamp_len(lens[p], width, page);
+    f.full = uint32_t(f.len) / page;
+    f.tail = uint32_t(f.len) % page;
+    bool first = true;
+    for (uint32_t e = 0; e < w; e++) first = first && parents[e] != p;
+    f.copy = f.tail > 0 && !first;
+    return f;
+}
+
+}  // namespace ocr

@@ -109,6 +109,14 @@ SIGNATURES = {
     "ocr_pp_line_box": (ctypes.c_int, [P, F32, U32, U32, P]),
     "ocr_pp_line_images": (ctypes.c_int, [P, P, U32, U32, P, U32, U32, P]),
     "ocr_line_images": (ctypes.c_int, [P, P, U32, U32, P, U32, P, U32, P, U32, U32, P]),
+    "ocr_stream_acquire": (ctypes.c_int, [P, P]),
+    "ocr_stream_release": (ctypes.c_int, [P, P]),
+    "ocr_kv_append_device": (ctypes.c_int, [P, P, P, P]),
+    "ocr_kv_read_device": (ctypes.c_int, [P, P, P, P, U32, I32, P, P]),
+    "ocr_attention_device": (ctypes.c_int, [P, P]),
+    "ocr_decode_attention_device": (ctypes.c_int, [P, P, P, P]),
+    "ocr_beam_select_device": (ctypes.c_int, [P, P]),
+    "ocr_kv_fork_device": (ctypes.c_int, [P, P, P, P, P, U32, P, P, P, P]),
 }
 
 
@@ -298,6 +306,7 @@ class Context:
     """Gpu::new (src/gpu.rs:850): device, stream and scratch pool."""
 
     def __init__(self, lines: int = 8, pool_mb: int = 8192, device: int = 0):
+        self.device = device
         opts = ocr_opts(lines, pool_mb, device)
         self.handle = lib().ocr_create(ctypes.byref(opts))
         if not self.handle:
@@ -305,6 +314,15 @@ class Context:
 
     def synchronize(self):
         _check(lib().ocr_synchronize(self.handle))
+
+    def acquire(self, stream: int = 0):
+        """What is queued on the context from now on comes after everything queued on `stream` (a
+        hipStream_t as an integer, such as torch's Stream.cuda_stream; 0: the default stream)."""
+        _check(lib().ocr_stream_acquire(self.handle, stream or None))
+
+    def release(self, stream: int = 0):
+        """What is queued on `stream` from now on comes after everything queued on the context."""
+        _check(lib().ocr_stream_release(self.handle, stream or None))
 
     def alloc(self, nbytes: int) -> DeviceBuffer:
         return DeviceBuffer(self, nbytes)
@@ -559,6 +577,7 @@ ND_FAMILIES = ("conv3x3_dma", "gemm_dma", "conv_narrow", "conv_igemm", "conv_mfm
                "nd_gemm_rows", "nd_head", "nd_attention", "nd_bgemm", "nd_conv_generic", "nd_conv_transpose", "nd_elementwise", "nd_copy",
                "nd_reduce", "nd_layer_norm", "nd_softmax", "nd_argmax", "nd_pool", "nd_resize", "nd_det_prep",
                "nd_threshold")
+TEXT_FAMILIES = ("text_append", "text_read", "text_attention", "text_decode", "text_fork", "beam_select")
 
 
 def probe_start(family: str):
@@ -861,3 +880,6 @@ def pp_line_images(ctx: Context, rgb: np.ndarray, lines, wb: int) -> np.ndarray:
     _check(lib().ocr_pp_line_images(ctx.handle, _ptr(rgb), rgb.shape[1], rgb.shape[0], _ptr(ln), len(ln), wb,
                                     _ptr(out)))
     return out
+
+
+from .text import DeviceArray, KvCache, attention, beam_select  # noqa: E402,F401
