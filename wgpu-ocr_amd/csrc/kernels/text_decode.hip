@@ -1,4 +1,10 @@
 // Attention of single tokens over the paged cache.
+//
+// Every cached vector is needed once for each of the group's query heads, so a step is bound by the
+// cache's bytes: a workgroup reads one key head's vectors of a part of a sequence once for all of
+// its (up to 16) query heads, and the parts of a sequence are joined afterwards. Products run on the
+// matrix cores, 16 queries wide, with keys as rows: S^T = K Q^T, O^T = V^T P^T. A lane of the first's
+// result holds four keys of one query, which is what the second takes from it as it is.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -10,8 +16,7 @@ namespace ocr {
 
 namespace {
 
-// A head's vectors in a sequence's pages; a position whose page there is not holds minus infinity's
-// worth: its key scores nothing.
+// A head's vectors in a sequence's pages; a position whose page there is not holds zeros.
 template <class C> struct PagedKv {
     KvCache c;
     const int32_t *row;
@@ -30,6 +35,7 @@ template <class C> struct PagedKv {
     }
 };
 
+// Vectors that are no whole 16-byte pieces: one wavefront a (sequence, head), by the formula.
 template <class T, class C> __global__ __launch_bounds__(64) void decode_row_kernel(DecodeArgs a) {
     __shared__ float s_q[256];
     const int64_t r = blockIdx.x;
@@ -43,17 +49,319 @@ template <class T, class C> __global__ __launch_bounds__(64) void decode_row_ker
     attend_row(kv, s_q, dim, 0, len, len - 1, a.cap, a.slopes ? a.slopes[h] : 0.f, [&](int c, float o) { out[c] = T(o); });
 }
 
+// Weights are held as 2^6 times their value relative to the maximum's reference, which may lie up to
+// 2^8 under the true maximum: at most 2^14, within float16, and 2^-24 (its last step) is 2^-30 of
+// the reference. The factor is common to the sums and leaves with them.
+constexpr float kLift = 6.f, kSlack = 8.f;
+
+// Parts of a sequence joined: part [row][head][parts] holds dim normalised values, then log2 of the
+// sum of weights.
+constexpr int kPartTail = 4;  // keeps the rows' 16-byte alignment
+
+template <class C, class M, int DP> __global__ __launch_bounds__(256) void decode_kernel(DecodeArgs a, uint32_t parts, float *part) {
+    constexpr int NU = DP * int(sizeof(C)) / 64;    // 16-byte pieces of a vector that a lane holds
+    constexpr int NS = DP / 32;                     // steps of 32 values of the first product
+    constexpr int NB = DP / 16;                     // blocks of 16 values of the second
+    constexpr int PITCH = DP * int(sizeof(C)) + 16; // a value vector's bytes in LDS: rows start four banks apart
+    constexpr int CH = 512;                         // positions looked up at a time
+    constexpr int JOIN = 2 * 16 * (DP + 4) * 4;     // the waves' sums on their way to each other
+    constexpr int STAGE = 4 * 32 * PITCH;
+    __shared__ __align__(16) char s_mem[STAGE > JOIN ? STAGE : JOIN];
+    __shared__ int64_t s_vec[CH];  // a position's vector in the pool, -1: none
+    __shared__ __align__(16) float s_ks[scaled<C> ? CH : 4], s_vs[scaled<C> ? CH : 4];
+    __shared__ float s_ml[2][2][16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g4 = lane >> 4;
+    const int64_t r = blockIdx.x;
+    const int group = a.q_heads / a.kv.heads, blocks = (group + 15) / 16;
+    const int hk = blockIdx.y / blocks, q0 = int(blockIdx.y) % blocks * 16, dim = a.kv.dim;
+    const int h = hk * group + q0 + n;  // the lane's query head
+    const bool real = q0 + n < group;
+    const int len = clamp_len(a.lens[r], a.table.width, a.kv.page);
+    const Parts ps = parts_of(len, parts);
+    const int lo = int(blockIdx.z) * ps.each, hi = min(len, lo + ps.each);
+    if (parts > 1 && lo >= hi) return;
+
+    // The lane's query, in the order of its key pieces; bfloat16 queries over an 8-bit cache as
+    // float16 with their largest value's exponent taken out.
+    M qf[NS][8];
+    float score_scale = a.scale * 1.4426950408889634f;
+    {
+        const int64_t at = r * a.q_stride + int64_t(h) * dim;
+        float x[NS][8], top = 0.f;
+#pragma unroll
+        for (int s = 0; s < NS; s++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int c = sizeof(C) == 1 ? 64 * (s >> 1) + 16 * g4 + 8 * (s & 1) + i : 32 * s + 8 * g4 + i;
+                x[s][i] = real && c < dim ? load16(a.q, a.type, at + c) : 0.f;
+                top = fmaxf(top, fabsf(x[s][i]));
+            }
+        float down = 1.f;
+        if (sizeof(C) == 1 && a.type == T_BF16) {
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const int e = top > 0.f && top < INFINITY ? max(-100, min(100, ilogbf(top))) : 0;
+            down = ldexpf(1.f, -e);
+            score_scale *= ldexpf(1.f, e);
+        }
+#pragma unroll
+        for (int s = 0; s < NS; s++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) qf[s][i] = M(x[s][i] * down);
+    }
+    const float slope = a.slopes && real ? a.slopes[h] * 1.4426950408889634f : 0.f;
+
+    typedef M mvec __attribute__((ext_vector_type(8)));
+    f32x4 o[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) o[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    float vtop = 0.f, vinv = 0.f;  // a power of two over all value scales so far, and one over it
+    char *const s_v = s_mem + wave * 32 * PITCH;
+    const int pieces = dim * int(sizeof(C)) / 16;
+    const int64_t vec_bytes = int64_t(dim) * sizeof(C);
+
+    for (int c0 = lo; c0 < hi; c0 += CH) {
+        if (c0 != lo) __syncthreads();
+        const int cn = min(CH, hi - c0);
+        for (int i = tid; i < (cn + 31 & ~31); i += 256) {
+            int64_t vec = -1;
+            if (i < cn) {
+                const int32_t p = page_of(a.table.p + r * a.table.width, a.table.width, a.kv.page, a.kv.pages, c0 + i);
+                if (p >= 0) vec = slot_of(p, a.kv.heads, a.kv.page, hk, uint32_t(c0 + i) % a.kv.page);
+            }
+            s_vec[i] = vec;
+            if constexpr (scaled<C>) {
+                s_ks[i] = vec < 0 ? 0.f : a.kv.k_scale[vec];
+                s_vs[i] = vec < 0 ? 0.f : a.kv.v_scale[vec];
+            }
+        }
+        __syncthreads();
+        u32x4 kr[2][NU], vr[2][NU];
+        auto load = [&](int t0) {
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const int64_t vec = t0 < cn ? s_vec[t0 + 16 * t + n] : -1;
+                const char *kp = static_cast<const char *>(a.kv.k) + vec * vec_bytes, *vp = static_cast<const char *>(a.kv.v) + vec * vec_bytes;
+#pragma unroll
+                for (int u = 0; u < NU; u++) {
+                    const int piece = 4 * u + g4;
+                    const bool there = vec >= 0 && piece < pieces;
+                    kr[t][u] = there ? *reinterpret_cast<const u32x4 *>(kp + 16 * piece) : u32x4{0, 0, 0, 0};
+                    vr[t][u] = there ? *reinterpret_cast<const u32x4 *>(vp + 16 * piece) : u32x4{0, 0, 0, 0};
+                }
+            }
+        };
+        load(wave * 32);
+        for (int t0 = wave * 32; t0 < cn; t0 += 128) {
+            f32x4 s[2];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int st = 0; st < NS; st++) {
+                    mvec kf, q;
+                    if constexpr (sizeof(C) == 1) kf = widen8<C>(kr[t][st >> 1][2 * (st & 1)], kr[t][st >> 1][2 * (st & 1) + 1]);
+                    else kf = __builtin_bit_cast(mvec, kr[t][st]);
+                    for (int i = 0; i < 8; i++) q[i] = qf[st][i];
+                    s[t] = mfma16(kf, q, s[t]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int u = 0; u < NU; u++)
+                    if (4 * u + g4 < pieces) *reinterpret_cast<u32x4 *>(s_v + (16 * t + n) * PITCH + 16 * (4 * u + g4)) = vr[t][u];
+            load(t0 + 128);
+            // Scores in units of log2.
+            float top = -INFINITY, sc[2][4];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const int j0 = t0 + 16 * t + 4 * g4;
+                f32x4 ks{1.f, 1.f, 1.f, 1.f};
+                if constexpr (scaled<C>) ks = *reinterpret_cast<const f32x4 *>(&s_ks[j0]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float x = s[t][i] * score_scale * ks[i];
+                    if (a.cap > 0.f) x = cap_log2(x, a.cap);
+                    x -= slope * float(len - 1 - (c0 + j0 + i));
+                    sc[t][i] = j0 + i < cn ? x : -INFINITY;
+                    top = fmaxf(top, sc[t][i]);
+                }
+            }
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            if (__any(top > m + kSlack)) {
+                const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : exp2_f32(m - mn);
+                l *= f;
+#pragma unroll
+                for (int b = 0; b < NB; b++) o[b] *= f;
+                m = mn;
+            }
+            const float ref = m == -INFINITY ? 0.f : m - kLift;
+            mvec p;
+            float vs[2][4], vmax = 0.f;
+            if constexpr (scaled<C>) {
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    const f32x4 x = *reinterpret_cast<const f32x4 *>(&s_vs[t0 + 16 * t + 4 * g4]);
+                    for (int i = 0; i < 4; i++) vs[t][i] = x[i], vmax = fmaxf(vmax, fabsf(x[i]));
+                }
+                if (__any(vmax > vtop)) {
+                    vmax = fmaxf(vmax, __shfl_xor(vmax, 16));
+                    vmax = fmaxf(vmax, __shfl_xor(vmax, 32));
+                    if (vmax > vtop) {
+                        const float vn = __uint_as_float(min((__float_as_uint(vmax) & 0x7f800000u) + 0x00800000u, 0x7e800000u)), f = vtop / vn;
+#pragma unroll
+                        for (int b = 0; b < NB; b++) o[b] *= f;
+                        vtop = vn, vinv = 1.f / vn;
+                    }
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float w = exp2_f32(sc[t][i] - ref);
+                    l += w;
+                    if constexpr (scaled<C>) w *= vs[t][i] * vinv;
+                    p[4 * t + i] = M(w);
+                }
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                if (16 * b >= dim) continue;
+                mvec vf;
+                if constexpr (sizeof(C) == 1) {
+                    const int row = (lane & 15) >> 1;
+                    const u32x2 x = lds_read_tr8(s_v + (16 * (row >> 2) + 4 * g4 + (row & 3)) * PITCH + 16 * b + 8 * (lane & 1));
+                    vf = widen8<C>(x[0], x[1]);
+                } else {
+                    const int row = 4 * g4 + ((lane & 15) >> 2);
+                    const u32x2 x = lds_read_tr16(s_v + row * PITCH + 32 * b + 8 * (lane & 3));
+                    const u32x2 y = lds_read_tr16(s_v + (16 + row) * PITCH + 32 * b + 8 * (lane & 3));
+                    vf = __builtin_bit_cast(mvec, u32x4{x[0], x[1], y[0], y[1]});
+                }
+                o[b] = mfma16(vf, p, o[b]);
+            }
+        }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    // True scale: the lift taken out with room for the sums of the largest values.
+    const float back = scaled<C> ? vtop * 0x1p-14f : 0x1p-14f;
+#pragma unroll
+    for (int b = 0; b < NB; b++) o[b] *= back;
+    l *= 0x1p-14f;
+    // Waves 2 and 3 hand their sums to 0 and 1, then 1 to 0.
+    float *const s_o = reinterpret_cast<float *>(s_mem);
+#pragma unroll
+    for (int step = 2; step >= 1; step >>= 1) {
+        __syncthreads();
+        if (wave >= step && wave < 2 * step) {
+            float *dst = s_o + ((wave - step) * 16 + n) * (DP + 4);
+#pragma unroll
+            for (int b = 0; b < NB; b++) *reinterpret_cast<f32x4 *>(dst + 16 * b + 4 * g4) = o[b];
+            if (g4 == 0) s_ml[wave - step][0][n] = m, s_ml[wave - step][1][n] = l;
+        }
+        __syncthreads();
+        if (wave < step) {
+            const float *src = s_o + (wave * 16 + n) * (DP + 4);
+            const float m2 = s_ml[wave][0][n], l2 = s_ml[wave][1][n], mn = fmaxf(m, m2);
+            const float f = mn == -INFINITY ? 0.f : exp2_f32(m - mn), f2 = mn == -INFINITY ? 0.f : exp2_f32(m2 - mn);
+            l = l * f + l2 * f2;
+#pragma unroll
+            for (int b = 0; b < NB; b++) o[b] = o[b] * f + *reinterpret_cast<const f32x4 *>(src + 16 * b + 4 * g4) * f2;
+            m = mn;
+        }
+    }
+    if (wave != 0 || !real) return;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (part) {
+        float *dst = part + ((r * a.q_heads + h) * parts + blockIdx.z) * (dim + kPartTail);
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+            if (16 * b + 4 * g4 < dim) *reinterpret_cast<f32x4 *>(dst + 16 * b + 4 * g4) = o[b] * inv;
+        if (g4 == 0) dst[dim] = l == 0.f ? -INFINITY : m + log2f(l);
+    } else {
+        const int64_t at = r * a.out_stride + int64_t(h) * dim;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+            for (int i = 0; i < 4; i++)
+                if (16 * b + 4 * g4 < dim) store16(a.out, a.type, at + 16 * b + 4 * g4 + i, o[b][i] * inv);
+    }
+}
+
+// One workgroup a (sequence, head): 16-byte pieces of the parts side by side.
+__global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a, uint32_t parts, const float *part) {
+    __shared__ float s_w[kMostParts], s_o[256 * 4];
+    const int64_t r = blockIdx.x;
+    const int h = blockIdx.y, dim = a.kv.dim, tid = threadIdx.x;
+    const int len = clamp_len(a.lens[r], a.table.width, a.kv.page), count = parts_of(len, parts).count;
+    const float *src = part + (r * a.q_heads + h) * parts * (dim + kPartTail);
+    float lse = -INFINITY, m;
+    if (tid < count) lse = src[int64_t(tid) * (dim + kPartTail) + dim];
+    if (tid < kMostParts) s_w[tid] = lse;
+    __syncthreads();
+    m = -INFINITY;
+    for (int i = 0; i < count; i++) m = fmaxf(m, s_w[i]);
+    __syncthreads();
+    const float w = tid < count ? (lse == -INFINITY ? 0.f : exp2_f32(lse - m)) : 0.f;
+    if (tid < kMostParts) s_w[tid] = w;
+    __syncthreads();
+    const int lanes = dim / 4, side = 256 / lanes, c = tid % lanes, k = tid / lanes;
+    f32x4 o{0.f, 0.f, 0.f, 0.f};
+    float total = 0.f;
+    for (int i = 0; i < count; i++) total += s_w[i];
+    if (k < side)
+        for (int i = k; i < count; i += side) o += *reinterpret_cast<const f32x4 *>(src + int64_t(i) * (dim + kPartTail) + 4 * c) * s_w[i];
+    *reinterpret_cast<f32x4 *>(&s_o[tid * 4]) = o;
+    __syncthreads();
+    if (k != 0) return;
+    for (int i = 1; i < side; i++) o += *reinterpret_cast<const f32x4 *>(&s_o[(tid + i * lanes) * 4]);
+    const int64_t at = r * a.out_stride + int64_t(h) * dim + 4 * c;
+    for (int i = 0; i < 4; i++) store16(a.out, a.type, at + i, total == 0.f ? 0.f : o[i] / total);
+}
+
+template <class C, class M> void launch_tiles(const DecodeArgs &a, uint32_t parts, float *part, hipStream_t s) {
+    const dim3 grid(a.table.rows, a.kv.heads * ((a.q_heads / a.kv.heads + 15) / 16), parts);
+    if (a.kv.dim <= 64) hipLaunchKernelGGL((decode_kernel<C, M, 64>), grid, dim3(256), 0, s, a, parts, part);
+    else if (a.kv.dim <= 128) hipLaunchKernelGGL((decode_kernel<C, M, 128>), grid, dim3(256), 0, s, a, parts, part);
+    else hipLaunchKernelGGL((decode_kernel<C, M, 256>), grid, dim3(256), 0, s, a, parts, part);
+    OCR_HIP(hipGetLastError());
+}
+
 }  // namespace
 
-void launch_decode(Ctx &, const DecodeArgs &a, hipStream_t s) {
+void launch_decode(Ctx &c, const DecodeArgs &a, hipStream_t s) {
     ProbeScope probe("text_decode", s, 4.0 * a.table.rows * a.table.width * a.kv.page * a.q_heads * a.kv.dim,
                      2.0 * a.table.rows * a.table.width * a.kv.page * a.kv.heads * a.kv.dim * type_bytes(a.kv.type));
-    with_type16(a.type, [&](auto t) {
-        with_cache(a.kv.type, [&](auto c) {
-            hipLaunchKernelGGL((decode_row_kernel<decltype(t), decltype(c)>), dim3(a.table.rows, a.q_heads), dim3(64), 0, s, a);
+    const bool pieces = a.kv.dim * type_bytes(a.kv.type) % 16 == 0 && reinterpret_cast<uintptr_t>(a.kv.k) % 16 == 0 &&
+                        reinterpret_cast<uintptr_t>(a.kv.v) % 16 == 0;
+    if (!pieces) {
+        with_type16(a.type, [&](auto t) {
+            with_cache(a.kv.type, [&](auto k) {
+                if constexpr (scaled<decltype(k)> || std::is_same_v<decltype(t), decltype(k)>)
+                    hipLaunchKernelGGL((decode_row_kernel<decltype(t), decltype(k)>), dim3(a.table.rows, a.q_heads), dim3(64), 0, s, a);
+            });
         });
+        OCR_HIP(hipGetLastError());
+        return;
+    }
+    // Parts until there are a few workgroups for every compute unit; a sequence has as many as its
+    // own length gives work to.
+    const uint64_t heads = uint64_t(a.table.rows) * a.kv.heads * ((a.q_heads / a.kv.heads + 15) / 16);
+    const uint64_t most = uint64_t(a.table.width) * a.kv.page;
+    const uint32_t parts = uint32_t(std::max<uint64_t>(1, std::min<uint64_t>({kMostParts, (2048 + heads - 1) / heads, (most + kLeastPart - 1) / kLeastPart})));
+    DBuf part;
+    if (parts > 1) part = DBuf(&c, size_t(a.table.rows) * a.q_heads * parts * (a.kv.dim + kPartTail) * 4, s);
+    with_cache(a.kv.type, [&](auto k) {
+        using C = decltype(k);
+        launch_tiles<C, std::conditional_t<std::is_same_v<C, bf16>, bf16, f16>>(a, parts, part.as<float>(), s);
     });
-    OCR_HIP(hipGetLastError());
+    if (parts > 1) {
+        hipLaunchKernelGGL(decode_join_kernel, dim3(a.table.rows, a.q_heads), dim3(256), 0, s, a, parts, part.as<float>());
+        OCR_HIP(hipGetLastError());
+    }
 }
 
 }  // namespace ocr

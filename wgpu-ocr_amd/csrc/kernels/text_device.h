@@ -38,6 +38,67 @@ __device__ inline float to_f32(bf16 v) { return float(v); }
 __device__ inline float to_f32(int8_t v) { return float(v); }
 __device__ inline float to_f32(e4m3 v) { return __builtin_amdgcn_cvt_f32_fp8(int(v.bits), 0); }
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef f16 f16x2 __attribute__((ext_vector_type(2)));
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// 16-bit values whose type is known at run time (uniform).
+__device__ inline float load16(const void *p, int type, int64_t i) {
+    return type == T_F16 ? float(static_cast<const f16 *>(p)[i]) : float(static_cast<const bf16 *>(p)[i]);
+}
+__device__ inline void store16(void *p, int type, int64_t i, float v) {
+    if (type == T_F16) static_cast<f16 *>(p)[i] = f16(v);
+    else static_cast<bf16 *>(p)[i] = bf16(v);
+}
+
+// D[16][16] += A[16][32] B[32][16]: lane l holds A's row and B's column l % 16, values 8 (l / 16) on
+// of the 32; of D, column l % 16 and rows 4 (l / 16) on.
+__device__ inline f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ inline f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// Transposing reads of LDS. 16 lanes name 4 rows of 16 values of 16 bits (lanes 4 r to 4 r + 3 the
+// four quarters of row r), or 8 rows of 16 bytes (lanes 2 r, 2 r + 1 the halves); each gets its column.
+__device__ inline u32x2 lds_read_tr16(const char *p) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)p));
+}
+__device__ inline u32x2 lds_read_tr8(const char *p) {
+    typedef int i2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i2 *)p));
+}
+
+// Eight codes of an 8-bit cache as float16, exactly.
+template <class C> __device__ inline f16x8 widen8(uint32_t a, uint32_t b) {
+    f16x2 x[4];
+    if constexpr (std::is_same_v<C, int8_t>) {
+        // 0x6400 | u is 1024 + u.
+        a ^= 0x80808080u, b ^= 0x80808080u;
+        const f16x2 off{f16(1152.f), f16(1152.f)};
+        x[0] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u)) - off;
+        x[1] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u)) - off;
+        x[2] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) - off;
+        x[3] = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) - off;
+    } else {
+        x[0] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, false));
+        x[1] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, true));
+        x[2] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, false));
+        x[3] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, true));
+    }
+    return f16x8{x[0][0], x[0][1], x[1][0], x[1][1], x[2][0], x[2][1], x[3][0], x[3][1]};
+}
+
+// 2^x; results under the normal range are zero.
+__device__ inline float exp2_f32(float x) { return __builtin_amdgcn_exp2f(x); }
+// A score in units of log2 through the cap: cap tanh(s / cap), tanh(y) = 1 - 2 / (e^2y + 1).
+__device__ inline float cap_log2(float x, float cap) {
+    const float c = cap * 1.4426950408889634f;
+    return c - 2.f * c * __builtin_amdgcn_rcpf(exp2_f32(x * (2.f / cap)) + 1.f);
+}
+
 // The code of a value already divided by its vector's scale (rounded to nearest, ties to even).
 template <class C> __device__ inline C code_of(float v) {
     if constexpr (std::is_same_v<C, int8_t>) return int8_t(rintf(v));

@@ -83,4 +83,18 @@ OCR_HD Fork fork_of(const int32_t *parents, uint32_t beams, uint32_t w, const in
     return f;
 }
 
+// How a sequence of len positions is cut for single-token attention: at most `parts` parts of at
+// least kLeastPart positions, whole tiles of 32.
+constexpr int kLeastPart = 256;
+constexpr uint32_t kMostParts = 128;
+struct Parts {
+    int count, each;
+};
+OCR_HD Parts parts_of(int len, uint32_t parts) {
+    if (len <= 0) return {0, kLeastPart};
+    const int want = int((uint32_t(len) + parts - 1) / parts);
+    const int each = want <= kLeastPart ? kLeastPart : (want + 31) & ~31;
+    return parts == 1 ? Parts{1, len} : Parts{int((uint32_t(len) + uint32_t(each) - 1) / uint32_t(each)), each};
+}
+
 }  // namespace ocr
