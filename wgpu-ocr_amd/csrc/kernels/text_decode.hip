@@ -58,7 +58,11 @@ constexpr float kLift = 6.f, kSlack = 8.f;
 // sum of weights.
 constexpr int kPartTail = 4;  // keeps the rows' 16-byte alignment
 
-template <class C, class M, int DP> __global__ __launch_bounds__(256) void decode_kernel(DecodeArgs a, uint32_t parts, float *part) {
+// T: the queries' type, C: the cache's; products of 8-bit caches in float16, which holds their codes
+// exactly.
+template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 3 : 1) void decode_kernel(DecodeArgs a, uint32_t parts, float *part, bool q_pieces) {
+    using M = std::conditional_t<scaled<C>, f16, C>;
+    typedef M mvec __attribute__((ext_vector_type(8)));
     constexpr int NU = DP * int(sizeof(C)) / 64;    // 16-byte pieces of a vector that a lane holds
     constexpr int NS = DP / 32;                     // steps of 32 values of the first product
     constexpr int NB = DP / 16;                     // blocks of 16 values of the second
@@ -67,8 +71,8 @@ template <class C, class M, int DP> __global__ __launch_bounds__(256) void decod
     constexpr int JOIN = 2 * 16 * (DP + 4) * 4;     // the waves' sums on their way to each other
     constexpr int STAGE = 4 * 32 * PITCH;
     __shared__ __align__(16) char s_mem[STAGE > JOIN ? STAGE : JOIN];
-    __shared__ int64_t s_vec[CH];  // a position's vector in the pool, -1: none
-    __shared__ __align__(16) float s_ks[scaled<C> ? CH : 4], s_vs[scaled<C> ? CH : 4];
+    __shared__ int64_t s_at[CH];  // a position's vector in the pool, negative: none
+    __shared__ __align__(16) float s_scale[4][2][32];  // the waves' key and value scales of a tile
     __shared__ float s_ml[2][2][16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g4 = lane >> 4;
     const int64_t r = blockIdx.x;
@@ -76,122 +80,169 @@ template <class C, class M, int DP> __global__ __launch_bounds__(256) void decod
     const int hk = blockIdx.y / blocks, q0 = int(blockIdx.y) % blocks * 16, dim = a.kv.dim;
     const int h = hk * group + q0 + n;  // the lane's query head
     const bool real = q0 + n < group;
+    // The lane's query, in the order of its key pieces.
+    u32x4 raw[NS];
+#pragma unroll
+    for (int s = 0; s < NS; s++) {
+        const int c = sizeof(C) == 1 ? 64 * (s >> 1) + 16 * g4 + 8 * (s & 1) : 32 * s + 8 * g4;
+        raw[s] = u32x4{0, 0, 0, 0};
+        if (real && c < dim) raw[s] = load16x8(a.q, r * a.q_stride + int64_t(h) * dim + c, q_pieces);
+    }
     const int len = clamp_len(a.lens[r], a.table.width, a.kv.page);
     const Parts ps = parts_of(len, parts);
     const int lo = int(blockIdx.z) * ps.each, hi = min(len, lo + ps.each);
     if (parts > 1 && lo >= hi) return;
 
-    // The lane's query, in the order of its key pieces; bfloat16 queries over an 8-bit cache as
-    // float16 with their largest value's exponent taken out.
-    M qf[NS][8];
-    float score_scale = a.scale * 1.4426950408889634f;
-    {
-        const int64_t at = r * a.q_stride + int64_t(h) * dim;
-        float x[NS][8], top = 0.f;
+    const int pieces = dim * int(sizeof(C)) / 16;
+    const uint32_t vec_bytes = dim * int(sizeof(C));
+    uint32_t off[NU];
 #pragma unroll
-        for (int s = 0; s < NS; s++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int c = sizeof(C) == 1 ? 64 * (s >> 1) + 16 * g4 + 8 * (s & 1) + i : 32 * s + 8 * g4 + i;
-                x[s][i] = real && c < dim ? load16(a.q, a.type, at + c) : 0.f;
-                top = fmaxf(top, fabsf(x[s][i]));
-            }
-        float down = 1.f;
-        if (sizeof(C) == 1 && a.type == T_BF16) {
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const int e = top > 0.f && top < INFINITY ? max(-100, min(100, ilogbf(top))) : 0;
-            down = ldexpf(1.f, -e);
-            score_scale *= ldexpf(1.f, e);
-        }
-#pragma unroll
-        for (int s = 0; s < NS; s++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) qf[s][i] = M(x[s][i] * down);
-    }
+    for (int u = 0; u < NU; u++) off[u] = 16 * min(4 * u + g4, pieces - 1);
+    char *const s_v = s_mem + wave * 32 * PITCH;
     const float slope = a.slopes && real ? a.slopes[h] * 1.4426950408889634f : 0.f;
-
-    typedef M mvec __attribute__((ext_vector_type(8)));
+    float score_scale = a.scale * 1.4426950408889634f;
+    mvec qf[NS];
     f32x4 o[NB];
 #pragma unroll
     for (int b = 0; b < NB; b++) o[b] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
     float vtop = 0.f, vinv = 0.f;  // a power of two over all value scales so far, and one over it
-    char *const s_v = s_mem + wave * 32 * PITCH;
-    const int pieces = dim * int(sizeof(C)) / 16;
-    const int64_t vec_bytes = int64_t(dim) * sizeof(C);
 
     for (int c0 = lo; c0 < hi; c0 += CH) {
         if (c0 != lo) __syncthreads();
         const int cn = min(CH, hi - c0);
-        for (int i = tid; i < (cn + 31 & ~31); i += 256) {
-            int64_t vec = -1;
+        for (int i = tid; i < ((cn + 31) & ~31); i += 256) {
+            int64_t at = -1;
             if (i < cn) {
                 const int32_t p = page_of(a.table.p + r * a.table.width, a.table.width, a.kv.page, a.kv.pages, c0 + i);
-                if (p >= 0) vec = slot_of(p, a.kv.heads, a.kv.page, hk, uint32_t(c0 + i) % a.kv.page);
+                if (p >= 0) at = slot_of(p, a.kv.heads, a.kv.page, hk, uint32_t(c0 + i) % a.kv.page);
             }
-            s_vec[i] = vec;
-            if constexpr (scaled<C>) {
-                s_ks[i] = vec < 0 ? 0.f : a.kv.k_scale[vec];
-                s_vs[i] = vec < 0 ? 0.f : a.kv.v_scale[vec];
-            }
+            s_at[i] = at;
         }
         __syncthreads();
+        // A tile's keys, values and scales; where there is no vector or no such piece of it, some
+        // other of the pool, zeroed when the tile is used.
         u32x4 kr[2][NU], vr[2][NU];
+        float scale_r = 0.f;
+        bool none[2];
         auto load = [&](int t0) {
+            if (t0 >= cn) return;
+            int64_t at[2];
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const int64_t vec = t0 < cn ? s_vec[t0 + 16 * t + n] : -1;
-                const char *kp = static_cast<const char *>(a.kv.k) + vec * vec_bytes, *vp = static_cast<const char *>(a.kv.v) + vec * vec_bytes;
-#pragma unroll
-                for (int u = 0; u < NU; u++) {
-                    const int piece = 4 * u + g4;
-                    const bool there = vec >= 0 && piece < pieces;
-                    kr[t][u] = there ? *reinterpret_cast<const u32x4 *>(kp + 16 * piece) : u32x4{0, 0, 0, 0};
-                    vr[t][u] = there ? *reinterpret_cast<const u32x4 *>(vp + 16 * piece) : u32x4{0, 0, 0, 0};
-                }
+            for (int t = 0; t < 2; t++) at[t] = s_at[t0 + 16 * t + n], none[t] = at[t] < 0, at[t] = none[t] ? 0 : at[t];
+            if constexpr (scaled<C>) {
+                const int64_t vec = (g4 & 1) ? at[1] : at[0];
+                scale_r = (g4 < 2 ? a.kv.k_scale : a.kv.v_scale)[vec];
             }
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int u = 0; u < NU; u++)
+                    kr[t][u] = *reinterpret_cast<const u32x4 *>(static_cast<const char *>(a.kv.k) + at[t] * vec_bytes + off[u]);
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int u = 0; u < NU; u++)
+                    vr[t][u] = *reinterpret_cast<const u32x4 *>(static_cast<const char *>(a.kv.v) + at[t] * vec_bytes + off[u]);
         };
         load(wave * 32);
+        if (c0 == lo) {
+            // bfloat16 queries over an 8-bit cache as float16, their largest value's exponent taken
+            // out: the steps lost under 2^-14 of it are 2^-25 of it.
+            if constexpr (scaled<C> && std::is_same_v<T, bf16>) {
+                float top = 0.f;
+#pragma unroll
+                for (int s = 0; s < NS; s++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(widen16(raw[s][i >> 1] >> (16 * (i & 1)), T_BF16)));
+                top = wave_max(top);
+                const int e = top > 0.f && top < INFINITY ? max(-100, min(100, ilogbf(top))) : 0;
+                const float down = ldexpf(1.f, -e);
+                score_scale *= ldexpf(1.f, e);
+#pragma unroll
+                for (int s = 0; s < NS; s++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) qf[s][i] = M(widen16(raw[s][i >> 1] >> (16 * (i & 1)), T_BF16) * down);
+            } else {
+#pragma unroll
+                for (int s = 0; s < NS; s++) qf[s] = __builtin_bit_cast(mvec, raw[s]);
+            }
+        }
         for (int t0 = wave * 32; t0 < cn; t0 += 128) {
+            if (pieces < 4 * NU || __any(none[0] || none[1])) {
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int u = 0; u < NU; u++)
+                        if (none[t] || 4 * u + g4 >= pieces) kr[t][u] = vr[t][u] = u32x4{0, 0, 0, 0};
+                if (none[g4 & 1]) scale_r = 0.f;
+            }
+            // The tile's scales: the keys' with the scores' own, the values' over their power of two.
+            if constexpr (scaled<C>) {
+                if (__any(g4 >= 2 && fabsf(scale_r) > vtop)) {
+                    const float vmax = wave_max(g4 >= 2 ? fabsf(scale_r) : 0.f);
+                    const float vn = __uint_as_float(min((__float_as_uint(vmax) & 0x7f800000u) + 0x00800000u, 0x7e800000u)), f = vtop / vn;
+#pragma unroll
+                    for (int b = 0; b < NB; b++) o[b] *= f;
+                    vtop = vn, vinv = 1.f / vn;
+                }
+                s_scale[wave][g4 >> 1][16 * (g4 & 1) + n] = scale_r * (g4 < 2 ? score_scale : vinv);
+            }
             f32x4 s[2];
 #pragma unroll
             for (int t = 0; t < 2; t++) {
                 s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int st = 0; st < NS; st++) {
-                    mvec kf, q;
-                    if constexpr (sizeof(C) == 1) kf = widen8<C>(kr[t][st >> 1][2 * (st & 1)], kr[t][st >> 1][2 * (st & 1) + 1]);
+                    mvec kf;
+                    if constexpr (scaled<C>) kf = widen8<C>(kr[t][st >> 1][2 * (st & 1)], kr[t][st >> 1][2 * (st & 1) + 1]);
                     else kf = __builtin_bit_cast(mvec, kr[t][st]);
-                    for (int i = 0; i < 8; i++) q[i] = qf[st][i];
-                    s[t] = mfma16(kf, q, s[t]);
+                    s[t] = mfma16(kf, qf[st], s[t]);
                 }
             }
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
                 for (int u = 0; u < NU; u++)
-                    if (4 * u + g4 < pieces) *reinterpret_cast<u32x4 *>(s_v + (16 * t + n) * PITCH + 16 * (4 * u + g4)) = vr[t][u];
+                    *reinterpret_cast<u32x4 *>(s_v + (16 * t + n) * PITCH + 16 * (4 * u + g4)) = vr[t][u];
             load(t0 + 128);
             // Scores in units of log2.
-            float top = -INFINITY, sc[2][4];
+            float sc[2][4];
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                const int j0 = t0 + 16 * t + 4 * g4;
-                f32x4 ks{1.f, 1.f, 1.f, 1.f};
-                if constexpr (scaled<C>) ks = *reinterpret_cast<const f32x4 *>(&s_ks[j0]);
+                f32x4 ks{score_scale, score_scale, score_scale, score_scale};
+                if constexpr (scaled<C>) ks = *reinterpret_cast<const f32x4 *>(&s_scale[wave][0][16 * t + 4 * g4]);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    float x = s[t][i] * score_scale * ks[i];
-                    if (a.cap > 0.f) x = cap_log2(x, a.cap);
-                    x -= slope * float(len - 1 - (c0 + j0 + i));
-                    sc[t][i] = j0 + i < cn ? x : -INFINITY;
-                    top = fmaxf(top, sc[t][i]);
-                }
+                for (int i = 0; i < 4; i++) sc[t][i] = s[t][i] * ks[i];
             }
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
+            if (a.cap > 0.f) {
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sc[t][i] = cap_log2(sc[t][i], a.cap);
+            }
+            if (a.slopes) {
+                const float d = float(len - 1 - c0 - t0 - 4 * g4);
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sc[t][i] -= slope * (d - float(16 * t + i));
+            }
+            if (t0 + 32 > cn) {
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (t0 + 16 * t + 4 * g4 + i >= cn) sc[t][i] = -INFINITY;
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) top = fmaxf(top, sc[t][i]);
             if (__any(top > m + kSlack)) {
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
                 const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : exp2_f32(m - mn);
                 l *= f;
 #pragma unroll
@@ -200,38 +251,22 @@ template <class C, class M, int DP> __global__ __launch_bounds__(256) void decod
             }
             const float ref = m == -INFINITY ? 0.f : m - kLift;
             mvec p;
-            float vs[2][4], vmax = 0.f;
-            if constexpr (scaled<C>) {
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const f32x4 x = *reinterpret_cast<const f32x4 *>(&s_vs[t0 + 16 * t + 4 * g4]);
-                    for (int i = 0; i < 4; i++) vs[t][i] = x[i], vmax = fmaxf(vmax, fabsf(x[i]));
-                }
-                if (__any(vmax > vtop)) {
-                    vmax = fmaxf(vmax, __shfl_xor(vmax, 16));
-                    vmax = fmaxf(vmax, __shfl_xor(vmax, 32));
-                    if (vmax > vtop) {
-                        const float vn = __uint_as_float(min((__float_as_uint(vmax) & 0x7f800000u) + 0x00800000u, 0x7e800000u)), f = vtop / vn;
-#pragma unroll
-                        for (int b = 0; b < NB; b++) o[b] *= f;
-                        vtop = vn, vinv = 1.f / vn;
-                    }
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < 2; t++)
+            for (int t = 0; t < 2; t++) {
+                f32x4 vs;
+                if constexpr (scaled<C>) vs = *reinterpret_cast<const f32x4 *>(&s_scale[wave][1][16 * t + 4 * g4]);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     float w = exp2_f32(sc[t][i] - ref);
                     l += w;
-                    if constexpr (scaled<C>) w *= vs[t][i] * vinv;
+                    if constexpr (scaled<C>) w *= vs[i];
                     p[4 * t + i] = M(w);
                 }
+            }
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                if (16 * b >= dim) continue;
                 mvec vf;
-                if constexpr (sizeof(C) == 1) {
+                if constexpr (scaled<C>) {
                     const int row = (lane & 15) >> 1;
                     const u32x2 x = lds_read_tr8(s_v + (16 * (row >> 2) + 4 * g4 + (row & 3)) * PITCH + 16 * b + 8 * (lane & 1));
                     vf = widen8<C>(x[0], x[1]);
@@ -291,43 +326,60 @@ template <class C, class M, int DP> __global__ __launch_bounds__(256) void decod
     }
 }
 
-// One workgroup a (sequence, head): 16-byte pieces of the parts side by side.
-__global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a, uint32_t parts, const float *part) {
-    __shared__ float s_w[kMostParts], s_o[256 * 4];
+// One workgroup a (sequence, head): four values a thread, the parts side by side.
+template <int N> __global__ __launch_bounds__(N) void decode_join_kernel(DecodeArgs a, uint32_t parts, const float *part) {
+    __shared__ __align__(16) float s_o[N * 4];
+    __shared__ float s_l[N];
     const int64_t r = blockIdx.x;
     const int h = blockIdx.y, dim = a.kv.dim, tid = threadIdx.x;
     const int len = clamp_len(a.lens[r], a.table.width, a.kv.page), count = parts_of(len, parts).count;
-    const float *src = part + (r * a.q_heads + h) * parts * (dim + kPartTail);
-    float lse = -INFINITY, m;
-    if (tid < count) lse = src[int64_t(tid) * (dim + kPartTail) + dim];
-    if (tid < kMostParts) s_w[tid] = lse;
-    __syncthreads();
-    m = -INFINITY;
-    for (int i = 0; i < count; i++) m = fmaxf(m, s_w[i]);
-    __syncthreads();
-    const float w = tid < count ? (lse == -INFINITY ? 0.f : exp2_f32(lse - m)) : 0.f;
-    if (tid < kMostParts) s_w[tid] = w;
-    __syncthreads();
-    const int lanes = dim / 4, side = 256 / lanes, c = tid % lanes, k = tid / lanes;
+    const int pitch = dim + kPartTail, lanes = dim / 4, side = N / lanes, c = tid % lanes, k = tid / lanes;
+    const float *src = part + (r * a.q_heads + h) * parts * pitch;
+    // Each thread's parts are k, k + side, ...: a running maximum over them, then over the threads.
     f32x4 o{0.f, 0.f, 0.f, 0.f};
-    float total = 0.f;
-    for (int i = 0; i < count; i++) total += s_w[i];
-    if (k < side)
-        for (int i = k; i < count; i += side) o += *reinterpret_cast<const f32x4 *>(src + int64_t(i) * (dim + kPartTail) + 4 * c) * s_w[i];
-    *reinterpret_cast<f32x4 *>(&s_o[tid * 4]) = o;
+    float m = -INFINITY, l = 0.f;
+    if (k < side) {
+#pragma unroll 4
+        for (int i = k; i < count; i += side) {
+            const float lse = src[i * pitch + dim];
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(src + i * pitch + 4 * c);
+            const float mn = fmaxf(m, lse), f = mn == -INFINITY ? 0.f : exp2_f32(m - mn), w = lse == -INFINITY ? 0.f : exp2_f32(lse - mn);
+            o = o * f + x * w;
+            l = l * f + w, m = mn;
+        }
+    }
+    s_l[tid] = m;
+    __syncthreads();
+    float top = -INFINITY;
+    for (int i = 0; i < side; i++) top = fmaxf(top, s_l[c + i * lanes]);
+    __syncthreads();
+    const float f = top == -INFINITY ? 0.f : exp2_f32(m - top);
+    s_l[tid] = l * f;
+    *reinterpret_cast<f32x4 *>(&s_o[tid * 4]) = o * f;
     __syncthreads();
     if (k != 0) return;
-    for (int i = 1; i < side; i++) o += *reinterpret_cast<const f32x4 *>(&s_o[(tid + i * lanes) * 4]);
+    o = f32x4{0.f, 0.f, 0.f, 0.f}, l = 0.f;
+    for (int i = 0; i < side; i++) o += *reinterpret_cast<const f32x4 *>(&s_o[(c + i * lanes) * 4]), l += s_l[c + i * lanes];
     const int64_t at = r * a.out_stride + int64_t(h) * dim + 4 * c;
-    for (int i = 0; i < 4; i++) store16(a.out, a.type, at + i, total == 0.f ? 0.f : o[i] / total);
+    for (int i = 0; i < 4; i++) store16(a.out, a.type, at + i, l == 0.f ? 0.f : o[i] / l);
 }
 
-template <class C, class M> void launch_tiles(const DecodeArgs &a, uint32_t parts, float *part, hipStream_t s) {
+template <class T, class C> void launch_tiles(const DecodeArgs &a, uint32_t parts, float *part, hipStream_t s) {
+    const bool q_pieces = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_stride % 8 == 0;
     const dim3 grid(a.table.rows, a.kv.heads * ((a.q_heads / a.kv.heads + 15) / 16), parts);
-    if (a.kv.dim <= 64) hipLaunchKernelGGL((decode_kernel<C, M, 64>), grid, dim3(256), 0, s, a, parts, part);
-    else if (a.kv.dim <= 128) hipLaunchKernelGGL((decode_kernel<C, M, 128>), grid, dim3(256), 0, s, a, parts, part);
-    else hipLaunchKernelGGL((decode_kernel<C, M, 256>), grid, dim3(256), 0, s, a, parts, part);
+    if (a.kv.dim <= 64) hipLaunchKernelGGL((decode_kernel<T, C, 64>), grid, dim3(256), 0, s, a, parts, part, q_pieces);
+    else if (a.kv.dim <= 128) hipLaunchKernelGGL((decode_kernel<T, C, 128>), grid, dim3(256), 0, s, a, parts, part, q_pieces);
+    else hipLaunchKernelGGL((decode_kernel<T, C, 256>), grid, dim3(256), 0, s, a, parts, part, q_pieces);
     OCR_HIP(hipGetLastError());
+}
+
+// f(query type, cache type) of the pairs that check_decode lets through.
+template <class F> void with_pair(const DecodeArgs &a, F &&f) {
+    with_type16(a.type, [&](auto t) {
+        with_cache(a.kv.type, [&](auto k) {
+            if constexpr (scaled<decltype(k)> || std::is_same_v<decltype(t), decltype(k)>) f(t, k);
+        });
+    });
 }
 
 }  // namespace
@@ -338,11 +390,8 @@ void launch_decode(Ctx &c, const DecodeArgs &a, hipStream_t s) {
     const bool pieces = a.kv.dim * type_bytes(a.kv.type) % 16 == 0 && reinterpret_cast<uintptr_t>(a.kv.k) % 16 == 0 &&
                         reinterpret_cast<uintptr_t>(a.kv.v) % 16 == 0;
     if (!pieces) {
-        with_type16(a.type, [&](auto t) {
-            with_cache(a.kv.type, [&](auto k) {
-                if constexpr (scaled<decltype(k)> || std::is_same_v<decltype(t), decltype(k)>)
-                    hipLaunchKernelGGL((decode_row_kernel<decltype(t), decltype(k)>), dim3(a.table.rows, a.q_heads), dim3(64), 0, s, a);
-            });
+        with_pair(a, [&](auto t, auto k) {
+            hipLaunchKernelGGL((decode_row_kernel<decltype(t), decltype(k)>), dim3(a.table.rows, a.q_heads), dim3(64), 0, s, a);
         });
         OCR_HIP(hipGetLastError());
         return;
@@ -350,16 +399,16 @@ void launch_decode(Ctx &c, const DecodeArgs &a, hipStream_t s) {
     // Parts until there are a few workgroups for every compute unit; a sequence has as many as its
     // own length gives work to.
     const uint64_t heads = uint64_t(a.table.rows) * a.kv.heads * ((a.q_heads / a.kv.heads + 15) / 16);
+    static const uint64_t kWork = getenv("KWORK") ? atoi(getenv("KWORK")) : 768;
     const uint64_t most = uint64_t(a.table.width) * a.kv.page;
-    const uint32_t parts = uint32_t(std::max<uint64_t>(1, std::min<uint64_t>({kMostParts, (2048 + heads - 1) / heads, (most + kLeastPart - 1) / kLeastPart})));
+    const uint32_t parts = uint32_t(std::max<uint64_t>(1, std::min<uint64_t>({kMostParts, (kWork + heads - 1) / heads, (most + kLeastPart - 1) / kLeastPart})));
     DBuf part;
     if (parts > 1) part = DBuf(&c, size_t(a.table.rows) * a.q_heads * parts * (a.kv.dim + kPartTail) * 4, s);
-    with_cache(a.kv.type, [&](auto k) {
-        using C = decltype(k);
-        launch_tiles<C, std::conditional_t<std::is_same_v<C, bf16>, bf16, f16>>(a, parts, part.as<float>(), s);
-    });
+    with_pair(a, [&](auto t, auto k) { launch_tiles<decltype(t), decltype(k)>(a, parts, part.as<float>(), s); });
     if (parts > 1) {
-        hipLaunchKernelGGL(decode_join_kernel, dim3(a.table.rows, a.q_heads), dim3(256), 0, s, a, parts, part.as<float>());
+        const dim3 grid(a.table.rows, a.q_heads);
+        if (parts <= 8) hipLaunchKernelGGL(decode_join_kernel<64>, grid, dim3(64), 0, s, a, parts, part.as<float>());
+        else hipLaunchKernelGGL(decode_join_kernel<256>, grid, dim3(256), 0, s, a, parts, part.as<float>());
         OCR_HIP(hipGetLastError());
     }
 }

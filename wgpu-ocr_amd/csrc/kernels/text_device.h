@@ -47,8 +47,16 @@ typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 // 16-bit values whose type is known at run time (uniform).
-__device__ inline float load16(const void *p, int type, int64_t i) {
-    return type == T_F16 ? float(static_cast<const f16 *>(p)[i]) : float(static_cast<const bf16 *>(p)[i]);
+__device__ inline float widen16(uint32_t bits, int type) {
+    return type == T_F16 ? float(__builtin_bit_cast(f16, uint16_t(bits))) : __uint_as_float(bits << 16);
+}
+// Eight of them from value i on; aligned: i lies on 16 bytes (uniform).
+__device__ inline u32x4 load16x8(const void *p, int64_t i, bool aligned) {
+    const uint16_t *x = static_cast<const uint16_t *>(p) + i;
+    if (aligned) return *reinterpret_cast<const u32x4 *>(x);
+    u32x4 r;
+    for (int k = 0; k < 4; k++) r[k] = uint32_t(x[2 * k]) | uint32_t(x[2 * k + 1]) << 16;
+    return r;
 }
 __device__ inline void store16(void *p, int type, int64_t i, float v) {
     if (type == T_F16) static_cast<f16 *>(p)[i] = f16(v);

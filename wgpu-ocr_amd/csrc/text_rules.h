@@ -17,7 +17,7 @@ namespace ocr {
 // there is none: a position outside the table, an entry that names no page of the pool.
 OCR_HD int32_t page_of(const int32_t *row, uint32_t width, uint32_t page, uint32_t pages, int64_t pos) {
     if (pos < 0 || pos >= int64_t(width) * page) return -1;
-    const int32_t p = row[pos / page];
+    const int32_t p = row[uint32_t(pos) / page];  // within 31 bits: width * page is (check_table)
     return p >= 0 && uint32_t(p) < pages ? p : -1;
 }
 

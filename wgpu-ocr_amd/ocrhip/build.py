@@ -16,6 +16,9 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 # Packed FP32 is disabled: this pool has seen wrong results from some v_pk_* f32 forms.
 DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+# Matrix products whose sums stay in ordinary registers: softmax kernels read and rescale them all
+# the time, and each move to and from the accumulation registers is an instruction.
+FILE_FLAGS = {f"text_{n}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"] for n in ("attn", "decode")}
 COMMON = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function"]
 
 
@@ -30,7 +33,7 @@ def sources():
 
 def _compile(src: str) -> str:
     obj = os.path.join(OBJ, os.path.relpath(src, CSRC).replace(os.sep, "_") + ".o")
-    cmd = [HIPCC, *COMMON, *DEVICE_FLAGS, "-c", src, "-o", obj]
+    cmd = [HIPCC, *COMMON, *DEVICE_FLAGS, *FILE_FLAGS.get(os.path.basename(src), []), "-c", src, "-o", obj]
     r = subprocess.run(cmd, capture_output=True, text=True)
     noise = "is not a recognized feature for this target"
     err = "\n".join(l for l in (r.stderr or "").splitlines() if noise not in l)
