@@ -67,7 +67,7 @@ template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 
     constexpr int NS = DP / 32;                     // steps of 32 values of the first product
     constexpr int NB = DP / 16;                     // blocks of 16 values of the second
     constexpr int PITCH = DP * int(sizeof(C)) + 16; // a value vector's bytes in LDS: rows start four banks apart
-    constexpr int CH = 512;                         // positions looked up at a time
+    constexpr int CH = 1024;                        // positions looked up at a time
     constexpr int JOIN = 2 * 16 * (DP + 4) * 4;     // the waves' sums on their way to each other
     constexpr int STAGE = 4 * 32 * PITCH;
     __shared__ __align__(16) char s_mem[STAGE > JOIN ? STAGE : JOIN];
@@ -396,10 +396,11 @@ void launch_decode(Ctx &c, const DecodeArgs &a, hipStream_t s) {
         OCR_HIP(hipGetLastError());
         return;
     }
-    // Parts until there are a few workgroups for every compute unit; a sequence has as many as its
-    // own length gives work to.
+    // Parts until there are two workgroups for every compute unit; a sequence has as many as its own
+    // length gives work to. 4 sequences of 131 072: 512 workgroups 197 us, 768 the same, 1024 212 to
+    // 230; 144 of 700, 576 workgroups: one part 29 us, two 32 and 4 more for the join.
+    constexpr uint64_t kWork = 512;
     const uint64_t heads = uint64_t(a.table.rows) * a.kv.heads * ((a.q_heads / a.kv.heads + 15) / 16);
-    static const uint64_t kWork = getenv("KWORK") ? atoi(getenv("KWORK")) : 768;
     const uint64_t most = uint64_t(a.table.width) * a.kv.page;
     const uint32_t parts = uint32_t(std::max<uint64_t>(1, std::min<uint64_t>({kMostParts, (kWork + heads - 1) / heads, (most + kLeastPart - 1) / kLeastPart})));
     DBuf part;
