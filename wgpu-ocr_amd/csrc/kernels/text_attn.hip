@@ -1,10 +1,18 @@
 // Attention over a packed row of documents: scores capped by a tanh, a bias that falls with the
 // distance, document and prefix masks.
+//
+// One pass over the keys with the running maximum and sum of the softmax. Both products have the
+// keys as rows: S^T = K Q^T, O^T = V^T P^T, so that a lane holds all of its share of a query's
+// scores and hands them to the second product from the registers they are in: of 32 x 32 results, lane
+// l has column l % 32 and rows 8 i + 4 (l / 32) + 0 .. 3, and as the second product's 16 keys a step it
+// gives rows 8 i .. 8 i + 15 in that order, which the value side follows. Values come transposed out
+// of LDS by its transposing reads.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 
 #include "../runtime.h"
+#include "lds_dma.h"
 #include "text_device.h"
 
 namespace ocr {
@@ -18,26 +26,241 @@ template <class T> struct DenseKv {
     __device__ float v(int j, int c) const { return to_f32(vp[j * vs + c]); }
 };
 
-// One wavefront a (token, head), by the formula.
-template <class T> __global__ __launch_bounds__(64) void attention_row_kernel(AttentionArgs a) {
-    __shared__ float s_q[256];
-    const int64_t i = blockIdx.x;
-    const int h = blockIdx.y, dim = a.dim, hk = h / int(a.q_heads / a.kv_heads);
+// Token i, head h by one wavefront, by the formula; s_q: 256 floats of the wavefront's own.
+template <class T> __device__ inline void attention_row(const AttentionArgs &a, int64_t i, int h, float *s_q) {
+    const int dim = a.dim, hk = h / int(a.q_heads / a.kv_heads);
     const T *q = static_cast<const T *>(a.q) + i * a.q_stride + int64_t(h) * dim;
-    for (int c = threadIdx.x; c < dim; c += 64) s_q[c] = to_f32(q[c]) * a.scale;
-    __syncthreads();
+    for (int c = threadIdx.x & 63; c < dim; c += 64) s_q[c] = to_f32(q[c]) * a.scale;
+    __builtin_amdgcn_wave_barrier();
     const KeyRange r = key_range(int(i), int(a.n), a.docs, int(a.ndocs), a.prefix);
     const DenseKv<T> kv{static_cast<const T *>(a.k) + int64_t(hk) * dim, static_cast<const T *>(a.v) + int64_t(hk) * dim, a.k_stride, a.v_stride};
     T *out = static_cast<T *>(a.out) + i * a.out_stride + int64_t(h) * dim;
     attend_row(kv, s_q, dim, r.lo, r.hi, int(i), a.cap, a.slopes ? a.slopes[h] : 0.f, [&](int c, float o) { out[c] = T(o); });
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Vectors that do not lie on 16-byte pieces.
+template <class T> __global__ __launch_bounds__(64) void attention_row_kernel(AttentionArgs a) {
+    __shared__ float s_q[256];
+    attention_row<T>(a, blockIdx.x, blockIdx.y, s_q);
+}
+
+// 128 queries of one head, 32 a wavefront, over tiles of KT keys that come into LDS by DMA while the
+// tile before is worked on. DP: the head's values rounded up to 32; BIAS: scores are capped or get
+// the distance's bias.
+template <class T, int DP, bool BIAS> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_tile_kernel(AttentionArgs a, int tiles) {
+    typedef T tvec __attribute__((ext_vector_type(8)));
+    constexpr int PW = DP <= 64 ? 64 : DP <= 128 ? 128 : 256;  // a vector's values in LDS
+    constexpr int PP = PW / 8;                                 // its 16-byte pieces
+    constexpr int KT = PW == 256 ? 32 : 64, KB = KT / 32;
+    constexpr int KS = DP / 16, NB = DP / 32;
+    constexpr int TILE = KT * PW * 2;
+    constexpr int ND = KT * PP / 256;  // copies a lane for a tile's keys
+    __shared__ __align__(16) char s_kv[2][2][TILE];
+    __shared__ int s_lo[4], s_hi[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+    const HeadTile w = head_tile(blockIdx.x, tiles, a.q_heads, a.kv_heads);
+    if (w.head < 0) return;
+    const int h = w.head, hk = h / int(a.q_heads / a.kv_heads), dim = a.dim;
+    const int i = w.tile * 128 + 32 * wave + (lane & 31);
+    const KeyRange r = key_range(i, int(a.n), a.docs, int(a.ndocs), a.prefix);
+    const bool sees = r.lo < r.hi;
+    // The wavefront's keys: some query sees those in [wlo, whi), all do those in [flo, fhi).
+    const int wlo = wave_min_i(sees ? r.lo : 0x7fffffff), whi = wave_max_i(sees ? r.hi : 0);
+    const int flo = wave_max_i(sees ? r.lo : 0), fhi = wave_min_i(sees ? r.hi : 0x7fffffff);
+    if (lane == 0) s_lo[wave] = wlo, s_hi[wave] = whi;
+
+    const int pieces = dim / 8;
+    tvec qf[KS];
+    {
+        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0;
+        const char *q = static_cast<const char *>(a.q) + (int64_t(min(i, int(a.n) - 1)) * a.q_stride + int64_t(h) * dim) * 2;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            u32x4 x{0, 0, 0, 0};
+            if (2 * s + half < pieces) x = *reinterpret_cast<const u32x4 *>(q + 16 * (2 * s + half));
+            qf[s] = __builtin_bit_cast(tvec, x ^ flip);
+        }
+    }
+    if (pieces < PP) {  // pieces that no copy writes count nothing
+        for (int x = tid; x < 4 * KT * PP; x += 256) *reinterpret_cast<u32x4 *>(&s_kv[0][0][0] + 16 * x) = u32x4{0, 0, 0, 0};
+    }
+    __syncthreads();
+    const int jlo = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3])), jhi = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
+
+    // Copies: a lane's pieces of a tile lie in LDS in order, each row's exchanged so that the reads
+    // below touch every bank (swap_of), by the choice of the piece that the lane copies.
+    auto swap_of = [](int row) { return PP == 8 ? (row >> 1 & 1) << 2 | (row >> 2 & 3) : (row & 3) << 2 | (row >> 2 & 3); };
+    const char *kbase = static_cast<const char *>(a.k) + int64_t(hk) * dim * 2, *vbase = static_cast<const char *>(a.v) + int64_t(hk) * dim * 2;
+    const unsigned lds0 = lds_addr(&s_kv[0][0][0]) + wave * 1024;
+    auto copy = [&](int j0, int buf) {
+        const bool whole = j0 + KT <= jhi;
+        const char *kb = kbase + int64_t(j0) * a.k_stride * 2, *vb = vbase + int64_t(j0) * a.v_stride * 2;
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+            const int at = (4 * d + wave) * 64 + lane, row = at / PP, piece = at % PP ^ swap_of(row);
+            const int from = whole ? row : min(row, jhi - 1 - j0);
+            if (piece < pieces) {
+                dma16s_to(kb, unsigned(from) * unsigned(a.k_stride * 2) + 16 * piece, lds0 + (2 * buf + 0) * TILE + d * 4096);
+                dma16s_to(vb, unsigned(from) * unsigned(a.v_stride * 2) + 16 * piece, lds0 + (2 * buf + 1) * TILE + d * 4096);
+            }
+        }
+    };
+    int koff[KS], voff[NB][2];
+#pragma unroll
+    for (int s = 0; s < KS; s++) koff[s] = (lane & 31) * PW * 2 + ((2 * s + half) ^ swap_of(lane & 15)) * 16;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int row = 4 * half + ((lane & 15) >> 2) + 8 * e;
+            voff[b][e] = row * PW * 2 + ((4 * b + 2 * (lane >> 4 & 1) + (lane >> 1 & 1)) ^ swap_of(row)) * 16 + 8 * (lane & 1);
+        }
+
+    f32x16 o[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[b][e] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    const float c = fabsf(a.scale) * 1.4426950408889634f;
+    const float slope = BIAS && a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.f;
+
+    if (jlo < jhi) copy(jlo, 0);
+    int buf = 0;
+    for (int j0 = jlo; j0 < jhi; j0 += KT, buf ^= 1) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        lds_barrier();  // the tile is there, and all have left the other buffer
+        if (j0 + KT < jhi) copy(j0 + KT, buf ^ 1);
+        if (j0 >= whi || j0 + KT <= wlo) continue;
+        const char *const sk = s_kv[buf][0], *const sv = s_kv[buf][1];
+        f32x16 s[KB];
+#pragma unroll
+        for (int t = 0; t < KB; t++) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[t][e] = 0.f;
+#pragma unroll
+            for (int st = 0; st < KS; st++)
+                s[t] = mfma32(*reinterpret_cast<const tvec *>(sk + koff[st] + t * 32 * PW * 2), qf[st], s[t]);
+        }
+        const bool whole = j0 >= flo && j0 + KT <= fhi;
+        float top = -INFINITY;
+        if (BIAS || !whole) {
+#pragma unroll
+            for (int t = 0; t < KB; t++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[t][e] *= c;
+            if (BIAS && a.cap > 0.f) {
+#pragma unroll
+                for (int t = 0; t < KB; t++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) s[t][e] = cap_log2(s[t][e], a.cap);
+            }
+            if (BIAS && a.slopes) {
+                const float d = float(i - j0 - 4 * half);
+#pragma unroll
+                for (int t = 0; t < KB; t++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) s[t][e] -= slope * fabsf(d - float(32 * t + 8 * (e / 4) + e % 4));
+            }
+            if (!whole) {
+                const unsigned first = unsigned(j0 + 4 * half - r.lo), count = unsigned(r.hi - r.lo);
+#pragma unroll
+                for (int t = 0; t < KB; t++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        if (first + unsigned(32 * t + 8 * (e / 4) + e % 4) >= count) s[t][e] = -INFINITY;
+            }
+#pragma unroll
+            for (int t = 0; t < KB; t++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) top = fmaxf(top, s[t][e]);
+        } else {
+#pragma unroll
+            for (int t = 0; t < KB; t++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) top = fmaxf(top, s[t][e]);
+            top *= c;
+        }
+        if (__any(top > m + kSlack)) {
+            const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32))), f = mn == -INFINITY ? 1.f : exp2_f32(m - mn);
+            l *= f;
+#pragma unroll
+            for (int b = 0; b < NB; b++) o[b] *= f;
+            m = mn;
+        }
+        const float ref = m == -INFINITY ? 0.f : m - kLift, mul = BIAS || !whole ? 1.f : c;
+        tvec p[KB][2];
+#pragma unroll
+        for (int t = 0; t < KB; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const float x = exp2_f32(__fmaf_rn(s[t][e], mul, -ref));
+                l += x;
+                p[t][e / 8][e % 8] = T(x);
+            }
+#pragma unroll
+        for (int t = 0; t < KB; t++)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    const u32x2 x = lds_read_tr16(sv + voff[b][0] + (32 * t + 16 * u) * PW * 2);
+                    const u32x2 y = lds_read_tr16(sv + voff[b][1] + (32 * t + 16 * u) * PW * 2);
+                    o[b] = mfma32(__builtin_bit_cast(tvec, u32x4{x[0], x[1], y[0], y[1]}), p[t][u], o[b]);
+                }
+    }
+    l += __shfl_xor(l, 32);
+    // A value that is not finite spoils the sums of every query of its tile, also where the mask
+    // gives it no weight: those queries again, by the formula.
+    float bad = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) bad += o[b][e] * 0.f;
+    const unsigned long long spoilt = __ballot(sees && !(bad == 0.f));
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (i < int(a.n) && !((spoilt >> (lane & 31) | spoilt >> ((lane & 31) + 32)) & 1)) {
+        T *out = static_cast<T *>(a.out) + int64_t(i) * a.out_stride + int64_t(h) * dim;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int col = 32 * b + 2 * e + 4 * half;
+                typedef T t4 __attribute__((ext_vector_type(4)));
+                if (col < dim)
+                    *reinterpret_cast<t4 *>(out + col) = sees ? t4{T(o[b][e] * inv), T(o[b][e + 1] * inv), T(o[b][e + 2] * inv), T(o[b][e + 3] * inv)}
+                                                              : t4{T(0.f), T(0.f), T(0.f), T(0.f)};
+            }
+    }
+    __syncthreads();
+    for (unsigned todo = unsigned(spoilt | spoilt >> 32); todo; todo &= todo - 1)
+        attention_row<T>(a, w.tile * 128 + 32 * wave + __builtin_ctz(todo), h, reinterpret_cast<float *>(&s_kv[0][0][0]) + 256 * wave);
+}
+
+template <class T, bool BIAS> void launch_tiles(const AttentionArgs &a, hipStream_t s) {
+    const int tiles = int((a.n + 127) / 128);
+    const dim3 grid(unsigned(head_blocks(tiles, a.q_heads, a.kv_heads)));
+    if (a.dim <= 32) hipLaunchKernelGGL((attention_tile_kernel<T, 32, BIAS>), grid, dim3(256), 0, s, a, tiles);
+    else if (a.dim <= 64) hipLaunchKernelGGL((attention_tile_kernel<T, 64, BIAS>), grid, dim3(256), 0, s, a, tiles);
+    else if (a.dim <= 96) hipLaunchKernelGGL((attention_tile_kernel<T, 96, BIAS>), grid, dim3(256), 0, s, a, tiles);
+    else if (a.dim <= 128) hipLaunchKernelGGL((attention_tile_kernel<T, 128, BIAS>), grid, dim3(256), 0, s, a, tiles);
+    else hipLaunchKernelGGL((attention_tile_kernel<T, 256, BIAS>), grid, dim3(256), 0, s, a, tiles);
 }
 
 }  // namespace
 
 void launch_attention(const AttentionArgs &a, hipStream_t s) {
     ProbeScope probe("text_attention", s, 2.0 * a.n * a.n * a.q_heads * a.dim, 4.0 * a.n * (a.q_heads + a.kv_heads) * a.dim);
+    // Whole 16-byte pieces, and rows of a tile within 32 bits of each other.
+    bool pieces = a.dim % 8 == 0 && head_blocks((a.n + 127) / 128, a.q_heads, a.kv_heads) < 1 << 24;
+    for (const void *p : {a.q, a.k, a.v, static_cast<const void *>(a.out)}) pieces = pieces && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+    for (int64_t st : {a.q_stride, a.k_stride, a.v_stride, a.out_stride}) pieces = pieces && st % 8 == 0 && st < 1 << 24;
     with_type16(a.type, [&](auto t) {
-        hipLaunchKernelGGL((attention_row_kernel<decltype(t)>), dim3(a.n, a.q_heads), dim3(64), 0, s, a);
+        using T = decltype(t);
+        if (!pieces) hipLaunchKernelGGL((attention_row_kernel<T>), dim3(a.n, a.q_heads), dim3(64), 0, s, a);
+        else if (a.cap > 0.f || a.slopes) launch_tiles<T, true>(a, s);
+        else launch_tiles<T, false>(a, s);
     });
     OCR_HIP(hipGetLastError());
 }

@@ -49,11 +49,6 @@ template <class T, class C> __global__ __launch_bounds__(64) void decode_row_ker
     attend_row(kv, s_q, dim, 0, len, len - 1, a.cap, a.slopes ? a.slopes[h] : 0.f, [&](int c, float o) { out[c] = T(o); });
 }
 
-// Weights are held as 2^6 times their value relative to the maximum's reference, which may lie up to
-// 2^8 under the true maximum: at most 2^14, within float16, and 2^-24 (its last step) is 2^-30 of
-// the reference. The factor is common to the sums and leaves with them.
-constexpr float kLift = 6.f, kSlack = 8.f;
-
 // Parts of a sequence joined: part [row][head][parts] holds dim normalised values, then log2 of the
 // sum of weights.
 constexpr int kPartTail = 4;  // keeps the rows' 16-byte alignment

@@ -68,6 +68,11 @@ __device__ inline void store16(void *p, int type, int64_t i, float v) {
 __device__ inline f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ inline f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
+// D[32][32] += A[32][16] B[16][32]: lane l holds A's row and B's column l % 32, values 8 (l / 32) on of
+// the 16; of D, column l % 32 and rows 8 i + 4 (l / 32) + 0 .. 3 in element 4 i on.
+__device__ inline f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ inline f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+
 // Transposing reads of LDS. 16 lanes name 4 rows of 16 values of 16 bits (lanes 4 r to 4 r + 3 the
 // four quarters of row r), or 8 rows of 16 bytes (lanes 2 r, 2 r + 1 the halves); each gets its column.
 __device__ inline u32x2 lds_read_tr16(const char *p) {
@@ -99,6 +104,11 @@ template <class C> __device__ inline f16x8 widen8(uint32_t a, uint32_t b) {
     return f16x8{x[0][0], x[0][1], x[1][0], x[1][1], x[2][0], x[2][1], x[3][0], x[3][1]};
 }
 
+// Weights are held as 2^6 times their value relative to the maximum's reference, which may lie up to
+// 2^8 under the true maximum: at most 2^14, within float16, and 2^-24 (its last step) is 2^-30 of
+// the reference. The factor is common to the sums and leaves with them.
+constexpr float kLift = 6.f, kSlack = 8.f;
+
 // 2^x; results under the normal range are zero.
 __device__ inline float exp2_f32(float x) { return __builtin_amdgcn_exp2f(x); }
 // A score in units of log2 through the cap: cap tanh(s / cap), tanh(y) = 1 - 2 / (e^2y + 1).
@@ -125,6 +135,12 @@ __device__ inline float wave_sum(float v) {
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
+
+__device__ inline int wave_max_i(int v) {
+    for (int o = 32; o; o >>= 1) v = max(v, __shfl_xor(v, o));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ inline int wave_min_i(int v) { return -1 - wave_max_i(-1 - v); }
 
 // A scaled score through the cap and the distance bias.
 __device__ inline float score_of(float s, float cap, float slope, int distance) {

@@ -97,4 +97,34 @@ OCR_HD Parts parts_of(int len, uint32_t parts) {
     return parts == 1 ? Parts{1, len} : Parts{int((uint32_t(len) + uint32_t(each) - 1) / uint32_t(each)), each};
 }
 
+// Which tile of queries and which head workgroup x of a prompt's attention takes. Workgroups go to
+// the eight compute dies in turn, each with a level-two cache of its own, so a die gets the query
+// heads of as few key heads as there are; later tiles, which see more of their document, come first.
+// Workgroups past the last have head -1.
+struct HeadTile {
+    int tile, head;
+};
+OCR_HD int64_t head_blocks(int64_t tiles, uint32_t q_heads, uint32_t kv_heads) {
+    const int64_t group = q_heads / kv_heads;
+    if (kv_heads < 8 && 8 % kv_heads == 0) {
+        const int64_t sharing = 8 / kv_heads;
+        return 8 * ((group * tiles + sharing - 1) / sharing);
+    }
+    return tiles * q_heads;
+}
+OCR_HD HeadTile head_tile(uint32_t x, int tiles, uint32_t q_heads, uint32_t kv_heads) {
+    const uint32_t group = q_heads / kv_heads, die = x % 8;
+    uint32_t hk, at;  // the key head, the place among its group * tiles pieces
+    if (kv_heads < 8 && 8 % kv_heads == 0) {
+        hk = die % kv_heads, at = x / 8 * (8 / kv_heads) + die / kv_heads;
+        if (at >= group * uint32_t(tiles)) return {0, -1};
+    } else if (kv_heads % 8 == 0) {
+        at = x / 8 % (group * uint32_t(tiles));
+        hk = x / 8 / (group * uint32_t(tiles)) * 8 + die;
+    } else {
+        hk = x % kv_heads, at = x / kv_heads;
+    }
+    return {tiles - 1 - int(at / group), int(hk * group + at % group)};
+}
+
 }  // namespace ocr
