@@ -543,8 +543,8 @@ int ocr_decode_attention_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const o
  * group scores scores[w] + log-softmax(logits of w)[t]; a beam whose finished flag is set keeps its
  * score with token eos and has no other. The best `beams` (at most 32) of each group in order, ties
  * to the lower w * vocab + t: out_scores, parents (w), tokens (t), out_finished (finished, or t ==
- * eos; may be NULL), each [groups][beams]. NaN logits weigh nothing, scores that are not numbers
- * count as minus infinity. finished may be NULL, eos negative (none) then. out_scores and
+ * eos; may be NULL), each [groups][beams]. NaN logits weigh nothing, scores that are not
+ * finite count as minus infinity. finished may be NULL, eos negative (none) then. out_scores and
  * out_finished may be scores and finished. */
 typedef struct ocr_beam_args {
     const void *logits;

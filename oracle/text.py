@@ -100,7 +100,7 @@ def beam_select(logits, scores, finished, eos):
         s = np.where(finished[..., None] != 0, np.where(np.arange(vocab) == eos, 0.0, -np.inf), s)
     with np.errstate(invalid="ignore"):
         s = s + scores.astype(np.float64)[..., None]
-    s = np.where(np.isnan(s), -np.inf, s).reshape(groups, -1)
+    s = np.where(np.isfinite(s), s, -np.inf).reshape(groups, -1)
     at = np.argsort(-s, axis=1, kind="stable")[:, :beams]
     parents, tokens = at // vocab, at % vocab
     fin = np.zeros_like(parents) if finished is None else np.take_along_axis(finished, parents, 1)

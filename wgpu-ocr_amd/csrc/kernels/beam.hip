@@ -1,4 +1,12 @@
 // A step of beam search: log-softmax of every beam's logits, the best of all beams' continuations.
+//
+// The logits are read once: a wavefront takes a block of a row, keeps it in registers, and writes
+// the block's maximum and the sum of its exponentials. What can be among a row's best `beams` lies in
+// the blocks whose maximum is at least the beams-th largest of the maxima, so the second kernel, one
+// workgroup a group and a wavefront a beam, reads only those again. Values order as 32-bit keys
+// (order_of); the beams-th largest of a set of keys is found bit by bit with ballots.
+//
+// Within a beam continuations order by their logits, between beams by float64 scores.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -11,119 +19,319 @@ namespace ocr {
 
 namespace {
 
-// A continuation: larger score first, then the lower index.
-struct Cand {
-    double score;
-    int at;
+constexpr int kChunk = 2048;       // logits that a wavefront holds: four times eight a lane
+constexpr int kMostBlocks = 512;   // blocks of a row: a lane of the second kernel holds eight
+constexpr int kOneLaunch = 2048;   // rows up to here need no first kernel
+constexpr int kList = 256;         // continuations that a wavefront sorts
+
+// Keys that order as the values do; NaN as minus infinity, the zeros alike.
+__device__ inline uint32_t order_of(float x) {
+    const uint32_t u = __float_as_uint(x == x ? x + 0.f : -INFINITY);
+    return u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
+}
+__device__ inline float value_of(uint32_t key) { return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu)); }
+
+// Eight logits of a row from index i on, those past the last minus infinity. aligned: rows and i lie
+// on 16 bytes (uniform).
+template <class T> __device__ inline void load8(const T *row, int i, int vocab, bool aligned, float *x) {
+    if (aligned && i + 8 <= vocab) {
+        constexpr int N = 16 / sizeof(T);
+        u32x4 raw[8 / N];
+#pragma unroll
+        for (int k = 0; k < 8 / N; k++) raw[k] = *reinterpret_cast<const u32x4 *>(row + i + k * N);
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            if constexpr (sizeof(T) == 4) x[k] = __uint_as_float(raw[k / 4][k % 4]);
+            else x[k] = widen16(raw[0][k / 2] >> (16 * (k % 2)), std::is_same_v<T, f16> ? T_F16 : T_BF16);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] = i + k < vocab ? to_f32(row[i + k]) : -INFINITY;
+    }
+}
+
+__device__ inline unsigned long long uniform(unsigned long long x) {
+    return uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(x >> 32)))) << 32 | uint32_t(__builtin_amdgcn_readfirstlane(int(x)));
+}
+
+// Whether a beam's continuations have scores of their own: not if it is finished, or no score.
+__device__ inline bool is_open(const BeamArgs &a, int64_t row) {
+    return !(a.finished && a.finished[row]) && fabsf(a.scores[row]) < INFINITY;
+}
+
+struct Block {
+    float top, sum;  // the largest logit (never NaN), the sum of e^(x - top)
 };
-__device__ inline bool before(const Cand &a, const Cand &b) { return a.score > b.score || (a.score == b.score && a.at < b.at); }
-__device__ inline Cand wave_best(Cand c) {
-    for (int o = 32; o; o >>= 1) {
-        const Cand d{__shfl_xor(c.score, o), __shfl_xor(c.at, o)};
-        if (before(d, c)) c = d;
+// [i0, i1) of a row by one wavefront. Sums in float32: 32 terms a lane, then six steps.
+template <class T> __device__ inline Block block_of(const T *row, int i0, int i1, int vocab, bool aligned) {
+    const int lane = threadIdx.x & 63;
+    float top = -INFINITY, sum = 0.f;
+    for (int c = i0; c < i1; c += kChunk) {
+        float x[4][8], t = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 4; u++) load8(row, c + 512 * u + 8 * lane, vocab, aligned, x[u]);
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) t = fmaxf(t, x[u][k]);
+        t = wave_max(t);
+        if (t > top) {
+            sum *= exp2_f32((top - t) * 1.4426950408889634f);
+            top = t;
+        }
+        if (top == -INFINITY) continue;
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float e = exp2_f32((x[u][k] - top) * 1.4426950408889634f);
+                sum += x[u][k] == x[u][k] ? e : 0.f;
+            }
     }
-    return c;
+    return {top, wave_sum(sum)};
 }
 
-// One workgroup a beam: its best `beams` continuations in order.
-template <class T> __global__ __launch_bounds__(256) void beam_rows_kernel(BeamArgs a, Cand *cand) {
-    __shared__ double s_d[4];
-    __shared__ float s_m[4];
-    __shared__ Cand s_c[4];
+// A wavefront a block of a row. 512 rows of 128 000 bfloat16 values.
+template <class T> __global__ __launch_bounds__(256) void beam_blocks_kernel(BeamArgs a, int blocks, int size, bool aligned, Block *out) {
     const int64_t row = blockIdx.x;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, v = a.vocab;
-    const T *x = static_cast<const T *>(a.logits) + row * a.stride;
-    const double cum = a.scores[row];
-    const bool over = a.finished && a.finished[row];
-    auto logit = [&](int t) {  // NaN weighs nothing
-        const float f = to_f32(x[t]);
-        return f == f ? f : -INFINITY;
-    };
-    float m = -INFINITY;
-    for (int t = threadIdx.x; t < v; t += 256) m = fmaxf(m, logit(t));
-    m = wave_max(m);
-    if (lane == 0) s_m[wave] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-    double sum = 0;
-    for (int t = threadIdx.x; t < v; t += 256) sum += exp(double(logit(t)) - double(m));
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-    if (lane == 0) s_d[wave] = sum;
-    __syncthreads();
-    const double lse = double(m) + log(s_d[0] + s_d[1] + s_d[2] + s_d[3]);
-    auto score = [&](int t) {
-        const double s = over ? (t == a.eos ? cum : -INFINITY) : cum + (double(logit(t)) - lse);
-        return s == s ? s : -INFINITY;
-    };
-    Cand last{INFINITY, -1};
-    for (int k = 0; k < int(a.beams); k++) {
-        Cand best{-INFINITY, 0x7fffffff};
-        for (int t = threadIdx.x; t < v; t += 256) {
-            const Cand c{score(t), t};
-            if (before(last, c) && before(c, best)) best = c;
-        }
-        best = wave_best(best);
-        __syncthreads();
-        if (lane == 0) s_c[wave] = best;
-        __syncthreads();
-        for (int o = 0; o < 4; o++)
-            if (before(s_c[o], best)) best = s_c[o];
-        if (threadIdx.x == 0) cand[row * a.beams + k] = best;
-        last = best;
-    }
+    const int b = blockIdx.y * 4 + (threadIdx.x >> 6), v = a.vocab;
+    if (b >= blocks || !is_open(a, row)) return;
+    const Block s = block_of(static_cast<const T *>(a.logits) + row * a.stride, b * size, min(v, (b + 1) * size), v, aligned);
+    if ((threadIdx.x & 63) == 0) out[row * blocks + b] = s;
 }
 
-// One wavefront a group.
-__global__ __launch_bounds__(64) void beam_groups_kernel(BeamArgs a, const Cand *cand) {
-    const int g = blockIdx.x, w = a.beams, n = w * w, lane = threadIdx.x;
-    struct Pick {
-        Cand c;
-        int beam;
-    };
-    int fin[2] = {0, 0};
-    Cand last{INFINITY, -1};
-    int last_beam = -1;
-    for (int k = 0; k < w; k++) {
-        Cand best{-INFINITY, 0x7fffffff};
-        int beam = w;
-        auto better = [](const Cand &c, int cb, const Cand &d, int db) {
-            return c.score > d.score || (c.score == d.score && (cb < db || (cb == db && c.at < d.at)));
-        };
-        for (int i = lane; i < n; i += 64) {
-            const Cand c = cand[int64_t(g) * n + i];
-            if (c.at == 0x7fffffff) continue;
-            if (better(last, last_beam, c, i / w) && better(c, i / w, best, beam)) best = c, beam = i / w;
-        }
-        for (int o = 32; o; o >>= 1) {
-            const Cand d{__shfl_xor(best.score, o), __shfl_xor(best.at, o)};
-            const int db = __shfl_xor(beam, o);
-            if (better(d, db, best, beam)) best = d, beam = db;
-        }
-        if (lane == k) fin[0] = (a.finished && a.finished[g * w + beam]) || (a.eos >= 0 && best.at == a.eos);
-        if (lane == 0) {
-            a.parents[g * w + k] = beam;
-            a.tokens[g * w + k] = best.at;
-        }
-        if (lane == k) fin[1] = __float_as_int(float(best.score));
-        last = best, last_beam = beam;
+// The n-th largest of all lanes' keys (0 where there are fewer): count(t) says how many keys of the
+// lane are t or more.
+template <class Count> __device__ inline uint32_t nth_largest(int n, Count &&count) {
+    uint32_t t = 0;
+    for (int bit = 31; bit >= 0; bit--) {
+        const uint32_t next = t | 1u << bit;
+        if (count(next) >= n) t = next;
     }
-    if (lane < w) {  // every score and flag of the group has been read: the outputs may be the inputs
-        a.out_scores[g * w + lane] = __int_as_float(fin[1]);
-        if (a.out_finished) a.out_finished[g * w + lane] = fin[0];
+    return t;
+}
+
+// A row's best `want` keys in order into top (the wavefront's own LDS, as list): a logit's key, then the index, lower
+// ones larger. sel: one bit a block to look at, most: the threshold known so far.
+template <class T>
+__device__ inline void row_best(const T *row, int vocab, bool aligned, int size, const unsigned long long *sel, int words, uint32_t floor,
+                                int want, uint64_t *list, uint64_t *top) {
+    const int lane = threadIdx.x & 63;
+    // f(first index, the lane's eight keys) over the blocks in order.
+    auto each = [&](auto &&f) {
+        for (int w = 0; w < words; w++)
+            for (unsigned long long bits = uniform(sel[w]); bits; bits &= bits - 1) {
+                const int b = 64 * w + __builtin_ctzll(bits);
+                const int i1 = min(vocab, (b + 1) * size);
+                for (int c = b * size; c < i1; c += 512) {
+                    float x[8];
+                    load8(row, c + 8 * lane, vocab, aligned, x);
+                    f(c + 8 * lane, x);
+                }
+            }
+    };
+    uint32_t best = 0;
+    each([&](int i, const float *x) {
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (i + k < vocab) best = max(best, order_of(x[k]));
+    });
+    uint32_t t = max(floor, nth_largest(want, [&](uint32_t key) { return __popcll(__ballot(best >= key)); }));
+    int greater, n;
+    for (int round = 0;; round++) {
+        greater = 0, n = 0;
+        int equal = 0;
+        each([&](int i, const float *x) {
+            int ne = 0;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const uint32_t key = order_of(x[k]);
+                const bool in = i + k < vocab;
+                ne += in && key == t;
+                const unsigned long long g = __ballot(in && key > t);
+                if (g) {
+                    const int at = greater + __popcll(g & ((1ull << lane) - 1));
+                    if (in && key > t && at < kList - int(kMostBeams)) list[at] = uint64_t(key) << 32 | uint32_t(~(i + k));
+                    greater += __popcll(g);
+                }
+            }
+            // Of the keys that equal the threshold the lowest `want` indices.
+            if (equal < want && __ballot(ne)) {
+                int before = ne;
+                for (int o = 1; o < 64; o <<= 1) {
+                    const int d = __shfl_up(before, o);
+                    if (lane >= o) before += d;
+                }
+                const int all = __shfl(before, 63);
+                before -= ne;
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (i + k < vocab && order_of(x[k]) == t) {
+                        if (equal + before < want) list[kList - 1 - (equal + before)] = uint64_t(t) << 32 | uint32_t(~(i + k));
+                        before++;
+                    }
+                equal += all;
+            }
+        });
+        n = min(equal, want);
+        if (greater <= kList - int(kMostBeams) || round) break;
+        // More than fit: the exact threshold, which fewer than `want` exceed.
+        t = nth_largest(want, [&](uint32_t key) {
+            int c = 0;
+            each([&](int i, const float *x) {
+                for (int k = 0; k < 8; k++) c += i + k < vocab && order_of(x[k]) >= key;
+            });
+            for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o);
+            return c;
+        });
+    }
+    __builtin_amdgcn_wave_barrier();
+    // Their places by counting.
+    const int total = greater + n;
+    for (int i = lane; i < total; i += 64) {
+        const uint64_t key = list[i < greater ? i : kList - 1 - (i - greater)];
+        int place = 0;
+        for (int j = 0; j < total; j++) place += list[j < greater ? j : kList - 1 - (j - greater)] > key;
+        if (place < want) top[place] = key;
+    }
+    for (int i = total + lane; i < want; i += 64) top[i] = 0;  // fewer tokens than beams
+}
+
+template <class T> __global__ __launch_bounds__(512) void beam_groups_kernel(BeamArgs a, int blocks, int size, bool aligned, const Block *stats) {
+    __shared__ uint64_t s_list[8][kList], s_top[kMostBeams * kMostBeams];
+    __shared__ double s_score[kMostBeams * kMostBeams];
+    __shared__ unsigned long long s_sel[8][kMostBlocks / 64];
+    const int64_t g = blockIdx.x;
+    const int w = a.beams, v = a.vocab, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, want = min(w, v);
+    for (int beam = wave; beam < w; beam += waves) {
+        const int64_t r = g * w + beam;
+        const T *row = static_cast<const T *>(a.logits) + r * a.stride;
+        uint64_t *const top = s_top + beam * w;
+        const double cum = a.scores[r];
+        const bool over = a.finished && a.finished[r];
+        double m = -INFINITY, sum = 0;
+        float bt[kMostBlocks / 64], bs[kMostBlocks / 64];
+        bool open = is_open(a, r);
+        if (open) {
+            if (!stats) {
+                const Block s = block_of(row, 0, v, v, aligned);
+                m = s.top, sum = s.sum;
+            } else {
+                float t = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < kMostBlocks / 64; k++) {
+                    const bool in = 64 * k + lane < blocks;
+                    const Block s = in ? stats[r * blocks + 64 * k + lane] : Block{-INFINITY, 0.f};
+                    bt[k] = s.top, bs[k] = s.sum;
+                    t = fmaxf(t, s.top);
+                }
+                m = wave_max(t);
+#pragma unroll
+                for (int k = 0; k < kMostBlocks / 64; k++)
+                    if (64 * k < blocks && bt[k] > -INFINITY) sum += double(bs[k]) * exp(double(bt[k]) - m);
+                for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+            }
+            open = m > -INFINITY && m < INFINITY;
+        }
+        const double lse = open ? m + log(sum) : 0.0;
+        if (open) {
+            uint32_t t = 0;
+            int words = 1;
+            if (!stats) {
+                if (lane == 0) s_sel[wave][0] = 1;
+            } else {
+                uint32_t key[kMostBlocks / 64];
+                words = (blocks + 63) / 64;
+#pragma unroll
+                for (int k = 0; k < kMostBlocks / 64; k++) key[k] = 64 * k + lane < blocks ? order_of(bt[k]) : 0;
+                t = nth_largest(want, [&](uint32_t x) {
+                    int c = 0;
+#pragma unroll
+                    for (int k = 0; k < kMostBlocks / 64; k++)
+                        if (k < words) c += __popcll(__ballot(key[k] >= x));
+                    return c;
+                });
+#pragma unroll
+                for (int k = 0; k < kMostBlocks / 64; k++) {
+                    const unsigned long long in = __ballot(key[k] >= t && 64 * k + lane < blocks);
+                    if (lane == 0) s_sel[wave][k] = in;
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+            row_best(row, v, aligned, stats ? size : v, s_sel[wave], words, t, want, s_list[wave], top);
+            for (int i = want + lane; i < w; i += 64) top[i] = 0;
+        } else {
+            // A finished beam's only continuation is its end; what scores nothing comes in order.
+            const bool kept = over && fabs(cum) < INFINITY;
+            for (int i = lane; i < w; i += 64) {
+                const int at = !kept ? i : i == 0 ? a.eos : i - 1 + (i - 1 >= a.eos);
+                top[i] = at >= 0 && at < v ? uint64_t(kept && i == 0) << 32 | uint32_t(~at) : 0;
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+        for (int i = lane; i < w; i += 64) {
+            double s = -INFINITY;
+            if (open) {
+                const float x = value_of(uint32_t(top[i] >> 32));
+                if (top[i] && x > -INFINITY) s = cum + (double(x) - lse);
+            } else if (top[i] >> 32) {
+                s = cum;
+            }
+            s_score[beam * w + i] = s == s ? s : -INFINITY;
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    // The group's best by counting those before each: beams' lists are in order, ties go to the lower
+    // beam, then the lower token. All of the group's inputs have been read.
+    for (int c = threadIdx.x; c < w * w; c += blockDim.x) {
+        const int beam = c / w, at = int(~uint32_t(s_top[c]));
+        if (!s_top[c]) continue;
+        const double s = s_score[c];
+        int place = 0;
+        for (int o = 0; o < w * w; o++) {
+            if (!s_top[o] || o == c) continue;
+            const double d = s_score[o];
+            const int ob = o / w;
+            place += d > s || (d == s && (ob < beam || (ob == beam && int(~uint32_t(s_top[o])) < at)));
+        }
+        if (place >= w) continue;
+        const int64_t out = g * w + place;
+        const bool over = a.finished && a.finished[g * w + beam];
+        s_list[0][place] = uint64_t(uint32_t(beam)) << 32 | uint32_t(c) << 1 | uint32_t(over || (a.eos >= 0 && at == a.eos));
+        a.parents[out] = beam;
+        a.tokens[out] = at;
+    }
+    __syncthreads();
+    for (int k = threadIdx.x; k < w; k += blockDim.x) {
+        const uint32_t x = uint32_t(s_list[0][k]);
+        a.out_scores[g * w + k] = float(s_score[x >> 1]);
+        if (a.out_finished) a.out_finished[g * w + k] = x & 1;
     }
 }
 
 }  // namespace
 
 void launch_beam(Ctx &c, const BeamArgs &a, hipStream_t s) {
-    const int rows = int(a.groups * a.beams);
-    ProbeScope probe("beam_select", s, 3.0 * rows * a.vocab, double(rows) * a.vocab * type_bytes(a.type));
-    DBuf cand(&c, size_t(rows) * a.beams * sizeof(Cand), s);
+    const int64_t rows = int64_t(a.groups) * a.beams;
+    const size_t bytes = type_bytes(a.type);
+    ProbeScope probe("beam_select", s, 3.0 * rows * a.vocab, double(rows) * a.vocab * bytes);
+    const bool aligned = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.stride * bytes % 16 == 0;
+    // Blocks of whole chunks, few enough for the second kernel's registers.
+    const int chunks = int((a.vocab + kChunk - 1) / kChunk), size = (chunks + kMostBlocks - 1) / kMostBlocks * kChunk;
+    const int blocks = int((a.vocab + size - 1) / size);
+    const bool two = a.vocab > kOneLaunch;
+    DBuf stats;
+    if (two) stats = DBuf(&c, size_t(rows) * blocks * sizeof(Block), s);
     with_type(a.type, [&](auto t) {
-        hipLaunchKernelGGL((beam_rows_kernel<decltype(t)>), dim3(rows), dim3(256), 0, s, a, cand.as<Cand>());
+        using T = decltype(t);
+        if (two) {
+            hipLaunchKernelGGL((beam_blocks_kernel<T>), dim3(unsigned(rows), (blocks + 3) / 4), dim3(256), 0, s, a, blocks, size, aligned, stats.as<Block>());
+            OCR_HIP(hipGetLastError());
+        }
+        hipLaunchKernelGGL((beam_groups_kernel<T>), dim3(a.groups), dim3(64 * std::min(a.beams, 8u)), 0, s, a, blocks, size, aligned,
+                           static_cast<const Block *>(stats.as<Block>()));
     });
-    OCR_HIP(hipGetLastError());
-    hipLaunchKernelGGL(beam_groups_kernel, dim3(a.groups), dim3(64), 0, s, a, cand.as<Cand>());
     OCR_HIP(hipGetLastError());
 }
 
