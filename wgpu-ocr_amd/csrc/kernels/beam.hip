@@ -1,9 +1,9 @@
 // A step of beam search: log-softmax of every beam's logits, the best of all beams' continuations.
 //
 // The logits are read once: a wavefront takes a block of a row, keeps it in registers, and writes
-// the block's maximum and the sum of its exponentials. What can be among a row's best `beams` lies in
-// the blocks whose maximum is at least the beams-th largest of the maxima, so the second kernel, one
-// workgroup a group and a wavefront a beam, reads only those again. Values order as 32-bit keys
+// the maxima of the block's four parts and the sum of its exponentials. What can be among a row's
+// best `beams` lies in the parts whose maximum is at least the beams-th largest of the maxima, so the
+// second kernel, one workgroup a group and a wavefront a beam, reads only those again. Values order as 32-bit keys
 // (order_of); the beams-th largest of a set of keys is found bit by bit with ballots.
 //
 // Within a beam continuations order by their logits, between beams by float64 scores.
@@ -20,8 +20,10 @@ namespace ocr {
 namespace {
 
 constexpr int kChunk = 2048;       // logits that a wavefront holds: four times eight a lane
-constexpr int kMostBlocks = 512;   // blocks of a row: a lane of the second kernel holds eight
-constexpr int kOneLaunch = 2048;   // rows up to here need no first kernel
+constexpr int kPart = 512;         // a part of a chunk: eight a lane
+constexpr int kMostBlocks = 128;   // blocks of a row
+constexpr int kHeld = kMostBlocks * 4 / 64;  // parts' maxima that a lane of the second kernel holds
+constexpr int kOneLaunch = kChunk; // rows up to here need no first kernel
 constexpr int kList = 256;         // continuations that a wavefront sorts
 
 // Keys that order as the values do; NaN as minus infinity, the zeros alike.
@@ -60,35 +62,39 @@ __device__ inline bool is_open(const BeamArgs &a, int64_t row) {
 }
 
 struct Block {
-    float top, sum;  // the largest logit (never NaN), the sum of e^(x - top)
+    float part[4];  // the parts' largest logits (never NaN)
+    float top, sum; // the largest of all, the sum of e^(x - top)
 };
-// [i0, i1) of a row by one wavefront. Sums in float32: 32 terms a lane, then six steps.
+// [i0, i1) of a row by one wavefront. Sums in float32: 32 terms a lane and chunk, then six steps.
 template <class T> __device__ inline Block block_of(const T *row, int i0, int i1, int vocab, bool aligned) {
     const int lane = threadIdx.x & 63;
-    float top = -INFINITY, sum = 0.f;
+    Block b{{-INFINITY, -INFINITY, -INFINITY, -INFINITY}, -INFINITY, 0.f};
     for (int c = i0; c < i1; c += kChunk) {
-        float x[4][8], t = -INFINITY;
+        float x[4][8];
 #pragma unroll
-        for (int u = 0; u < 4; u++) load8(row, c + 512 * u + 8 * lane, vocab, aligned, x[u]);
+        for (int u = 0; u < 4; u++) load8(row, c + kPart * u + 8 * lane, vocab, aligned, x[u]);
+        float top = b.top;
 #pragma unroll
-        for (int u = 0; u < 4; u++)
+        for (int u = 0; u < 4; u++) {
+            float t = -INFINITY;
 #pragma unroll
             for (int k = 0; k < 8; k++) t = fmaxf(t, x[u][k]);
-        t = wave_max(t);
-        if (t > top) {
-            sum *= exp2_f32((top - t) * 1.4426950408889634f);
-            top = t;
+            b.part[u] = fmaxf(b.part[u], wave_max(t));
+            top = fmaxf(top, b.part[u]);
         }
         if (top == -INFINITY) continue;
+        b.sum *= exp2_f32((b.top - top) * 1.4426950408889634f);
+        b.top = top;
 #pragma unroll
         for (int u = 0; u < 4; u++)
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 const float e = exp2_f32((x[u][k] - top) * 1.4426950408889634f);
-                sum += x[u][k] == x[u][k] ? e : 0.f;
+                b.sum += x[u][k] == x[u][k] ? e : 0.f;
             }
     }
-    return {top, wave_sum(sum)};
+    b.sum = wave_sum(b.sum);
+    return b;
 }
 
 // A wavefront a block of a row. 512 rows of 128 000 bfloat16 values.
@@ -111,34 +117,64 @@ template <class Count> __device__ inline uint32_t nth_largest(int n, Count &&cou
     return t;
 }
 
-// A row's best `want` keys in order into top (the wavefront's own LDS, as list): a logit's key, then the index, lower
-// ones larger. sel: one bit a block to look at, most: the threshold known so far.
+// A row's best `want` keys in order into top (the wavefront's own LDS, as list): a logit's key, then
+// the index, lower ones larger. sel: one bit a part to look at (parts of blocks of `size`, all within
+// `words`); threshold: a key that at least `want` of the row reach, 0 if none is known.
 template <class T>
-__device__ inline void row_best(const T *row, int vocab, bool aligned, int size, const unsigned long long *sel, int words, uint32_t floor,
+__device__ inline void row_best(const T *row, int vocab, bool aligned, int size, const unsigned long long *sel, int words, uint32_t threshold,
                                 int want, uint64_t *list, uint64_t *top) {
     const int lane = threadIdx.x & 63;
-    // f(first index, the lane's eight keys) over the blocks in order.
+    // f(first index, the lane's eight logits) over the parts in order, four on their way at a time.
     auto each = [&](auto &&f) {
-        for (int w = 0; w < words; w++)
-            for (unsigned long long bits = uniform(sel[w]); bits; bits &= bits - 1) {
-                const int b = 64 * w + __builtin_ctzll(bits);
-                const int i1 = min(vocab, (b + 1) * size);
-                for (int c = b * size; c < i1; c += 512) {
-                    float x[8];
-                    load8(row, c + 8 * lane, vocab, aligned, x);
-                    f(c + 8 * lane, x);
-                }
-            }
-    };
-    uint32_t best = 0;
-    each([&](int i, const float *x) {
+        int at[4], held = 0;
+        auto flush = [&] {
+            float x[4][8];
 #pragma unroll
-        for (int k = 0; k < 8; k++)
-            if (i + k < vocab) best = max(best, order_of(x[k]));
-    });
-    uint32_t t = max(floor, nth_largest(want, [&](uint32_t key) { return __popcll(__ballot(best >= key)); }));
+            for (int u = 0; u < 4; u++)
+                if (u < held) load8(row, at[u] + 8 * lane, vocab, aligned, x[u]);
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (u < held) f(at[u] + 8 * lane, x[u]);
+            held = 0;
+        };
+        auto put = [&](int i) {
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (u == held) at[u] = i;
+            if (++held == 4) flush();
+        };
+        for (int w = 0; w < words; w++)
+            for (unsigned long long bits = uniform(sel[w]); bits;) {
+                const int b = 16 * w + __builtin_ctzll(bits) / 4, first = 4 * (b - 16 * w);
+                const unsigned parts = unsigned(bits >> first) & 15;
+                for (int c = b * size; c < min(vocab, (b + 1) * size); c += kChunk)
+                    for (unsigned p = parts; p; p &= p - 1)
+                        if (c + kPart * __builtin_ctz(p) < vocab) put(c + kPart * __builtin_ctz(p));
+                bits &= ~(15ull << first);
+            }
+        flush();
+    };
+    uint32_t t = threshold;
     int greater, n;
-    for (int round = 0;; round++) {
+    for (int round = t ? 0 : 1;; round++) {
+        if (round == 1) {  // of the lanes' largest keys
+            uint32_t best = 0;
+            each([&](int i, const float *x) {
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (i + k < vocab) best = max(best, order_of(x[k]));
+            });
+            t = max(t, nth_largest(want, [&](uint32_t key) { return __popcll(__ballot(best >= key)); }));
+        } else if (round == 2) {  // the exact one, which fewer than `want` exceed
+            t = nth_largest(want, [&](uint32_t key) {
+                int c = 0;
+                each([&](int i, const float *x) {
+                    for (int k = 0; k < 8; k++) c += i + k < vocab && order_of(x[k]) >= key;
+                });
+                for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o);
+                return c;
+            });
+        }
         greater = 0, n = 0;
         int equal = 0;
         each([&](int i, const float *x) {
@@ -174,16 +210,7 @@ __device__ inline void row_best(const T *row, int vocab, bool aligned, int size,
             }
         });
         n = min(equal, want);
-        if (greater <= kList - int(kMostBeams) || round) break;
-        // More than fit: the exact threshold, which fewer than `want` exceed.
-        t = nth_largest(want, [&](uint32_t key) {
-            int c = 0;
-            each([&](int i, const float *x) {
-                for (int k = 0; k < 8; k++) c += i + k < vocab && order_of(x[k]) >= key;
-            });
-            for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o);
-            return c;
-        });
+        if (greater <= kList - int(kMostBeams)) break;
     }
     __builtin_amdgcn_wave_barrier();
     // Their places by counting.
@@ -200,7 +227,7 @@ __device__ inline void row_best(const T *row, int vocab, bool aligned, int size,
 template <class T> __global__ __launch_bounds__(512) void beam_groups_kernel(BeamArgs a, int blocks, int size, bool aligned, const Block *stats) {
     __shared__ uint64_t s_list[8][kList], s_top[kMostBeams * kMostBeams];
     __shared__ double s_score[kMostBeams * kMostBeams];
-    __shared__ unsigned long long s_sel[8][kMostBlocks / 64];
+    __shared__ unsigned long long s_sel[8][kHeld];
     const int64_t g = blockIdx.x;
     const int w = a.beams, v = a.vocab, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, want = min(w, v);
     for (int beam = wave; beam < w; beam += waves) {
@@ -210,25 +237,31 @@ template <class T> __global__ __launch_bounds__(512) void beam_groups_kernel(Bea
         const double cum = a.scores[r];
         const bool over = a.finished && a.finished[r];
         double m = -INFINITY, sum = 0;
-        float bt[kMostBlocks / 64], bs[kMostBlocks / 64];
+        uint32_t key[kHeld];  // of the parts' maxima, 0 where there is no part
+        const int words = stats ? (4 * blocks + 63) / 64 : 1;
         bool open = is_open(a, r);
         if (open) {
             if (!stats) {
                 const Block s = block_of(row, 0, v, v, aligned);
                 m = s.top, sum = s.sum;
             } else {
-                float t = -INFINITY;
+                float t[kMostBlocks / 64], bs[kMostBlocks / 64], best = -INFINITY;
 #pragma unroll
                 for (int k = 0; k < kMostBlocks / 64; k++) {
+                    const Block *b = stats + r * blocks + 64 * k + lane;
                     const bool in = 64 * k + lane < blocks;
-                    const Block s = in ? stats[r * blocks + 64 * k + lane] : Block{-INFINITY, 0.f};
-                    bt[k] = s.top, bs[k] = s.sum;
-                    t = fmaxf(t, s.top);
+                    t[k] = in ? b->top : -INFINITY, bs[k] = in ? b->sum : 0.f;
+                    best = fmaxf(best, t[k]);
                 }
-                m = wave_max(t);
+#pragma unroll
+                for (int k = 0; k < kHeld; k++) {
+                    const int part = 64 * k + lane;
+                    key[k] = part < 4 * blocks ? order_of(stats[r * blocks + part / 4].part[part % 4]) : 0;
+                }
+                m = wave_max(best);
 #pragma unroll
                 for (int k = 0; k < kMostBlocks / 64; k++)
-                    if (64 * k < blocks && bt[k] > -INFINITY) sum += double(bs[k]) * exp(double(bt[k]) - m);
+                    if (64 * k < blocks && t[k] > -INFINITY) sum += double(bs[k]) * exp(double(t[k]) - m);
                 for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
             }
             open = m > -INFINITY && m < INFINITY;
@@ -236,24 +269,19 @@ template <class T> __global__ __launch_bounds__(512) void beam_groups_kernel(Bea
         const double lse = open ? m + log(sum) : 0.0;
         if (open) {
             uint32_t t = 0;
-            int words = 1;
             if (!stats) {
-                if (lane == 0) s_sel[wave][0] = 1;
+                if (lane == 0) s_sel[wave][0] = 15;
             } else {
-                uint32_t key[kMostBlocks / 64];
-                words = (blocks + 63) / 64;
-#pragma unroll
-                for (int k = 0; k < kMostBlocks / 64; k++) key[k] = 64 * k + lane < blocks ? order_of(bt[k]) : 0;
                 t = nth_largest(want, [&](uint32_t x) {
                     int c = 0;
 #pragma unroll
-                    for (int k = 0; k < kMostBlocks / 64; k++)
+                    for (int k = 0; k < kHeld; k++)
                         if (k < words) c += __popcll(__ballot(key[k] >= x));
                     return c;
                 });
 #pragma unroll
-                for (int k = 0; k < kMostBlocks / 64; k++) {
-                    const unsigned long long in = __ballot(key[k] >= t && 64 * k + lane < blocks);
+                for (int k = 0; k < kHeld; k++) {
+                    const unsigned long long in = __ballot(key[k] >= t && key[k]);
                     if (lane == 0) s_sel[wave][k] = in;
                 }
             }

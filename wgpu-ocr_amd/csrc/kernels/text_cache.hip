@@ -102,31 +102,42 @@ template <class C, class O> __global__ __launch_bounds__(256) void read_kernel(R
     }
 }
 
-// One workgroup a sequence.
-__global__ __launch_bounds__(256) void fork_kernel(ForkArgs a) {
-    const uint32_t r = blockIdx.x, w = r % a.beams, g = r - w;
+// One workgroup a (sequence, head): the head's part of a copied page, the first also the table's row.
+// P: what a thread copies at once.
+template <class P> __global__ __launch_bounds__(256) void fork_kernel(ForkArgs a) {
+    const uint32_t r = blockIdx.x, h = blockIdx.y, w = r % a.beams, g = r - w;
     const Fork f = fork_of(a.parents + g, a.beams, w, a.lens + g, a.table.width, a.kv.page);
     const int32_t p = a.parents[r];
     const bool ok = p >= 0 && uint32_t(p) < a.beams;
     const int32_t *from = a.table.p + size_t(g + (ok ? p : 0)) * a.table.width;
-    int32_t *to = a.table_out + size_t(r) * a.table.width;
-    const uint32_t cols = ok ? f.full + (f.tail > 0) : 0;
-    for (uint32_t i = threadIdx.x; i < a.table.width; i += 256)
-        to[i] = i >= cols ? -1 : i == f.full && f.copy ? a.spare[r] : from[i];
-    if (threadIdx.x == 0) a.lens_out[r] = f.len, a.used[r] = f.copy;
+    if (h == 0) {
+        int32_t *to = a.table_out + size_t(r) * a.table.width;
+        const uint32_t cols = ok ? f.full + (f.tail > 0) : 0;
+        for (uint32_t i = threadIdx.x; i < a.table.width; i += 256)
+            to[i] = i >= cols ? -1 : i == f.full && f.copy ? a.spare[r] : from[i];
+        if (threadIdx.x == 0) a.lens_out[r] = f.len, a.used[r] = f.copy;
+    }
     if (!f.copy) return;
     const int32_t src = from[f.full], dst = a.spare[r];
     if (src < 0 || uint32_t(src) >= a.kv.pages || dst < 0 || uint32_t(dst) >= a.kv.pages || src == dst) return;
-    const size_t vec = size_t(a.kv.dim) * (a.kv.type == T_I8 || a.kv.type == T_E4M3 ? 1 : 2);
-    for (uint32_t h = 0; h < a.kv.heads; h++) {
-        const int64_t s0 = slot_of(src, a.kv.heads, a.kv.page, h, 0), d0 = slot_of(dst, a.kv.heads, a.kv.page, h, 0);
-        const char *ks = static_cast<const char *>(a.kv.k) + s0 * vec, *vs = static_cast<const char *>(a.kv.v) + s0 * vec;
-        char *kd = static_cast<char *>(a.kv.k) + d0 * vec, *vd = static_cast<char *>(a.kv.v) + d0 * vec;
-        for (size_t i = threadIdx.x; i < f.tail * vec; i += 256) kd[i] = ks[i], vd[i] = vs[i];
-        if (a.kv.type == T_I8 || a.kv.type == T_E4M3)
-            for (uint32_t i = threadIdx.x; i < f.tail; i += 256)
-                a.kv.k_scale[d0 + i] = a.kv.k_scale[s0 + i], a.kv.v_scale[d0 + i] = a.kv.v_scale[s0 + i];
+    const bool coded = a.kv.type == T_I8 || a.kv.type == T_E4M3;
+    const size_t vec = size_t(a.kv.dim) * (coded ? 1 : 2);
+    const int64_t s0 = slot_of(src, a.kv.heads, a.kv.page, h, 0), d0 = slot_of(dst, a.kv.heads, a.kv.page, h, 0);
+    const P *ks = reinterpret_cast<const P *>(static_cast<const char *>(a.kv.k) + s0 * vec), *vs = reinterpret_cast<const P *>(static_cast<const char *>(a.kv.v) + s0 * vec);
+    P *kd = reinterpret_cast<P *>(static_cast<char *>(a.kv.k) + d0 * vec), *vd = reinterpret_cast<P *>(static_cast<char *>(a.kv.v) + d0 * vec);
+    const uint32_t n = uint32_t(f.tail * vec / sizeof(P));
+    uint32_t i = threadIdx.x;
+    for (; i + 768 < n; i += 1024) {  // all on their way before the first is written
+        P x[4], y[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) x[u] = ks[i + 256 * u], y[u] = vs[i + 256 * u];
+#pragma unroll
+        for (int u = 0; u < 4; u++) kd[i + 256 * u] = x[u], vd[i + 256 * u] = y[u];
     }
+    for (; i < n; i += 256) kd[i] = ks[i], vd[i] = vs[i];
+    if (coded)
+        for (uint32_t e = threadIdx.x; e < f.tail; e += 256)
+            a.kv.k_scale[d0 + e] = a.kv.k_scale[s0 + e], a.kv.v_scale[d0 + e] = a.kv.v_scale[s0 + e];
 }
 
 }  // namespace
@@ -157,7 +168,9 @@ void launch_read(const ReadArgs &a, hipStream_t s) {
 
 void launch_fork(const ForkArgs &a, hipStream_t s) {
     ProbeScope probe("text_fork", s, 0, 8.0 * a.table.rows * a.table.width);
-    hipLaunchKernelGGL(fork_kernel, dim3(a.table.rows), dim3(256), 0, s, a);
+    const dim3 grid(a.table.rows, a.kv.heads);
+    if (whole_pieces(a.kv)) hipLaunchKernelGGL(fork_kernel<u32x4>, grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(fork_kernel<uint8_t>, grid, dim3(256), 0, s, a);
     OCR_HIP(hipGetLastError());
 }
 

@@ -382,9 +382,7 @@ template <class F> void with_pair(const DecodeArgs &a, F &&f) {
 void launch_decode(Ctx &c, const DecodeArgs &a, hipStream_t s) {
     ProbeScope probe("text_decode", s, 4.0 * a.table.rows * a.table.width * a.kv.page * a.q_heads * a.kv.dim,
                      2.0 * a.table.rows * a.table.width * a.kv.page * a.kv.heads * a.kv.dim * type_bytes(a.kv.type));
-    const bool pieces = a.kv.dim * type_bytes(a.kv.type) % 16 == 0 && reinterpret_cast<uintptr_t>(a.kv.k) % 16 == 0 &&
-                        reinterpret_cast<uintptr_t>(a.kv.v) % 16 == 0;
-    if (!pieces) {
+    if (!whole_pieces(a.kv)) {
         with_pair(a, [&](auto t, auto k) {
             hipLaunchKernelGGL((decode_row_kernel<decltype(t), decltype(k)>), dim3(a.table.rows, a.q_heads), dim3(64), 0, s, a);
         });

@@ -127,15 +127,26 @@ template <class C> constexpr float code_max = std::is_same_v<C, int8_t> ? 127.f 
 // Vectors whose largest value is under this are held as zeros: 448 over it still is a float.
 constexpr float kTinyMax = 1e-30f;
 
+// Over a wavefront, without LDS: each row of 16 lanes, then the rows in order; the last lane has the
+// result.
+template <int Ctrl, int Rows> __device__ inline float dpp_f32(float old, float v) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(__float_as_uint(old), __float_as_uint(v), Ctrl, Rows, 15, false));
+}
+template <class Op> __device__ inline float wave_reduce(float v, float none, Op &&op) {
+    v = op(v, dpp_f32<0x111, 15>(none, v));  // from 1, 2, 4, 8 lanes before
+    v = op(v, dpp_f32<0x112, 15>(none, v));
+    v = op(v, dpp_f32<0x114, 15>(none, v));
+    v = op(v, dpp_f32<0x118, 15>(none, v));
+    v = op(v, dpp_f32<0x142, 10>(none, v));  // a row's last lane to the next row (rows 1 and 3)
+    v = op(v, dpp_f32<0x143, 12>(none, v));  // lane 31 to rows 2 and 3
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 63));
+}
 __device__ inline float wave_max(float v) {
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+    return wave_reduce(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ inline float wave_sum(float v) {
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+    return wave_reduce(v, 0.f, [](float a, float b) { return a + b; });
 }
-
 __device__ inline int wave_max_i(int v) {
     for (int o = 32; o; o >>= 1) v = max(v, __shfl_xor(v, o));
     return __builtin_amdgcn_readfirstlane(v);

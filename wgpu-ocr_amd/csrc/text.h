@@ -25,6 +25,11 @@ struct KvCache {
     int type;
 };
 
+// Whether its vectors are whole 16-byte pieces.
+inline bool whole_pieces(const KvCache &c) {
+    return c.dim * type_bytes(c.type) % 16 == 0 && reinterpret_cast<uintptr_t>(c.k) % 16 == 0 && reinterpret_cast<uintptr_t>(c.v) % 16 == 0;
+}
+
 // Every sequence's pages: rows of width entries, a negative one where there is none.
 struct PageTable {
     const int32_t *p;
