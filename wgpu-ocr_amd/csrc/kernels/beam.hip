@@ -24,6 +24,7 @@ constexpr int kPart = 512;         // a part of a chunk: eight a lane
 constexpr int kMostBlocks = 128;   // blocks of a row
 constexpr int kHeld = kMostBlocks * 4 / 64;  // parts' maxima that a lane of the second kernel holds
 constexpr int kOneLaunch = kChunk; // rows up to here need no first kernel
+constexpr int kRough = 20;         // bits of a threshold that need not be exact
 constexpr int kList = 256;         // continuations that a wavefront sorts
 
 // Keys that order as the values do; NaN as minus infinity, the zeros alike.
@@ -31,6 +32,7 @@ __device__ inline uint32_t order_of(float x) {
     const uint32_t u = __float_as_uint(x == x ? x + 0.f : -INFINITY);
     return u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
 }
+constexpr uint32_t kNothing = 0x007fffffu;  // the key of minus infinity
 __device__ inline float value_of(uint32_t key) { return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu)); }
 
 // Eight logits of a row from index i on, those past the last minus infinity. aligned: rows and i lie
@@ -106,15 +108,15 @@ template <class T> __global__ __launch_bounds__(256) void beam_blocks_kernel(Bea
     if ((threadIdx.x & 63) == 0) out[row * blocks + b] = s;
 }
 
-// The n-th largest of all lanes' keys (0 where there are fewer): count(t) says how many keys of the
-// lane are t or more.
-template <class Count> __device__ inline uint32_t nth_largest(int n, Count &&count) {
+// The n-th largest of all lanes' keys as far as `bits` of it go, the others zero: at least n keys
+// reach it. count(t) says how many keys are t or more. Never under minus infinity's key.
+template <class Count> __device__ inline uint32_t nth_largest(int n, int bits, Count &&count) {
     uint32_t t = 0;
-    for (int bit = 31; bit >= 0; bit--) {
+    for (int bit = 31; bit >= 32 - bits; bit--) {
         const uint32_t next = t | 1u << bit;
         if (count(next) >= n) t = next;
     }
-    return t;
+    return max(t, kNothing);
 }
 
 // A row's best `want` keys in order into top (the wavefront's own LDS, as list): a logit's key, then
@@ -154,58 +156,59 @@ __device__ inline void row_best(const T *row, int vocab, bool aligned, int size,
             }
         flush();
     };
-    uint32_t t = threshold;
+    float t = value_of(threshold);
     int greater, n;
-    for (int round = t ? 0 : 1;; round++) {
-        if (round == 1) {  // of the lanes' largest keys
+    for (int round = threshold ? 0 : 1;; round++) {
+        if (round == 1) {  // of the lanes' largest
             uint32_t best = 0;
             each([&](int i, const float *x) {
+                float m = -INFINITY;
 #pragma unroll
-                for (int k = 0; k < 8; k++)
-                    if (i + k < vocab) best = max(best, order_of(x[k]));
+                for (int k = 0; k < 8; k++) m = fmaxf(m, x[k]);
+                if (i < vocab) best = max(best, order_of(m));
             });
-            t = max(t, nth_largest(want, [&](uint32_t key) { return __popcll(__ballot(best >= key)); }));
+            t = value_of(max(threshold, nth_largest(want, kRough, [&](uint32_t key) { return __popcll(__ballot(best >= key)); })));
         } else if (round == 2) {  // the exact one, which fewer than `want` exceed
-            t = nth_largest(want, [&](uint32_t key) {
+            t = value_of(nth_largest(want, 32, [&](uint32_t key) {
                 int c = 0;
                 each([&](int i, const float *x) {
                     for (int k = 0; k < 8; k++) c += i + k < vocab && order_of(x[k]) >= key;
                 });
                 for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o);
                 return c;
-            });
+            }));
         }
         greater = 0, n = 0;
         int equal = 0;
         each([&](int i, const float *x) {
-            int ne = 0;
+            unsigned over = 0, same = 0;  // bits of the lane's eight
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const uint32_t key = order_of(x[k]);
-                const bool in = i + k < vocab;
-                ne += in && key == t;
-                const unsigned long long g = __ballot(in && key > t);
-                if (g) {
-                    const int at = greater + __popcll(g & ((1ull << lane) - 1));
-                    if (in && key > t && at < kList - int(kMostBeams)) list[at] = uint64_t(key) << 32 | uint32_t(~(i + k));
-                    greater += __popcll(g);
-                }
+                over |= unsigned(x[k] > t) << k;
+                same |= unsigned(x[k] == t || (x[k] != x[k] && t == -INFINITY)) << k;
             }
-            // Of the keys that equal the threshold the lowest `want` indices.
-            if (equal < want && __ballot(ne)) {
-                int before = ne;
+            same &= vocab - i >= 8 ? 255u : (1u << max(vocab - i, 0)) - 1;
+            for (unsigned long long g; (g = __ballot(over)) != 0; over &= over - 1) {
+                const int at = greater + __popcll(g & ((1ull << lane) - 1)), k = __builtin_ctz(over | 256);
+                if (over && at < kList - int(kMostBeams)) {
+                    float v = x[0];
+#pragma unroll
+                    for (int e = 1; e < 8; e++) v = e == k ? x[e] : v;
+                    list[at] = uint64_t(order_of(v)) << 32 | uint32_t(~(i + k));
+                }
+                greater += __popcll(g);
+            }
+            // Of those that equal the threshold the `want` lowest indices.
+            if (equal < want && __ballot(same)) {
+                int before = __popc(same);
                 for (int o = 1; o < 64; o <<= 1) {
                     const int d = __shfl_up(before, o);
                     if (lane >= o) before += d;
                 }
                 const int all = __shfl(before, 63);
-                before -= ne;
-#pragma unroll
-                for (int k = 0; k < 8; k++)
-                    if (i + k < vocab && order_of(x[k]) == t) {
-                        if (equal + before < want) list[kList - 1 - (equal + before)] = uint64_t(t) << 32 | uint32_t(~(i + k));
-                        before++;
-                    }
+                before += equal - __popc(same);
+                for (; same && before < want; same &= same - 1, before++)
+                    list[kList - 1 - before] = uint64_t(order_of(t)) << 32 | uint32_t(~(i + __builtin_ctz(same)));
                 equal += all;
             }
         });
@@ -227,6 +230,7 @@ __device__ inline void row_best(const T *row, int vocab, bool aligned, int size,
 template <class T> __global__ __launch_bounds__(512) void beam_groups_kernel(BeamArgs a, int blocks, int size, bool aligned, const Block *stats) {
     __shared__ uint64_t s_list[8][kList], s_top[kMostBeams * kMostBeams];
     __shared__ double s_score[kMostBeams * kMostBeams];
+    __shared__ int s_place[kMostBeams * kMostBeams];
     __shared__ unsigned long long s_sel[8][kHeld];
     const int64_t g = blockIdx.x;
     const int w = a.beams, v = a.vocab, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, want = min(w, v);
@@ -272,13 +276,10 @@ template <class T> __global__ __launch_bounds__(512) void beam_groups_kernel(Bea
             if (!stats) {
                 if (lane == 0) s_sel[wave][0] = 15;
             } else {
-                t = nth_largest(want, [&](uint32_t x) {
-                    int c = 0;
+                uint32_t most = 0;
 #pragma unroll
-                    for (int k = 0; k < kHeld; k++)
-                        if (k < words) c += __popcll(__ballot(key[k] >= x));
-                    return c;
-                });
+                for (int k = 0; k < kHeld; k++) most = max(most, key[k]);
+                t = nth_largest(want, kRough, [&](uint32_t x) { return __popcll(__ballot(most >= x)); });
 #pragma unroll
                 for (int k = 0; k < kHeld; k++) {
                     const unsigned long long in = __ballot(key[k] >= t && key[k]);
@@ -310,25 +311,33 @@ template <class T> __global__ __launch_bounds__(512) void beam_groups_kernel(Bea
         __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();
-    // The group's best by counting those before each: beams' lists are in order, ties go to the lower
-    // beam, then the lower token. All of the group's inputs have been read.
-    for (int c = threadIdx.x; c < w * w; c += blockDim.x) {
-        const int beam = c / w, at = int(~uint32_t(s_top[c]));
+    // The group's best by counting those before each, list by list: the lists are in order, ties go
+    // to the lower beam, then the lower token.
+    for (int c = threadIdx.x; c < w * w; c += blockDim.x) s_place[c] = 0;
+    __syncthreads();
+    for (int x = threadIdx.x; x < w * w * w; x += blockDim.x) {
+        const int o = x / (w * w), c = x - o * w * w, beam = c / w, at = int(~uint32_t(s_top[c]));
         if (!s_top[c]) continue;
         const double s = s_score[c];
-        int place = 0;
-        for (int o = 0; o < w * w; o++) {
-            if (!s_top[o] || o == c) continue;
-            const double d = s_score[o];
-            const int ob = o / w;
-            place += d > s || (d == s && (ob < beam || (ob == beam && int(~uint32_t(s_top[o])) < at)));
+        int lo = 0, hi = w;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            const double d = s_score[o * w + mid];
+            const uint64_t k = s_top[o * w + mid];
+            if (k && (d > s || (d == s && (o < beam || (o == beam && int(~uint32_t(k)) < at))))) lo = mid + 1;
+            else hi = mid;
         }
-        if (place >= w) continue;
-        const int64_t out = g * w + place;
+        if (lo) atomicAdd(&s_place[c], lo);
+    }
+    __syncthreads();
+    // All of the group's inputs have been read but the flags of the winners.
+    for (int c = threadIdx.x; c < w * w; c += blockDim.x) {
+        const int place = s_place[c], beam = c / w, at = int(~uint32_t(s_top[c]));
+        if (!s_top[c] || place >= w) continue;
         const bool over = a.finished && a.finished[g * w + beam];
-        s_list[0][place] = uint64_t(uint32_t(beam)) << 32 | uint32_t(c) << 1 | uint32_t(over || (a.eos >= 0 && at == a.eos));
-        a.parents[out] = beam;
-        a.tokens[out] = at;
+        s_list[0][place] = uint32_t(c) << 1 | uint32_t(over || (a.eos >= 0 && at == a.eos));
+        a.parents[g * w + place] = beam;
+        a.tokens[g * w + place] = at;
     }
     __syncthreads();
     for (int k = threadIdx.x; k < w; k += blockDim.x) {
