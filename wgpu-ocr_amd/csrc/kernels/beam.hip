@@ -35,23 +35,32 @@ __device__ inline uint32_t order_of(float x) {
 constexpr uint32_t kNothing = 0x007fffffu;  // the key of minus infinity
 __device__ inline float value_of(uint32_t key) { return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu)); }
 
-// Eight logits of a row from index i on, those past the last minus infinity. aligned: rows and i lie
-// on 16 bytes (uniform).
-template <class T> __device__ inline void load8(const T *row, int i, int vocab, bool aligned, float *x) {
-    if (aligned && i + 8 <= vocab) {
-        constexpr int N = 16 / sizeof(T);
-        u32x4 raw[8 / N];
+// Eight logits from index i on, all in the row, as they are in memory (rows lie on no more than a
+// logit's size, which global loads take at any width).
+template <class T> struct Raw {
+    u32x4 x[8 * sizeof(T) / 16];
+};
+template <class T> __device__ inline Raw<T> load_raw(const T *row, int i) {
+    typedef uint32_t loose __attribute__((ext_vector_type(4), aligned(2)));
+    Raw<T> r;
 #pragma unroll
-        for (int k = 0; k < 8 / N; k++) raw[k] = *reinterpret_cast<const u32x4 *>(row + i + k * N);
+    for (int k = 0; k < int(8 * sizeof(T) / 16); k++) r.x[k] = *reinterpret_cast<const loose *>(reinterpret_cast<const char *>(row + i) + 16 * k);
+    return r;
+}
+template <class T> __device__ inline void values(const Raw<T> &r, float *x) {
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            if constexpr (sizeof(T) == 4) x[k] = __uint_as_float(raw[k / 4][k % 4]);
-            else x[k] = widen16(raw[0][k / 2] >> (16 * (k % 2)), std::is_same_v<T, f16> ? T_F16 : T_BF16);
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; k++) x[k] = i + k < vocab ? to_f32(row[i + k]) : -INFINITY;
+    for (int k = 0; k < 8; k++) {
+        if constexpr (sizeof(T) == 4) x[k] = __uint_as_float(r.x[k / 4][k % 4]);
+        else x[k] = widen16(r.x[0][k / 2] >> (16 * (k % 2)), std::is_same_v<T, f16> ? T_F16 : T_BF16);
     }
+}
+// The same at a row's end: minus infinity past the last.
+template <class T> __device__ inline void last_values(const T *row, int i, int vocab, float *x) {
+    T v[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = row[min(i + k, vocab - 1)];
+#pragma unroll
+    for (int k = 0; k < 8; k++) x[k] = i + k < vocab ? to_f32(v[k]) : -INFINITY;
 }
 
 __device__ inline unsigned long long uniform(unsigned long long x) {
@@ -68,13 +77,21 @@ struct Block {
     float top, sum; // the largest of all, the sum of e^(x - top)
 };
 // [i0, i1) of a row by one wavefront. Sums in float32: 32 terms a lane and chunk, then six steps.
-template <class T> __device__ inline Block block_of(const T *row, int i0, int i1, int vocab, bool aligned) {
+template <class T> __device__ inline Block block_of(const T *row, int i0, int i1, int vocab) {
     const int lane = threadIdx.x & 63;
     Block b{{-INFINITY, -INFINITY, -INFINITY, -INFINITY}, -INFINITY, 0.f};
     for (int c = i0; c < i1; c += kChunk) {
         float x[4][8];
+        if (c + kChunk <= vocab) {
+            Raw<T> raw[4];
 #pragma unroll
-        for (int u = 0; u < 4; u++) load8(row, c + kPart * u + 8 * lane, vocab, aligned, x[u]);
+            for (int u = 0; u < 4; u++) raw[u] = load_raw(row, c + kPart * u + 8 * lane);
+#pragma unroll
+            for (int u = 0; u < 4; u++) values(raw[u], x[u]);
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; u++) last_values(row, c + kPart * u + 8 * lane, vocab, x[u]);
+        }
         float top = b.top;
 #pragma unroll
         for (int u = 0; u < 4; u++) {
@@ -100,11 +117,11 @@ template <class T> __device__ inline Block block_of(const T *row, int i0, int i1
 }
 
 // A wavefront a block of a row. 512 rows of 128 000 bfloat16 values.
-template <class T> __global__ __launch_bounds__(256) void beam_blocks_kernel(BeamArgs a, int blocks, int size, bool aligned, Block *out) {
+template <class T> __global__ __launch_bounds__(256) void beam_blocks_kernel(BeamArgs a, int blocks, int size, Block *out) {
     const int64_t row = blockIdx.x;
     const int b = blockIdx.y * 4 + (threadIdx.x >> 6), v = a.vocab;
     if (b >= blocks || !is_open(a, row)) return;
-    const Block s = block_of(static_cast<const T *>(a.logits) + row * a.stride, b * size, min(v, (b + 1) * size), v, aligned);
+    const Block s = block_of(static_cast<const T *>(a.logits) + row * a.stride, b * size, min(v, (b + 1) * size), v);
     if ((threadIdx.x & 63) == 0) out[row * blocks + b] = s;
 }
 
@@ -123,112 +140,133 @@ template <class Count> __device__ inline uint32_t nth_largest(int n, int bits, C
 // the index, lower ones larger. sel: one bit a part to look at (parts of blocks of `size`, all within
 // `words`); threshold: a key that at least `want` of the row reach, 0 if none is known.
 template <class T>
-__device__ inline void row_best(const T *row, int vocab, bool aligned, int size, const unsigned long long *sel, int words, uint32_t threshold,
-                                int want, uint64_t *list, uint64_t *top) {
+__device__ inline void row_best(const T *row, int vocab, int size, const unsigned long long *sel, int words, uint32_t threshold, int want,
+                                uint32_t *list, uint64_t *keys, uint64_t *top) {
     const int lane = threadIdx.x & 63;
-    // f(first index, the lane's eight logits) over the parts in order, four on their way at a time.
+    // f(x, at) over the parts in order, four at a time: a lane's eight logits of each, minus infinity
+    // past the row's end and for NaN, and the part's first index, vocab if there is none.
     auto each = [&](auto &&f) {
-        int at[4], held = 0;
-        auto flush = [&] {
+        int at[4] = {vocab, vocab, vocab, vocab}, held = 0;
+        auto flush = [&](bool whole) {
             float x[4][8];
+            if (whole) {
+                Raw<T> raw[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) raw[u] = load_raw(row, (u < held ? at[u] : at[0]) + 8 * lane);
+#pragma unroll
+                for (int u = 0; u < 4; u++) values(raw[u], x[u]);
+            } else {
+                last_values(row, at[0] + 8 * lane, vocab, x[0]);
+            }
 #pragma unroll
             for (int u = 0; u < 4; u++)
-                if (u < held) load8(row, at[u] + 8 * lane, vocab, aligned, x[u]);
 #pragma unroll
-            for (int u = 0; u < 4; u++)
-                if (u < held) f(at[u] + 8 * lane, x[u]);
+                for (int k = 0; k < 8; k++)
+                    if (u >= held || x[u][k] != x[u][k]) x[u][k] = -INFINITY;
+            f(x, at);
             held = 0;
-        };
-        auto put = [&](int i) {
-#pragma unroll
-            for (int u = 0; u < 4; u++)
-                if (u == held) at[u] = i;
-            if (++held == 4) flush();
+            at[0] = at[1] = at[2] = at[3] = vocab;
         };
         for (int w = 0; w < words; w++)
             for (unsigned long long bits = uniform(sel[w]); bits;) {
-                const int b = 16 * w + __builtin_ctzll(bits) / 4, first = 4 * (b - 16 * w);
+                const int b = 16 * w + __builtin_ctzll(bits) / 4, first = 4 * (b - 16 * w), end = min(vocab, (b + 1) * size);
                 const unsigned parts = unsigned(bits >> first) & 15;
-                for (int c = b * size; c < min(vocab, (b + 1) * size); c += kChunk)
-                    for (unsigned p = parts; p; p &= p - 1)
-                        if (c + kPart * __builtin_ctz(p) < vocab) put(c + kPart * __builtin_ctz(p));
                 bits &= ~(15ull << first);
+                for (int c = b * size; c < end; c += kChunk)
+                    for (unsigned p = parts; p; p &= p - 1) {
+                        const int i = c + kPart * __builtin_ctz(p);
+                        if (i >= vocab) break;
+                        const bool last = i + kPart > vocab;
+                        if (held == 4 || (last && held)) flush(true);
+#pragma unroll
+                        for (int u = 0; u < 4; u++)
+                            if (u == held) at[u] = i;
+                        held++;
+                        if (last) flush(false);
+                    }
             }
-        flush();
+        if (held) flush(true);
     };
     float t = value_of(threshold);
     int greater, n;
     for (int round = threshold ? 0 : 1;; round++) {
         if (round == 1) {  // of the lanes' largest
             uint32_t best = 0;
-            each([&](int i, const float *x) {
+            each([&](const float (*x)[8], const int *at) {
                 float m = -INFINITY;
 #pragma unroll
-                for (int k = 0; k < 8; k++) m = fmaxf(m, x[k]);
-                if (i < vocab) best = max(best, order_of(m));
+                for (int u = 0; u < 4; u++)
+#pragma unroll
+                    for (int k = 0; k < 8; k++) m = fmaxf(m, x[u][k]);
+                if (at[0] + 8 * lane < vocab) best = max(best, order_of(m));
             });
             t = value_of(max(threshold, nth_largest(want, kRough, [&](uint32_t key) { return __popcll(__ballot(best >= key)); })));
         } else if (round == 2) {  // the exact one, which fewer than `want` exceed
             t = value_of(nth_largest(want, 32, [&](uint32_t key) {
                 int c = 0;
-                each([&](int i, const float *x) {
-                    for (int k = 0; k < 8; k++) c += i + k < vocab && order_of(x[k]) >= key;
+                each([&](const float (*x)[8], const int *at) {
+                    for (int u = 0; u < 4; u++)
+                        for (int k = 0; k < 8; k++) c += at[u] + 8 * lane + k < vocab && order_of(x[u][k]) >= key;
                 });
                 for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o);
                 return c;
             }));
         }
         greater = 0, n = 0;
-        int equal = 0;
-        each([&](int i, const float *x) {
-            unsigned over = 0, same = 0;  // bits of the lane's eight
+        each([&](const float (*x)[8], const int *at) {
+            unsigned over = 0, same = 0;  // a bit a logit
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                over |= unsigned(x[k] > t) << k;
-                same |= unsigned(x[k] == t || (x[k] != x[k] && t == -INFINITY)) << k;
-            }
-            same &= vocab - i >= 8 ? 255u : (1u << max(vocab - i, 0)) - 1;
-            for (unsigned long long g; (g = __ballot(over)) != 0; over &= over - 1) {
-                const int at = greater + __popcll(g & ((1ull << lane) - 1)), k = __builtin_ctz(over | 256);
-                if (over && at < kList - int(kMostBeams)) {
-                    float v = x[0];
+            for (int u = 0; u < 4; u++) {
 #pragma unroll
-                    for (int e = 1; e < 8; e++) v = e == k ? x[e] : v;
-                    list[at] = uint64_t(order_of(v)) << 32 | uint32_t(~(i + k));
+                for (int k = 0; k < 8; k++) {
+                    over |= unsigned(x[u][k] > t) << (8 * u + k);
+                    same |= unsigned(x[u][k] == t) << (8 * u + k);
                 }
+            }
+            for (unsigned long long g; (g = __ballot(over)) != 0; over &= over - 1) {
+                const int place = greater + __popcll(g & ((1ull << lane) - 1)), k = __builtin_ctz(over | 1u << 31);
+                if (over && place < kList - int(kMostBeams)) list[place] = (k < 16 ? k < 8 ? at[0] : at[1] : k < 24 ? at[2] : at[3]) + 8 * lane + k % 8;
                 greater += __popcll(g);
             }
             // Of those that equal the threshold the `want` lowest indices.
-            if (equal < want && __ballot(same)) {
-                int before = __popc(same);
+            for (int u = 0; u < 4 && n < want && __ballot(same); u++, same >>= 8) {
+                const int i = (u < 2 ? u == 0 ? at[0] : at[1] : u == 2 ? at[2] : at[3]) + 8 * lane;
+                unsigned mine = same & (vocab - i >= 8 ? 255u : (1u << max(vocab - i, 0)) - 1);
+                if (!__ballot(mine)) continue;
+                int before = __popc(mine);
                 for (int o = 1; o < 64; o <<= 1) {
                     const int d = __shfl_up(before, o);
                     if (lane >= o) before += d;
                 }
-                const int all = __shfl(before, 63);
-                before += equal - __popc(same);
-                for (; same && before < want; same &= same - 1, before++)
-                    list[kList - 1 - before] = uint64_t(order_of(t)) << 32 | uint32_t(~(i + __builtin_ctz(same)));
-                equal += all;
+                const int all = n + __shfl(before, 63);
+                before += n - __popc(mine);
+                for (; mine && before < want; mine &= mine - 1, before++) list[kList - 1 - before] = i + __builtin_ctz(mine);
+                n = min(all, want);
             }
         });
-        n = min(equal, want);
         if (greater <= kList - int(kMostBeams)) break;
     }
     __builtin_amdgcn_wave_barrier();
     // Their places by counting.
     const int total = greater + n;
     for (int i = lane; i < total; i += 64) {
-        const uint64_t key = list[i < greater ? i : kList - 1 - (i - greater)];
+        const uint32_t at = list[i < greater ? i : kList - 1 - (i - greater)];
+        keys[i] = uint64_t(order_of(to_f32(row[at]))) << 32 | uint32_t(~at);
+    }
+    __builtin_amdgcn_wave_barrier();
+    for (int i = lane; i < total; i += 64) {
+        const uint64_t key = keys[i];
         int place = 0;
-        for (int j = 0; j < total; j++) place += list[j < greater ? j : kList - 1 - (j - greater)] > key;
+#pragma unroll 4
+        for (int j = 0; j < total; j++) place += keys[j] > key;
         if (place < want) top[place] = key;
     }
     for (int i = total + lane; i < want; i += 64) top[i] = 0;  // fewer tokens than beams
 }
 
-template <class T> __global__ __launch_bounds__(512) void beam_groups_kernel(BeamArgs a, int blocks, int size, bool aligned, const Block *stats) {
-    __shared__ uint64_t s_list[8][kList], s_top[kMostBeams * kMostBeams];
+template <class T> __global__ __launch_bounds__(512) void beam_groups_kernel(BeamArgs a, int blocks, int size, const Block *stats) {
+    __shared__ uint32_t s_list[8][kList];
+    __shared__ uint64_t s_keys[8][kList], s_top[kMostBeams * kMostBeams];
     __shared__ double s_score[kMostBeams * kMostBeams];
     __shared__ int s_place[kMostBeams * kMostBeams];
     __shared__ unsigned long long s_sel[8][kHeld];
@@ -246,7 +284,7 @@ template <class T> __global__ __launch_bounds__(512) void beam_groups_kernel(Bea
         bool open = is_open(a, r);
         if (open) {
             if (!stats) {
-                const Block s = block_of(row, 0, v, v, aligned);
+                const Block s = block_of(row, 0, v, v);
                 m = s.top, sum = s.sum;
             } else {
                 float t[kMostBlocks / 64], bs[kMostBlocks / 64], best = -INFINITY;
@@ -287,7 +325,7 @@ template <class T> __global__ __launch_bounds__(512) void beam_groups_kernel(Bea
                 }
             }
             __builtin_amdgcn_wave_barrier();
-            row_best(row, v, aligned, stats ? size : v, s_sel[wave], words, t, want, s_list[wave], top);
+            row_best(row, v, stats ? size : v, s_sel[wave], words, t, want, s_list[wave], s_keys[wave], top);
             for (int i = want + lane; i < w; i += 64) top[i] = 0;
         } else {
             // A finished beam's only continuation is its end; what scores nothing comes in order.
@@ -353,7 +391,6 @@ void launch_beam(Ctx &c, const BeamArgs &a, hipStream_t s) {
     const int64_t rows = int64_t(a.groups) * a.beams;
     const size_t bytes = type_bytes(a.type);
     ProbeScope probe("beam_select", s, 3.0 * rows * a.vocab, double(rows) * a.vocab * bytes);
-    const bool aligned = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.stride * bytes % 16 == 0;
     // Blocks of whole chunks, few enough for the second kernel's registers.
     const int chunks = int((a.vocab + kChunk - 1) / kChunk), size = (chunks + kMostBlocks - 1) / kMostBlocks * kChunk;
     const int blocks = int((a.vocab + size - 1) / size);
@@ -363,10 +400,10 @@ void launch_beam(Ctx &c, const BeamArgs &a, hipStream_t s) {
     with_type(a.type, [&](auto t) {
         using T = decltype(t);
         if (two) {
-            hipLaunchKernelGGL((beam_blocks_kernel<T>), dim3(unsigned(rows), (blocks + 3) / 4), dim3(256), 0, s, a, blocks, size, aligned, stats.as<Block>());
+            hipLaunchKernelGGL((beam_blocks_kernel<T>), dim3(unsigned(rows), (blocks + 3) / 4), dim3(256), 0, s, a, blocks, size, stats.as<Block>());
             OCR_HIP(hipGetLastError());
         }
-        hipLaunchKernelGGL((beam_groups_kernel<T>), dim3(a.groups), dim3(64 * std::min(a.beams, 8u)), 0, s, a, blocks, size, aligned,
+        hipLaunchKernelGGL((beam_groups_kernel<T>), dim3(a.groups), dim3(64 * std::min(a.beams, 8u)), 0, s, a, blocks, size,
                            static_cast<const Block *>(stats.as<Block>()));
     });
     OCR_HIP(hipGetLastError());
