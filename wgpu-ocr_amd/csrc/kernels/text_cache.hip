@@ -1,5 +1,6 @@
 // The text decoder's cache: a step's projections normed, rotated and written into pages, pages read
-// back, beams' pages reordered.
+// back, beams' pages reordered. All are bound by the bytes they move: a lane takes eight values of a
+// vector at a time, and as many lanes as it has eights (a power of two) share it.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -12,8 +13,19 @@ namespace ocr {
 
 namespace {
 
-// One wavefront a (token, head): lane l holds values l, l + 64, ... of the head's vector.
-template <class T, class O, class C> __global__ __launch_bounds__(64) void append_kernel(AppendArgs a) {
+constexpr int kAppendTokens = 4, kReadTokens = 16;  // tokens of a workgroup
+
+// The cosine and sine of pair i of rot / 2 at a position. The turns in float64: float32 angles of far
+// positions would be off by whole steps of the rotation.
+__device__ inline float2 turn_of(int pos, int i, int rot, double log2_theta) {
+    const double turns = double(pos) * (exp2(-2.0 * i / double(rot) * log2_theta) * 0.15915494309189533577);
+    float2 r;
+    sincospif(2.f * float(turns - rint(turns)), &r.y, &r.x);
+    return r;
+}
+
+// Vectors that are no whole eights, or whose rotated halves are not: one wavefront a (token, head), lane l holds values l, l + 64, ... of the head's vector.
+template <class T, class O, class C> __global__ __launch_bounds__(64) void append_row_kernel(AppendArgs a) {
     __shared__ float s_x[256];
     const int lane = threadIdx.x, dim = a.kv.dim, heads = a.kv.heads;
     const int64_t t = blockIdx.x;
@@ -42,9 +54,8 @@ template <class T, class O, class C> __global__ __launch_bounds__(64) void appen
             const int i = a.adjacent ? c >> 1 : c % half;
             const bool second = a.adjacent ? c & 1 : c >= half;
             const int other = a.adjacent ? c ^ 1 : second ? c - half : c + half;
-            const double turns = double(pos) * (exp2(-2.0 * i / double(a.rot) * a.log2_theta) * 0.15915494309189533577);
-            float sn, cs;
-            sincospif(2.f * float(turns - rint(turns)), &sn, &cs);
+            const float2 r = turn_of(pos, i, a.rot, a.log2_theta);
+            const float cs = r.x, sn = r.y;
             x[u] = second ? x[u] * cs + s_x[other] * sn : x[u] * cs - s_x[other] * sn;
         }
     }
@@ -83,7 +94,153 @@ template <class T, class O, class C> __global__ __launch_bounds__(64) void appen
         if (lane + 64 * u < dim) dst[lane + 64 * u] = code_of<C>(x[u] * inv);
 }
 
-template <class C, class O> __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
+// Eight values at p, which lies on no more than a value's size.
+template <class T> struct Eight {
+    uint32_t x[2 * sizeof(T)];
+};
+template <class T> __device__ inline Eight<T> load_eight(const T *p) {
+    typedef uint32_t loose __attribute__((ext_vector_type(sizeof(T) == 1 ? 2 : 4), aligned(sizeof(T) > 2 ? 4 : sizeof(T))));
+    constexpr int N = sizeof(T) == 1 ? 2 : 4;
+    Eight<T> r;
+#pragma unroll
+    for (int k = 0; k < int(2 * sizeof(T)) / N; k++) {
+        const loose y = reinterpret_cast<const loose *>(p)[k];
+#pragma unroll
+        for (int e = 0; e < N; e++) r.x[N * k + e] = y[e];
+    }
+    return r;
+}
+template <class T> __device__ inline void store_eight(T *p, const Eight<T> &r) {
+    typedef uint32_t loose __attribute__((ext_vector_type(sizeof(T) == 1 ? 2 : 4), aligned(sizeof(T))));
+    if constexpr (sizeof(T) == 1) *reinterpret_cast<loose *>(p) = loose{r.x[0], r.x[1]};
+    else *reinterpret_cast<loose *>(p) = loose{r.x[0], r.x[1], r.x[2], r.x[3]};
+}
+template <class T> __device__ inline float value_at(const Eight<T> &r, int k) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(r.x[k]);
+    else if constexpr (sizeof(T) == 2) return widen16(r.x[k / 2] >> (16 * (k % 2)), std::is_same_v<T, f16> ? T_F16 : T_BF16);
+    else return to_f32(__builtin_bit_cast(T, uint8_t(r.x[k / 4] >> (8 * (k % 4)))));
+}
+// Eight values rounded to T (codes: already divided by the vector's scale).
+template <class T> __device__ inline Eight<T> eight_of(const float *x) {
+    Eight<T> r;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            r.x[k] = uint32_t(__builtin_bit_cast(uint16_t, T(x[2 * k]))) | uint32_t(__builtin_bit_cast(uint16_t, T(x[2 * k + 1]))) << 16;
+    } else if constexpr (std::is_same_v<T, e4m3>) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * k], x[4 * k + 1], 0, false);
+            r.x[k] = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * k + 2], x[4 * k + 3], lo, true);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            r.x[k] = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) r.x[k] |= uint32_t(uint8_t(code_of<int8_t>(x[4 * k + e]))) << (8 * e);
+        }
+    }
+    return r;
+}
+
+// `each` tokens a workgroup, W lanes a vector. The tokens' turns and places are looked up once for
+// all heads; a group of lanes takes a vector after the other, the next on its way. A prompt of 20 500
+// tokens of 48 bfloat16 heads of 128 into e4m3.
+template <class T, class O, class C, int W> __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int each) {
+    __shared__ float2 s_turn[kAppendTokens][128];
+    __shared__ int64_t s_vec[kAppendTokens];  // head 0's vector in the pool, negative: none
+    const int tid = threadIdx.x, c = tid % W, dim = a.kv.dim, heads = a.kv.heads, all = a.q_heads + 2 * heads, half = a.rot / 2;
+    const int64_t t0 = int64_t(blockIdx.x) * each;
+    const int n = int(min<int64_t>(each, a.n - t0)), items = n * all;
+    const bool in = 8 * c < dim;
+    auto load = [&](int item) {
+        const int t = item / all, h = item - t * all;
+        return load_eight(static_cast<const T *>(a.qkv) + (t0 + t) * a.stride + int64_t(h) * dim + 8 * (in ? c : 0));
+    };
+    Eight<T> raw = load(min(tid / W, items - 1));
+    float norm[2][8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        norm[0][k] = a.q_norm && in ? a.q_norm[8 * c + k] : 1.f;
+        norm[1][k] = a.k_norm && in ? a.k_norm[8 * c + k] : 1.f;
+    }
+    for (int x = tid; x < n * half; x += 256) {
+        const int t = x / half, i = x - t * half;
+        s_turn[t][i] = turn_of(a.pos[t0 + t], i, a.rot, a.log2_theta);
+    }
+    if (tid < n) {
+        const int seq = a.seq[t0 + tid], pos = a.pos[t0 + tid];
+        int page = -1;
+        if (seq >= 0 && seq < int(a.table.rows)) page = page_of(a.table.p + size_t(seq) * a.table.width, a.table.width, a.kv.page, a.kv.pages, pos);
+        s_vec[tid] = page < 0 ? -1 : slot_of(page, heads, a.kv.page, 0, uint32_t(pos) % a.kv.page);
+    }
+    __syncthreads();
+    for (int item = tid / W; item < items; item += 256 / W) {
+        const int t = item / all, h = item - t * all;
+        const int kind = h < int(a.q_heads) ? 0 : h < int(a.q_heads) + heads ? 1 : 2;  // q, k, v
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] = in ? value_at(raw, k) : 0.f;
+        raw = load(min(item + 256 / W, items - 1));
+        if (kind < 2) {
+            if (kind == 0 ? a.q_norm : a.k_norm) {
+                float ss = 0.f;
+#pragma unroll
+                for (int k = 0; k < 8; k++) ss = __fmaf_rn(x[k], x[k], ss);
+                for (int o = W / 2; o; o >>= 1) ss += __shfl_xor(ss, o);
+                const float r = 1.f / sqrtf(ss / float(dim) + a.eps);
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[k] = x[k] * r * (kind == 0 ? norm[0][k] : norm[1][k]);
+            }
+            if (a.rot && a.adjacent) {
+#pragma unroll
+                for (int k = 0; k < 8; k += 2)
+                    if (8 * c + k < int(a.rot)) {
+                        const float2 r = s_turn[t][4 * c + k / 2];
+                        const float y = x[k];
+                        x[k] = y * r.x - x[k + 1] * r.y;
+                        x[k + 1] = x[k + 1] * r.x + y * r.y;
+                    }
+            } else if (a.rot) {
+                const bool turns = 8 * c < int(a.rot), second = 8 * c >= half;
+                const int lane = tid & 63, other = !turns ? lane : second ? lane - half / 8 : lane + half / 8;
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float y = __shfl(x[k], other);
+                    if (turns) {
+                        const float2 r = s_turn[t][8 * c + k - (second ? half : 0)];
+                        x[k] = second ? x[k] * r.x + y * r.y : x[k] * r.x - y * r.y;
+                    }
+                }
+            }
+        }
+        const int hk = h - int(a.q_heads) - (kind == 2 ? heads : 0);
+        if (kind == 0) {
+            if (in) store_eight(static_cast<O *>(a.q) + ((t0 + t) * a.q_heads + h) * dim + 8 * c, eight_of<O>(x));
+            continue;
+        }
+        if (kind == 1 && a.k && in) store_eight(static_cast<O *>(a.k) + ((t0 + t) * heads + hk) * dim + 8 * c, eight_of<O>(x));
+        const int64_t vec = s_vec[t] + int64_t(hk) * a.kv.page;
+        if (s_vec[t] < 0) continue;
+        if constexpr (scaled<C>) {
+            uint32_t top = 0;  // of the magnitudes' bits: infinities and NaN come above every number
+#pragma unroll
+            for (int k = 0; k < 8; k++) top = max(top, __float_as_uint(x[k]) & 0x7fffffffu);
+            for (int o = W / 2; o; o >>= 1) top = max(top, uint32_t(__shfl_xor(int(top), o)));
+            const float m = __uint_as_float(top);
+            const bool fine = top < 0x7f800000u, some = fine && m > kTinyMax;
+            const float inv = some ? code_max<C> / m : 0.f;
+            if (c == 0) (kind == 1 ? a.kv.k_scale : a.kv.v_scale)[vec] = some ? m / code_max<C> : fine ? 0.f : NAN;
+#pragma unroll
+            for (int k = 0; k < 8; k++) x[k] = some ? x[k] * inv : 0.f;
+        }
+        if (in) store_eight(static_cast<C *>(kind == 1 ? a.kv.k : a.kv.v) + vec * dim + 8 * c, eight_of<C>(x));
+    }
+}
+
+// Vectors that are no whole eights: one workgroup a position of a sequence.
+template <class C, class O> __global__ __launch_bounds__(256) void read_row_kernel(ReadArgs a) {
     const int dim = a.kv.dim, heads = a.kv.heads;
     const int64_t pos = blockIdx.x, seq = blockIdx.y;
     const bool there = pos < clamp_len(a.lens[seq], a.table.width, a.kv.page);
@@ -99,6 +256,53 @@ template <class C, class O> __global__ __launch_bounds__(256) void read_kernel(R
         }
         static_cast<O *>(a.k)[out + i] = O(k);
         static_cast<O *>(a.v)[out + i] = O(v);
+    }
+}
+
+// kReadTokens positions of a sequence a workgroup, W lanes a vector, two vectors' keys and values on
+// their way at a time.
+template <class C, class O, int W> __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
+    __shared__ int64_t s_vec[kReadTokens];
+    const int tid = threadIdx.x, c = tid % W, dim = a.kv.dim, heads = a.kv.heads;
+    const uint32_t blocks = (a.most + kReadTokens - 1) / kReadTokens;
+    const int64_t seq = blockIdx.x / blocks, p0 = int64_t(blockIdx.x % blocks) * kReadTokens;
+    const int n = int(min<int64_t>(kReadTokens, a.most - p0)), items = n * heads;
+    if (tid < n) {
+        int64_t vec = -1;
+        if (p0 + tid < clamp_len(a.lens[seq], a.table.width, a.kv.page)) {
+            const int32_t page = page_of(a.table.p + seq * a.table.width, a.table.width, a.kv.page, a.kv.pages, p0 + tid);
+            if (page >= 0) vec = slot_of(page, heads, a.kv.page, 0, uint32_t(p0 + tid) % a.kv.page);
+        }
+        s_vec[tid] = vec;
+    }
+    __syncthreads();
+    if (8 * c >= dim) return;
+    constexpr int G = 256 / W;
+    for (int item = tid / W; item < items; item += 2 * G) {
+        Eight<C> raw[2][2];
+        float scale[2][2];
+        bool there[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int i = min(item + u * G, items - 1), p = i / heads;
+            there[u] = s_vec[p] >= 0;
+            const int64_t vec = there[u] ? s_vec[p] + int64_t(i - p * heads) * a.kv.page : 0;
+            raw[u][0] = load_eight(static_cast<const C *>(a.kv.k) + vec * dim + 8 * c);
+            raw[u][1] = load_eight(static_cast<const C *>(a.kv.v) + vec * dim + 8 * c);
+            scale[u][0] = scaled<C> ? a.kv.k_scale[vec] : 1.f;
+            scale[u][1] = scaled<C> ? a.kv.v_scale[vec] : 1.f;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            if (item + u * G >= items) break;
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                float x[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[k] = there[u] ? value_at(raw[u][y], k) * scale[u][y] : 0.f;
+                store_eight(static_cast<O *>(y ? a.v : a.k) + ((seq * a.most + p0) * heads + item + u * G) * dim + 8 * c, eight_of<O>(x));
+            }
+        }
     }
 }
 
@@ -140,16 +344,35 @@ template <class P> __global__ __launch_bounds__(256) void fork_kernel(ForkArgs a
             a.kv.k_scale[d0 + e] = a.kv.k_scale[s0 + e], a.kv.v_scale[d0 + e] = a.kv.v_scale[s0 + e];
 }
 
+// f(lanes of a vector): the power of two that holds its eights.
+template <class F> void with_lanes(uint32_t dim, F &&f) {
+    if (dim <= 32) f(std::integral_constant<int, 4>{});
+    else if (dim <= 64) f(std::integral_constant<int, 8>{});
+    else if (dim <= 128) f(std::integral_constant<int, 16>{});
+    else f(std::integral_constant<int, 32>{});
+}
+
 }  // namespace
 
 void launch_append(const AppendArgs &a, hipStream_t s) {
     const double values = double(a.n) * (a.q_heads + 2 * a.kv.heads) * a.kv.dim;
     ProbeScope probe("text_append", s, 10 * values, values * (type_bytes(a.type) + 2));
-    const dim3 grid(a.n, a.q_heads + 2 * a.kv.heads);
+    const bool eights = a.kv.dim % 8 == 0 && (a.adjacent || a.rot % 16 == 0);
+    // Four tokens a workgroup share their lookups once that leaves work for every compute unit.
+    const int each = a.n >= 4096 ? kAppendTokens : 1;
     with_type(a.type, [&](auto t) {
         with_type16(a.out_type, [&](auto o) {
             with_cache(a.kv.type, [&](auto c) {
-                hipLaunchKernelGGL((append_kernel<decltype(t), decltype(o), decltype(c)>), grid, dim3(64), 0, s, a);
+                using T = decltype(t);
+                using O = decltype(o);
+                using C = decltype(c);
+                if (!eights) {
+                    hipLaunchKernelGGL((append_row_kernel<T, O, C>), dim3(a.n, a.q_heads + 2 * a.kv.heads), dim3(64), 0, s, a);
+                    return;
+                }
+                with_lanes(a.kv.dim, [&](auto w) {
+                    hipLaunchKernelGGL((append_kernel<T, O, C, decltype(w)::value>), dim3((a.n + each - 1) / each), dim3(256), 0, s, a, each);
+                });
             });
         });
     });
@@ -159,9 +382,14 @@ void launch_append(const AppendArgs &a, hipStream_t s) {
 void launch_read(const ReadArgs &a, hipStream_t s) {
     const double values = 2.0 * a.table.rows * a.most * a.kv.heads * a.kv.dim;
     ProbeScope probe("text_read", s, values, values * (type_bytes(a.kv.type) + 2));
-    const dim3 grid(a.most, a.table.rows);
+    const int64_t blocks = (int64_t(a.most) + kReadTokens - 1) / kReadTokens * a.table.rows;
     with_cache(a.kv.type, [&](auto c) {
-        with_type16(a.type, [&](auto o) { hipLaunchKernelGGL((read_kernel<decltype(c), decltype(o)>), grid, dim3(256), 0, s, a); });
+        with_type16(a.type, [&](auto o) {
+            using C = decltype(c);
+            using O = decltype(o);
+            if (a.kv.dim % 8 || blocks > 0x7fffff) hipLaunchKernelGGL((read_row_kernel<C, O>), dim3(a.most, a.table.rows), dim3(256), 0, s, a);
+            else with_lanes(a.kv.dim, [&](auto w) { hipLaunchKernelGGL((read_kernel<C, O, decltype(w)::value>), dim3(unsigned(blocks)), dim3(256), 0, s, a); });
+        });
     });
     OCR_HIP(hipGetLastError());
 }
