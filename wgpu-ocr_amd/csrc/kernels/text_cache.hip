@@ -94,48 +94,53 @@ template <class T, class O, class C> __global__ __launch_bounds__(64) void appen
         if (lane + 64 * u < dim) dst[lane + 64 * u] = code_of<C>(x[u] * inv);
 }
 
-// Eight values at p, which lies on no more than a value's size.
-template <class T> struct Eight {
-    uint32_t x[2 * sizeof(T)];
+// N (four or eight) values at p, which lies on no more than a value's size.
+template <class T, int N> struct Some {
+    uint32_t x[N * sizeof(T) / 4];
 };
-template <class T> __device__ inline Eight<T> load_eight(const T *p) {
-    typedef uint32_t loose __attribute__((ext_vector_type(sizeof(T) == 1 ? 2 : 4), aligned(sizeof(T) > 2 ? 4 : sizeof(T))));
-    constexpr int N = sizeof(T) == 1 ? 2 : 4;
-    Eight<T> r;
+template <class T, int N> struct loose_of {
+    static constexpr int words = N * sizeof(T) / 4 < 4 ? N * sizeof(T) / 4 : 4;
+    typedef uint32_t type __attribute__((ext_vector_type(words), aligned(sizeof(T))));
+};
+template <class T, int N> __device__ inline Some<T, N> load_some(const T *p) {
+    using L = loose_of<T, N>;
+    Some<T, N> r;
 #pragma unroll
-    for (int k = 0; k < int(2 * sizeof(T)) / N; k++) {
-        const loose y = reinterpret_cast<const loose *>(p)[k];
+    for (int k = 0; k < int(N * sizeof(T) / 4) / L::words; k++) {
+        const typename L::type y = reinterpret_cast<const typename L::type *>(p)[k];
 #pragma unroll
-        for (int e = 0; e < N; e++) r.x[N * k + e] = y[e];
+        for (int e = 0; e < L::words; e++) r.x[L::words * k + e] = y[e];
     }
     return r;
 }
-template <class T> __device__ inline void store_eight(T *p, const Eight<T> &r) {
-    typedef uint32_t loose __attribute__((ext_vector_type(sizeof(T) == 1 ? 2 : 4), aligned(sizeof(T))));
-    if constexpr (sizeof(T) == 1) *reinterpret_cast<loose *>(p) = loose{r.x[0], r.x[1]};
-    else *reinterpret_cast<loose *>(p) = loose{r.x[0], r.x[1], r.x[2], r.x[3]};
+template <class T, int N> __device__ inline void store_some(T *p, const Some<T, N> &r) {
+    using L = loose_of<T, N>;
+    typename L::type y;
+#pragma unroll
+    for (int e = 0; e < L::words; e++) y[e] = r.x[e];
+    *reinterpret_cast<typename L::type *>(p) = y;
 }
-template <class T> __device__ inline float value_at(const Eight<T> &r, int k) {
+template <class T, int N> __device__ inline float value_at(const Some<T, N> &r, int k) {
     if constexpr (sizeof(T) == 4) return __uint_as_float(r.x[k]);
     else if constexpr (sizeof(T) == 2) return widen16(r.x[k / 2] >> (16 * (k % 2)), std::is_same_v<T, f16> ? T_F16 : T_BF16);
     else return to_f32(__builtin_bit_cast(T, uint8_t(r.x[k / 4] >> (8 * (k % 4)))));
 }
-// Eight values rounded to T (codes: already divided by the vector's scale).
-template <class T> __device__ inline Eight<T> eight_of(const float *x) {
-    Eight<T> r;
+// Values rounded to T (codes: already divided by the vector's scale).
+template <class T, int N> __device__ inline Some<T, N> some_of(const float *x) {
+    Some<T, N> r;
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int k = 0; k < 4; k++)
+        for (int k = 0; k < N / 2; k++)
             r.x[k] = uint32_t(__builtin_bit_cast(uint16_t, T(x[2 * k]))) | uint32_t(__builtin_bit_cast(uint16_t, T(x[2 * k + 1]))) << 16;
     } else if constexpr (std::is_same_v<T, e4m3>) {
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
+        for (int k = 0; k < N / 4; k++) {
             const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * k], x[4 * k + 1], 0, false);
             r.x[k] = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * k + 2], x[4 * k + 3], lo, true);
         }
     } else {
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
+        for (int k = 0; k < N / 4; k++) {
             r.x[k] = 0;
 #pragma unroll
             for (int e = 0; e < 4; e++) r.x[k] |= uint32_t(uint8_t(code_of<int8_t>(x[4 * k + e]))) << (8 * e);
@@ -145,25 +150,42 @@ template <class T> __device__ inline Eight<T> eight_of(const float *x) {
 }
 
 // `each` tokens a workgroup, W lanes a vector. The tokens' turns and places are looked up once for
-// all heads; a group of lanes takes a vector after the other, the next on its way. A prompt of 20 500
-// tokens of 48 bfloat16 heads of 128 into e4m3.
+// all heads; a group of lanes takes a vector after the other, the next two on their way. A lane has
+// two fours of a vector: those that it rotates with each other where pairs are halves apart, two
+// neighbours otherwise. A prompt of 23 600 tokens of 48 bfloat16 heads of 128 into e4m3.
 template <class T, class O, class C, int W> __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int each) {
-    __shared__ float2 s_turn[kAppendTokens][128];
+    __shared__ __align__(16) float2 s_turn[kAppendTokens][128];
+    __shared__ __align__(16) float s_norm[2][8 * W];
     __shared__ int64_t s_vec[kAppendTokens];  // head 0's vector in the pool, negative: none
     const int tid = threadIdx.x, c = tid % W, dim = a.kv.dim, heads = a.kv.heads, all = a.q_heads + 2 * heads, half = a.rot / 2;
     const int64_t t0 = int64_t(blockIdx.x) * each;
-    const int n = int(min<int64_t>(each, a.n - t0)), items = n * all;
-    const bool in = 8 * c < dim;
-    auto load = [&](int item) {
-        const int t = item / all, h = item - t * all;
-        return load_eight(static_cast<const T *>(a.qkv) + (t0 + t) * a.stride + int64_t(h) * dim + 8 * (in ? c : 0));
+    const int n = int(min<int64_t>(each, a.n - t0));
+    const bool in = 8 * c < dim, turns = 8 * c < int(a.rot), apart = turns && !a.adjacent;
+    const int at[2] = {!in ? 0 : apart ? 4 * c : 8 * c, !in ? 0 : apart ? half + 4 * c : 8 * c + 4};
+    // A group's vectors: every G-th of the tokens' heads.
+    constexpr int G = 256 / W;
+    const int dt = G / all, dh = G - dt * all;
+    struct Item {
+        int t, h;
     };
-    Eight<T> raw = load(min(tid / W, items - 1));
-    float norm[2][8];
-#pragma unroll
-    for (int k = 0; k < 8; k++) {
-        norm[0][k] = a.q_norm && in ? a.q_norm[8 * c + k] : 1.f;
-        norm[1][k] = a.k_norm && in ? a.k_norm[8 * c + k] : 1.f;
+    auto after = [&](Item i) {
+        i.t += dt, i.h += dh;
+        if (i.h >= all) i.h -= all, i.t++;
+        return i;
+    };
+    struct Vec {
+        Some<T, 4> x[2];
+    };
+    const T *const base = static_cast<const T *>(a.qkv) + t0 * a.stride;
+    auto load = [&](Item i) {
+        const T *src = base + (i.t < n ? i.t * a.stride + uint32_t(i.h * dim) : 0);
+        return Vec{load_some<T, 4>(src + at[0]), load_some<T, 4>(src + at[1])};
+    };
+    Item item{tid / W / all, tid / W % all}, ahead = after(item);
+    Vec next[2] = {load(item), load(ahead)};
+    for (int k = tid; k < 2 * dim; k += 256) {
+        const float *w = k < dim ? a.q_norm : a.k_norm;
+        s_norm[k >= dim][k < dim ? k : k - dim] = w ? w[k < dim ? k : k - dim] : 1.f;
     }
     for (int x = tid; x < n * half; x += 256) {
         const int t = x / half, i = x - t * half;
@@ -176,66 +198,79 @@ template <class T, class O, class C, int W> __global__ __launch_bounds__(256) vo
         s_vec[tid] = page < 0 ? -1 : slot_of(page, heads, a.kv.page, 0, uint32_t(pos) % a.kv.page);
     }
     __syncthreads();
-    for (int item = tid / W; item < items; item += 256 / W) {
-        const int t = item / all, h = item - t * all;
+    auto store = [&](auto *dst, const float *x) {
+        using D = std::remove_pointer_t<decltype(dst)>;
+        if (!in) return;
+        if (apart) {
+            store_some(dst + at[0], some_of<D, 4>(x));
+            store_some(dst + at[1], some_of<D, 4>(x + 4));
+        } else {
+            store_some(dst + at[0], some_of<D, 8>(x));
+        }
+    };
+    for (; item.t < n; item = after(item)) {
+        const int t = item.t, h = item.h;
         const int kind = h < int(a.q_heads) ? 0 : h < int(a.q_heads) + heads ? 1 : 2;  // q, k, v
         float x[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) x[k] = in ? value_at(raw, k) : 0.f;
-        raw = load(min(item + 256 / W, items - 1));
+        for (int k = 0; k < 8; k++) x[k] = value_at(next[0].x[k / 4], k % 4);
+        if (dim < 8 * W && !in)
+#pragma unroll
+            for (int k = 0; k < 8; k++) x[k] = 0.f;
+        ahead = after(ahead);
+        next[0] = next[1];
+        next[1] = load(ahead);
         if (kind < 2) {
             if (kind == 0 ? a.q_norm : a.k_norm) {
                 float ss = 0.f;
 #pragma unroll
                 for (int k = 0; k < 8; k++) ss = __fmaf_rn(x[k], x[k], ss);
-                for (int o = W / 2; o; o >>= 1) ss += __shfl_xor(ss, o);
-                const float r = 1.f / sqrtf(ss / float(dim) + a.eps);
+                ss = group_reduce<W>(ss, [](float a, float b) { return a + b; });
+                const float ms = ss * (1.f / float(dim)) + a.eps;
+                const float r = ms > 1e-30f ? __builtin_amdgcn_rsqf(ms) : 1.f / sqrtf(ms);  // the instruction takes no subnormals
+                const f32x4 w0 = *reinterpret_cast<const f32x4 *>(&s_norm[kind][at[0]]), w1 = *reinterpret_cast<const f32x4 *>(&s_norm[kind][at[1]]);
 #pragma unroll
-                for (int k = 0; k < 8; k++) x[k] = x[k] * r * (kind == 0 ? norm[0][k] : norm[1][k]);
+                for (int k = 0; k < 8; k++) x[k] = x[k] * r * (k < 4 ? w0[k] : w1[k - 4]);
             }
-            if (a.rot && a.adjacent) {
+            if (turns) {
+                const f32x4 r01 = *reinterpret_cast<const f32x4 *>(&s_turn[t][4 * c]), r23 = *reinterpret_cast<const f32x4 *>(&s_turn[t][4 * c + 2]);
+                const float cs[4] = {r01[0], r01[2], r23[0], r23[2]}, sn[4] = {r01[1], r01[3], r23[1], r23[3]};
+                auto turn = [](float &p, float &q, float c, float s) {
+                    const float y = p;
+                    p = y * c - q * s;
+                    q = q * c + y * s;
+                };
 #pragma unroll
-                for (int k = 0; k < 8; k += 2)
-                    if (8 * c + k < int(a.rot)) {
-                        const float2 r = s_turn[t][4 * c + k / 2];
-                        const float y = x[k];
-                        x[k] = y * r.x - x[k + 1] * r.y;
-                        x[k + 1] = x[k + 1] * r.x + y * r.y;
-                    }
-            } else if (a.rot) {
-                const bool turns = 8 * c < int(a.rot), second = 8 * c >= half;
-                const int lane = tid & 63, other = !turns ? lane : second ? lane - half / 8 : lane + half / 8;
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const float y = __shfl(x[k], other);
-                    if (turns) {
-                        const float2 r = s_turn[t][8 * c + k - (second ? half : 0)];
-                        x[k] = second ? x[k] * r.x + y * r.y : x[k] * r.x - y * r.y;
-                    }
+                for (int k = 0; k < 4; k++) {
+                    if (!a.adjacent) turn(x[k], x[4 + k], cs[k], sn[k]);
+                    else if (8 * c + 2 * k < int(a.rot)) turn(x[2 * k], x[2 * k + 1], cs[k], sn[k]);
                 }
             }
         }
         const int hk = h - int(a.q_heads) - (kind == 2 ? heads : 0);
         if (kind == 0) {
-            if (in) store_eight(static_cast<O *>(a.q) + ((t0 + t) * a.q_heads + h) * dim + 8 * c, eight_of<O>(x));
+            store(static_cast<O *>(a.q) + ((t0 + t) * a.q_heads + h) * dim, x);
             continue;
         }
-        if (kind == 1 && a.k && in) store_eight(static_cast<O *>(a.k) + ((t0 + t) * heads + hk) * dim + 8 * c, eight_of<O>(x));
+        if (kind == 1 && a.k) store(static_cast<O *>(a.k) + ((t0 + t) * heads + hk) * dim, x);
         const int64_t vec = s_vec[t] + int64_t(hk) * a.kv.page;
         if (s_vec[t] < 0) continue;
         if constexpr (scaled<C>) {
             uint32_t top = 0;  // of the magnitudes' bits: infinities and NaN come above every number
 #pragma unroll
             for (int k = 0; k < 8; k++) top = max(top, __float_as_uint(x[k]) & 0x7fffffffu);
-            for (int o = W / 2; o; o >>= 1) top = max(top, uint32_t(__shfl_xor(int(top), o)));
+            top = group_reduce<W>(top, [](uint32_t a, uint32_t b) { return max(a, b); });
             const float m = __uint_as_float(top);
             const bool fine = top < 0x7f800000u, some = fine && m > kTinyMax;
-            const float inv = some ? code_max<C> / m : 0.f;
-            if (c == 0) (kind == 1 ? a.kv.k_scale : a.kv.v_scale)[vec] = some ? m / code_max<C> : fine ? 0.f : NAN;
+            const float scale = m * (1.f / code_max<C>), inv = __builtin_amdgcn_rcpf(scale);  // from 2e-33 to 3e36: its reciprocal is normal
+            if (c == 0) (kind == 1 ? a.kv.k_scale : a.kv.v_scale)[vec] = some ? scale : fine ? 0.f : NAN;
 #pragma unroll
-            for (int k = 0; k < 8; k++) x[k] = some ? x[k] * inv : 0.f;
+            for (int k = 0; k < 8; k++) x[k] *= inv;
+            if (!some)
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[k] = 0.f;
         }
-        if (in) store_eight(static_cast<C *>(kind == 1 ? a.kv.k : a.kv.v) + vec * dim + 8 * c, eight_of<C>(x));
+        store(static_cast<C *>(kind == 1 ? a.kv.k : a.kv.v) + vec * dim, x);
     }
 }
 
@@ -279,7 +314,7 @@ template <class C, class O, int W> __global__ __launch_bounds__(256) void read_k
     if (8 * c >= dim) return;
     constexpr int G = 256 / W;
     for (int item = tid / W; item < items; item += 2 * G) {
-        Eight<C> raw[2][2];
+        Some<C, 8> raw[2][2];
         float scale[2][2];
         bool there[2];
 #pragma unroll
@@ -287,8 +322,8 @@ template <class C, class O, int W> __global__ __launch_bounds__(256) void read_k
             const int i = min(item + u * G, items - 1), p = i / heads;
             there[u] = s_vec[p] >= 0;
             const int64_t vec = there[u] ? s_vec[p] + int64_t(i - p * heads) * a.kv.page : 0;
-            raw[u][0] = load_eight(static_cast<const C *>(a.kv.k) + vec * dim + 8 * c);
-            raw[u][1] = load_eight(static_cast<const C *>(a.kv.v) + vec * dim + 8 * c);
+            raw[u][0] = load_some<C, 8>(static_cast<const C *>(a.kv.k) + vec * dim + 8 * c);
+            raw[u][1] = load_some<C, 8>(static_cast<const C *>(a.kv.v) + vec * dim + 8 * c);
             scale[u][0] = scaled<C> ? a.kv.k_scale[vec] : 1.f;
             scale[u][1] = scaled<C> ? a.kv.v_scale[vec] : 1.f;
         }
@@ -300,7 +335,7 @@ template <class C, class O, int W> __global__ __launch_bounds__(256) void read_k
                 float x[8];
 #pragma unroll
                 for (int k = 0; k < 8; k++) x[k] = there[u] ? value_at(raw[u][y], k) * scale[u][y] : 0.f;
-                store_eight(static_cast<O *>(y ? a.v : a.k) + ((seq * a.most + p0) * heads + item + u * G) * dim + 8 * c, eight_of<O>(x));
+                store_some(static_cast<O *>(y ? a.v : a.k) + ((seq * a.most + p0) * heads + item + u * G) * dim + 8 * c, some_of<O, 8>(x));
             }
         }
     }
@@ -357,7 +392,7 @@ template <class F> void with_lanes(uint32_t dim, F &&f) {
 void launch_append(const AppendArgs &a, hipStream_t s) {
     const double values = double(a.n) * (a.q_heads + 2 * a.kv.heads) * a.kv.dim;
     ProbeScope probe("text_append", s, 10 * values, values * (type_bytes(a.type) + 2));
-    const bool eights = a.kv.dim % 8 == 0 && (a.adjacent || a.rot % 16 == 0);
+    const bool eights = a.kv.dim % 8 == 0 && (a.adjacent || a.rot % 8 == 0);
     // Four tokens a workgroup share their lookups once that leaves work for every compute unit.
     const int each = a.n >= 4096 ? kAppendTokens : 1;
     with_type(a.type, [&](auto t) {

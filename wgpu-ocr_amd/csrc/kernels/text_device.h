@@ -147,6 +147,19 @@ __device__ inline float wave_max(float v) {
 __device__ inline float wave_sum(float v) {
     return wave_reduce(v, 0.f, [](float a, float b) { return a + b; });
 }
+// Over groups of W lanes, all of which get the result.
+template <int W, class V, class Op> __device__ inline V group_reduce(V v, Op &&op) {
+    auto from = [](V x, auto ctrl) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, x);
+        return __builtin_bit_cast(V, uint32_t(__builtin_amdgcn_update_dpp(u, u, decltype(ctrl)::value, 15, 15, false)));
+    };
+    v = op(v, from(v, std::integral_constant<int, 0xb1>{}));                          // neighbours
+    v = op(v, from(v, std::integral_constant<int, 0x4e>{}));                          // pairs of four
+    if constexpr (W > 4) v = op(v, from(v, std::integral_constant<int, 0x141>{}));    // eight, mirrored
+    if constexpr (W > 8) v = op(v, from(v, std::integral_constant<int, 0x140>{}));    // sixteen, mirrored
+    if constexpr (W > 16) v = op(v, V(__shfl_xor(v, 16)));
+    return v;
+}
 __device__ inline int wave_max_i(int v) {
     for (int o = 32; o; o >>= 1) v = max(v, __shfl_xor(v, o));
     return __builtin_amdgcn_readfirstlane(v);
