@@ -1,5 +1,5 @@
 """Builds libocrhip.so for gfx950 in-tree: every HIP kernel file and host C++ file with hipcc,
-in parallel, then one link. Run as `python -m ocrhip.build` from wgpu-ocr_amd/, or call build()."""
+in parallel, then one link; and the text decoder's calls on torch tensors with the host compiler. Run as `python -m ocrhip.build` from wgpu-ocr_amd/, or call build()."""
 from __future__ import annotations
 
 import concurrent.futures as cf
@@ -12,6 +12,7 @@ ROOT = os.path.dirname(PKG)  # wgpu-ocr_amd/
 CSRC = os.path.join(ROOT, "csrc")
 OBJ = os.path.join(ROOT, "_build")
 LIB = os.path.join(PKG, "libocrhip.so")
+CXX = os.environ.get("CXX", "g++")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 # Packed FP32 is disabled: this pool has seen wrong results from some v_pk_* f32 forms.
@@ -44,12 +45,36 @@ def _compile(src: str) -> str:
     return obj
 
 
+def _tensors() -> None:
+    """ocrhip._tensors, the text decoder's calls on torch tensors (csrc/python/tensors.cpp)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    out = os.path.join(PKG, "_tensors.so")
+    tmp = out + f".tmp{os.getpid()}"
+    include = [sysconfig.get_paths()["include"], *cpp_extension.include_paths()]
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-isystem{p}" for p in include], os.path.join(CSRC, "python", "tensors.cpp"), "-o", tmp, "-L" + lib, "-ltorch_python",
+           "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stderr}")
+    if r.stderr.strip():
+        sys.stderr.write(r.stderr)
+    os.replace(tmp, out)
+
+
 def build(jobs: int | None = None) -> str:
     os.makedirs(OBJ, exist_ok=True)
     srcs = sources()
     jobs = jobs or min(len(srcs), max(1, min(16, os.cpu_count() or 4)))
     with cf.ThreadPoolExecutor(jobs) as ex:
+        tensors = ex.submit(_tensors)
         objs = list(ex.map(_compile, srcs))
+        tensors.result()
     tmp = LIB + f".tmp{os.getpid()}"
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs, "-lz"]
     r = subprocess.run(cmd, capture_output=True, text=True)

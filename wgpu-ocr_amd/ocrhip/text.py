@@ -90,6 +90,30 @@ def _call(name, *args):
         raise root.OcrError(root.lib().ocr_last_error().decode())
 
 
+_tensors = None
+
+
+def _native(name, ctx, *args):
+    """The call on torch tensors by ocrhip._tensors; False if that leaves it to the checks here, which
+    say what is wrong or take arrays of another kind."""
+    global _tensors
+    if _tensors is None:
+        if "torch" not in sys.modules:
+            return False
+        try:
+            from . import _tensors as module
+        except ImportError as e:
+            raise _error(f"ocrhip._tensors is not built (run __graft_entry__.build() or python -m ocrhip.build): {e}")
+        lib = _root().lib()
+        module.bind(*[ctypes.cast(getattr(lib, f"ocr_{f}_device"), ctypes.c_void_p).value
+                      for f in ("kv_append", "kv_read", "attention", "decode_attention", "beam_select", "kv_fork")])
+        _tensors = module
+    rc = getattr(_tensors, name)(ctx.handle, ctx.device, *args)
+    if rc > 0 or rc == -1:
+        raise _error(_root().lib().ocr_last_error().decode())
+    return rc == 0
+
+
 def _code(x, what):
     code = _known.get(x.dtype)
     if code is None:
@@ -150,6 +174,7 @@ def _tokens(ctx, x, what, types, n=None, heads=None, dim=None):
 
 
 _I32, _F32, _F16, _ANY = (5,), (0,), (1, 2), (0, 1, 2)
+_PAIRS = {"halves": False, "adjacent": True}
 
 
 class KvCache:
@@ -180,6 +205,7 @@ class KvCache:
             raise _error("cache: an 8-bit cache needs scales")
         self._c = ocr_kv_cache(_array(ctx, self.k, "cache keys", (code,), shape), _array(ctx, self.v, "cache values", (code,), shape),
                                *scales, pages, heads, page, dim, code)
+        self._at = ctypes.addressof(self._c)
 
     def _table(self, table):
         if len(table.shape) != 2:
@@ -194,6 +220,9 @@ class KvCache:
         values, all of them by default; pairs "halves" or "adjacent"); queries into q [n][q_heads][dim], keys and values
         into the cache, keys into k [n][heads][dim] too if given (ocr_kv_append_device)."""
         ctx, types = self.ctx, _F16
+        rot = self.dim if rot is None else rot
+        if pairs in _PAIRS and _native("append", ctx, self._at, table, seq, pos, qkv, q, k, q_norm, k_norm, eps, rot, theta, _PAIRS[pairs]):
+            return
         qp, n, q_heads, dim, stride = _tokens(ctx, q, "queries", types, dim=self.dim)
         if stride != q_heads * dim:
             raise _error("queries: its values do not lie one after another")
@@ -202,22 +231,23 @@ class KvCache:
         code = _code(qkv, "projections")
         if code not in _ANY or tuple(qkv.shape) != (n, width) or (n and qkv.stride()[1] != 1):
             raise _error(f"projections: rows [{n}][{width}] of f32, f16 or bf16 are wanted, not {tuple(qkv.shape)} of {qkv.dtype}")
-        if pairs not in ("halves", "adjacent"):
+        if pairs not in _PAIRS:
             raise _error(f'pairs: "halves" or "adjacent" is wanted, not {pairs!r}')
-        rot = dim if rot is None else rot
         if theta <= 0 or rot < 0:
             raise _error(f"a rotation of {rot} values to the base {theta}")
         out = _code(q, "queries")
         args = ocr_kv_append_args(_array(ctx, seq, "sequence numbers", _I32, (n,)), _array(ctx, pos, "positions", _I32, (n,)),
                                   qkv.data_ptr() or None, code, n, q_heads, qkv.stride()[0] if n > 1 else width,
                                   _array(ctx, q_norm, "q_norm", _F32, (dim,)), _array(ctx, k_norm, "k_norm", _F32, (dim,)), eps, rot,
-                                  theta, pairs == "adjacent", qp, _array(ctx, k, "keys", (out,), (n, self.heads, dim)), out)
+                                  theta, _PAIRS[pairs], qp, _array(ctx, k, "keys", (out,), (n, self.heads, dim)), out)
         _call("ocr_kv_append_device", ctx.handle, ctypes.byref(self._c), ctypes.byref(self._table(table)), ctypes.byref(args))
 
     def read(self, table, lens, k, v):
         """The cached keys and values of every sequence's first positions into k and v
         [sequences][positions][heads][dim] (float16 or bfloat16), zeros past its length (lens
         [sequences]; ocr_kv_read_device)."""
+        if _native("read", self.ctx, self._at, table, lens, k, v):
+            return
         t = self._table(table)
         if len(k.shape) != 4:
             raise _error(f"keys: shape [sequences][positions][heads][dim] is wanted, not {tuple(k.shape)}")
@@ -230,18 +260,24 @@ class KvCache:
     def attend(self, table, lens, q, out, scale: float | None = None, cap: float = 0.0, slopes=None):
         """Attention of every sequence's last token (lens [sequences] counts it) over its cached
         vectors: q, out [sequences][q_heads][dim] (ocr_decode_attention_device)."""
-        ctx, t = self.ctx, self._table(table)
+        ctx = self.ctx
+        scale = self.dim ** -0.5 if scale is None else scale
+        if _native("attend", ctx, self._at, table, lens, q, out, scale, cap, slopes):
+            return
+        t = self._table(table)
         qp, n, q_heads, dim, qs = _tokens(ctx, q, "queries", _F16, n=t.rows, dim=self.dim)
         code = _code(q, "queries")
         op, _, _, _, os = _tokens(ctx, out, "outputs", (code,), n, q_heads, dim)
         args = ocr_decode_args(_array(ctx, lens, "lengths", _I32, (n,)), qp, op, code, q_heads, qs, os,
-                               dim ** -0.5 if scale is None else scale, cap, _array(ctx, slopes, "slopes", _F32, (q_heads,)))
+                               scale, cap, _array(ctx, slopes, "slopes", _F32, (q_heads,)))
         _call("ocr_decode_attention_device", ctx.handle, ctypes.byref(self._c), ctypes.byref(t), ctypes.byref(args))
 
     def fork(self, table, lens, parents, spare, table_out, lens_out, used):
         """The tables and lengths of every group's beams after a step that continued `parents`
         [groups][beams]: whole pages shared, part-filled ones copied into spare [sequences] for all
         but their first child; used [sequences] says where that was (ocr_kv_fork_device)."""
+        if _native("fork", self.ctx, self._at, table, lens, parents, spare, table_out, lens_out, used):
+            return
         ctx, t = self.ctx, self._table(table)
         if len(parents.shape) != 2 or parents.shape[0] * parents.shape[1] != t.rows:
             raise _error(f"parents: shape [groups][beams] of {t.rows} sequences is wanted, not {tuple(parents.shape)}")
@@ -256,6 +292,10 @@ def attention(ctx, q, k, v, out, docs=None, prefix=None, scale: float | None = N
     [n][kv_heads][dim], docs [documents + 1] rising offsets (None: one document), prefix
     [documents] tokens at each one's start that all of it sees, slopes [q_heads] of the distance
     bias, cap of the scores' tanh (0: none)."""
+    if scale is None:
+        scale = q.shape[2] ** -0.5 if len(q.shape) == 3 and q.shape[2] else 1.0
+    if _native("attention", ctx, q, k, v, out, docs, prefix, scale, cap, slopes):
+        return
     qp, n, q_heads, dim, qs = _tokens(ctx, q, "queries", _F16)
     code = _code(q, "queries")
     kp, _, kv_heads, _, ks = _tokens(ctx, k, "keys", (code,), n, dim=dim)
@@ -268,7 +308,7 @@ def attention(ctx, q, k, v, out, docs=None, prefix=None, scale: float | None = N
         ndocs = docs.shape[0] - 1
     args = ocr_attention_args(qp, kp, vp, op, code, n, q_heads, kv_heads, dim, qs, ks, vs, os,
                               None if docs is None else _array(ctx, docs, "documents", _I32, (ndocs + 1,)), ndocs,
-                              _array(ctx, prefix, "prefix", _I32, (ndocs,)), dim ** -0.5 if scale is None else scale, cap,
+                              _array(ctx, prefix, "prefix", _I32, (ndocs,)), scale, cap,
                               _array(ctx, slopes, "slopes", _F32, (q_heads,)))
     _call("ocr_attention_device", ctx.handle, ctypes.byref(args))
 
@@ -278,6 +318,8 @@ def beam_select(ctx, logits, scores, finished, eos: int | None, out_scores, pare
     [groups][beams] float32, finished [groups][beams] int32 or None, the end token or None; the
     best continuations of every group into out_scores, parents, tokens and out_finished
     [groups][beams]."""
+    if _native("beam_select", ctx, logits, scores, finished, eos, out_scores, parents, tokens, out_finished):
+        return
     if len(scores.shape) != 2 or len(logits.shape) != 2:
         raise _error(f"logits [groups * beams][vocab] and scores [groups][beams] are wanted, not {tuple(logits.shape)} and {tuple(scores.shape)}")
     shape = tuple(scores.shape)
