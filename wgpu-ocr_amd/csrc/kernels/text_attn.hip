@@ -45,10 +45,32 @@ template <class T> __global__ __launch_bounds__(64) void attention_row_kernel(At
     attention_row<T>(a, blockIdx.x, blockIdx.y, s_q);
 }
 
+// What scores go through besides the scale: nothing, the cap, or the distance's bias and perhaps the cap.
+enum Scores { kPlain, kCapped, kAny };
+
+// cap tanh(s / cap) of unscaled scores as s times a polynomial of their squares, which lasts to half
+// the cap: tanh(y) / y by powers of y^2, interpolated at the Chebyshev points of [0, 1/4], off by
+// 2^-25. In units of log2; the exponential's and the reciprocal's way takes half again as long.
+struct SmallCap {
+    float k[5], most;
+    __device__ SmallCap(float scale, float cap) {
+        const float y = scale / cap, t = y * y;
+        k[0] = scale * 1.4426950408889634f;
+        const float part[5] = {1.f, -0.3333306908607483f, 0.133247509598732f, -0.05298423767089844f, 0.017131345346570015f};
+        float power = k[0];
+#pragma unroll
+        for (int e = 1; e < 5; e++) power *= t, k[e] = part[e] * power;
+        most = y < 1e3f ? 0.5f / y : -1.f;  // beyond, the powers leave float32
+    }
+    __device__ float factor(float s) const {
+        const float t = s * s;
+        return __fmaf_rn(__fmaf_rn(__fmaf_rn(__fmaf_rn(k[4], t, k[3]), t, k[2]), t, k[1]), t, k[0]);
+    }
+};
+
 // 128 queries of one head, 32 a wavefront, over tiles of KT keys that come into LDS by DMA while the
-// tile before is worked on. DP: the head's values rounded up to 32; BIAS: scores are capped or get
-// the distance's bias.
-template <class T, int DP, bool BIAS> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_tile_kernel(AttentionArgs a, int tiles) {
+// tile before is worked on. DP: the head's values rounded up to 32.
+template <class T, int DP, Scores KIND> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_tile_kernel(AttentionArgs a, int tiles) {
     typedef T tvec __attribute__((ext_vector_type(8)));
     constexpr int PW = DP <= 64 ? 64 : DP <= 128 ? 128 : 256;  // a vector's values in LDS
     constexpr int PP = PW / 8;                                 // its 16-byte pieces
@@ -123,8 +145,10 @@ template <class T, int DP, bool BIAS> __global__ __launch_bounds__(256, DP <= 12
 #pragma unroll
         for (int e = 0; e < 16; e++) o[b][e] = 0.f;
     float m = -INFINITY, l = 0.f;
-    const float c = fabsf(a.scale) * 1.4426950408889634f;
-    const float slope = BIAS && a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.f;
+    const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);  // not 0: masked scores stay minus infinity
+    const float slope = KIND == kAny && a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.f;
+
+    const SmallCap small(fabsf(a.scale), KIND != kPlain && a.cap > 0.f ? a.cap : 1.f);
 
     if (jlo < jhi) copy(jlo, 0);
     int buf = 0;
@@ -143,45 +167,53 @@ template <class T, int DP, bool BIAS> __global__ __launch_bounds__(256, DP <= 12
             for (int st = 0; st < KS; st++)
                 s[t] = mfma32(*reinterpret_cast<const tvec *>(sk + koff[st] + t * 32 * PW * 2), qf[st], s[t]);
         }
-        const bool whole = j0 >= flo && j0 + KT <= fhi;
-        float top = -INFINITY;
-        if (BIAS || !whole) {
-#pragma unroll
-            for (int t = 0; t < KB; t++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) s[t][e] *= c;
-            if (BIAS && a.cap > 0.f) {
+        // Scores in units of log2 over `unit`, in place.
+        constexpr bool scaled_later = KIND == kPlain;
+        const float unit = scaled_later ? c : 1.f;
+        if (!scaled_later) {
+            float top = 0.f;
+            if (a.cap > 0.f) {
 #pragma unroll
                 for (int t = 0; t < KB; t++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) s[t][e] = cap_log2(s[t][e], a.cap);
+                    for (int e = 0; e < 16; e++) top = fmaxf(top, fabsf(s[t][e]));
             }
-            if (BIAS && a.slopes) {
+            if (a.cap > 0.f && __any(top > small.most)) {
+#pragma unroll
+                for (int t = 0; t < KB; t++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) s[t][e] = cap_log2(s[t][e] * c, a.cap);
+            } else if (a.cap > 0.f) {
+#pragma unroll
+                for (int t = 0; t < KB; t++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) s[t][e] *= small.factor(s[t][e]);
+            } else {
+#pragma unroll
+                for (int t = 0; t < KB; t++) s[t] *= c;
+            }
+            if (KIND == kAny) {
                 const float d = float(i - j0 - 4 * half);
 #pragma unroll
                 for (int t = 0; t < KB; t++)
 #pragma unroll
                     for (int e = 0; e < 16; e++) s[t][e] -= slope * fabsf(d - float(32 * t + 8 * (e / 4) + e % 4));
             }
-            if (!whole) {
-                const unsigned first = unsigned(j0 + 4 * half - r.lo), count = unsigned(r.hi - r.lo);
-#pragma unroll
-                for (int t = 0; t < KB; t++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        if (first + unsigned(32 * t + 8 * (e / 4) + e % 4) >= count) s[t][e] = -INFINITY;
-            }
-#pragma unroll
-            for (int t = 0; t < KB; t++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) top = fmaxf(top, s[t][e]);
-        } else {
-#pragma unroll
-            for (int t = 0; t < KB; t++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) top = fmaxf(top, s[t][e]);
-            top *= c;
         }
+        if (j0 < flo || j0 + KT > fhi) {
+            const unsigned first = unsigned(j0 + 4 * half - r.lo), count = unsigned(r.hi - r.lo);
+#pragma unroll
+            for (int t = 0; t < KB; t++)
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    if (first + unsigned(32 * t + 8 * (e / 4) + e % 4) >= count) s[t][e] = -INFINITY;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int t = 0; t < KB; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) top = fmaxf(top, s[t][e]);
+        top *= unit;
         if (__any(top > m + kSlack)) {
             const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32))), f = mn == -INFINITY ? 1.f : exp2_f32(m - mn);
             l *= f;
@@ -189,13 +221,13 @@ template <class T, int DP, bool BIAS> __global__ __launch_bounds__(256, DP <= 12
             for (int b = 0; b < NB; b++) o[b] *= f;
             m = mn;
         }
-        const float ref = m == -INFINITY ? 0.f : m - kLift, mul = BIAS || !whole ? 1.f : c;
+        const float ref = m == -INFINITY ? 0.f : m - kLift;
         tvec p[KB][2];
 #pragma unroll
         for (int t = 0; t < KB; t++)
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-                const float x = exp2_f32(__fmaf_rn(s[t][e], mul, -ref));
+                const float x = exp2_f32(scaled_later ? __fmaf_rn(s[t][e], unit, -ref) : s[t][e] - ref);
                 l += x;
                 p[t][e / 8][e % 8] = T(x);
             }
@@ -238,14 +270,14 @@ template <class T, int DP, bool BIAS> __global__ __launch_bounds__(256, DP <= 12
         attention_row<T>(a, w.tile * 128 + 32 * wave + __builtin_ctz(todo), h, reinterpret_cast<float *>(&s_kv[0][0][0]) + 256 * wave);
 }
 
-template <class T, bool BIAS> void launch_tiles(const AttentionArgs &a, hipStream_t s) {
+template <class T, Scores KIND> void launch_tiles(const AttentionArgs &a, hipStream_t s) {
     const int tiles = int((a.n + 127) / 128);
     const dim3 grid(unsigned(head_blocks(tiles, a.q_heads, a.kv_heads)));
-    if (a.dim <= 32) hipLaunchKernelGGL((attention_tile_kernel<T, 32, BIAS>), grid, dim3(256), 0, s, a, tiles);
-    else if (a.dim <= 64) hipLaunchKernelGGL((attention_tile_kernel<T, 64, BIAS>), grid, dim3(256), 0, s, a, tiles);
-    else if (a.dim <= 96) hipLaunchKernelGGL((attention_tile_kernel<T, 96, BIAS>), grid, dim3(256), 0, s, a, tiles);
-    else if (a.dim <= 128) hipLaunchKernelGGL((attention_tile_kernel<T, 128, BIAS>), grid, dim3(256), 0, s, a, tiles);
-    else hipLaunchKernelGGL((attention_tile_kernel<T, 256, BIAS>), grid, dim3(256), 0, s, a, tiles);
+    if (a.dim <= 32) hipLaunchKernelGGL((attention_tile_kernel<T, 32, KIND>), grid, dim3(256), 0, s, a, tiles);
+    else if (a.dim <= 64) hipLaunchKernelGGL((attention_tile_kernel<T, 64, KIND>), grid, dim3(256), 0, s, a, tiles);
+    else if (a.dim <= 96) hipLaunchKernelGGL((attention_tile_kernel<T, 96, KIND>), grid, dim3(256), 0, s, a, tiles);
+    else if (a.dim <= 128) hipLaunchKernelGGL((attention_tile_kernel<T, 128, KIND>), grid, dim3(256), 0, s, a, tiles);
+    else hipLaunchKernelGGL((attention_tile_kernel<T, 256, KIND>), grid, dim3(256), 0, s, a, tiles);
 }
 
 }  // namespace
@@ -259,8 +291,9 @@ void launch_attention(const AttentionArgs &a, hipStream_t s) {
     with_type16(a.type, [&](auto t) {
         using T = decltype(t);
         if (!pieces) hipLaunchKernelGGL((attention_row_kernel<T>), dim3(a.n, a.q_heads), dim3(64), 0, s, a);
-        else if (a.cap > 0.f || a.slopes) launch_tiles<T, true>(a, s);
-        else launch_tiles<T, false>(a, s);
+        else if (a.slopes) launch_tiles<T, kAny>(a, s);
+        else if (a.cap > 0.f) launch_tiles<T, kCapped>(a, s);
+        else launch_tiles<T, kPlain>(a, s);
     });
     OCR_HIP(hipGetLastError());
 }
