@@ -68,23 +68,27 @@ struct SmallCap {
     }
 };
 
-// 128 queries of one head, 32 a wavefront, over tiles of KT keys that come into LDS by DMA while the
-// tile before is worked on. DP: the head's values rounded up to 32.
-template <class T, int DP, Scores KIND> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_tile_kernel(AttentionArgs a, int tiles) {
+// 32 queries of one head a wavefront over tiles of KT keys that come into LDS by DMA while the tile
+// before is worked on. DP: the head's values rounded up to 32. QW: of the four wavefronts, those with
+// queries of their own; where it is two, the other two take the same queries over the other half of
+// each tile's keys, and their sums are joined at the end.
+template <class T, int DP, Scores KIND, int QW> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attention_tile_kernel(AttentionArgs a, int tiles) {
     typedef T tvec __attribute__((ext_vector_type(8)));
     constexpr int PW = DP <= 64 ? 64 : DP <= 128 ? 128 : 256;  // a vector's values in LDS
     constexpr int PP = PW / 8;                                 // its 16-byte pieces
-    constexpr int KT = PW == 256 ? 32 : 64, KB = KT / 32;
+    constexpr int KT = PW == 256 ? 32 : 64, KB = KT / 32 * QW / 4;  // a tile's keys, blocks of 32 of a wavefront's part
+    static_assert(KB >= 1, "a wavefront's part of a tile");
     constexpr int KS = DP / 16, NB = DP / 32;
     constexpr int TILE = KT * PW * 2;
     constexpr int ND = KT * PP / 256;  // copies a lane for a tile's keys
     __shared__ __align__(16) char s_kv[2][2][TILE];
     __shared__ int s_lo[4], s_hi[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+    const int qw = wave % QW, part = wave / QW * KB * 32;  // its queries, the first of its keys of a tile
     const HeadTile w = head_tile(blockIdx.x, tiles, a.q_heads, a.kv_heads);
     if (w.head < 0) return;
     const int h = w.head, hk = h / int(a.q_heads / a.kv_heads), dim = a.dim;
-    const int i = w.tile * 128 + 32 * wave + (lane & 31);
+    const int i = w.tile * (32 * QW) + 32 * qw + (lane & 31);
     const KeyRange r = key_range(i, int(a.n), a.docs, int(a.ndocs), a.prefix);
     const bool sees = r.lo < r.hi;
     // The wavefront's keys: some query sees those in [wlo, whi), all do those in [flo, fhi).
@@ -108,23 +112,40 @@ template <class T, int DP, Scores KIND> __global__ __launch_bounds__(256, DP <= 
         for (int x = tid; x < 4 * KT * PP; x += 256) *reinterpret_cast<u32x4 *>(&s_kv[0][0][0] + 16 * x) = u32x4{0, 0, 0, 0};
     }
     __syncthreads();
-    const int jlo = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3])), jhi = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
+    int jlo = s_lo[0], jhi = s_hi[0];
+#pragma unroll
+    for (int x = 1; x < 4; x++) jlo = min(jlo, s_lo[x]), jhi = max(jhi, s_hi[x]);
+    jlo = __builtin_amdgcn_readfirstlane(jlo), jhi = __builtin_amdgcn_readfirstlane(jhi);
 
     // Copies: a lane's pieces of a tile lie in LDS in order, each row's exchanged so that the reads
     // below touch every bank (swap_of), by the choice of the piece that the lane copies.
     auto swap_of = [](int row) { return PP == 8 ? (row >> 1 & 1) << 2 | (row >> 2 & 3) : (row & 3) << 2 | (row >> 2 & 3); };
-    const char *kbase = static_cast<const char *>(a.k) + int64_t(hk) * dim * 2, *vbase = static_cast<const char *>(a.v) + int64_t(hk) * dim * 2;
+    const char *kbase = static_cast<const char *>(a.k) + (int64_t(jlo) * a.k_stride + int64_t(hk) * dim) * 2;
+    const char *vbase = static_cast<const char *>(a.v) + (int64_t(jlo) * a.v_stride + int64_t(hk) * dim) * 2;
     const unsigned lds0 = lds_addr(&s_kv[0][0][0]) + wave * 1024;
-    auto copy = [&](int j0, int buf) {
-        const bool whole = j0 + KT <= jhi;
-        const char *kb = kbase + int64_t(j0) * a.k_stride * 2, *vb = vbase + int64_t(j0) * a.v_stride * 2;
+    const unsigned kstep = unsigned(a.k_stride * 2), vstep = unsigned(a.v_stride * 2);
+    auto row_of = [&](int d) { return ((4 * d + wave) * 64 + lane) / PP; };
+    auto piece_of = [&](int d) { return ((4 * d + wave) * 64 + lane) % PP ^ swap_of(row_of(d)); };
+    unsigned kat[ND], vat[ND];
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-            const int at = (4 * d + wave) * 64 + lane, row = at / PP, piece = at % PP ^ swap_of(row);
-            const int from = whole ? row : min(row, jhi - 1 - j0);
-            if (piece < pieces) {
-                dma16s_to(kb, unsigned(from) * unsigned(a.k_stride * 2) + 16 * piece, lds0 + (2 * buf + 0) * TILE + d * 4096);
-                dma16s_to(vb, unsigned(from) * unsigned(a.v_stride * 2) + 16 * piece, lds0 + (2 * buf + 1) * TILE + d * 4096);
+    for (int d = 0; d < ND; d++) kat[d] = row_of(d) * kstep + 16 * piece_of(d), vat[d] = row_of(d) * vstep + 16 * piece_of(d);
+    auto copy = [&](int j0, int buf) {
+        const char *kb = kbase + int64_t(j0 - jlo) * kstep, *vb = vbase + int64_t(j0 - jlo) * vstep;
+        const unsigned to = lds0 + buf * 2 * TILE;
+        if (j0 + KT <= jhi && pieces == PP) {
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                dma16s_to(kb, kat[d], to + d * 4096);
+                dma16s_to(vb, vat[d], to + TILE + d * 4096);
+            }
+            return;
+        }
+#pragma unroll
+        for (int d = 0; d < ND; d++) {  // past the last row: that again
+            const unsigned over = unsigned(max(0, row_of(d) - (jhi - 1 - j0)));
+            if (piece_of(d) < pieces) {
+                dma16s_to(kb, kat[d] - over * kstep, to + d * 4096);
+                dma16s_to(vb, vat[d] - over * vstep, to + TILE + d * 4096);
             }
         }
     };
@@ -150,14 +171,9 @@ template <class T, int DP, Scores KIND> __global__ __launch_bounds__(256, DP <= 
 
     const SmallCap small(fabsf(a.scale), KIND != kPlain && a.cap > 0.f ? a.cap : 1.f);
 
-    if (jlo < jhi) copy(jlo, 0);
-    int buf = 0;
-    for (int j0 = jlo; j0 < jhi; j0 += KT, buf ^= 1) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        lds_barrier();  // the tile is there, and all have left the other buffer
-        if (j0 + KT < jhi) copy(j0 + KT, buf ^ 1);
-        if (j0 >= whi || j0 + KT <= wlo) continue;
-        const char *const sk = s_kv[buf][0], *const sv = s_kv[buf][1];
+    // 32 KB keys from jw on, in LDS at sk, and their values at sv.
+    auto turn = [&](int jw, const char *sk, const char *sv) __attribute__((always_inline)) {
+        if (jw >= whi || jw + 32 * KB <= wlo) return;
         f32x16 s[KB];
 #pragma unroll
         for (int t = 0; t < KB; t++) {
@@ -193,15 +209,15 @@ template <class T, int DP, Scores KIND> __global__ __launch_bounds__(256, DP <= 
                 for (int t = 0; t < KB; t++) s[t] *= c;
             }
             if (KIND == kAny) {
-                const float d = float(i - j0 - 4 * half);
+                const float d = float(i - jw - 4 * half);
 #pragma unroll
                 for (int t = 0; t < KB; t++)
 #pragma unroll
                     for (int e = 0; e < 16; e++) s[t][e] -= slope * fabsf(d - float(32 * t + 8 * (e / 4) + e % 4));
             }
         }
-        if (j0 < flo || j0 + KT > fhi) {
-            const unsigned first = unsigned(j0 + 4 * half - r.lo), count = unsigned(r.hi - r.lo);
+        if (jw < flo || jw + 32 * KB > fhi) {
+            const unsigned first = unsigned(jw + 4 * half - r.lo), count = unsigned(r.hi - r.lo);
 #pragma unroll
             for (int t = 0; t < KB; t++)
 #pragma unroll
@@ -241,8 +257,38 @@ template <class T, int DP, Scores KIND> __global__ __launch_bounds__(256, DP <= 
                     const u32x2 y = lds_read_tr16(sv + voff[b][1] + (32 * t + 16 * u) * PW * 2);
                     o[b] = mfma32(__builtin_bit_cast(tvec, u32x4{x[0], x[1], y[0], y[1]}), p[t][u], o[b]);
                 }
+    };
+    auto step = [&](int j0, auto which) __attribute__((always_inline)) {
+        constexpr int buf = decltype(which)::value;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        lds_barrier();  // the tile is there, and all have left the other buffer
+        if (j0 + KT < jhi) copy(j0 + KT, buf ^ 1);
+        turn(j0 + part, s_kv[buf][0] + part * PW * 2, s_kv[buf][1] + part * PW * 2);
+    };
+    if (jlo < jhi) copy(jlo, 0);
+    for (int j0 = jlo; j0 < jhi; j0 += 2 * KT) {
+        step(j0, std::integral_constant<int, 0>{});
+        if (j0 + KT < jhi) step(j0 + KT, std::integral_constant<int, 1>{});
     }
     l += __shfl_xor(l, 32);
+    if constexpr (QW < 4) {
+        static_assert(2 * 64 * (16 * NB + 2) * 4 <= int(sizeof(s_kv)), "the sums' way");
+        __syncthreads();
+        float *const s_o = reinterpret_cast<float *>(&s_kv[0][0][0]) + qw * 64 * (16 * NB + 2) + lane;
+        if (wave >= QW) {
+#pragma unroll
+            for (int e = 0; e < 16 * NB; e++) s_o[64 * e] = o[e / 16][e % 16];
+            s_o[64 * 16 * NB] = m, s_o[64 * (16 * NB + 1)] = l;
+        }
+        __syncthreads();
+        if (wave < QW) {
+            const float m2 = s_o[64 * 16 * NB], l2 = s_o[64 * (16 * NB + 1)], mn = fmaxf(m, m2);
+            const float f = mn == -INFINITY ? 1.f : exp2_f32(m - mn), f2 = mn == -INFINITY ? 1.f : exp2_f32(m2 - mn);
+            l = l * f + l2 * f2;
+#pragma unroll
+            for (int e = 0; e < 16 * NB; e++) o[e / 16][e % 16] = o[e / 16][e % 16] * f + s_o[64 * e] * f2;
+        }
+    }
     // A value that is not finite spoils the sums of every query of its tile, also where the mask
     // gives it no weight: those queries again, by the formula.
     float bad = 0.f;
@@ -250,9 +296,9 @@ template <class T, int DP, Scores KIND> __global__ __launch_bounds__(256, DP <= 
     for (int b = 0; b < NB; b++)
 #pragma unroll
         for (int e = 0; e < 16; e++) bad += o[b][e] * 0.f;
-    const unsigned long long spoilt = __ballot(sees && !(bad == 0.f));
+    const unsigned long long spoilt = wave < QW ? __ballot(sees && !(bad == 0.f)) : 0;
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (i < int(a.n) && !((spoilt >> (lane & 31) | spoilt >> ((lane & 31) + 32)) & 1)) {
+    if (wave < QW && i < int(a.n) && !((spoilt >> (lane & 31) | spoilt >> ((lane & 31) + 32)) & 1)) {
         T *out = static_cast<T *>(a.out) + int64_t(i) * a.out_stride + int64_t(h) * dim;
 #pragma unroll
         for (int b = 0; b < NB; b++)
@@ -267,17 +313,24 @@ template <class T, int DP, Scores KIND> __global__ __launch_bounds__(256, DP <= 
     }
     __syncthreads();
     for (unsigned todo = unsigned(spoilt | spoilt >> 32); todo; todo &= todo - 1)
-        attention_row<T>(a, w.tile * 128 + 32 * wave + __builtin_ctz(todo), h, reinterpret_cast<float *>(&s_kv[0][0][0]) + 256 * wave);
+        attention_row<T>(a, w.tile * (32 * QW) + 32 * qw + __builtin_ctz(todo), h, reinterpret_cast<float *>(&s_kv[0][0][0]) + 256 * wave);
 }
 
-template <class T, Scores KIND> void launch_tiles(const AttentionArgs &a, hipStream_t s) {
-    const int tiles = int((a.n + 127) / 128);
-    const dim3 grid(unsigned(head_blocks(tiles, a.q_heads, a.kv_heads)));
-    if (a.dim <= 32) hipLaunchKernelGGL((attention_tile_kernel<T, 32, KIND>), grid, dim3(256), 0, s, a, tiles);
-    else if (a.dim <= 64) hipLaunchKernelGGL((attention_tile_kernel<T, 64, KIND>), grid, dim3(256), 0, s, a, tiles);
-    else if (a.dim <= 96) hipLaunchKernelGGL((attention_tile_kernel<T, 96, KIND>), grid, dim3(256), 0, s, a, tiles);
-    else if (a.dim <= 128) hipLaunchKernelGGL((attention_tile_kernel<T, 128, KIND>), grid, dim3(256), 0, s, a, tiles);
-    else hipLaunchKernelGGL((attention_tile_kernel<T, 256, KIND>), grid, dim3(256), 0, s, a, tiles);
+template <class T, int DP, Scores KIND, int QW> void launch_tiles(const AttentionArgs &a, hipStream_t s) {
+    const int tiles = int((a.n + 32 * QW - 1) / (32 * QW));
+    hipLaunchKernelGGL((attention_tile_kernel<T, DP, KIND, QW>), dim3(unsigned(head_blocks(tiles, a.q_heads, a.kv_heads))), dim3(256), 0, s, a, tiles);
+}
+template <class T, Scores KIND> void launch_dims(const AttentionArgs &a, hipStream_t s) {
+    // Tiles of 64 queries while those of 128 would leave compute units empty, but they bring every key
+    // from level two twice as often. 36 documents of up to 130 tokens, 16 heads of 64 (336 tiles of
+    // 128; four workgroups of it fit a compute unit): 11.9 us with 64 queries, 12.9 with 128; one of
+    // 2929, 16 heads of 128 (368 tiles; two fit): 103 and 87 us.
+    const bool few = int64_t((a.n + 127) / 128) * a.q_heads <= (a.dim <= 64 ? 768 : 256);
+    if (a.dim <= 32) few ? launch_tiles<T, 32, KIND, 2>(a, s) : launch_tiles<T, 32, KIND, 4>(a, s);
+    else if (a.dim <= 64) few ? launch_tiles<T, 64, KIND, 2>(a, s) : launch_tiles<T, 64, KIND, 4>(a, s);
+    else if (a.dim <= 96) few ? launch_tiles<T, 96, KIND, 2>(a, s) : launch_tiles<T, 96, KIND, 4>(a, s);
+    else if (a.dim <= 128) few ? launch_tiles<T, 128, KIND, 2>(a, s) : launch_tiles<T, 128, KIND, 4>(a, s);
+    else launch_tiles<T, 256, KIND, 4>(a, s);
 }
 
 }  // namespace
@@ -285,15 +338,15 @@ template <class T, Scores KIND> void launch_tiles(const AttentionArgs &a, hipStr
 void launch_attention(const AttentionArgs &a, hipStream_t s) {
     ProbeScope probe("text_attention", s, 2.0 * a.n * a.n * a.q_heads * a.dim, 4.0 * a.n * (a.q_heads + a.kv_heads) * a.dim);
     // Whole 16-byte pieces, and rows of a tile within 32 bits of each other.
-    bool pieces = a.dim % 8 == 0 && head_blocks((a.n + 127) / 128, a.q_heads, a.kv_heads) < 1 << 24;
+    bool pieces = a.dim % 8 == 0 && head_blocks((a.n + 63) / 64, a.q_heads, a.kv_heads) < 1 << 24;
     for (const void *p : {a.q, a.k, a.v, static_cast<const void *>(a.out)}) pieces = pieces && reinterpret_cast<uintptr_t>(p) % 16 == 0;
     for (int64_t st : {a.q_stride, a.k_stride, a.v_stride, a.out_stride}) pieces = pieces && st % 8 == 0 && st < 1 << 24;
     with_type16(a.type, [&](auto t) {
         using T = decltype(t);
         if (!pieces) hipLaunchKernelGGL((attention_row_kernel<T>), dim3(a.n, a.q_heads), dim3(64), 0, s, a);
-        else if (a.slopes) launch_tiles<T, kAny>(a, s);
-        else if (a.cap > 0.f) launch_tiles<T, kCapped>(a, s);
-        else launch_tiles<T, kPlain>(a, s);
+        else if (a.slopes) launch_dims<T, kAny>(a, s);
+        else if (a.cap > 0.f) launch_dims<T, kCapped>(a, s);
+        else launch_dims<T, kPlain>(a, s);
     });
     OCR_HIP(hipGetLastError());
 }
