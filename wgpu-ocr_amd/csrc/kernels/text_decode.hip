@@ -115,16 +115,20 @@ template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 
             s_at[i] = at;
         }
         __syncthreads();
-        // A tile's keys, values and scales; where there is no vector or no such piece of it, some
-        // other of the pool, zeroed when the tile is used.
+        // A tile's keys, values and scales; where there is no vector or no such piece of it, the
+        // pool's first, zeroed when the tile is used. (Past the last tile too: loads under a condition
+        // would be waited for where the paths meet.)
         u32x4 kr[2][NU], vr[2][NU];
         float scale_r = 0.f;
         bool none[2];
         auto load = [&](int t0) {
-            if (t0 >= cn) return;
             int64_t at[2];
 #pragma unroll
-            for (int t = 0; t < 2; t++) at[t] = s_at[t0 + 16 * t + n], none[t] = at[t] < 0, at[t] = none[t] ? 0 : at[t];
+            for (int t = 0; t < 2; t++) {
+                at[t] = s_at[min(t0, CH - 32) + 16 * t + n];
+                none[t] = t0 >= cn || at[t] < 0;
+                at[t] = none[t] ? 0 : at[t];
+            }
             if constexpr (scaled<C>) {
                 const int64_t vec = (g4 & 1) ? at[1] : at[0];
                 scale_r = (g4 < 2 ? a.kv.k_scale : a.kv.v_scale)[vec];
