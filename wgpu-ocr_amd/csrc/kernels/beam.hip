@@ -76,52 +76,60 @@ struct Block {
     float part[4];  // the parts' largest logits (never NaN)
     float top, sum; // the largest of all, the sum of e^(x - top)
 };
-// [i0, i1) of a row by one wavefront. Sums in float32: 32 terms a lane and chunk, then six steps.
-template <class T> __device__ inline Block block_of(const T *row, int i0, int i1, int vocab) {
+// A chunk's logits: eight of each part a lane, minus infinity past the row's end.
+template <class T> __device__ inline void load_chunk(const T *row, int c, int vocab, float (*x)[8]) {
     const int lane = threadIdx.x & 63;
-    Block b{{-INFINITY, -INFINITY, -INFINITY, -INFINITY}, -INFINITY, 0.f};
-    for (int c = i0; c < i1; c += kChunk) {
-        float x[4][8];
-        if (c + kChunk <= vocab) {
-            Raw<T> raw[4];
+    if (c + kChunk <= vocab) {
+        Raw<T> raw[4];
 #pragma unroll
-            for (int u = 0; u < 4; u++) raw[u] = load_raw(row, c + kPart * u + 8 * lane);
+        for (int u = 0; u < 4; u++) raw[u] = load_raw(row, c + kPart * u + 8 * lane);
 #pragma unroll
-            for (int u = 0; u < 4; u++) values(raw[u], x[u]);
-        } else {
-#pragma unroll
-            for (int u = 0; u < 4; u++) last_values(row, c + kPart * u + 8 * lane, vocab, x[u]);
-        }
-        float top = b.top;
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            float t = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < 8; k++) t = fmaxf(t, x[u][k]);
-            b.part[u] = fmaxf(b.part[u], wave_max(t));
-            top = fmaxf(top, b.part[u]);
-        }
-        if (top == -INFINITY) continue;
-        b.sum *= exp2_f32((b.top - top) * 1.4426950408889634f);
-        b.top = top;
-#pragma unroll
-        for (int u = 0; u < 4; u++)
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const float e = exp2_f32((x[u][k] - top) * 1.4426950408889634f);
-                b.sum += x[u][k] == x[u][k] ? e : 0.f;
-            }
+        for (int u = 0; u < 4; u++) values(raw[u], x[u]);
+        return;
     }
-    b.sum = wave_sum(b.sum);
-    return b;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[u][k] = -INFINITY;
+        if (c + kPart * u < vocab) last_values(row, c + kPart * u + 8 * lane, vocab, x[u]);
+    }
 }
+// A chunk added to a block (its sum still a lane's). Sums in float32: 32 terms a lane and chunk.
+__device__ inline void add_chunk(const float (*x)[8], Block &b) {
+    float top = b.top;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        float t = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 8; k++) t = fmaxf(t, x[u][k]);
+        b.part[u] = fmaxf(b.part[u], wave_max(t));
+        top = fmaxf(top, b.part[u]);
+    }
+    if (top == -INFINITY) return;
+    b.sum *= exp2_f32((b.top - top) * 1.4426950408889634f);
+    b.top = top;
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const float e = exp2_f32((x[u][k] - top) * 1.4426950408889634f);
+            b.sum += x[u][k] == x[u][k] ? e : 0.f;
+        }
+}
+constexpr Block kNoBlock{{-INFINITY, -INFINITY, -INFINITY, -INFINITY}, -INFINITY, 0.f};
 
 // A wavefront a block of a row. 512 rows of 128 000 bfloat16 values.
 template <class T> __global__ __launch_bounds__(256) void beam_blocks_kernel(BeamArgs a, int blocks, int size, Block *out) {
     const int64_t row = blockIdx.x;
     const int b = blockIdx.y * 4 + (threadIdx.x >> 6), v = a.vocab;
     if (b >= blocks || !is_open(a, row)) return;
-    const Block s = block_of(static_cast<const T *>(a.logits) + row * a.stride, b * size, min(v, (b + 1) * size), v);
+    Block s = kNoBlock;
+    for (int c = b * size; c < min(v, (b + 1) * size); c += kChunk) {
+        float x[4][8];
+        load_chunk(static_cast<const T *>(a.logits) + row * a.stride, c, v, x);
+        add_chunk(x, s);
+    }
+    s.sum = wave_sum(s.sum);
     if ((threadIdx.x & 63) == 0) out[row * blocks + b] = s;
 }
 
@@ -129,6 +137,7 @@ template <class T> __global__ __launch_bounds__(256) void beam_blocks_kernel(Bea
 // reach it. count(t) says how many keys are t or more. Never under minus infinity's key.
 template <class Count> __device__ inline uint32_t nth_largest(int n, int bits, Count &&count) {
     uint32_t t = 0;
+#pragma unroll 1
     for (int bit = 31; bit >= 32 - bits; bit--) {
         const uint32_t next = t | 1u << bit;
         if (count(next) >= n) t = next;
@@ -136,59 +145,62 @@ template <class Count> __device__ inline uint32_t nth_largest(int n, int bits, C
     return max(t, kNothing);
 }
 
-// A row's best `want` keys in order into top (the wavefront's own LDS, as list): a logit's key, then
-// the index, lower ones larger. sel: one bit a part to look at (parts of blocks of `size`, all within
-// `words`); threshold: a key that at least `want` of the row reach, 0 if none is known.
-template <class T>
-__device__ inline void row_best(const T *row, int vocab, int size, const unsigned long long *sel, int words, uint32_t threshold, int want,
-                                uint32_t *list, uint64_t *keys, uint64_t *top) {
+// f(x, at) over a row's parts (sel: one bit a part, of blocks of `size`, all within `words`) in order,
+// four at a time: a lane's eight logits of each, minus infinity past the row's end and for NaN, and
+// the part's first index, vocab if there is none.
+template <class T, class F> __device__ inline void each_part(const T *row, int vocab, int size, const unsigned long long *sel, int words, F &&f) {
     const int lane = threadIdx.x & 63;
-    // f(x, at) over the parts in order, four at a time: a lane's eight logits of each, minus infinity
-    // past the row's end and for NaN, and the part's first index, vocab if there is none.
-    auto each = [&](auto &&f) {
-        int at[4] = {vocab, vocab, vocab, vocab}, held = 0;
-        auto flush = [&](bool whole) {
-            float x[4][8];
-            if (whole) {
-                Raw<T> raw[4];
+    int at[4] = {vocab, vocab, vocab, vocab}, held = 0;
+    auto flush = [&](bool whole) {
+        float x[4][8];
+        if (whole) {
+            Raw<T> raw[4];
 #pragma unroll
-                for (int u = 0; u < 4; u++) raw[u] = load_raw(row, (u < held ? at[u] : at[0]) + 8 * lane);
+            for (int u = 0; u < 4; u++) raw[u] = load_raw(row, (u < held ? at[u] : at[0]) + 8 * lane);
 #pragma unroll
-                for (int u = 0; u < 4; u++) values(raw[u], x[u]);
-            } else {
-                last_values(row, at[0] + 8 * lane, vocab, x[0]);
-            }
+            for (int u = 0; u < 4; u++) values(raw[u], x[u]);
+        } else {
+            last_values(row, at[0] + 8 * lane, vocab, x[0]);
+        }
 #pragma unroll
-            for (int u = 0; u < 4; u++)
+        for (int u = 0; u < 4; u++)
 #pragma unroll
-                for (int k = 0; k < 8; k++)
-                    if (u >= held || x[u][k] != x[u][k]) x[u][k] = -INFINITY;
-            f(x, at);
-            held = 0;
-            at[0] = at[1] = at[2] = at[3] = vocab;
-        };
-        for (int w = 0; w < words; w++)
-            for (unsigned long long bits = uniform(sel[w]); bits;) {
-                const int b = 16 * w + __builtin_ctzll(bits) / 4, first = 4 * (b - 16 * w), end = min(vocab, (b + 1) * size);
-                const unsigned parts = unsigned(bits >> first) & 15;
-                bits &= ~(15ull << first);
-                for (int c = b * size; c < end; c += kChunk)
-                    for (unsigned p = parts; p; p &= p - 1) {
-                        const int i = c + kPart * __builtin_ctz(p);
-                        if (i >= vocab) break;
-                        const bool last = i + kPart > vocab;
-                        if (held == 4 || (last && held)) flush(true);
-#pragma unroll
-                        for (int u = 0; u < 4; u++)
-                            if (u == held) at[u] = i;
-                        held++;
-                        if (last) flush(false);
-                    }
-            }
-        if (held) flush(true);
+            for (int k = 0; k < 8; k++)
+                if (u >= held || x[u][k] != x[u][k]) x[u][k] = -INFINITY;
+        f(x, at);
+        held = 0;
+        at[0] = at[1] = at[2] = at[3] = vocab;
     };
+    for (int w = 0; w < words; w++)
+        for (unsigned long long bits = uniform(sel[w]); bits;) {
+            const int b = 16 * w + __builtin_ctzll(bits) / 4, first = 4 * (b - 16 * w), end = min(vocab, (b + 1) * size);
+            const unsigned parts = unsigned(bits >> first) & 15;
+            bits &= ~(15ull << first);
+            for (int c = b * size; c < end; c += kChunk)
+                for (unsigned p = parts; p; p &= p - 1) {
+                    const int i = c + kPart * __builtin_ctz(p);
+                    if (i >= vocab) break;
+                    const bool last = i + kPart > vocab;
+                    if (held == 4 || (last && held)) flush(true);
+#pragma unroll
+                    for (int u = 0; u < 4; u++)
+                        if (u == held) at[u] = i;
+                    held++;
+                    if (last) flush(false);
+                }
+        }
+    if (held) flush(true);
+}
+
+// A row's best `want` keys in order into top (the wavefront's own LDS, as list and keys): a logit's
+// key, then the index, lower ones larger. each(f): each_part over what can be among them; threshold:
+// a key that at least `want` of the row reach, 0 if none is known.
+template <class T, class Each>
+__device__ inline void row_best(const T *row, int vocab, Each &&each, uint32_t threshold, int want, uint32_t *list, uint64_t *keys, uint64_t *top) {
+    const int lane = threadIdx.x & 63;
     float t = value_of(threshold);
     int greater, n;
+#pragma unroll 1
     for (int round = threshold ? 0 : 1;; round++) {
         if (round == 1) {  // of the lanes' largest
             uint32_t best = 0;
@@ -205,7 +217,9 @@ __device__ inline void row_best(const T *row, int vocab, int size, const unsigne
             t = value_of(nth_largest(want, 32, [&](uint32_t key) {
                 int c = 0;
                 each([&](const float (*x)[8], const int *at) {
+#pragma unroll
                     for (int u = 0; u < 4; u++)
+#pragma unroll
                         for (int k = 0; k < 8; k++) c += at[u] + 8 * lane + k < vocab && order_of(x[u][k]) >= key;
                 });
                 for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o);
@@ -229,17 +243,17 @@ __device__ inline void row_best(const T *row, int vocab, int size, const unsigne
                 greater += __popcll(g);
             }
             // Of those that equal the threshold the `want` lowest indices.
+#pragma unroll 1
             for (int u = 0; u < 4 && n < want && __ballot(same); u++, same >>= 8) {
                 const int i = (u < 2 ? u == 0 ? at[0] : at[1] : u == 2 ? at[2] : at[3]) + 8 * lane;
                 unsigned mine = same & (vocab - i >= 8 ? 255u : (1u << max(vocab - i, 0)) - 1);
                 if (!__ballot(mine)) continue;
-                int before = __popc(mine);
-                for (int o = 1; o < 64; o <<= 1) {
-                    const int d = __shfl_up(before, o);
-                    if (lane >= o) before += d;
+                int before = n, all = n;
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const unsigned long long g = __ballot(mine >> k & 1);
+                    before += __popcll(g & ((1ull << lane) - 1)), all += __popcll(g);
                 }
-                const int all = n + __shfl(before, 63);
-                before += n - __popc(mine);
                 for (; mine && before < want; mine &= mine - 1, before++) list[kList - 1 - before] = i + __builtin_ctz(mine);
                 n = min(all, want);
             }
@@ -264,7 +278,7 @@ __device__ inline void row_best(const T *row, int vocab, int size, const unsigne
     for (int i = total + lane; i < want; i += 64) top[i] = 0;  // fewer tokens than beams
 }
 
-template <class T> __global__ __launch_bounds__(512) void beam_groups_kernel(BeamArgs a, int blocks, int size, const Block *stats) {
+template <class T, bool ONE> __global__ __launch_bounds__(512) void beam_groups_kernel(BeamArgs a, int blocks, int size, const Block *stats) {
     __shared__ uint32_t s_list[8][kList];
     __shared__ uint64_t s_keys[8][kList], s_top[kMostBeams * kMostBeams];
     __shared__ double s_score[kMostBeams * kMostBeams];
@@ -279,27 +293,45 @@ template <class T> __global__ __launch_bounds__(512) void beam_groups_kernel(Bea
         const double cum = a.scores[r];
         const bool over = a.finished && a.finished[r];
         double m = -INFINITY, sum = 0;
+        float x[4][8];        // a row of one chunk
         uint32_t key[kHeld];  // of the parts' maxima, 0 where there is no part
-        const int words = stats ? (4 * blocks + 63) / 64 : 1;
+        const int words = (4 * blocks + 63) / 64;
+        // All of the row's loads before the first is looked at.
+        float t[kMostBlocks / 64], bs[kMostBlocks / 64], held[kHeld];
+        if constexpr (ONE) {
+            load_chunk(row, 0, v, x);
+        } else {
+#pragma unroll
+            for (int k = 0; k < kMostBlocks / 64; k++) {
+                const Block *b = stats + r * blocks + min(64 * k + lane, blocks - 1);
+                t[k] = b->top, bs[k] = b->sum;
+            }
+#pragma unroll
+            for (int k = 0; k < kHeld; k++) {
+                const int part = min(64 * k + lane, 4 * blocks - 1);
+                held[k] = stats[r * blocks + part / 4].part[part % 4];
+            }
+        }
         bool open = is_open(a, r);
         if (open) {
-            if (!stats) {
-                const Block s = block_of(row, 0, v, v);
-                m = s.top, sum = s.sum;
+            if constexpr (ONE) {
+                Block s = kNoBlock;
+                add_chunk(x, s);
+                m = s.top, sum = wave_sum(s.sum);
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        if (x[u][k] != x[u][k]) x[u][k] = -INFINITY;
             } else {
-                float t[kMostBlocks / 64], bs[kMostBlocks / 64], best = -INFINITY;
+                float best = -INFINITY;
 #pragma unroll
                 for (int k = 0; k < kMostBlocks / 64; k++) {
-                    const Block *b = stats + r * blocks + 64 * k + lane;
-                    const bool in = 64 * k + lane < blocks;
-                    t[k] = in ? b->top : -INFINITY, bs[k] = in ? b->sum : 0.f;
+                    if (64 * k + lane >= blocks) t[k] = -INFINITY;
                     best = fmaxf(best, t[k]);
                 }
 #pragma unroll
-                for (int k = 0; k < kHeld; k++) {
-                    const int part = 64 * k + lane;
-                    key[k] = part < 4 * blocks ? order_of(stats[r * blocks + part / 4].part[part % 4]) : 0;
-                }
+                for (int k = 0; k < kHeld; k++) key[k] = 64 * k + lane < 4 * blocks ? order_of(held[k]) : 0;
                 m = wave_max(best);
 #pragma unroll
                 for (int k = 0; k < kMostBlocks / 64; k++)
@@ -311,8 +343,9 @@ template <class T> __global__ __launch_bounds__(512) void beam_groups_kernel(Bea
         const double lse = open ? m + log(sum) : 0.0;
         if (open) {
             uint32_t t = 0;
-            if (!stats) {
-                if (lane == 0) s_sel[wave][0] = 15;
+            if constexpr (ONE) {
+                const int at[4] = {0, min(kPart, v), min(2 * kPart, v), min(3 * kPart, v)};
+                row_best(row, v, [&](auto &&f) { f(x, at); }, 0, want, s_list[wave], s_keys[wave], top);
             } else {
                 uint32_t most = 0;
 #pragma unroll
@@ -323,9 +356,9 @@ template <class T> __global__ __launch_bounds__(512) void beam_groups_kernel(Bea
                     const unsigned long long in = __ballot(key[k] >= t && key[k]);
                     if (lane == 0) s_sel[wave][k] = in;
                 }
+                __builtin_amdgcn_wave_barrier();
+                row_best(row, v, [&](auto &&f) { each_part(row, v, size, s_sel[wave], words, f); }, t, want, s_list[wave], s_keys[wave], top);
             }
-            __builtin_amdgcn_wave_barrier();
-            row_best(row, v, stats ? size : v, s_sel[wave], words, t, want, s_list[wave], s_keys[wave], top);
             for (int i = want + lane; i < w; i += 64) top[i] = 0;
         } else {
             // A finished beam's only continuation is its end; what scores nothing comes in order.
@@ -403,8 +436,9 @@ void launch_beam(Ctx &c, const BeamArgs &a, hipStream_t s) {
             hipLaunchKernelGGL((beam_blocks_kernel<T>), dim3(unsigned(rows), (blocks + 3) / 4), dim3(256), 0, s, a, blocks, size, stats.as<Block>());
             OCR_HIP(hipGetLastError());
         }
-        hipLaunchKernelGGL((beam_groups_kernel<T>), dim3(a.groups), dim3(64 * std::min(a.beams, 8u)), 0, s, a, blocks, size,
-                           static_cast<const Block *>(stats.as<Block>()));
+        const dim3 threads(64 * std::min(a.beams, 8u));
+        if (two) hipLaunchKernelGGL((beam_groups_kernel<T, false>), dim3(a.groups), threads, 0, s, a, blocks, size, static_cast<const Block *>(stats.as<Block>()));
+        else hipLaunchKernelGGL((beam_groups_kernel<T, true>), dim3(a.groups), threads, 0, s, a, blocks, size, static_cast<const Block *>(nullptr));
     });
     OCR_HIP(hipGetLastError());
 }
