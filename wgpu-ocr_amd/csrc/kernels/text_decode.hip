@@ -49,13 +49,20 @@ template <class T, class C> __global__ __launch_bounds__(64) void decode_row_ker
     attend_row(kv, s_q, dim, 0, len, len - 1, a.cap, a.slopes ? a.slopes[h] : 0.f, [&](int c, float o) { out[c] = T(o); });
 }
 
+// What a launch's workgroups share. shift: a page's positions as a power of two, -1 if they are none.
+struct DecodePlan {
+    uint32_t parts;
+    int group, blocks, shift;  // query heads a key head, blocks of 16 of them
+    bool q_pieces;
+};
+
 // Parts of a sequence joined: part [row][head][parts] holds dim normalised values, then log2 of the
 // sum of weights.
 constexpr int kPartTail = 4;  // keeps the rows' 16-byte alignment
 
 // T: the queries' type, C: the cache's; products of 8-bit caches in float16, which holds their codes
 // exactly.
-template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 3 : 1) void decode_kernel(DecodeArgs a, uint32_t parts, float *part, bool q_pieces) {
+template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 3 : 1) void decode_kernel(DecodeArgs a, DecodePlan plan, float *part) {
     using M = std::conditional_t<scaled<C>, f16, C>;
     typedef M mvec __attribute__((ext_vector_type(8)));
     constexpr int NU = DP * int(sizeof(C)) / 64;    // 16-byte pieces of a vector that a lane holds
@@ -71,8 +78,9 @@ template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 
     __shared__ float s_ml[2][2][16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g4 = lane >> 4;
     const int64_t r = blockIdx.x;
-    const int group = a.q_heads / a.kv.heads, blocks = (group + 15) / 16;
-    const int hk = blockIdx.y / blocks, q0 = int(blockIdx.y) % blocks * 16, dim = a.kv.dim;
+    const uint32_t parts = plan.parts;
+    const int hk = plan.blocks == 1 ? blockIdx.y : blockIdx.y / plan.blocks, q0 = (int(blockIdx.y) - hk * plan.blocks) * 16, dim = a.kv.dim;
+    const int group = plan.group;
     const int h = hk * group + q0 + n;  // the lane's query head
     const bool real = q0 + n < group;
     // The lane's query, in the order of its key pieces.
@@ -81,7 +89,7 @@ template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 
     for (int s = 0; s < NS; s++) {
         const int c = sizeof(C) == 1 ? 64 * (s >> 1) + 16 * g4 + 8 * (s & 1) : 32 * s + 8 * g4;
         raw[s] = u32x4{0, 0, 0, 0};
-        if (real && c < dim) raw[s] = load16x8(a.q, r * a.q_stride + int64_t(h) * dim + c, q_pieces);
+        if (real && c < dim) raw[s] = load16x8(a.q, r * a.q_stride + int64_t(h) * dim + c, plan.q_pieces);
     }
     const int len = clamp_len(a.lens[r], a.table.width, a.kv.page);
     const Parts ps = parts_of(len, parts);
@@ -109,8 +117,9 @@ template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 
         for (int i = tid; i < ((cn + 31) & ~31); i += 256) {
             int64_t at = -1;
             if (i < cn) {
-                const int32_t p = page_of(a.table.p + r * a.table.width, a.table.width, a.kv.page, a.kv.pages, c0 + i);
-                if (p >= 0) at = slot_of(p, a.kv.heads, a.kv.page, hk, uint32_t(c0 + i) % a.kv.page);
+                const uint32_t pos = c0 + i, entry = plan.shift >= 0 ? pos >> plan.shift : pos / a.kv.page;
+                const int32_t p = page_at(a.table.p + r * a.table.width, a.table.width, a.kv.pages, entry);
+                if (p >= 0) at = slot_of(p, a.kv.heads, a.kv.page, hk, pos - entry * a.kv.page);
             }
             s_at[i] = at;
         }
@@ -364,11 +373,13 @@ template <int N> __global__ __launch_bounds__(N) void decode_join_kernel(DecodeA
 }
 
 template <class T, class C> void launch_tiles(const DecodeArgs &a, uint32_t parts, float *part, hipStream_t s) {
-    const bool q_pieces = reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_stride % 8 == 0;
-    const dim3 grid(a.table.rows, a.kv.heads * ((a.q_heads / a.kv.heads + 15) / 16), parts);
-    if (a.kv.dim <= 64) hipLaunchKernelGGL((decode_kernel<T, C, 64>), grid, dim3(256), 0, s, a, parts, part, q_pieces);
-    else if (a.kv.dim <= 128) hipLaunchKernelGGL((decode_kernel<T, C, 128>), grid, dim3(256), 0, s, a, parts, part, q_pieces);
-    else hipLaunchKernelGGL((decode_kernel<T, C, 256>), grid, dim3(256), 0, s, a, parts, part, q_pieces);
+    const int group = int(a.q_heads / a.kv.heads);
+    const DecodePlan plan{parts, group, (group + 15) / 16, a.kv.page & (a.kv.page - 1) ? -1 : __builtin_ctz(a.kv.page),
+                          reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_stride % 8 == 0};
+    const dim3 grid(a.table.rows, a.kv.heads * plan.blocks, parts);
+    if (a.kv.dim <= 64) hipLaunchKernelGGL((decode_kernel<T, C, 64>), grid, dim3(256), 0, s, a, plan, part);
+    else if (a.kv.dim <= 128) hipLaunchKernelGGL((decode_kernel<T, C, 128>), grid, dim3(256), 0, s, a, plan, part);
+    else hipLaunchKernelGGL((decode_kernel<T, C, 256>), grid, dim3(256), 0, s, a, plan, part);
     OCR_HIP(hipGetLastError());
 }
 

@@ -15,10 +15,14 @@ namespace ocr {
 
 // The page that holds position pos of a sequence (its row of the table, width entries), or -1 where
 // there is none: a position outside the table, an entry that names no page of the pool.
+OCR_HD int32_t page_at(const int32_t *row, uint32_t width, uint32_t pages, uint32_t entry) {
+    if (entry >= width) return -1;
+    const int32_t p = row[entry];
+    return p >= 0 && uint32_t(p) < pages ? p : -1;
+}
 OCR_HD int32_t page_of(const int32_t *row, uint32_t width, uint32_t page, uint32_t pages, int64_t pos) {
     if (pos < 0 || pos >= int64_t(width) * page) return -1;
-    const int32_t p = row[uint32_t(pos) / page];  // within 31 bits: width * page is (check_table)
-    return p >= 0 && uint32_t(p) < pages ? p : -1;
+    return page_at(row, width, pages, uint32_t(pos) / page);  // within 31 bits: width * page is (check_table)
 }
 
 // Vector index of (page p, head, slot) in a pool laid out [pages][heads][page].
