@@ -129,17 +129,17 @@ constexpr float kTinyMax = 1e-30f;
 
 // Over a wavefront, without LDS: each row of 16 lanes, then the rows in order; the last lane has the
 // result.
-template <int Ctrl, int Rows> __device__ inline float dpp_f32(float old, float v) {
-    return __uint_as_float(__builtin_amdgcn_update_dpp(__float_as_uint(old), __float_as_uint(v), Ctrl, Rows, 15, false));
+template <int Ctrl, int Rows, class V> __device__ inline V dpp(V old, V v) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, old), __builtin_bit_cast(int, v), Ctrl, Rows, 15, false));
 }
-template <class Op> __device__ inline float wave_reduce(float v, float none, Op &&op) {
-    v = op(v, dpp_f32<0x111, 15>(none, v));  // from 1, 2, 4, 8 lanes before
-    v = op(v, dpp_f32<0x112, 15>(none, v));
-    v = op(v, dpp_f32<0x114, 15>(none, v));
-    v = op(v, dpp_f32<0x118, 15>(none, v));
-    v = op(v, dpp_f32<0x142, 10>(none, v));  // a row's last lane to the next row (rows 1 and 3)
-    v = op(v, dpp_f32<0x143, 12>(none, v));  // lane 31 to rows 2 and 3
-    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 63));
+template <class V, class Op> __device__ inline V wave_reduce(V v, V none, Op &&op) {
+    v = op(v, dpp<0x111, 15>(none, v));  // from 1, 2, 4, 8 lanes before
+    v = op(v, dpp<0x112, 15>(none, v));
+    v = op(v, dpp<0x114, 15>(none, v));
+    v = op(v, dpp<0x118, 15>(none, v));
+    v = op(v, dpp<0x142, 10>(none, v));  // a row's last lane to the next row (rows 1 and 3)
+    v = op(v, dpp<0x143, 12>(none, v));  // lane 31 to rows 2 and 3
+    return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 __device__ inline float wave_max(float v) {
     return wave_reduce(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
@@ -161,8 +161,7 @@ template <int W, class V, class Op> __device__ inline V group_reduce(V v, Op &&o
     return v;
 }
 __device__ inline int wave_max_i(int v) {
-    for (int o = 32; o; o >>= 1) v = max(v, __shfl_xor(v, o));
-    return __builtin_amdgcn_readfirstlane(v);
+    return wave_reduce(v, int(0x80000000), [](int a, int b) { return max(a, b); });
 }
 __device__ inline int wave_min_i(int v) { return -1 - wave_max_i(-1 - v); }
 
