@@ -152,7 +152,9 @@ template <class T, int N> __device__ inline Some<T, N> some_of(const float *x) {
 // `each` tokens a workgroup, W lanes a vector. The tokens' turns and places are looked up once for
 // all heads; a group of lanes takes a vector after the other, the next two on their way. A lane has
 // two fours of a vector: those that it rotates with each other where pairs are halves apart, two
-// neighbours otherwise. A prompt of 23 600 tokens of 48 bfloat16 heads of 128 into e4m3.
+// neighbours otherwise. A prompt of 23 600 tokens of 48 bfloat16 heads of 128 into e4m3: 533 MB in
+// 115 us, 4.6 TB/s (a large copy reaches 5.2); with the rotation's other half from a neighbouring
+// lane and exact divisions 157, bound by vector instructions.
 template <class T, class O, class C, int W> __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int each) {
     __shared__ __align__(16) float2 s_turn[kAppendTokens][128];
     __shared__ __align__(16) float s_norm[2][8 * W];
@@ -295,7 +297,7 @@ template <class C, class O> __global__ __launch_bounds__(256) void read_row_kern
 }
 
 // kReadTokens positions of a sequence a workgroup, W lanes a vector, two vectors' keys and values on
-// their way at a time.
+// their way at a time. Eight prompts of 4096, 8 heads of 128 from e4m3: 182 MB in 38 us, 4.8 TB/s.
 template <class C, class O, int W> __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
     __shared__ int64_t s_vec[kReadTokens];
     const int tid = threadIdx.x, c = tid % W, dim = a.kv.dim, heads = a.kv.heads;
@@ -342,7 +344,8 @@ template <class C, class O, int W> __global__ __launch_bounds__(256) void read_k
 }
 
 // One workgroup a (sequence, head): the head's part of a copied page, the first also the table's row.
-// P: what a thread copies at once.
+// P: what a thread copies at once. 512 beams, 64-position pages of 4 bfloat16 heads of 128: 12 us, 4.2
+// TB/s of the copies; one workgroup a sequence and bytes: 127.
 template <class P> __global__ __launch_bounds__(256) void fork_kernel(ForkArgs a) {
     const uint32_t r = blockIdx.x, h = blockIdx.y, w = r % a.beams, g = r - w;
     const Fork f = fork_of(a.parents + g, a.beams, w, a.lens + g, a.table.width, a.kv.page);

@@ -5,6 +5,9 @@
 // its (up to 16) query heads, and the parts of a sequence are joined afterwards. Products run on the
 // matrix cores, 16 queries wide, with keys as rows: S^T = K Q^T, O^T = V^T P^T. A lane of the first's
 // result holds four keys of one query, which is what the second takes from it as it is.
+// 4 sequences of 131 072 and less over 8 heads of 128 in e4m3 (981 MB): 186 us with the join, 5.3
+// TB/s, as fast as a large copy. 144 of up to 700 in int8 (71 MB): 27 us; of those 4 pass before the
+// first keys are asked for, and the longest sequences end 10 after the median.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
