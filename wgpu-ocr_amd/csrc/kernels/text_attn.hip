@@ -54,23 +54,23 @@ template <class T> __global__ __launch_bounds__(64) void attention_row_kernel(At
 // What scores go through besides the scale: nothing, the cap, or the distance's bias and perhaps the cap.
 enum Scores { kPlain, kCapped, kAny };
 
-// cap tanh(s / cap) of unscaled scores as s times a polynomial of their squares, which lasts to half
-// the cap: tanh(y) / y by powers of y^2, interpolated at the Chebyshev points of [0, 1/4], off by
-// 2^-25. In units of log2; the exponential's and the reciprocal's way takes half again as long.
+// cap tanh(s / cap) of unscaled scores as s times a polynomial of their squares, which lasts to 0.35
+// of the cap: tanh(y) / y by powers of y^2, interpolated at the Chebyshev points of [0, 0.35^2], off
+// by 2^-24. In units of log2; the exponential's and the reciprocal's way takes half again as long.
 struct SmallCap {
-    float k[5], most;
+    float k[4], most;
     __device__ SmallCap(float scale, float cap) {
         const float y = scale / cap, t = y * y;
         k[0] = scale * 1.4426950408889634f;
-        const float part[5] = {1.f, -0.3333306908607483f, 0.133247509598732f, -0.05298423767089844f, 0.017131345346570015f};
+        const float part[4] = {1.f, -0.3333241939544678f, 0.13295751810073853f, -0.04895563796162605f};
         float power = k[0];
 #pragma unroll
-        for (int e = 1; e < 5; e++) power *= t, k[e] = part[e] * power;
-        most = y < 1e3f ? 0.5f / y : -1.f;  // beyond, the powers leave float32
+        for (int e = 1; e < 4; e++) power *= t, k[e] = part[e] * power;
+        most = y < 1e3f ? 0.35f / y : -1.f;  // beyond, the powers leave float32
     }
     __device__ float factor(float s) const {
         const float t = s * s;
-        return __fmaf_rn(__fmaf_rn(__fmaf_rn(__fmaf_rn(k[4], t, k[3]), t, k[2]), t, k[1]), t, k[0]);
+        return __fmaf_rn(__fmaf_rn(__fmaf_rn(k[3], t, k[2]), t, k[1]), t, k[0]);
     }
 };
 
@@ -91,7 +91,7 @@ template <class T, int DP, Scores KIND, int QW> __global__ __launch_bounds__(256
     __shared__ int s_lo[4], s_hi[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     const int qw = wave % QW, part = wave / QW * KB * 32;  // its queries, the first of its keys of a tile
-    const HeadTile w = head_tile(blockIdx.x, tiles, a.q_heads, a.kv_heads);
+    const HeadTile w = head_tile(blockIdx.x, tiles, a.q_heads, a.kv_heads, PW == 128 ? 32 : 0);
     if (w.head < 0) return;
     const int h = w.head, hk = h / int(a.q_heads / a.kv_heads), dim = a.dim;
     const int i = w.tile * (32 * QW) + 32 * qw + (lane & 31);
