@@ -284,6 +284,41 @@ def test_decode_of_what_is_not_a_number(ctx):
     close(got[fine], want[fine], size[fine], top, EPS["f16"], 3)
 
 
+def test_largest_bfloat16_values(ctx):
+    """Values near the type's largest: their weighted means are, the sums on the way must be."""
+    g = gen(25)
+    n, dim, page = 120, 64, 16
+    q, k = (rn(g, n, h, dim).bfloat16().cuda() for h in (4, 1))
+    v = ((0.5 + 0.4 * torch.rand(n, 1, dim, generator=g)) * 3.3e38 / n).bfloat16()
+    v[:60] = -v[:60]
+    v = v.cuda()
+    got = attend(ctx, q, k, v)
+    want, size, top = plain.attention(host(q), host(k), host(v), plain.key_ranges(n, None, None), dim ** -0.5)
+    close(got / 1e36, want / 1e36, size / 1e36, top, EPS["bf16"])
+    pages = -(-n // page)
+    mem = [torch.zeros(pages, 1, page, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2)] + [None, None]
+    for m, x in zip(mem, (k, v)):
+        m.view(-1, dim)[:n] = x[:, 0]
+    cache = ocrhip.KvCache(ctx, pages, page, 1, dim, "bf16", memory=mem)
+    got = decode(ctx, cache, [list(range(pages))], [n], q[-1:])
+    close(got / 1e36, want[-1:] / 1e36, size[-1:] / 1e36, top, EPS["bf16"], 3)
+
+
+def test_read_past_a_grid(ctx):
+    """More pieces of sequences than a launch has workgroups."""
+    rows, most, dim = 2 ** 22 + 5, 3, 8
+    mem = [torch.arange(2 * 4 * dim, dtype=torch.float32).view(2, 1, 4, dim).half().cuda() for _ in range(2)] + [None, None]
+    cache = ocrhip.KvCache(ctx, 2, 4, 1, dim, "f16", memory=mem)
+    table = (torch.arange(rows, device="cuda", dtype=torch.int32) % 2)[:, None].contiguous()
+    lens = torch.full((rows,), 2, dtype=torch.int32, device="cuda")
+    k, v = (torch.full((rows, most, 1, dim), 9.0, dtype=torch.float16, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    cache.read(table, lens, k, v)
+    ctx.synchronize()
+    want = torch.cat([mem[0][:, 0, :2], torch.zeros(2, 1, dim, device="cuda", dtype=torch.float16)], 1)[table[:, 0].long()]
+    assert torch.equal(k[:, :, 0], want) and torch.equal(v, k)
+
+
 @pytest.mark.parametrize("fmt", ["i8", "f16"])
 def test_pools_past_32_bits(ctx, fmt):
     """Vectors whose first byte is more than 2^32 into the pool: written, read and attended to."""

@@ -243,7 +243,7 @@ template <class T, int DP, Scores KIND, int QW> __global__ __launch_bounds__(256
             for (int b = 0; b < NB; b++) o[b] *= f;
             m = mn;
         }
-        const float ref = m == -INFINITY ? 0.f : m - kLift;
+        const float ref = m == -INFINITY ? 0.f : m - lift<T>;
         tvec p[KB][2];
 #pragma unroll
         for (int t = 0; t < KB; t++)

@@ -279,20 +279,22 @@ template <class T, class O, class C, int W> __global__ __launch_bounds__(256) vo
 // Vectors that are no whole eights: one workgroup a position of a sequence.
 template <class C, class O> __global__ __launch_bounds__(256) void read_row_kernel(ReadArgs a) {
     const int dim = a.kv.dim, heads = a.kv.heads;
-    const int64_t pos = blockIdx.x, seq = blockIdx.y;
-    const bool there = pos < clamp_len(a.lens[seq], a.table.width, a.kv.page);
-    const int page = there ? page_of(a.table.p + seq * a.table.width, a.table.width, a.kv.page, a.kv.pages, pos) : -1;
-    const int64_t out = (seq * a.most + pos) * heads * dim;
-    for (int i = threadIdx.x; i < heads * dim; i += 256) {
-        float k = 0.f, v = 0.f;
-        if (page >= 0) {
-            const int64_t slot = slot_of(page, heads, a.kv.page, i / dim, pos % a.kv.page);
-            k = to_f32(static_cast<const C *>(a.kv.k)[slot * dim + i % dim]);
-            v = to_f32(static_cast<const C *>(a.kv.v)[slot * dim + i % dim]);
-            if constexpr (scaled<C>) k *= a.kv.k_scale[slot], v *= a.kv.v_scale[slot];
+    for (int64_t block = blockIdx.x; block < int64_t(a.most) * a.table.rows; block += gridDim.x) {
+        const int64_t seq = block / a.most, pos = block - seq * a.most;
+        const bool there = pos < clamp_len(a.lens[seq], a.table.width, a.kv.page);
+        const int page = there ? page_of(a.table.p + seq * a.table.width, a.table.width, a.kv.page, a.kv.pages, pos) : -1;
+        const int64_t out = block * heads * dim;
+        for (int i = threadIdx.x; i < heads * dim; i += 256) {
+            float k = 0.f, v = 0.f;
+            if (page >= 0) {
+                const int64_t slot = slot_of(page, heads, a.kv.page, i / dim, pos % a.kv.page);
+                k = to_f32(static_cast<const C *>(a.kv.k)[slot * dim + i % dim]);
+                v = to_f32(static_cast<const C *>(a.kv.v)[slot * dim + i % dim]);
+                if constexpr (scaled<C>) k *= a.kv.k_scale[slot], v *= a.kv.v_scale[slot];
+            }
+            static_cast<O *>(a.k)[out + i] = O(k);
+            static_cast<O *>(a.v)[out + i] = O(v);
         }
-        static_cast<O *>(a.k)[out + i] = O(k);
-        static_cast<O *>(a.v)[out + i] = O(v);
     }
 }
 
@@ -301,45 +303,47 @@ template <class C, class O> __global__ __launch_bounds__(256) void read_row_kern
 template <class C, class O, int W> __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
     __shared__ int64_t s_vec[kReadTokens];
     const int tid = threadIdx.x, c = tid % W, dim = a.kv.dim, heads = a.kv.heads;
-    const uint32_t blocks = (a.most + kReadTokens - 1) / kReadTokens;
-    const int64_t seq = blockIdx.x / blocks, p0 = int64_t(blockIdx.x % blocks) * kReadTokens;
-    const int n = int(min<int64_t>(kReadTokens, a.most - p0)), items = n * heads;
-    if (tid < n) {
-        int64_t vec = -1;
-        if (p0 + tid < clamp_len(a.lens[seq], a.table.width, a.kv.page)) {
-            const int32_t page = page_of(a.table.p + seq * a.table.width, a.table.width, a.kv.page, a.kv.pages, p0 + tid);
-            if (page >= 0) vec = slot_of(page, heads, a.kv.page, 0, uint32_t(p0 + tid) % a.kv.page);
-        }
-        s_vec[tid] = vec;
-    }
-    __syncthreads();
-    if (8 * c >= dim) return;
+    const int64_t blocks = (int64_t(a.most) + kReadTokens - 1) / kReadTokens;
     constexpr int G = 256 / W;
-    for (int item = tid / W; item < items; item += 2 * G) {
-        Some<C, 8> raw[2][2];
-        float scale[2][2];
-        bool there[2];
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int i = min(item + u * G, items - 1), p = i / heads;
-            there[u] = s_vec[p] >= 0;
-            const int64_t vec = there[u] ? s_vec[p] + int64_t(i - p * heads) * a.kv.page : 0;
-            raw[u][0] = load_some<C, 8>(static_cast<const C *>(a.kv.k) + vec * dim + 8 * c);
-            raw[u][1] = load_some<C, 8>(static_cast<const C *>(a.kv.v) + vec * dim + 8 * c);
-            scale[u][0] = scaled<C> ? a.kv.k_scale[vec] : 1.f;
-            scale[u][1] = scaled<C> ? a.kv.v_scale[vec] : 1.f;
+    for (int64_t block = blockIdx.x; block < blocks * a.table.rows; block += gridDim.x) {
+        const int64_t seq = block / blocks, p0 = (block - seq * blocks) * kReadTokens;
+        const int n = int(min<int64_t>(kReadTokens, a.most - p0)), items = n * heads;
+        if (tid < n) {
+            int64_t vec = -1;
+            if (p0 + tid < clamp_len(a.lens[seq], a.table.width, a.kv.page)) {
+                const int32_t page = page_of(a.table.p + seq * a.table.width, a.table.width, a.kv.page, a.kv.pages, p0 + tid);
+                if (page >= 0) vec = slot_of(page, heads, a.kv.page, 0, uint32_t(p0 + tid) % a.kv.page);
+            }
+            s_vec[tid] = vec;
         }
+        __syncthreads();
+        for (int item = tid / W; item < items && 8 * c < dim; item += 2 * G) {
+            Some<C, 8> raw[2][2];
+            float scale[2][2];
+            bool there[2];
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            if (item + u * G >= items) break;
+            for (int u = 0; u < 2; u++) {
+                const int i = min(item + u * G, items - 1), p = i / heads;
+                there[u] = s_vec[p] >= 0;
+                const int64_t vec = there[u] ? s_vec[p] + int64_t(i - p * heads) * a.kv.page : 0;
+                raw[u][0] = load_some<C, 8>(static_cast<const C *>(a.kv.k) + vec * dim + 8 * c);
+                raw[u][1] = load_some<C, 8>(static_cast<const C *>(a.kv.v) + vec * dim + 8 * c);
+                scale[u][0] = scaled<C> ? a.kv.k_scale[vec] : 1.f;
+                scale[u][1] = scaled<C> ? a.kv.v_scale[vec] : 1.f;
+            }
 #pragma unroll
-            for (int y = 0; y < 2; y++) {
-                float x[8];
+            for (int u = 0; u < 2; u++) {
+                if (item + u * G >= items) break;
 #pragma unroll
-                for (int k = 0; k < 8; k++) x[k] = there[u] ? value_at(raw[u][y], k) * scale[u][y] : 0.f;
-                store_some(static_cast<O *>(y ? a.v : a.k) + ((seq * a.most + p0) * heads + item + u * G) * dim + 8 * c, some_of<O, 8>(x));
+                for (int y = 0; y < 2; y++) {
+                    float x[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) x[k] = there[u] ? value_at(raw[u][y], k) * scale[u][y] : 0.f;
+                    store_some(static_cast<O *>(y ? a.v : a.k) + ((seq * a.most + p0) * heads + item + u * G) * dim + 8 * c, some_of<O, 8>(x));
+                }
             }
         }
+        __syncthreads();
     }
 }
 
@@ -420,13 +424,18 @@ void launch_append(const AppendArgs &a, hipStream_t s) {
 void launch_read(const ReadArgs &a, hipStream_t s) {
     const double values = 2.0 * a.table.rows * a.most * a.kv.heads * a.kv.dim;
     ProbeScope probe("text_read", s, values, values * (type_bytes(a.kv.type) + 2));
-    const int64_t blocks = (int64_t(a.most) + kReadTokens - 1) / kReadTokens * a.table.rows;
+    // Workgroups go on to further positions past what a grid holds.
+    const auto grid = [](int64_t blocks) { return dim3(unsigned(std::min<int64_t>(blocks, 1 << 22))); };
     with_cache(a.kv.type, [&](auto c) {
         with_type16(a.type, [&](auto o) {
             using C = decltype(c);
             using O = decltype(o);
-            if (a.kv.dim % 8 || blocks > 0x7fffff) hipLaunchKernelGGL((read_row_kernel<C, O>), dim3(a.most, a.table.rows), dim3(256), 0, s, a);
-            else with_lanes(a.kv.dim, [&](auto w) { hipLaunchKernelGGL((read_kernel<C, O, decltype(w)::value>), dim3(unsigned(blocks)), dim3(256), 0, s, a); });
+            if (a.kv.dim % 8) {
+                hipLaunchKernelGGL((read_row_kernel<C, O>), grid(int64_t(a.most) * a.table.rows), dim3(256), 0, s, a);
+                return;
+            }
+            const int64_t blocks = (int64_t(a.most) + kReadTokens - 1) / kReadTokens * a.table.rows;
+            with_lanes(a.kv.dim, [&](auto w) { hipLaunchKernelGGL((read_kernel<C, O, decltype(w)::value>), grid(blocks), dim3(256), 0, s, a); });
         });
     });
     OCR_HIP(hipGetLastError());

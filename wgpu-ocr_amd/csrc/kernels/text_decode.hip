@@ -260,7 +260,7 @@ template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 
                 for (int b = 0; b < NB; b++) o[b] *= f;
                 m = mn;
             }
-            const float ref = m == -INFINITY ? 0.f : m - kLift;
+            const float ref = m == -INFINITY ? 0.f : m - lift<M>;
             mvec p;
 #pragma unroll
             for (int t = 0; t < 2; t++) {
@@ -293,11 +293,12 @@ template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    // True scale: the lift taken out with room for the sums of the largest values.
-    const float back = scaled<C> ? vtop * 0x1p-14f : 0x1p-14f;
+    // The weights' most taken out, and the values' scales put in.
+    constexpr float most = lift<M> > 0.f ? 0x1p-14f : 1.f;
+    const float back = scaled<C> ? vtop * most : most;
 #pragma unroll
     for (int b = 0; b < NB; b++) o[b] *= back;
-    l *= 0x1p-14f;
+    l *= most;
     // Waves 2 and 3 hand their sums to 0 and 1, then 1 to 0.
     float *const s_o = reinterpret_cast<float *>(s_mem);
 #pragma unroll

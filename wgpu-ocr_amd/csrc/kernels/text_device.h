@@ -104,10 +104,12 @@ template <class C> __device__ inline f16x8 widen8(uint32_t a, uint32_t b) {
     return f16x8{x[0][0], x[0][1], x[1][0], x[1][1], x[2][0], x[2][1], x[3][0], x[3][1]};
 }
 
-// Weights are held as 2^6 times their value relative to the maximum's reference, which may lie up to
-// 2^8 under the true maximum: at most 2^14, within float16, and 2^-24 (its last step) is 2^-30 of
-// the reference. The factor is common to the sums and leaves with them.
-constexpr float kLift = 6.f, kSlack = 8.f;
+// A softmax's reference may lie up to 2^8 under the true maximum before the sums are scaled again.
+// Weights in float16 are held as 2^6 times their value relative to it: at most 2^14, within the type,
+// and its last step 2^-24 is 2^-30 of the reference. bfloat16 has the range to hold them under one,
+// which leaves the sums that of their values. The factor is common to the sums and leaves with them.
+constexpr float kSlack = 8.f;
+template <class M> constexpr float lift = std::is_same_v<M, f16> ? 6.f : -kSlack;
 
 // 2^x; results under the normal range are zero.
 __device__ inline float exp2_f32(float x) { return __builtin_amdgcn_exp2f(x); }

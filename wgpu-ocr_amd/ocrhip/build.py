@@ -49,8 +49,11 @@ def _tensors() -> None:
     """ocrhip._tensors, the text decoder's calls on torch tensors (csrc/python/tensors.cpp)."""
     import sysconfig
 
-    import torch
-    from torch.utils import cpp_extension
+    try:
+        import torch
+        from torch.utils import cpp_extension
+    except ImportError:  # the library needs none of it, and without torch nothing here calls it
+        return
 
     out = os.path.join(PKG, "_tensors.so")
     tmp = out + f".tmp{os.getpid()}"
