@@ -122,6 +122,7 @@ template <class T, int DP, Scores KIND, int QW> __global__ __launch_bounds__(256
 #pragma unroll
     for (int x = 1; x < 4; x++) jlo = min(jlo, s_lo[x]), jhi = max(jhi, s_hi[x]);
     jlo = __builtin_amdgcn_readfirstlane(jlo), jhi = __builtin_amdgcn_readfirstlane(jhi);
+    if (jlo >= jhi) jlo = jhi = 0;  // nothing is seen: jlo is the largest int, and tiles on from it none
 
     // Copies: a lane's pieces of a tile lie in LDS in order, each row's exchanged so that the reads
     // below touch every bank (swap_of), by the choice of the piece that the lane copies.
