@@ -156,7 +156,7 @@ template <class T, int N> __device__ inline Some<T, N> some_of(const float *x) {
 // 115 us, 4.6 TB/s (a large copy reaches 5.2); with the rotation's other half from a neighbouring
 // lane and exact divisions 157, bound by vector instructions.
 template <class T, class O, class C, int W> __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int each) {
-    __shared__ __align__(16) float2 s_turn[kAppendTokens][128];
+    __shared__ __align__(16) float s_cos[kAppendTokens][128], s_sin[kAppendTokens][128];
     __shared__ __align__(16) float s_norm[2][8 * W];
     __shared__ int64_t s_vec[kAppendTokens];  // head 0's vector in the pool, negative: none
     const int tid = threadIdx.x, c = tid % W, dim = a.kv.dim, heads = a.kv.heads, all = a.q_heads + 2 * heads, half = a.rot / 2;
@@ -191,7 +191,8 @@ template <class T, class O, class C, int W> __global__ __launch_bounds__(256) vo
     }
     for (int x = tid; x < n * half; x += 256) {
         const int t = x / half, i = x - t * half;
-        s_turn[t][i] = turn_of(a.pos[t0 + t], i, a.rot, a.log2_theta);
+        const float2 r = turn_of(a.pos[t0 + t], i, a.rot, a.log2_theta);
+        s_cos[t][i] = r.x, s_sin[t][i] = r.y;
     }
     if (tid < n) {
         const int seq = a.seq[t0 + tid], pos = a.pos[t0 + tid];
@@ -235,8 +236,7 @@ template <class T, class O, class C, int W> __global__ __launch_bounds__(256) vo
                 for (int k = 0; k < 8; k++) x[k] = x[k] * r * (k < 4 ? w0[k] : w1[k - 4]);
             }
             if (turns) {
-                const f32x4 r01 = *reinterpret_cast<const f32x4 *>(&s_turn[t][4 * c]), r23 = *reinterpret_cast<const f32x4 *>(&s_turn[t][4 * c + 2]);
-                const float cs[4] = {r01[0], r01[2], r23[0], r23[2]}, sn[4] = {r01[1], r01[3], r23[1], r23[3]};
+                const f32x4 cs = *reinterpret_cast<const f32x4 *>(&s_cos[t][4 * c]), sn = *reinterpret_cast<const f32x4 *>(&s_sin[t][4 * c]);
                 auto turn = [](float &p, float &q, float c, float s) {
                     const float y = p;
                     p = y * c - q * s;
