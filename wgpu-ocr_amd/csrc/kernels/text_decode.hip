@@ -65,7 +65,7 @@ constexpr int kPartTail = 4;  // keeps the rows' 16-byte alignment
 
 // T: the queries' type, C: the cache's; products of 8-bit caches in float16, which holds their codes
 // exactly.
-template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 3 : 1) void decode_kernel(DecodeArgs a, DecodePlan plan, float *part) {
+template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void decode_kernel(DecodeArgs a, DecodePlan plan, float *part) {
     using M = std::conditional_t<scaled<C>, f16, C>;
     typedef M mvec __attribute__((ext_vector_type(8)));
     constexpr int NU = DP * int(sizeof(C)) / 64;    // 16-byte pieces of a vector that a lane holds
