@@ -94,6 +94,11 @@ template <class T, class O, class C> __global__ __launch_bounds__(64) void appen
         if (lane + 64 * u < dim) dst[lane + 64 * u] = code_of<C>(x[u] * inv);
 }
 
+// Outputs that the level-two caches (eight of 4 MiB) cannot hold are stored past them: what is left
+// there at a kernel's end is written out before the next one starts. 144 sequences' 88 MB read back:
+// 25 us for the step, 33 with ordinary stores; a prompt's 380 MB 149 and 157.
+constexpr double kHeld = 32.0 * (1 << 20);
+
 // N (four or eight) values at p, which lies on no more than a value's size.
 template <class T, int N> struct Some {
     uint32_t x[N * sizeof(T) / 4];
@@ -113,12 +118,18 @@ template <class T, int N> __device__ inline Some<T, N> load_some(const T *p) {
     }
     return r;
 }
-template <class T, int N> __device__ inline void store_some(T *p, const Some<T, N> &r) {
+template <class T, int N> __device__ inline void store_some(T *p, const Some<T, N> &r, bool past) {
     using L = loose_of<T, N>;
     typename L::type y;
 #pragma unroll
     for (int e = 0; e < L::words; e++) y[e] = r.x[e];
-    *reinterpret_cast<typename L::type *>(p) = y;
+    if (past) {
+        asm volatile("" ::: "memory");  // on both sides: else the compiler makes one ordinary store of the two
+        __builtin_nontemporal_store(y, reinterpret_cast<typename L::type *>(p));
+        asm volatile("" ::: "memory");
+    } else {
+        *reinterpret_cast<typename L::type *>(p) = y;
+    }
 }
 template <class T, int N> __device__ inline float value_at(const Some<T, N> &r, int k) {
     if constexpr (sizeof(T) == 4) return __uint_as_float(r.x[k]);
@@ -155,7 +166,7 @@ template <class T, int N> __device__ inline Some<T, N> some_of(const float *x) {
 // neighbours otherwise. A prompt of 23 600 tokens of 48 bfloat16 heads of 128 into e4m3: 533 MB in
 // 115 us, 4.6 TB/s (a large copy reaches 5.2); with the rotation's other half from a neighbouring
 // lane and exact divisions 157, bound by vector instructions.
-template <class T, class O, class C, int W> __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int each) {
+template <class T, class O, class C, int W> __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int each, bool past) {
     __shared__ __align__(16) float s_cos[kAppendTokens][128], s_sin[kAppendTokens][128];
     __shared__ __align__(16) float s_norm[2][8 * W];
     __shared__ int64_t s_vec[kAppendTokens];  // head 0's vector in the pool, negative: none
@@ -205,10 +216,10 @@ template <class T, class O, class C, int W> __global__ __launch_bounds__(256) vo
         using D = std::remove_pointer_t<decltype(dst)>;
         if (!in) return;
         if (apart) {
-            store_some(dst + at[0], some_of<D, 4>(x));
-            store_some(dst + at[1], some_of<D, 4>(x + 4));
+            store_some(dst + at[0], some_of<D, 4>(x), past);
+            store_some(dst + at[1], some_of<D, 4>(x + 4), past);
         } else {
-            store_some(dst + at[0], some_of<D, 8>(x));
+            store_some(dst + at[0], some_of<D, 8>(x), past);
         }
     };
     for (; item.t < n; item = after(item)) {
@@ -300,7 +311,7 @@ template <class C, class O> __global__ __launch_bounds__(256) void read_row_kern
 
 // kReadTokens positions of a sequence a workgroup, W lanes a vector, two vectors' keys and values on
 // their way at a time. Eight prompts of 4096, 8 heads of 128 from e4m3: 182 MB in 38 us, 4.8 TB/s.
-template <class C, class O, int W> __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
+template <class C, class O, int W> __global__ __launch_bounds__(256) void read_kernel(ReadArgs a, bool past) {
     __shared__ int64_t s_vec[kReadTokens];
     const int tid = threadIdx.x, c = tid % W, dim = a.kv.dim, heads = a.kv.heads;
     const int64_t blocks = (int64_t(a.most) + kReadTokens - 1) / kReadTokens;
@@ -339,7 +350,7 @@ template <class C, class O, int W> __global__ __launch_bounds__(256) void read_k
                     float x[8];
 #pragma unroll
                     for (int k = 0; k < 8; k++) x[k] = there[u] ? value_at(raw[u][y], k) * scale[u][y] : 0.f;
-                    store_some(static_cast<O *>(y ? a.v : a.k) + ((seq * a.most + p0) * heads + item + u * G) * dim + 8 * c, some_of<O, 8>(x));
+                    store_some(static_cast<O *>(y ? a.v : a.k) + ((seq * a.most + p0) * heads + item + u * G) * dim + 8 * c, some_of<O, 8>(x), past);
                 }
             }
         }
@@ -402,6 +413,7 @@ void launch_append(const AppendArgs &a, hipStream_t s) {
     const bool eights = a.kv.dim % 8 == 0 && (a.adjacent || a.rot % 8 == 0);
     // Four tokens a workgroup share their lookups once that leaves work for every compute unit.
     const int each = a.n >= 4096 ? kAppendTokens : 1;
+    const bool past = double(a.n) * a.kv.dim * (2.0 * a.q_heads + 2.0 * a.kv.heads * type_bytes(a.kv.type)) > kHeld;
     with_type(a.type, [&](auto t) {
         with_type16(a.out_type, [&](auto o) {
             with_cache(a.kv.type, [&](auto c) {
@@ -413,7 +425,7 @@ void launch_append(const AppendArgs &a, hipStream_t s) {
                     return;
                 }
                 with_lanes(a.kv.dim, [&](auto w) {
-                    hipLaunchKernelGGL((append_kernel<T, O, C, decltype(w)::value>), dim3((a.n + each - 1) / each), dim3(256), 0, s, a, each);
+                    hipLaunchKernelGGL((append_kernel<T, O, C, decltype(w)::value>), dim3((a.n + each - 1) / each), dim3(256), 0, s, a, each, past);
                 });
             });
         });
@@ -435,7 +447,7 @@ void launch_read(const ReadArgs &a, hipStream_t s) {
                 return;
             }
             const int64_t blocks = (int64_t(a.most) + kReadTokens - 1) / kReadTokens * a.table.rows;
-            with_lanes(a.kv.dim, [&](auto w) { hipLaunchKernelGGL((read_kernel<C, O, decltype(w)::value>), grid(blocks), dim3(256), 0, s, a); });
+            with_lanes(a.kv.dim, [&](auto w) { hipLaunchKernelGGL((read_kernel<C, O, decltype(w)::value>), grid(blocks), dim3(256), 0, s, a, 2 * values > kHeld); });
         });
     });
     OCR_HIP(hipGetLastError());
