@@ -99,7 +99,9 @@ template <class T, class O, class C> __global__ __launch_bounds__(64) void appen
 // 25 us for the step, 33 with ordinary stores; a prompt's 380 MB 149 and 157.
 constexpr double kHeld = 32.0 * (1 << 20);
 
-// N (four or eight) values at p, which lies on no more than a value's size.
+// N (four or eight) values at p, which lies on no more than a value's size. ONCE: the caches need not
+// keep them (a prompt's projections: 147 us for writing and reading, 151 without; codes read back so: 32
+// instead of 25 for 144 sequences, whose neighbouring heads share lines).
 template <class T, int N> struct Some {
     uint32_t x[N * sizeof(T) / 4];
 };
@@ -107,12 +109,12 @@ template <class T, int N> struct loose_of {
     static constexpr int words = N * sizeof(T) / 4 < 4 ? N * sizeof(T) / 4 : 4;
     typedef uint32_t type __attribute__((ext_vector_type(words), aligned(sizeof(T))));
 };
-template <class T, int N> __device__ inline Some<T, N> load_some(const T *p) {
+template <class T, int N, bool ONCE = false> __device__ inline Some<T, N> load_some(const T *p) {
     using L = loose_of<T, N>;
     Some<T, N> r;
 #pragma unroll
     for (int k = 0; k < int(N * sizeof(T) / 4) / L::words; k++) {
-        const typename L::type y = reinterpret_cast<const typename L::type *>(p)[k];
+        const typename L::type *from = reinterpret_cast<const typename L::type *>(p) + k, y = ONCE ? __builtin_nontemporal_load(from) : *from;
 #pragma unroll
         for (int e = 0; e < L::words; e++) r.x[L::words * k + e] = y[e];
     }
@@ -192,7 +194,7 @@ template <class T, class O, class C, int W> __global__ __launch_bounds__(256) vo
     const T *const base = static_cast<const T *>(a.qkv) + t0 * a.stride;
     auto load = [&](Item i) {
         const T *src = base + (i.t < n ? i.t * a.stride + uint32_t(i.h * dim) : 0);
-        return Vec{load_some<T, 4>(src + at[0]), load_some<T, 4>(src + at[1])};
+        return Vec{load_some<T, 4, true>(src + at[0]), load_some<T, 4, true>(src + at[1])};
     };
     Item item{tid / W / all, tid / W % all}, ahead = after(item);
     Vec next[2] = {load(item), load(ahead)};
