@@ -165,8 +165,8 @@ template <class T, int N> __device__ inline Some<T, N> some_of(const float *x) {
 // `each` tokens a workgroup, W lanes a vector. The tokens' turns and places are looked up once for
 // all heads; a group of lanes takes a vector after the other, the next two on their way. A lane has
 // two fours of a vector: those that it rotates with each other where pairs are halves apart, two
-// neighbours otherwise. A prompt of 23 600 tokens of 48 bfloat16 heads of 128 into e4m3: 533 MB in
-// 115 us, 4.6 TB/s (a large copy reaches 5.2); with the rotation's other half from a neighbouring
+// neighbours otherwise. A prompt of 23 600 tokens of 48 bfloat16 heads of 128 into e4m3: 532 MB in
+// 119 us, 4.5 TB/s (a large copy reaches 5.2); with the rotation's other half from a neighbouring
 // lane and exact divisions 157, bound by vector instructions.
 template <class T, class O, class C, int W> __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int each, bool past) {
     __shared__ __align__(16) float s_cos[kAppendTokens][128], s_sin[kAppendTokens][128];
@@ -312,7 +312,8 @@ template <class C, class O> __global__ __launch_bounds__(256) void read_row_kern
 }
 
 // kReadTokens positions of a sequence a workgroup, W lanes a vector, two vectors' keys and values on
-// their way at a time. Eight prompts of 4096, 8 heads of 128 from e4m3: 182 MB in 38 us, 4.8 TB/s.
+// their way at a time. Eight prompts of 4096, 8 heads of 128 from e4m3: 181 MB in 43 us, 4.2 TB/s; with
+// ordinary stores 38, and 8 more until the next kernel starts.
 template <class C, class O, int W> __global__ __launch_bounds__(256) void read_kernel(ReadArgs a, bool past) {
     __shared__ int64_t s_vec[kReadTokens];
     const int tid = threadIdx.x, c = tid % W, dim = a.kv.dim, heads = a.kv.heads;

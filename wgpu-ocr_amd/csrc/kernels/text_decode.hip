@@ -5,9 +5,10 @@
 // its (up to 16) query heads, and the parts of a sequence are joined afterwards. Products run on the
 // matrix cores, 16 queries wide, with keys as rows: S^T = K Q^T, O^T = V^T P^T. A lane of the first's
 // result holds four keys of one query, which is what the second takes from it as it is.
-// 4 sequences of 131 072 and less over 8 heads of 128 in e4m3 (981 MB): 186 us with the join, 5.3
-// TB/s, as fast as a large copy. 144 of up to 700 in int8 (71 MB): 27 us; of those 4 pass before the
-// first keys are asked for, and the longest sequences end 10 after the median.
+// 4 sequences of 131 072 and less over 8 heads of 128 in e4m3 (981 MB): 178 us with the join, 5.5
+// TB/s, faster than a large copy. 144 of up to 700 in int8 (71 MB): 24 us; of those 4 pass before the
+// first keys are asked for, and the longest sequences end well after the median. Registers for two
+// wavefronts a SIMD: for three some are spilled (186 and 27 us).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -409,8 +410,8 @@ void launch_decode(Ctx &c, const DecodeArgs &a, hipStream_t s) {
         return;
     }
     // Parts until there are two workgroups for every compute unit; a sequence has as many as its own
-    // length gives work to. 4 sequences of 131 072: 512 workgroups 197 us, 768 the same, 1024 212 to
-    // 230; 144 of 700, 576 workgroups: one part 29 us, two 32 and 4 more for the join.
+    // length gives work to. 4 sequences of 131 072: 256 workgroups 194 us, 384 204, 512 179, 1024
+    // 181; 144 of 700: one part (576) 24 us, two 30.
     constexpr uint64_t kWork = 512;
     const uint64_t heads = uint64_t(a.table.rows) * a.kv.heads * ((a.q_heads / a.kv.heads + 15) / 16);
     const uint64_t most = uint64_t(a.table.width) * a.kv.page;
