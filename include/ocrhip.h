@@ -541,8 +541,8 @@ int ocr_decode_attention_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const o
 /* A step of beam search: logits [groups * beams] rows of vocab values (type OCR_F32, OCR_F16 or
  * OCR_BF16) every stride values, scores [groups][beams]. A continuation (beam w, token t) of a
  * group scores scores[w] + log-softmax(logits of w)[t]; a beam whose finished flag is set keeps its
- * score with token eos and has no other. The best `beams` (at most 32) of each group in order, ties
- * to the lower w * vocab + t: out_scores, parents (w), tokens (t), out_finished (finished, or t ==
+ * score with token eos and has no other. The best `beams` (at most 32) of each group in order of their
+ * float64 scores, equal ones (logits that a large score absorbs among them) by the lower w * vocab + t: out_scores, parents (w), tokens (t), out_finished (finished, or t ==
  * eos; may be NULL), each [groups][beams]. NaN logits weigh nothing, scores that are not
  * finite count as minus infinity. finished may be NULL, eos negative (none) then. out_scores and
  * out_finished may be scores and finished. */

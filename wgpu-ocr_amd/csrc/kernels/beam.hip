@@ -6,7 +6,9 @@
 // second kernel, one workgroup a group and a wavefront a beam, reads only those again. Values order as 32-bit keys
 // (order_of); the beams-th largest of a set of keys is found bit by bit with ballots.
 //
-// Within a beam continuations order by their logits, between beams by float64 scores.
+// Continuations order by their float64 scores, then by beam and token. Within a beam that is the logits'
+// order wherever different logits score differently, which all do but next to nothing beside the log-sum or
+// under a score of 10^9 and more; a row's best are found by their logits, and settle_ties looks for that.
 //
 // 64 groups of 8 beams: the second kernel takes 20 us, 5 to the row's sums, 7 to its best and 2 to
 // the group's; one chain of latencies, on 64 of the compute units.
@@ -35,8 +37,6 @@ __device__ inline uint32_t order_of(float x) {
     const uint32_t u = __float_as_uint(x == x ? x + 0.f : -INFINITY);
     return u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
 }
-constexpr uint32_t kNothing = 0x007fffffu;  // the key of minus infinity
-__device__ inline float value_of(uint32_t key) { return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu)); }
 
 // Eight logits from index i on, all in the row, as they are in memory (rows lie on no more than a
 // logit's size, which global loads take at any width). ONCE: the caches need not keep them, which
@@ -286,6 +286,63 @@ __device__ inline void row_best(const T *row, int vocab, Each &&each, uint32_t t
     for (int i = total + lane; i < want; i += 64) top[i] = 0;  // fewer tokens than beams
 }
 
+// A row's `need` lowest tokens with logits in [lo, hi], of which there are that many: into top, as
+// keys of `hi`.
+template <class T> __device__ inline void lowest_of(const T *row, int vocab, uint32_t lo, uint32_t hi, int need, uint64_t *top) {
+    const int lane = threadIdx.x & 63;
+    const float least = value_of(lo), most = value_of(hi);
+    for (int c = 0, n = 0; c < vocab && n < need; c += kChunk) {
+        float x[4][8];
+        load_chunk(row, c, vocab, x);
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            unsigned mine = 0;  // a bit a logit; what is past the row's end is minus infinity, under every `lo`
+#pragma unroll
+            for (int k = 0; k < 8; k++) mine |= unsigned(x[u][k] >= least && x[u][k] <= most) << k;
+            if (!__ballot(mine)) continue;
+            int before = n, all = n;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const unsigned long long g = __ballot(mine >> k & 1);
+                before += __popcll(g & ((1ull << lane) - 1)), all += __popcll(g);
+            }
+            for (; mine && before < need; mine &= mine - 1, before++)
+                top[before] = uint64_t(hi) << 32 | uint32_t(~(c + kPart * u + 8 * lane + __builtin_ctz(mine)));
+            n = min(all, need);
+        }
+    }
+}
+
+// A row's best `want` (at most 32) keys, found by their logits, brought into the order of scores, then
+// tokens: where different logits score alike the lower tokens come first, those too that are not among
+// the best by logits.
+template <class T> __device__ inline void settle_ties(const T *row, int vocab, double cum, double lse, int want, uint64_t *top) {
+    const int lane = threadIdx.x & 63;
+    const uint64_t mine = lane < want ? top[lane] : 0;
+    const double s = score_of_key(uint32_t(mine >> 32), cum, lse);
+    const uint32_t last = uint32_t(__builtin_amdgcn_readlane(int(mine >> 32), want - 1));
+    const double least = score_of_key(last, cum, lse);
+    // The next logit under the last one's: what scores as that may be anywhere in the row.
+    if (last > kNothing && score_of_key(last - 1, cum, lse) == least) {
+        const int first = __builtin_ctzll(__ballot(lane < want && s == least));
+        const uint32_t hi = uint32_t(__builtin_amdgcn_readlane(int(mine >> 32), first));
+        lowest_of(row, vocab, lowest_alike(last, cum, lse), hi, want - first, top + first);
+        __builtin_amdgcn_wave_barrier();
+    }
+    const uint64_t key = lane < want ? top[lane] : 0;
+    const uint64_t next = __shfl_down(key, 1);
+    const double after = __shfl_down(s, 1);  // the scores in order are what they were
+    if (!__any(lane + 1 < want && s == after && uint32_t(key) < uint32_t(next))) return;  // ~token: the lower is the larger
+    int place = 0;
+    for (int j = 0; j < want; j++) {
+        const double d = __shfl(s, j);
+        const uint32_t t = uint32_t(__shfl(int(uint32_t(key)), j));
+        place += d > s || (d == s && t > uint32_t(key));
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (lane < want) top[place] = key;
+}
+
 template <class T, bool ONE> __global__ __launch_bounds__(512) void beam_groups_kernel(BeamArgs a, int blocks, int size, const Block *stats) {
     __shared__ uint32_t s_list[8][kList];
     __shared__ uint64_t s_keys[8][kList], s_top[kMostBeams * kMostBeams];
@@ -368,6 +425,8 @@ template <class T, bool ONE> __global__ __launch_bounds__(512) void beam_groups_
                 __builtin_amdgcn_wave_barrier();
                 row_best(row, v, [&](auto &&f) { each_part(row, v, size, s_sel[wave], words, f); }, t, want, s_list[wave], s_keys[wave], top);
             }
+            __builtin_amdgcn_wave_barrier();
+            settle_ties(row, v, cum, lse, want, top);
             for (int i = want + lane; i < w; i += 64) top[i] = 0;
         } else {
             // A finished beam's only continuation is its end; what scores nothing comes in order.
@@ -381,8 +440,7 @@ template <class T, bool ONE> __global__ __launch_bounds__(512) void beam_groups_
         for (int i = lane; i < w; i += 64) {
             double s = -INFINITY;
             if (open) {
-                const float x = value_of(uint32_t(top[i] >> 32));
-                if (top[i] && x > -INFINITY) s = cum + (double(x) - lse);
+                if (top[i]) s = score_of_key(uint32_t(top[i] >> 32), cum, lse);
             } else if (top[i] >> 32) {
                 s = cum;
             }
@@ -392,22 +450,14 @@ template <class T, bool ONE> __global__ __launch_bounds__(512) void beam_groups_
     }
     __syncthreads();
     // The group's best by counting those before each, list by list: the lists are in order, ties go
-    // to the lower beam, then the lower token.
+    // to the lower beam, then the lower token. No two count alike, so every place gets one.
     for (int c = threadIdx.x; c < w * w; c += blockDim.x) s_place[c] = 0;
     __syncthreads();
     for (int x = threadIdx.x; x < w * w * w; x += blockDim.x) {
-        const int o = x / (w * w), c = x - o * w * w, beam = c / w, at = int(~uint32_t(s_top[c]));
+        const int o = x / (w * w), c = x - o * w * w, beam = c / w;
         if (!s_top[c]) continue;
-        const double s = s_score[c];
-        int lo = 0, hi = w;
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            const double d = s_score[o * w + mid];
-            const uint64_t k = s_top[o * w + mid];
-            if (k && (d > s || (d == s && (o < beam || (o == beam && int(~uint32_t(k)) < at))))) lo = mid + 1;
-            else hi = mid;
-        }
-        if (lo) atomicAdd(&s_place[c], lo);
+        const int before = o == beam ? c - beam * w : before_other(s_score + o * w, want, s_score[c], o < beam);
+        if (before) atomicAdd(&s_place[c], before);
     }
     __syncthreads();
     // All of the group's inputs have been read but the flags of the winners.

@@ -87,6 +87,39 @@ OCR_HD Fork fork_of(const int32_t *parents, uint32_t beams, uint32_t w, const in
     return f;
 }
 
+// Logits as 32-bit keys that order as they do (the zeros next to each other); minus infinity's key.
+constexpr uint32_t kNothing = 0x007fffffu;
+OCR_HD float value_of(uint32_t key) { return __builtin_bit_cast(float, key ^ (key >> 31 ? 0x80000000u : 0xffffffffu)); }
+
+// A continuation's score: the beam's, and the logit of this key less the row's log-sum.
+OCR_HD double score_of_key(uint32_t key, double cum, double lse) {
+    return key > kNothing ? cum + (double(value_of(key)) - lse) : -__builtin_inf();
+}
+// The least key whose score is that of `key` (over minus infinity's): scores rise with the keys, but
+// not every step, since a large score absorbs logits, and a log-sum small ones.
+OCR_HD uint32_t lowest_alike(uint32_t key, double cum, double lse) {
+    const double s = score_of_key(key, cum, lse);
+    uint32_t under = kNothing;
+    while (key - under > 1) {
+        const uint32_t mid = under + (key - under) / 2;
+        if (score_of_key(mid, cum, lse) == s) key = mid;
+        else under = mid;
+    }
+    return key;
+}
+// How many of a beam's n continuations, whose scores fall, come before one of another beam that
+// scores s. lower: the list's beam comes before that other one, so its equal scores do. Within its own list a
+// continuation's place is where it stands, whatever its score: the places of all are different.
+OCR_HD int before_other(const double *list, int n, double s, bool lower) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (list[mid] > s || (lower && list[mid] == s)) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
 // How a sequence of len positions is cut for single-token attention: at most `parts` parts of at
 // least kLeastPart positions, whole tiles of 32.
 constexpr int kLeastPart = 256;
