@@ -1,0 +1,148 @@
+"""The text decoder's operators over the whole range of what they take: caps far over the scores,
+queries and value scales of very different size beside each other, scales and codes to the last
+bit. Against float64 (oracle/text.py). Tolerances count roundings: half a step of a type is EPS / 2
+of the value; weights are rounded once to 16 bits, an error of the sum of p |v|, an 8-bit cache's scaled ones once more,
+the output once. Scores are float32: 2^-20 of the largest that weighs anything, which the exponential passes on to the weights."""
+import numpy as np
+import pytest
+import torch
+
+import ocrhip
+from oracle import text as plain
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+EPS = {"f16": 2.0 ** -10, "bf16": 2.0 ** -7}
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def rn(g, *shape):
+    return torch.randn(*shape, generator=g)
+
+
+def i32(x):
+    return torch.as_tensor(np.asarray(x), dtype=torch.int32).to("cuda")
+
+
+def host(x):
+    torch.cuda.synchronize()
+    return x.cpu().double().numpy() if x.is_floating_point() else x.cpu().numpy()
+
+
+def close(got, want, size, top, eps, roundings=2):
+    tol = (roundings * eps / 2 + 2.0 ** -18 + 2.0 ** -20 * top) * size + eps / 2 * np.abs(want) * (1 + eps) + 2.0 ** -24
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (np.argwhere(bad)[:5], got[bad][:5], want[bad][:5], tol[bad][:5])
+
+
+def prompt(ctx, q, k, v, **kw):
+    out = torch.full_like(q, 9.0)
+    torch.cuda.synchronize()
+    ocrhip.attention(ctx, q, k, v, out, **kw)
+    ctx.synchronize()
+    return host(out)
+
+
+def single(ctx, cache, table, lens, q, **kw):
+    out = torch.full_like(q, 9.0)
+    t, n = i32(table), i32(lens)
+    torch.cuda.synchronize()
+    cache.attend(t, n, q, out, **kw)
+    ctx.synchronize()
+    return host(out)
+
+
+def held(ctx, fmt, k, v, ks=None, vs=None, page=16):
+    """(cache, table, k, v): one sequence whose vectors k, v [n][heads][dim] are codes (8-bit types, with
+    scales [n][heads]) or values; the float64 values they stand for."""
+    n, heads, dim = k.shape
+    pages = -(-n // page)
+    mem, val = [], []
+    for x, s in ((k, ks), (v, vs)):
+        if fmt == "i8":
+            x = x.to(torch.int8)
+            f = x.double()
+        elif fmt == "e4m3":
+            x = x.float().to(torch.float8_e4m3fn)
+            f = x.float().double()
+            x = x.view(torch.uint8)
+        else:
+            x = x.to(TYPES[fmt])
+            f = x.double()
+        m = torch.zeros(pages * page, heads, dim, dtype=x.dtype)
+        m[:n] = x
+        mem.append(m.view(pages, page, heads, dim).transpose(1, 2).contiguous().cuda())
+        if fmt in plain.QMAX:
+            m = torch.zeros(pages * page, heads)
+            m[:n] = s
+            mem.append(m.view(pages, page, heads).transpose(1, 2).contiguous().cuda())
+            f = f * s.double()[..., None]
+        else:
+            mem.append(None)
+        val.append(f.numpy())
+    cache = ocrhip.KvCache(ctx, pages, page, heads, dim, fmt, memory=(mem[0], mem[2], mem[1], mem[3]))
+    return cache, [list(range(pages))], val[0], val[1]
+
+
+CAPS = [(-0.3, 0.0), (0.0, 0.0), (1e-30, 0.0), (-0.2, 4.0), (2.0, 30.0), (0.05, 1000.0), (0.1, 1e-3), (1e3, 1e-2), (0.1, 1e4), (0.1, 1e6),
+        (0.1, 1e8), (0.1, 1e20), (0.1, 3e38), (0.1, float(np.finfo(np.float32).max)), (0.1, 1e-40)]
+
+
+@pytest.mark.parametrize("fmt,ty", [("f16", "f16"), ("bf16", "bf16"), ("i8", "bf16"), ("e4m3", "f16")])
+@pytest.mark.parametrize("dim", [128, 15])
+@pytest.mark.parametrize("scale,cap", CAPS)
+def test_single_tokens_of_any_cap(ctx, fmt, ty, dim, scale, cap):
+    """Scores of a few units under caps from nothing to the largest float, by the tiles (128) and by the formula (15)."""
+    g = gen(41)
+    n = 300
+    k, v = ((rn(g, n, 2, dim) * (40 if fmt == "i8" else 1)).round() if fmt in plain.QMAX else rn(g, n, 2, dim) for _ in range(2))
+    s = [0.02 * (0.5 + torch.rand(n, 2, generator=g)) for _ in range(2)] if fmt in plain.QMAX else [None, None]
+    cache, table, kf, vf = held(ctx, fmt, k, v, *s)
+    q = rn(g, 1, 4, dim).to(TYPES[ty]).cuda()
+    got = single(ctx, cache, table, [n], q, scale=scale, cap=cap)
+    want, size, top = plain.attention(host(q), kf, vf, ([0], [n]), scale, cap, pos=[n - 1])
+    close(got, want, size, min(top, cap) if cap else top, EPS[ty], 3)
+
+
+@pytest.mark.parametrize("ty", ["f16", "bf16"])
+@pytest.mark.parametrize("scale,cap", CAPS[8:])
+def test_prompts_of_any_cap(ctx, ty, scale, cap):
+    g = gen(42)
+    q, k, v = (rn(g, 200, h, 128).to(TYPES[ty]).cuda() for h in (4, 2, 2))
+    got = prompt(ctx, q, k, v, scale=scale, cap=cap)
+    want, size, top = plain.attention(host(q), host(k), host(v), plain.key_ranges(200, None, None), scale, cap)
+    close(got, want, size, min(top, cap), EPS[ty])
+
+
+@pytest.mark.parametrize("ty", ["f16", "bf16"])
+@pytest.mark.parametrize("cap", [1e4, 1e6])
+@pytest.mark.parametrize("form", ["prompt", "single"])
+@pytest.mark.parametrize("bias", [False, True])
+def test_capped_scores_of_very_different_size(ctx, ty, cap, form, bias):
+    """Scores of a few units beside some far under them, past a third of the cap, in every tile: those
+    weigh nothing, and the others must not feel the cap."""
+    g = gen(43)
+    n, dim = 260, 64
+    q, k = torch.zeros(n, 2, dim), torch.zeros(n, 1, dim)
+    q[..., 0] = 1.0
+    k[..., 0] = (torch.rand(n, 1, generator=g) * 4).to(TYPES[ty]).float()
+    k[5::9, :, 0] = -2.0 ** 15
+    v = rn(g, n, 1, dim)
+    q, k, v = (x.to(TYPES[ty]) for x in (q, k, v))
+    scale = cap / 2.0 ** 16  # half the cap
+    k = torch.where(k > -1000, (k.float() / scale).to(TYPES[ty]), k)  # the others: up to four units
+    sl = torch.tensor([0.02, 0.01]) if bias else None
+    kw = dict(scale=scale, cap=cap, slopes=None if sl is None else sl.cuda())
+    rows = [0, 4, 60, 199, 259]
+    want, size, _ = plain.attention(q.double().numpy()[rows], k.double().numpy(), v.double().numpy(), ([0] * 5, [r + 1 for r in rows]), scale, cap,
+                                    None if sl is None else sl.numpy(), pos=rows)
+    if form == "prompt":
+        got = prompt(ctx, q.cuda(), k.cuda(), v.cuda(), **kw)[rows]
+    else:
+        cache, table, *_ = held(ctx, ty, k, v)
+        got = np.concatenate([single(ctx, cache, table, [r + 1], q[r:r + 1].cuda(), **kw) for r in rows])
+    close(got, want, size, 4.0, EPS[ty], 3)

@@ -54,19 +54,17 @@ template <class T> __global__ __launch_bounds__(64) void attention_row_kernel(At
 // What scores go through besides the scale: nothing, the cap, or the distance's bias and perhaps the cap.
 enum Scores { kPlain, kCapped, kAny };
 
-// cap tanh(s / cap) of unscaled scores as s times a polynomial of their squares, which lasts to 0.35
-// of the cap: tanh(y) / y by powers of y^2, interpolated at the Chebyshev points of [0, 0.35^2], off
-// by 2^-24. In units of log2; the exponential's and the reciprocal's way takes half again as long.
+// cap tanh(s / cap) of unscaled scores as s times a polynomial of their squares (tanh_ratio, its powers
+// of scale / cap in the factors), which lasts to 0.35 of the cap. In units of log2; the exponential's and the reciprocal's way takes half again as long.
 struct SmallCap {
     float k[4], most;
     __device__ SmallCap(float scale, float cap) {
         const float y = scale / cap, t = y * y;
         k[0] = scale * 1.4426950408889634f;
-        const float part[4] = {1.f, -0.3333241939544678f, 0.13295751810073853f, -0.04895563796162605f};
         float power = k[0];
 #pragma unroll
-        for (int e = 1; e < 4; e++) power *= t, k[e] = part[e] * power;
-        most = y < 1e3f ? 0.35f / y : -1.f;  // beyond, the powers leave float32
+        for (int e = 1; e < 4; e++) power *= t, k[e] = kTanhPart[e] * power;
+        most = y >= 1e-6f && y < 1e3f ? kSmallTanh / y : -1.f;  // beyond, the powers leave float32
     }
     __device__ float factor(float s) const {
         const float t = s * s;
@@ -177,6 +175,7 @@ template <class T, int DP, Scores KIND, int QW> __global__ __launch_bounds__(256
     const float slope = KIND == kAny && a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.f;
 
     const SmallCap small(fabsf(a.scale), KIND != kPlain && a.cap > 0.f ? a.cap : 1.f);
+    const Cap cap = cap_of(a.cap, 1.4426950408889634f);
 
     // 32 KB keys from jw on, in LDS at sk, and their values at sv.
     auto turn = [&](int jw, const char *sk, const char *sv) __attribute__((always_inline)) {
@@ -205,7 +204,7 @@ template <class T, int DP, Scores KIND, int QW> __global__ __launch_bounds__(256
 #pragma unroll
                 for (int t = 0; t < KB; t++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) s[t][e] = cap_log2(s[t][e] * c, a.cap);
+                    for (int e = 0; e < 16; e++) s[t][e] = capped(cap, s[t][e] * c);
             } else if (a.cap > 0.f) {
 #pragma unroll
                 for (int t = 0; t < KB; t++)

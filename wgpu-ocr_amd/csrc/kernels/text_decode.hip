@@ -58,6 +58,7 @@ struct DecodePlan {
     uint32_t parts;
     int group, blocks, shift;  // query heads a key head, blocks of 16 of them
     bool q_pieces;
+    Cap cap;  // in units of log2
 };
 
 // Parts of a sequence joined: part [row][head][parts] holds dim normalised values, then log2 of the
@@ -228,10 +229,22 @@ template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 
                 for (int i = 0; i < 4; i++) sc[t][i] = s[t][i] * ks[i];
             }
             if (a.cap > 0.f) {
+                float far = 0.f;
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) sc[t][i] = cap_log2(sc[t][i], a.cap);
+                    for (int i = 0; i < 4; i++) far = fmaxf(far, fabsf(sc[t][i]));
+                if (__any(far > plan.cap.small)) {
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) sc[t][i] = capped(plan.cap, sc[t][i]);
+                } else {
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) sc[t][i] = small_capped(plan.cap, sc[t][i]);
+                }
             }
             if (a.slopes) {
                 const float d = float(len - 1 - c0 - t0 - 4 * g4);
@@ -380,7 +393,7 @@ template <int N> __global__ __launch_bounds__(N) void decode_join_kernel(DecodeA
 template <class T, class C> void launch_tiles(const DecodeArgs &a, uint32_t parts, float *part, hipStream_t s) {
     const int group = int(a.q_heads / a.kv.heads);
     const DecodePlan plan{parts, group, (group + 15) / 16, a.kv.page & (a.kv.page - 1) ? -1 : __builtin_ctz(a.kv.page),
-                          reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_stride % 8 == 0};
+                          reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_stride % 8 == 0, cap_of(a.cap, 1.4426950408889634f)};
     const dim3 grid(a.table.rows, a.kv.heads * plan.blocks, parts);
     if (a.kv.dim <= 64) hipLaunchKernelGGL((decode_kernel<T, C, 64>), grid, dim3(256), 0, s, a, plan, part);
     else if (a.kv.dim <= 128) hipLaunchKernelGGL((decode_kernel<T, C, 128>), grid, dim3(256), 0, s, a, plan, part);

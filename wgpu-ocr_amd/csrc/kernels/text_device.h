@@ -113,10 +113,10 @@ template <class M> constexpr float lift = std::is_same_v<M, f16> ? 6.f : -kSlack
 
 // 2^x; results under the normal range are zero.
 __device__ inline float exp2_f32(float x) { return __builtin_amdgcn_exp2f(x); }
-// A score in units of log2 through the cap: cap tanh(s / cap), tanh(y) = 1 - 2 / (e^2y + 1).
-__device__ inline float cap_log2(float x, float cap) {
-    const float c = cap * 1.4426950408889634f;
-    return c - 2.f * c * __builtin_amdgcn_rcpf(exp2_f32(x * (2.f / cap)) + 1.f);
+// A score through the cap: most tanh(y) = most (1 - 2 / (e^2y + 1)) past the small ones (text_rules.h).
+__device__ inline float capped(const Cap &c, float s) {
+    const float large = c.most * (1.f - 2.f * __builtin_amdgcn_rcpf(exp2_f32(s * c.inv * 2.8853900817779268f) + 1.f));
+    return fabsf(s) <= c.small ? small_capped(c, s) : large;
 }
 
 // The code of a value already divided by its vector's scale (rounded to nearest, ties to even).
@@ -167,12 +167,6 @@ __device__ inline int wave_max_i(int v) {
 }
 __device__ inline int wave_min_i(int v) { return -1 - wave_max_i(-1 - v); }
 
-// A scaled score through the cap and the distance bias.
-__device__ inline float score_of(float s, float cap, float slope, int distance) {
-    if (cap > 0.f) s = cap * tanhf(s / cap);
-    return s - slope * float(distance);
-}
-
 // One query's attention over keys [lo, hi) by one wavefront, by the formula: the scores' maximum
 // first, then exp(s - max) and the value sums, all in float32. q: the query's dim values in LDS,
 // scaled; kv.k(j, c) and kv.v(j, c): value c of key and value vector j. Scores of minus infinity
@@ -180,10 +174,12 @@ __device__ inline float score_of(float s, float cap, float slope, int distance) 
 template <class KV, class Done>
 __device__ inline void attend_row(const KV &kv, const float *q, int dim, int lo, int hi, int pos, float cap, float slope, Done &&done) {
     const int lane = threadIdx.x & 63;
+    const Cap most = cap_of(cap, 1.f);
     auto score = [&](int j) {
         float s = 0.f;
         for (int c = 0; c < dim; c++) s = __fmaf_rn(q[c], kv.k(j, c), s);
-        return score_of(s, cap, slope, pos > j ? pos - j : j - pos);
+        if (cap > 0.f) s = capped(most, s);
+        return s - slope * float(pos > j ? pos - j : j - pos);
     };
     float m = -INFINITY;
     for (int j = lo + lane; j < hi; j += 64) m = fmaxf(m, score(j));
