@@ -146,3 +146,47 @@ def test_capped_scores_of_very_different_size(ctx, ty, cap, form, bias):
         cache, table, *_ = held(ctx, ty, k, v)
         got = np.concatenate([single(ctx, cache, table, [r + 1], q[r:r + 1].cuda(), **kw) for r in rows])
     close(got, want, size, 4.0, EPS[ty], 3)
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("hq", [4, 16, 24])
+def test_queries_of_very_different_size(ctx, fmt, hq):
+    """bfloat16 heads of every size over one key head, each with scores of order one: a head's rounding is
+    its own, and an infinite one's is nobody else's."""
+    g = gen(44)
+    n, dim = 300, 64
+    k, v = ((rn(g, n, 1, dim) * 40).round() for _ in range(2))
+    s = [0.02 * (0.5 + torch.rand(n, 1, generator=g)) for _ in range(2)]
+    cache, table, kf, vf = held(ctx, fmt, k, v, *s)
+    q = rn(g, 1, hq, dim)
+    q[:, 0] *= 2.0 ** 20
+    q[:, 2] *= 2.0 ** 10
+    q = q.bfloat16()
+    def check(got, heads):
+        for h in heads:
+            want, size, top = plain.attention(q.double().numpy()[:, h:h + 1], kf, vf, ([0], [n]), dim ** -0.5, pos=[n - 1])
+            close(got[:, h:h + 1], want, size, top, EPS["bf16"], 3)
+
+    check(single(ctx, cache, table, [n], q.cuda()), range(1, hq))
+    q[:, 0, 3] = float("inf")
+    q[:, 1, 5] = float("nan")
+    got = single(ctx, cache, table, [n], q.cuda())
+    assert np.isnan(got[:, 1]).all()
+    check(got, range(2, hq))
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("up", [-126, -100, 100, 116, 120, 126])
+def test_queries_near_the_ends_of_bfloat16(ctx, fmt, up):
+    g = gen(45)
+    n, dim = 100, 64
+    k, v = ((rn(g, n, 1, dim) * 40).round() for _ in range(2))
+    # Scores of order one: 2^up of the queries, 2^-(up / 2) each of the keys' scales and the scores' own.
+    ks = 0.02 * 2.0 ** (-up / 2) * (0.5 + torch.rand(n, 1, generator=g))
+    vs = 0.02 * (0.5 + torch.rand(n, 1, generator=g))
+    cache, table, kf, vf = held(ctx, fmt, k, v, ks, vs)
+    q = (rn(g, 1, 4, dim).clamp(-1.9, 1.9).double() * 2.0 ** up).bfloat16()
+    scale = dim ** -0.5 * 2.0 ** (-up / 2)
+    got = single(ctx, cache, table, [n], q.cuda(), scale=scale)
+    want, size, top = plain.attention(q.double().numpy(), kf, vf, ([0], [n]), float(np.float32(scale)), pos=[n - 1])
+    close(got, want, size, top, EPS["bf16"], 3)

@@ -108,6 +108,9 @@ template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 
     for (int u = 0; u < NU; u++) off[u] = 16 * min(4 * u + g4, pieces - 1);
     char *const s_v = s_mem + wave * 32 * PITCH;
     const float slope = a.slopes && real ? a.slopes[h] * 1.4426950408889634f : 0.f;
+    // bfloat16 queries over an 8-bit cache are float16 in the products, each over a power of two of its own (below),
+    // which is in its lanes' score_scale.
+    constexpr bool own_scale = scaled<C> && std::is_same_v<T, bf16>;
     float score_scale = a.scale * 1.4426950408889634f;
     mvec qf[NS];
     f32x4 o[NB];
@@ -160,16 +163,20 @@ template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 
         };
         load(wave * 32);
         if (c0 == lo) {
-            // bfloat16 queries over an 8-bit cache as float16, their largest value's exponent taken
-            // out: the steps lost under 2^-14 of it are 2^-25 of it.
-            if constexpr (scaled<C> && std::is_same_v<T, bf16>) {
+            // The exponent of the query's largest finite value: float16 holds the others to 2^-11 of themselves down
+            // to 2^-14 of it, and to 2^-25 of it below.
+            if constexpr (own_scale) {
                 float top = 0.f;
 #pragma unroll
                 for (int s = 0; s < NS; s++)
 #pragma unroll
-                    for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(widen16(raw[s][i >> 1] >> (16 * (i & 1)), T_BF16)));
-                top = wave_max(top);
-                const int e = top > 0.f && top < INFINITY ? max(-100, min(100, ilogbf(top))) : 0;
+                    for (int i = 0; i < 8; i++) {
+                        const float x = fabsf(widen16(raw[s][i >> 1] >> (16 * (i & 1)), T_BF16));
+                        top = fmaxf(top, x < INFINITY ? x : 0.f);
+                    }
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const int e = top > 0.f ? max(-126, min(126, ilogbf(top))) : 0;
                 const float down = ldexpf(1.f, -e);
                 score_scale *= ldexpf(1.f, e);
 #pragma unroll
@@ -190,7 +197,7 @@ template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 
                         if (none[t] || 4 * u + g4 >= pieces) kr[t][u] = vr[t][u] = u32x4{0, 0, 0, 0};
                 if (none[g4 & 1]) scale_r = 0.f;
             }
-            // The tile's scales: the keys' with the scores' own, the values' over their power of two.
+            // The tile's scales: the keys' with the scores' own where that is one for all, the values' over their power of two.
             if constexpr (scaled<C>) {
                 if (__any(g4 >= 2 && fabsf(scale_r) > vtop)) {
                     const float vmax = wave_max(g4 >= 2 ? fabsf(scale_r) : 0.f);
@@ -199,7 +206,7 @@ template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 
                     for (int b = 0; b < NB; b++) o[b] *= f;
                     vtop = vn, vinv = 1.f / vn;
                 }
-                s_scale[wave][g4 >> 1][16 * (g4 & 1) + n] = scale_r * (g4 < 2 ? score_scale : vinv);
+                s_scale[wave][g4 >> 1][16 * (g4 & 1) + n] = scale_r * (g4 < 2 ? own_scale ? 1.f : score_scale : vinv);
             }
             f32x4 s[2];
 #pragma unroll
@@ -226,7 +233,7 @@ template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 
                 f32x4 ks{score_scale, score_scale, score_scale, score_scale};
                 if constexpr (scaled<C>) ks = *reinterpret_cast<const f32x4 *>(&s_scale[wave][0][16 * t + 4 * g4]);
 #pragma unroll
-                for (int i = 0; i < 4; i++) sc[t][i] = s[t][i] * ks[i];
+                for (int i = 0; i < 4; i++) sc[t][i] = (own_scale ? s[t][i] * score_scale : s[t][i]) * ks[i];
             }
             if (a.cap > 0.f) {
                 float far = 0.f;
