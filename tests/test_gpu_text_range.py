@@ -190,3 +190,49 @@ def test_queries_near_the_ends_of_bfloat16(ctx, fmt, up):
     got = single(ctx, cache, table, [n], q.cuda(), scale=scale)
     want, size, top = plain.attention(q.double().numpy(), kf, vf, ([0], [n]), float(np.float32(scale)), pos=[n - 1])
     close(got, want, size, top, EPS["bf16"], 3)
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("ty", ["f16", "bf16"])
+@pytest.mark.parametrize("apart", [12, 24, 32, 60, 100])
+@pytest.mark.parametrize("where", ["one tile", "before", "after", "everywhere"])
+def test_value_scales_far_apart(ctx, fmt, ty, apart, where):
+    """Keys that weigh nearly everything hold values far smaller than those of keys that weigh next to
+    nothing: 2^-(apart + 20) of them, so that theirs is all of the sum but 2^-20."""
+    g = gen(46)
+    n, dim = 700, 64
+    v = (rn(g, n, 1, dim) * 40).round().clamp(-120, 120)
+    k = torch.full((n, 1, dim), 8.0)
+    small = {"one tile": torch.arange(640, 672, 3), "before": torch.arange(0, 300), "after": torch.arange(400, 700),
+             "everywhere": torch.arange(0, 700, 2)}[where]
+    heavy = torch.zeros(n, dtype=torch.bool)
+    heavy[small] = True
+    vs = (0.02 * (0.5 + torch.rand(n, 1, generator=g)))
+    vs[~heavy] *= 2.0 ** apart
+    # Scores: q . k = 8 * 64 ks scale; the heavy ones higher by (apart + 20) bits.
+    ks = torch.full((n, 1), 1.0)
+    q = torch.full((1, 4, dim), 1.0).to(TYPES[ty])
+    ks[~heavy] = 1.0 - (apart + 20) / 128
+    scale = 128 * float(np.log(2)) / (8 * dim)
+    cache, table, kf, vf = held(ctx, fmt, k, v, ks, vs)
+    got = single(ctx, cache, table, [n], q.cuda(), scale=scale)
+    want, size, top = plain.attention(host(q), kf, vf, ([0], [n]), float(np.float32(scale)), pos=[n - 1])
+    close(got, want, size, top, EPS[ty], 3)
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("least", [2.0 ** -110, 2.0 ** -127, 2.0 ** -140, 2.0 ** -149])
+def test_value_scales_past_every_span(ctx, fmt, least):
+    """Scales down to float32's least beside ones: nothing beside those, in every tile."""
+    g = gen(48)
+    n, dim = 300, 64
+    k, v = ((rn(g, n, 1, dim) * 40).round() for _ in range(2))
+    ks, vs = (0.02 * (0.5 + torch.rand(n, 1, generator=g)) for _ in range(2))
+    vs[::7] = least
+    vs[::11] = 2.0 ** -30
+    vs[::13] = 0.0
+    cache, table, kf, vf = held(ctx, fmt, k, v, ks, vs)
+    q = rn(g, 1, 4, dim).half()
+    got = single(ctx, cache, table, [n], q.cuda())
+    want, size, top = plain.attention(host(q), kf, vf, ([0], [n]), dim ** -0.5, pos=[n - 1])
+    close(got, want, size, top, EPS["f16"], 3)

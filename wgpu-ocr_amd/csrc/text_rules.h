@@ -156,6 +156,22 @@ OCR_HD Parts parts_of(int len, uint32_t parts) {
     return parts == 1 ? Parts{1, len} : Parts{int((uint32_t(len) + uint32_t(each) - 1) / uint32_t(each)), each};
 }
 
+// The power of two over a positive number, at most 2^126.
+OCR_HD float over_pow2(float x) {
+    const uint32_t u = (__builtin_bit_cast(uint32_t, x) & 0x7f800000u) + 0x00800000u;
+    return __builtin_bit_cast(float, u < 0x7e800000u ? u : 0x7e800000u);
+}
+// Value scales (over the largest so far) that single-token attention's float16 weights hold at once: a
+// weight 2^-16 of the largest keeps eight bits under the least of them. Tiles of more take them a span at
+// a time, the largest first, each over a power of two of its own; those under the last span are nothing.
+// A span begins at its largest scale, so that each holds one and the next lies lower.
+constexpr float kScaleSpan = 0x1p-6f, kLastSpan = 0x1p-120f;
+struct ScaleSpan {
+    float over, low;  // the power of two, the least scale
+};
+OCR_HD bool more_spans(float largest) { return largest >= kLastSpan; }
+OCR_HD ScaleSpan span_of(float largest) { return {over_pow2(largest), over_pow2(largest) * kScaleSpan}; }
+
 // Which tile of queries and which head workgroup x of a prompt's attention takes. Workgroups go to
 // the eight compute dies in turn, each with a level-two cache of its own, so a die gets the query
 // heads of as few key heads as there are; later tiles, which see more of their document, come first.
