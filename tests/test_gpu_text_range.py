@@ -236,3 +236,23 @@ def test_value_scales_past_every_span(ctx, fmt, least):
     got = single(ctx, cache, table, [n], q.cuda())
     want, size, top = plain.attention(host(q), kf, vf, ([0], [n]), dim ** -0.5, pos=[n - 1])
     close(got, want, size, top, EPS["f16"], 3)
+
+
+def test_log_sums_to_the_last_bit(ctx):
+    """Rows of equal logits a block: the exponentials inside a block are ones, their sums whole, and what is left is the join
+    of the blocks, in float64. The score is that sum less itself, so no other rounding hides it."""
+    blocks, size = 40, 2048
+    for step in (0.37, 1.7, 0.011):
+        tops = -np.float32(step) * np.arange(blocks, dtype=np.float32)
+        x = torch.from_numpy(np.repeat(tops, size)[None]).cuda()
+        lse = float(np.log((size * np.exp(tops.astype(np.float64))).sum()))
+        scores = np.full((1, 1), np.float32(lse))
+        out = [torch.zeros(1, 1, device="cuda")] + [i32([[0]]) for _ in range(3)]
+        sc = torch.from_numpy(scores).cuda()
+        torch.cuda.synchronize()
+        ocrhip.beam_select(ctx, x, sc, None, None, *out)
+        ctx.synchronize()
+        assert int(out[2][0, 0]) == 0
+        # Forty float64 exponentials and a logarithm of numbers near ten: 2^-45; the result's own rounding 2^-24 of it.
+        want = float(scores[0, 0]) - lse
+        assert abs(float(out[0][0, 0]) - want) <= 2.0 ** -45 + 2.0 ** -24 * abs(want)

@@ -357,7 +357,8 @@ template <class T, bool ONE> __global__ __launch_bounds__(512) void beam_groups_
         uint64_t *const top = s_top + beam * w;
         const double cum = a.scores[r];
         const bool over = a.finished && a.finished[r];
-        float m = -INFINITY, sum = 0.f;
+        float m = -INFINITY;
+        double sum = 0.0;
         float x[4][8];        // a row of one chunk
         uint32_t key[kHeld];  // of the parts' maxima, 0 where there is no part
         const int words = (4 * blocks + 63) / 64;
@@ -400,13 +401,14 @@ template <class T, bool ONE> __global__ __launch_bounds__(512) void beam_groups_
                 m = wave_max(best);
 #pragma unroll
                 for (int k = 0; k < kMostBlocks / 64; k++)
-                    if (t[k] > -INFINITY) sum += bs[k] * exp2_f32((t[k] - m) * 1.4426950408889634f);
-                sum = wave_sum(sum);
+                    if (64 * k < blocks && t[k] > -INFINITY) sum += double(bs[k]) * exp(double(t[k]) - double(m));
+                for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
             }
             open = m > -INFINITY && m < INFINITY;
         }
-        // The float32 sums are good to 2^-22, the same error for all of a row; what it is added to is float64.
-        const double lse = open ? double(m) + log(double(sum)) : 0.0;
+        // The blocks' sums are float32 (off by some 2^-23, each its own way), what joins them, and what
+        // decides between beams, float64.
+        const double lse = open ? double(m) + log(sum) : 0.0;
         if (open) {
             uint32_t t = 0;
             if constexpr (ONE) {
