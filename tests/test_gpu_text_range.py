@@ -256,3 +256,56 @@ def test_log_sums_to_the_last_bit(ctx):
         # Forty float64 exponentials and a logarithm of numbers near ten: 2^-45; the result's own rounding 2^-24 of it.
         want = float(scores[0, 0]) - lse
         assert abs(float(out[0][0, 0]) - want) <= 2.0 ** -45 + 2.0 ** -24 * abs(want)
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 40, 20])
+def test_scales_and_codes_to_the_last_bit(ctx, fmt, dim):
+    """A vector's scale is the float32 quotient of its largest magnitude, and a code the value's own
+    rounding unless that lies within two float32 roundings of a border (2^-23 of the code): half of the values lie
+    just past that, by the tiles (64, 40) and by the row (20)."""
+    g = np.random.default_rng(47)
+    n, most = 400, plain.QMAX[fmt]
+    m = np.exp2(g.uniform(-20, 20, (n, 1))).astype(np.float32)
+    codes = g.integers(0, 126, (n, dim)) + 0.5 if fmt == "i8" else (8 + g.integers(0, 8, (n, dim)) + 0.5) * 2.0 ** g.integers(-3, 5, (n, dim))
+    x = (codes * (1 + g.choice([-1, 1], (n, dim)) * 2.0 ** -22.2) * m / most).astype(np.float32)
+    x[:, dim // 2:] = (g.uniform(-1, 1, (n, dim - dim // 2)) * m).astype(np.float32)
+    x = np.clip(x, -m, m)
+    x[:, 3:4] = m
+    mem = [torch.zeros(n, 1, 1, dim, dtype=torch.int8 if fmt == "i8" else torch.uint8, device="cuda") for _ in range(2)]
+    mem += [torch.zeros(n, 1, 1, device="cuda") for _ in range(2)]
+    cache = ocrhip.KvCache(ctx, n, 1, 1, dim, fmt, memory=mem)
+    q = torch.zeros(n, 1, dim, dtype=torch.float16, device="cuda")
+    table, seq, pos, xs = i32(np.arange(n)[None]), i32(np.zeros(n)), i32(np.arange(n)), torch.from_numpy(np.tile(x, (1, 3))).cuda()
+    torch.cuda.synchronize()
+    cache.append(table, seq, pos, xs, q, rot=0)
+    ctx.synchronize()
+    y = x.astype(np.float64) * most / m
+    for code, scale in ((mem[0], mem[2]), (mem[1], mem[3])):
+        assert np.array_equal(scale.cpu().numpy().reshape(n, 1), m / np.float32(most))
+        if fmt == "i8":
+            got, step = host(code).reshape(n, dim), np.ones_like(y)
+        else:
+            got = plain.e4m3_value(host(code)).reshape(n, dim)
+            step = 2.0 ** (np.floor(np.log2(np.maximum(np.abs(y), 2.0 ** -6))) - 3)
+        want = np.rint(y / step) * step
+        border = np.abs(np.abs(y / step - np.floor(y / step)) - 0.5) * step <= 2.0 ** -23 * np.abs(y)
+        assert np.array_equal(got[~border], want[~border]), (np.abs(got - want)[~border] > 0).sum()
+
+
+@pytest.mark.parametrize("dim", [64, 20])
+def test_norms_of_constant_vectors(ctx, dim):
+    """A constant vector c has sums without roundings: c / sqrt(c^2) is off by the reciprocal root's half step
+    and a quarter (what corrects it is float32 too), the product's and the scale's half: 1.75 x 2^-23."""
+    c = np.float32([3, 5, 7, 11, 13, 17, 19, 23, 29, 31, 37, 41, 43, 47, 53, 59, 61, 97, 101, 1.5, 0.375, 3 * 2.0 ** -40, 5 * 2.0 ** 40])
+    n = len(c)
+    mem = [torch.zeros(n, 1, 1, dim, dtype=torch.int8, device="cuda") for _ in range(2)] + [torch.zeros(n, 1, 1, device="cuda") for _ in range(2)]
+    cache = ocrhip.KvCache(ctx, n, 1, 1, dim, "i8", memory=mem)
+    q = torch.zeros(n, 1, dim, dtype=torch.float16, device="cuda")
+    ones = torch.ones(dim, device="cuda")
+    table, seq, pos, xs = i32(np.arange(n)[None]), i32(np.zeros(n)), i32(np.arange(n)), torch.from_numpy(np.repeat(c[:, None], 3 * dim, 1)).cuda()
+    torch.cuda.synchronize()
+    cache.append(table, seq, pos, xs, q, None, ones, ones, eps=0.0, rot=0)
+    ctx.synchronize()
+    assert (np.abs(host(mem[2]).reshape(n) * 127 - 1) <= 1.75 * 2.0 ** -23 * (1 + 2.0 ** -10)).all()
+    assert (host(mem[0]) == 127).all() and (host(q) == 1).all()

@@ -15,6 +15,24 @@ namespace {
 
 constexpr int kAppendTokens = 4, kReadTokens = 16;  // tokens of a workgroup
 
+// The instructions for reciprocals are off by up to a step, which moves codes over their borders; one Newton step on
+// the float32 remainder brings a division's half step back, in four instructions instead of ten.
+__device__ inline float root_reciprocal(float x) {
+    const float r = __builtin_amdgcn_rsqf(x), h = x * r;
+    return __fmaf_rn(__fmaf_rn(-h, r, 1.f), 0.5f * r, r);
+}
+// A vector's largest magnitude over its code, and the other way round (scale: the first of the two, from
+// 2e-33 to 3e36, whose reciprocal is normal).
+template <class C> __device__ inline float over_code_max(float m) {
+    constexpr float part = 1.f / code_max<C>;
+    const float s = m * part;
+    return __fmaf_rn(__fmaf_rn(-s, code_max<C>, m), part, s);
+}
+template <class C> __device__ inline float code_max_over(float m, float scale) {
+    const float r = __builtin_amdgcn_rcpf(scale);
+    return __fmaf_rn(__fmaf_rn(-m, r, code_max<C>), r * (1.f / code_max<C>), r);
+}
+
 // The cosine and sine of pair i of rot / 2 at a position. The turns in float64: float32 angles of far
 // positions would be off by whole steps of the rotation.
 __device__ inline float2 turn_of(int pos, int i, int rot, double log2_theta) {
@@ -167,7 +185,7 @@ template <class T, int N> __device__ inline Some<T, N> some_of(const float *x) {
 // two fours of a vector: those that it rotates with each other where pairs are halves apart, two
 // neighbours otherwise. A prompt of 23 600 tokens of 48 bfloat16 heads of 128 into e4m3: 532 MB in
 // 119 us, 4.5 TB/s (a large copy reaches 5.2); with the rotation's other half from a neighbouring
-// lane and exact divisions 157, bound by vector instructions.
+// lane and the compiler's divisions, the two together, 157, bound by vector instructions.
 template <class T, class O, class C, int W> __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, int each, bool past) {
     __shared__ __align__(16) float s_cos[kAppendTokens][128], s_sin[kAppendTokens][128];
     __shared__ __align__(16) float s_norm[2][8 * W];
@@ -243,7 +261,7 @@ template <class T, class O, class C, int W> __global__ __launch_bounds__(256) vo
                 for (int k = 0; k < 8; k++) ss = __fmaf_rn(x[k], x[k], ss);
                 ss = group_reduce<W>(ss, [](float a, float b) { return a + b; });
                 const float ms = ss * (1.f / float(dim)) + a.eps;
-                const float r = ms > 1e-30f ? __builtin_amdgcn_rsqf(ms) : 1.f / sqrtf(ms);  // the instruction takes no subnormals
+                const float r = ms > 1e-30f ? root_reciprocal(ms) : 1.f / sqrtf(ms);  // the instruction takes no subnormals
                 const f32x4 w0 = *reinterpret_cast<const f32x4 *>(&s_norm[kind][at[0]]), w1 = *reinterpret_cast<const f32x4 *>(&s_norm[kind][at[1]]);
 #pragma unroll
                 for (int k = 0; k < 8; k++) x[k] = x[k] * r * (k < 4 ? w0[k] : w1[k - 4]);
@@ -277,7 +295,7 @@ template <class T, class O, class C, int W> __global__ __launch_bounds__(256) vo
             top = group_reduce<W>(top, [](uint32_t a, uint32_t b) { return max(a, b); });
             const float m = __uint_as_float(top);
             const bool fine = top < 0x7f800000u, some = fine && m > kTinyMax;
-            const float scale = m * (1.f / code_max<C>), inv = __builtin_amdgcn_rcpf(scale);  // from 2e-33 to 3e36: its reciprocal is normal
+            const float scale = over_code_max<C>(m), inv = code_max_over<C>(m, scale);
             if (c == 0) (kind == 1 ? a.kv.k_scale : a.kv.v_scale)[vec] = some ? scale : fine ? 0.f : NAN;
 #pragma unroll
             for (int k = 0; k < 8; k++) x[k] *= inv;
