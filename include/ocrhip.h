@@ -445,7 +445,7 @@ typedef struct ocr_kv_cache {
 
 /* Which pages every sequence has: rows (sequences) of width entries, position p of a sequence in
  * the page that entry p / page names. An entry that is negative or names no page holds nothing:
- * writes there are dropped, reads give zeros. */
+ * writes there are dropped, reads give zeros. No rows: nothing to do (the table may be NULL). */
 typedef struct ocr_page_table {
     const int32_t *table;
     uint32_t rows;
