@@ -189,6 +189,8 @@ class KvCache:
             raise _error(f"cache: f16, bf16, i8 or e4m3 is wanted, not {dtype!r}")
         if min(pages, page, heads, dim) < 1:
             raise _error("cache: empty")
+        if max(pages, page, heads, dim) >= 2 ** 32:  # ctypes would cut them
+            raise _error(f"cache: sizes {(pages, page, heads, dim)} are past 32 bits")
         self.ctx, self.pages, self.page, self.heads, self.dim, self.dtype = ctx, pages, page, heads, dim, dtype
         code = _SHORT[dtype]
         shape = (pages, heads, page, dim)
@@ -233,7 +235,7 @@ class KvCache:
             raise _error(f"projections: rows [{n}][{width}] of f32, f16 or bf16 are wanted, not {tuple(qkv.shape)} of {qkv.dtype}")
         if pairs not in _PAIRS:
             raise _error(f'pairs: "halves" or "adjacent" is wanted, not {pairs!r}')
-        if theta <= 0 or rot < 0:
+        if theta <= 0 or not 0 <= rot < 2 ** 32:
             raise _error(f"a rotation of {rot} values to the base {theta}")
         out = _code(q, "queries")
         args = ocr_kv_append_args(_array(ctx, seq, "sequence numbers", _I32, (n,)), _array(ctx, pos, "positions", _I32, (n,)),
@@ -328,6 +330,8 @@ def beam_select(ctx, logits, scores, finished, eos: int | None, out_scores, pare
     code = _code(logits, "logits")
     if code not in _ANY or rows != shape[0] * shape[1] or (rows and vocab > 1 and logits.stride()[1] != 1):
         raise _error(f"logits: {shape[0] * shape[1]} rows of f32, f16 or bf16 are wanted, not {tuple(logits.shape)} of {logits.dtype}")
+    if eos is not None and not -2 ** 31 <= eos < 2 ** 31:
+        raise _error(f"the end token {eos} is not in the vocabulary")
     arr = lambda x, what, types: _array(ctx, x, what, types, shape)  # noqa: E731
     args = ocr_beam_args(logits.data_ptr() or None, code, shape[0], shape[1], vocab, logits.stride()[0] if rows > 1 else vocab,
                          arr(scores, "scores", _F32), arr(finished, "finished", _I32), -1 if eos is None else eos,
