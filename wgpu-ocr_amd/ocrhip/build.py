@@ -46,7 +46,9 @@ def _compile(src: str) -> str:
 
 
 def _tensors() -> None:
-    """ocrhip._tensors, the text decoder's calls on torch tensors (csrc/python/tensors.cpp)."""
+    """ocrhip._tensors, the text decoder's calls on torch tensors (csrc/python/tensors.cpp). Left out where torch, the
+    host compiler or a header is missing: the binding does without it."""
+    import shutil
     import sysconfig
 
     try:
@@ -58,6 +60,14 @@ def _tensors() -> None:
     out = os.path.join(PKG, "_tensors.so")
     tmp = out + f".tmp{os.getpid()}"
     include = [sysconfig.get_paths()["include"], *cpp_extension.include_paths()]
+    missing = [h for h in ("Python.h", "torch/csrc/autograd/python_variable.h") if not any(os.path.exists(os.path.join(p, h)) for p in include)]
+    if shutil.which(CXX) is None:
+        missing.insert(0, CXX)
+    if missing:
+        if os.path.exists(out):  # of another build: it may not fit the library
+            os.remove(out)
+        sys.stderr.write(f"_tensors.so is left out, for want of {', '.join(missing)}: calls on torch tensors are checked in Python\n")
+        return
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *[f"-isystem{p}" for p in include], os.path.join(CSRC, "python", "tensors.cpp"), "-o", tmp, "-L" + lib, "-ltorch_python",

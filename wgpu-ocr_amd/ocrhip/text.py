@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import sys
+import warnings
 
 P, U32, I32, I64, F32, F64 = ctypes.c_void_p, ctypes.c_uint32, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_double
 _TYPES = {"float32": 0, "float16": 1, "bfloat16": 2, "int8": 3, "uint8": 4, "float8_e4m3fn": 4, "int32": 5}
@@ -90,20 +91,24 @@ def _call(name, *args):
         raise root.OcrError(root.lib().ocr_last_error().decode())
 
 
-_tensors = None
+_tensors = None  # the module, False where it is not there
 
 
 def _native(name, ctx, *args):
     """The call on torch tensors by ocrhip._tensors; False if that leaves it to the checks here, which
-    say what is wrong or take arrays of another kind."""
+    say what is wrong or take arrays of another kind. Without the module they do all of it, a few
+    microseconds a call slower."""
     global _tensors
-    if _tensors is None:
-        if "torch" not in sys.modules:
+    if not _tensors:
+        if _tensors is False or "torch" not in sys.modules:
             return False
         try:
             from . import _tensors as module
         except ImportError as e:
-            raise _error(f"ocrhip._tensors is not built (run __graft_entry__.build() or python -m ocrhip.build): {e}")
+            warnings.warn(f"ocrhip._tensors is not there (python -m ocrhip.build makes it); calls on tensors are checked in Python: {e}",
+                          RuntimeWarning, stacklevel=3)
+            _tensors = False
+            return False
         lib = _root().lib()
         module.bind(*[ctypes.cast(getattr(lib, f"ocr_{f}_device"), ctypes.c_void_p).value
                       for f in ("kv_append", "kv_read", "attention", "decode_attention", "beam_select", "kv_fork")])
