@@ -196,7 +196,9 @@ int ocr_recognize_device(ocr_recognizer *rec, const ocr_batch *d_batches, uint32
  * "text_attention", "text_decode", "text_fork", "beam_select") is bracketed by HIP events on its
  * own stream. stop waits for them and returns the launches, their summed duration in ms and
  * their summed algorithmic FLOPs and bytes. Where a family has several kernels that a rule on
- * sizes picks from, each is a name of its own as well ("gemm_thin" of "gemm_dma"). */
+ * sizes picks from, each is a name of its own as well ("gemm_thin" of "gemm_dma"; "text_append_eights" and "_row",
+ * "text_read_eights" and "_row", "text_attention_64", "_128" and "_row", "text_decode_whole", "_parts" and "_row",
+ * "text_fork_pieces" and "_bytes", "beam_select_one" and "_two"). */
 int ocr_probe_start(const char *family);
 int ocr_probe_stop(const char *family, uint32_t *calls, double *ms, double *flops, double *bytes);
 

@@ -484,11 +484,11 @@ template <class T, bool ONE> __global__ __launch_bounds__(512) void beam_groups_
 void launch_beam(Ctx &c, const BeamArgs &a, hipStream_t s) {
     const int64_t rows = int64_t(a.groups) * a.beams;
     const size_t bytes = type_bytes(a.type);
-    ProbeScope probe("beam_select", s, 3.0 * rows * a.vocab, double(rows) * a.vocab * bytes);
     // Blocks of whole chunks, few enough for the second kernel's registers.
     const int chunks = int((a.vocab + kChunk - 1) / kChunk), size = (chunks + kMostBlocks - 1) / kMostBlocks * kChunk;
     const int blocks = int((a.vocab + size - 1) / size);
     const bool two = a.vocab > kOneLaunch;
+    ProbeScope probe("beam_select", s, 3.0 * rows * a.vocab, double(rows) * a.vocab * bytes, two ? "beam_select_two" : "beam_select_one");
     DBuf stats;
     if (two) stats = DBuf(&c, size_t(rows) * blocks * sizeof(Block), s);
     with_type(a.type, [&](auto t) {

@@ -326,12 +326,14 @@ template <class T, int DP, Scores KIND, int QW> void launch_tiles(const Attentio
     const int tiles = int((a.n + 32 * QW - 1) / (32 * QW));
     hipLaunchKernelGGL((attention_tile_kernel<T, DP, KIND, QW>), dim3(unsigned(head_blocks(tiles, a.q_heads, a.kv_heads))), dim3(256), 0, s, a, tiles);
 }
-template <class T, Scores KIND> void launch_dims(const AttentionArgs &a, hipStream_t s) {
-    // Tiles of 64 queries while those of 128 would leave compute units empty, but they bring every key
-    // from level two twice as often. 36 documents of up to 130 tokens, 16 heads of 64 (336 tiles of
-    // 128; four workgroups of it fit a compute unit): 11.9 us with 64 queries, 12.9 with 128; one of
-    // 2929, 16 heads of 128 (368 tiles; two fit): 103 and 87 us.
-    const bool few = int64_t((a.n + 127) / 128) * a.q_heads <= (a.dim <= 64 ? 768 : 256);
+// Tiles of 64 queries while those of 128 would leave compute units empty, but they bring every key
+// from level two twice as often. 36 documents of up to 130 tokens, 16 heads of 64 (336 tiles of
+// 128; four workgroups of it fit a compute unit): 11.9 us with 64 queries, 12.9 with 128; one of
+// 2929, 16 heads of 128 (368 tiles; two fit): 103 and 87 us.
+bool few_tiles(const AttentionArgs &a) {
+    return a.dim <= 128 && int64_t((a.n + 127) / 128) * a.q_heads <= (a.dim <= 64 ? 768 : 256);
+}
+template <class T, Scores KIND> void launch_dims(const AttentionArgs &a, bool few, hipStream_t s) {
     if (a.dim <= 32) few ? launch_tiles<T, 32, KIND, 2>(a, s) : launch_tiles<T, 32, KIND, 4>(a, s);
     else if (a.dim <= 64) few ? launch_tiles<T, 64, KIND, 2>(a, s) : launch_tiles<T, 64, KIND, 4>(a, s);
     else if (a.dim <= 96) few ? launch_tiles<T, 96, KIND, 2>(a, s) : launch_tiles<T, 96, KIND, 4>(a, s);
@@ -342,17 +344,19 @@ template <class T, Scores KIND> void launch_dims(const AttentionArgs &a, hipStre
 }  // namespace
 
 void launch_attention(const AttentionArgs &a, hipStream_t s) {
-    ProbeScope probe("text_attention", s, 2.0 * a.n * a.n * a.q_heads * a.dim, 4.0 * a.n * (a.q_heads + a.kv_heads) * a.dim);
     // Whole 16-byte pieces, and rows of a tile within 32 bits of each other.
     bool pieces = a.dim % 8 == 0 && head_blocks((a.n + 63) / 64, a.q_heads, a.kv_heads) < 1 << 24;
     for (const void *p : {a.q, a.k, a.v, static_cast<const void *>(a.out)}) pieces = pieces && reinterpret_cast<uintptr_t>(p) % 16 == 0;
     for (int64_t st : {a.q_stride, a.k_stride, a.v_stride, a.out_stride}) pieces = pieces && st % 8 == 0 && st < 1 << 24;
+    const bool few = few_tiles(a);
+    ProbeScope probe("text_attention", s, 2.0 * a.n * a.n * a.q_heads * a.dim, 4.0 * a.n * (a.q_heads + a.kv_heads) * a.dim,
+                     !pieces ? "text_attention_row" : few ? "text_attention_64" : "text_attention_128");
     with_type16(a.type, [&](auto t) {
         using T = decltype(t);
         if (!pieces) hipLaunchKernelGGL((attention_row_kernel<T>), dim3(a.n, a.q_heads), dim3(64), 0, s, a);
-        else if (a.slopes) launch_dims<T, kAny>(a, s);
-        else if (a.cap > 0.f) launch_dims<T, kCapped>(a, s);
-        else launch_dims<T, kPlain>(a, s);
+        else if (a.slopes) launch_dims<T, kAny>(a, few, s);
+        else if (a.cap > 0.f) launch_dims<T, kCapped>(a, few, s);
+        else launch_dims<T, kPlain>(a, few, s);
     });
     OCR_HIP(hipGetLastError());
 }

@@ -430,8 +430,8 @@ template <class F> void with_lanes(uint32_t dim, F &&f) {
 
 void launch_append(const AppendArgs &a, hipStream_t s) {
     const double values = double(a.n) * (a.q_heads + 2 * a.kv.heads) * a.kv.dim;
-    ProbeScope probe("text_append", s, 10 * values, values * (type_bytes(a.type) + 2));
     const bool eights = a.kv.dim % 8 == 0 && (a.adjacent || a.rot % 8 == 0);
+    ProbeScope probe("text_append", s, 10 * values, values * (type_bytes(a.type) + 2), eights ? "text_append_eights" : "text_append_row");
     // Four tokens a workgroup share their lookups once that leaves work for every compute unit.
     const int each = a.n >= 4096 ? kAppendTokens : 1;
     const bool past = double(a.n) * a.kv.dim * (2.0 * a.q_heads + 2.0 * a.kv.heads * type_bytes(a.kv.type)) > kHeld;
@@ -456,14 +456,15 @@ void launch_append(const AppendArgs &a, hipStream_t s) {
 
 void launch_read(const ReadArgs &a, hipStream_t s) {
     const double values = 2.0 * a.table.rows * a.most * a.kv.heads * a.kv.dim;
-    ProbeScope probe("text_read", s, values, values * (type_bytes(a.kv.type) + 2));
+    const bool eights = a.kv.dim % 8 == 0;
+    ProbeScope probe("text_read", s, values, values * (type_bytes(a.kv.type) + 2), eights ? "text_read_eights" : "text_read_row");
     // Workgroups go on to further positions past what a grid holds.
     const auto grid = [](int64_t blocks) { return dim3(unsigned(std::min<int64_t>(blocks, 1 << 22))); };
     with_cache(a.kv.type, [&](auto c) {
         with_type16(a.type, [&](auto o) {
             using C = decltype(c);
             using O = decltype(o);
-            if (a.kv.dim % 8) {
+            if (!eights) {
                 hipLaunchKernelGGL((read_row_kernel<C, O>), grid(int64_t(a.most) * a.table.rows), dim3(256), 0, s, a);
                 return;
             }
@@ -475,9 +476,10 @@ void launch_read(const ReadArgs &a, hipStream_t s) {
 }
 
 void launch_fork(const ForkArgs &a, hipStream_t s) {
-    ProbeScope probe("text_fork", s, 0, 8.0 * a.table.rows * a.table.width);
+    const bool pieces = whole_pieces(a.kv);
+    ProbeScope probe("text_fork", s, 0, 8.0 * a.table.rows * a.table.width, pieces ? "text_fork_pieces" : "text_fork_bytes");
     const dim3 grid(a.table.rows, a.kv.heads);
-    if (whole_pieces(a.kv)) hipLaunchKernelGGL(fork_kernel<u32x4>, grid, dim3(256), 0, s, a);
+    if (pieces) hipLaunchKernelGGL(fork_kernel<u32x4>, grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL(fork_kernel<uint8_t>, grid, dim3(256), 0, s, a);
     OCR_HIP(hipGetLastError());
 }

@@ -448,15 +448,7 @@ template <class F> void with_pair(const DecodeArgs &a, F &&f) {
 }  // namespace
 
 void launch_decode(Ctx &c, const DecodeArgs &a, hipStream_t s) {
-    ProbeScope probe("text_decode", s, 4.0 * a.table.rows * a.table.width * a.kv.page * a.q_heads * a.kv.dim,
-                     2.0 * a.table.rows * a.table.width * a.kv.page * a.kv.heads * a.kv.dim * type_bytes(a.kv.type));
-    if (!whole_pieces(a.kv)) {
-        with_pair(a, [&](auto t, auto k) {
-            hipLaunchKernelGGL((decode_row_kernel<decltype(t), decltype(k)>), dim3(a.table.rows, a.q_heads), dim3(64), 0, s, a);
-        });
-        OCR_HIP(hipGetLastError());
-        return;
-    }
+    const bool pieces = whole_pieces(a.kv);
     // Parts until there are two workgroups for every compute unit; a sequence has as many as its own
     // length gives work to. 4 sequences of 131 072: 256 workgroups 194 us, 384 204, 512 179, 1024
     // 181; 144 of 700: one part (576) 24 us, two 30.
@@ -464,6 +456,16 @@ void launch_decode(Ctx &c, const DecodeArgs &a, hipStream_t s) {
     const uint64_t heads = uint64_t(a.table.rows) * a.kv.heads * ((a.q_heads / a.kv.heads + 15) / 16);
     const uint64_t most = uint64_t(a.table.width) * a.kv.page;
     const uint32_t parts = uint32_t(std::max<uint64_t>(1, std::min<uint64_t>({kMostParts, (kWork + heads - 1) / heads, (most + kLeastPart - 1) / kLeastPart})));
+    ProbeScope probe("text_decode", s, 4.0 * a.table.rows * a.table.width * a.kv.page * a.q_heads * a.kv.dim,
+                     2.0 * a.table.rows * a.table.width * a.kv.page * a.kv.heads * a.kv.dim * type_bytes(a.kv.type),
+                     !pieces ? "text_decode_row" : parts > 1 ? "text_decode_parts" : "text_decode_whole");
+    if (!pieces) {
+        with_pair(a, [&](auto t, auto k) {
+            hipLaunchKernelGGL((decode_row_kernel<decltype(t), decltype(k)>), dim3(a.table.rows, a.q_heads), dim3(64), 0, s, a);
+        });
+        OCR_HIP(hipGetLastError());
+        return;
+    }
     DBuf part;
     if (parts > 1) part = DBuf(&c, size_t(a.table.rows) * a.q_heads * parts * (a.kv.dim + kPartTail) * 4, s);
     with_pair(a, [&](auto t, auto k) { launch_tiles<decltype(t), decltype(k)>(a, parts, part.as<float>(), s); });
