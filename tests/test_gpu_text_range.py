@@ -309,3 +309,17 @@ def test_norms_of_constant_vectors(ctx, dim):
     ctx.synchronize()
     assert (np.abs(host(mem[2]).reshape(n) * 127 - 1) <= 1.75 * 2.0 ** -23 * (1 + 2.0 ** -10)).all()
     assert (host(mem[0]) == 127).all() and (host(q) == 1).all()
+
+
+@pytest.mark.parametrize("ty", ["f16", "bf16"])
+@pytest.mark.parametrize("scale,cap,size", [(1e-12, 1.0, 2.0 ** 18), (1e-6, 1e5, 2.0 ** 6), (1e-25, 1e3, 2.0 ** 40), (1e6, 1e13, 2.0 ** -10), (3e-38, 1e-3, 2.0 ** 60)])
+def test_prompts_of_caps_whose_powers_are_no_floats(ctx, ty, scale, cap, size):
+    """scale / cap from 10^-28 to 10^-7: scores of a third of the cap and of next to nothing."""
+    if ty == "f16":
+        size = min(size, 2.0 ** 9)
+    g = gen(49)
+    q, k, v = (rn(g, 200, h, 128) for h in (4, 2, 2))
+    q, k, v = (x.to(TYPES[ty]).cuda() for x in (q * size, k * size, v))
+    got = prompt(ctx, q, k, v, scale=scale, cap=cap)
+    want, size, top = plain.attention(host(q), host(k), host(v), plain.key_ranges(200, None, None), float(np.float32(scale)), float(np.float32(cap)))
+    close(got, want, size, min(top, cap), EPS[ty])

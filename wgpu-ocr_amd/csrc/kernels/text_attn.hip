@@ -51,8 +51,12 @@ template <class T> __global__ __launch_bounds__(64) void attention_row_kernel(At
     attention_row<T>(a, blockIdx.x, blockIdx.y, s_q);
 }
 
-// What scores go through besides the scale: nothing, the cap, or the distance's bias and perhaps the cap.
-enum Scores { kPlain, kCapped, kAny };
+// What scores go through besides the scale: nothing, a fine cap, the distance's bias and perhaps a fine cap, or any cap
+// and perhaps the bias.
+//
+// A tile with a score past 0.35 of the cap takes the exponential's form, for all of its scores where the cap
+// is fine (kFineCap). Score by score it costs more: a page of 2929 tokens with scores past the cap: 104 us, so 135.
+enum Scores { kPlain, kCapped, kBias, kAny };
 
 // cap tanh(s / cap) of unscaled scores as s times a polynomial of their squares (tanh_ratio, its powers
 // of scale / cap in the factors), which lasts to 0.35 of the cap. In units of log2; the exponential's and the reciprocal's way takes half again as long.
@@ -64,7 +68,9 @@ struct SmallCap {
         float power = k[0];
 #pragma unroll
         for (int e = 1; e < 4; e++) power *= t, k[e] = kTanhPart[e] * power;
-        most = y >= 1e-6f && y < 1e3f ? kSmallTanh / y : -1.f;  // beyond, the powers leave float32
+        // Where the powers leave float32: as far as those that are left reach (the fourth power's part under 2^-25 of
+        // the score, the square's), and no score's square is infinite.
+        most = y >= 1e3f ? -1.f : fabsf(k[3]) >= 1e-36f ? kSmallTanh / y : fminf((fabsf(k[1]) >= 1e-36f ? 0.02f : 3e-4f) / y, 1e18f);
     }
     __device__ float factor(float s) const {
         const float t = s * s;
@@ -172,7 +178,7 @@ template <class T, int DP, Scores KIND, int QW> __global__ __launch_bounds__(256
         for (int e = 0; e < 16; e++) o[b][e] = 0.f;
     float m = -INFINITY, l = 0.f;
     const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);  // not 0: masked scores stay minus infinity
-    const float slope = KIND == kAny && a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.f;
+    const float slope = KIND >= kBias && a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.f;
 
     const SmallCap small(fabsf(a.scale), KIND != kPlain && a.cap > 0.f ? a.cap : 1.f);
     const Cap cap = cap_of(a.cap, 1.4426950408889634f);
@@ -204,7 +210,7 @@ template <class T, int DP, Scores KIND, int QW> __global__ __launch_bounds__(256
 #pragma unroll
                 for (int t = 0; t < KB; t++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) s[t][e] = capped(cap, s[t][e] * c);
+                    for (int e = 0; e < 16; e++) s[t][e] = KIND == kAny ? capped(cap, s[t][e] * c) : large_capped(cap, s[t][e] * c);
             } else if (a.cap > 0.f) {
 #pragma unroll
                 for (int t = 0; t < KB; t++)
@@ -214,7 +220,7 @@ template <class T, int DP, Scores KIND, int QW> __global__ __launch_bounds__(256
 #pragma unroll
                 for (int t = 0; t < KB; t++) s[t] *= c;
             }
-            if (KIND == kAny) {
+            if (KIND == kBias || (KIND == kAny && a.slopes)) {
                 const float d = float(i - jw - 4 * half);
 #pragma unroll
                 for (int t = 0; t < KB; t++)
@@ -354,7 +360,8 @@ void launch_attention(const AttentionArgs &a, hipStream_t s) {
     with_type16(a.type, [&](auto t) {
         using T = decltype(t);
         if (!pieces) hipLaunchKernelGGL((attention_row_kernel<T>), dim3(a.n, a.q_heads), dim3(64), 0, s, a);
-        else if (a.slopes) launch_dims<T, kAny>(a, few, s);
+        else if (cap_of(a.cap, 1.4426950408889634f).most > kFineCap) launch_dims<T, kAny>(a, few, s);
+        else if (a.slopes) launch_dims<T, kBias>(a, few, s);
         else if (a.cap > 0.f) launch_dims<T, kCapped>(a, few, s);
         else launch_dims<T, kPlain>(a, few, s);
     });

@@ -113,11 +113,12 @@ template <class M> constexpr float lift = std::is_same_v<M, f16> ? 6.f : -kSlack
 
 // 2^x; results under the normal range are zero.
 __device__ inline float exp2_f32(float x) { return __builtin_amdgcn_exp2f(x); }
-// A score through the cap: most tanh(y) = most (1 - 2 / (e^2y + 1)) past the small ones (text_rules.h).
-__device__ inline float capped(const Cap &c, float s) {
-    const float large = c.most * (1.f - 2.f * __builtin_amdgcn_rcpf(exp2_f32(s * c.inv * 2.8853900817779268f) + 1.f));
-    return fabsf(s) <= c.small ? small_capped(c, s) : large;
+// A score through the cap: most tanh(y) = most (1 - 2 / (e^2y + 1)), off by 2^-23 of the cap; and with the small
+// ones off by their own size (text_rules.h).
+__device__ inline float large_capped(const Cap &c, float s) {
+    return c.most * (1.f - 2.f * __builtin_amdgcn_rcpf(exp2_f32(s * c.inv * 2.8853900817779268f) + 1.f));
 }
+__device__ inline float capped(const Cap &c, float s) { return fabsf(s) <= c.small ? small_capped(c, s) : large_capped(c, s); }
 
 // The code of a value already divided by its vector's scale (rounded to nearest, ties to even).
 template <class C> __device__ inline C code_of(float v) {

@@ -100,6 +100,9 @@ OCR_HD float tanh_ratio(float u) {
 struct Cap {
     float most, inv, small;
 };
+// Up to here (in units of log2: a cap of 88) that error, 2^-16, is a thirtieth of a float16 weight's own rounding: one
+// form may do for all scores of a prompt's tile.
+constexpr float kFineCap = 128.f;
 OCR_HD Cap cap_of(float cap, float unit) {
     const float most = __builtin_fminf(cap * unit, 0x1.fffffep127f);
     return {most, most > 0.f ? __builtin_fminf(1.f / most, 1e30f) : 0.f, kSmallTanh * most};
