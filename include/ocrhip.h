@@ -416,7 +416,11 @@ int ocr_pp_line_images(ocr_ctx *ctx, const uint8_t *rgb, uint32_t page_w, uint32
  * tokens over the cache, beam search. All buffers are in device memory; the work is queued on the
  * context's stream (ocr_stream_acquire and ocr_stream_release order it with the caller's own
  * streams). Sizes and pointers are checked by the call. Lengths, positions and page numbers live in device memory
- * and are checked by the kernels: what lies outside the buffers is neither read nor written. */
+ * and are checked by the kernels: what lies outside the buffers is neither read nor written.
+ * Every size and alignment that the checks let through works; these are the fast ones, others go by the row or by the formula,
+ * three to a thousand times slower: append, dim and (pairs half a rotation apart) rot multiples of 8; read, dim a multiple of 8; attention, dim
+ * and strides multiples of 8 and addresses of 16 bytes; single tokens, vectors of the cache whole 16 bytes (dim a multiple of 16 in
+ * 8 bits, of 8 in 16) at addresses of 16 bytes. */
 
 /* Everything queued on `stream` (a hipStream_t of the context's device; NULL: the default stream)
  * so far comes before what is queued on the context from now on; and the other way round. */
@@ -569,7 +573,8 @@ int ocr_beam_select_device(ocr_ctx *ctx, const ocr_beam_args *args);
  * (parents, one a row, within the group). Whole pages are shared; a part-filled last page stays
  * with the lowest w that continues the parent, the others get its contents in their own page
  * spare[row] (used[row] = 1, else 0). Entries past the last page are -1. A parent outside the
- * group gives an empty sequence. Spare pages must be in no row of the table and all different;
+ * group gives an empty sequence. Where the parent's last page or the spare one is none of the pool's, nothing is copied
+ * (the table names the spare page all the same). Spare pages must be in no row of the table and all different;
  * table_out and lens_out must not overlap the old ones. */
 int ocr_kv_fork_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_table *pages, const int32_t *lens,
                        const int32_t *parents, uint32_t beams, const int32_t *spare, int32_t *table_out,
