@@ -94,8 +94,11 @@ def beam_select(logits, scores, finished, eos):
     x = np.where(np.isnan(x), -np.inf, x)
     with np.errstate(invalid="ignore", divide="ignore"):
         m = x.max(-1, keepdims=True)
-        lse = m + np.log(np.exp(x - m).sum(-1, keepdims=True))
-        s = x - lse
+        rest = np.log(np.exp(x - m).sum(-1, keepdims=True))
+        lse = m + rest
+        b = lse - m
+        lost = (m - (lse - b)) + (rest - b)  # all of rest, where a row's logits are very large
+        s = x - lse - lost
     if finished is not None:
         s = np.where(finished[..., None] != 0, np.where(np.arange(vocab) == eos, 0.0, -np.inf), s)
     with np.errstate(invalid="ignore"):

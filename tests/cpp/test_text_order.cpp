@@ -38,14 +38,22 @@ static void keys() {
 static void alike() {
     for (double cum : {0.0, -20.0, -1e9, -1e20, -1e30, -3.4028234663852886e38, 3.4028234663852886e38})
         for (float x : {0.f, 1e-17f, -1e-17f, 9.f, -9.f, 1e6f, -3e38f, 3e38f}) {
-            const double lse = std::log(97.0) + std::max(0.f, x);
+            const LogSum lse = log_sum(std::max(0.f, x), std::log(97.0));
             const uint32_t k = key_of(x), low = lowest_alike(k, cum, lse);
             const double s = score_of_key(k, cum, lse);
             check(low > kNothing && low <= k && score_of_key(low, cum, lse) == s, "the least scores alike", cum, x);
             check(score_of_key(low - 1, cum, lse) < s, "the next one less", cum, x);
         }
-    check(lowest_alike(key_of(9.f), -20.0, 10.0) == key_of(9.f), "ordinary logits differ", 0, 0);
-    check(lowest_alike(key_of(9.f), -1e30, 10.0) < key_of(-1e12f), "a large score absorbs them", 0, 0);
+    check(lowest_alike(key_of(9.f), -20.0, log_sum(9.0, 1.0)) == key_of(9.f), "ordinary logits differ", 0, 0);
+    for (float x : {-3.4028235e38f, 3.4028235e38f, 1e20f})
+        check(score_of_key(key_of(x), -2.0, log_sum(x, std::log(97.0))) == -2.0 - std::log(97.0), "a row of equal logits", x, 0);
+    // What an ordinary sum loses is under its last bit, and logits that it absorbs stay alike.
+    for (double top : {-3.0, 0.0, 1.25, 40.0}) {
+        const LogSum l = log_sum(top, std::log(20001.0));
+        check(std::fabs(l.lost) <= 0x1p-53 * std::fabs(l.whole), "what the sum lost", top, l.lost);
+        check(score_of_key(key_of(1e-17f), -1.0, l) == score_of_key(key_of(1.2e-16f), -1.0, l), "absorbed logits", top, 0);
+    }
+    check(lowest_alike(key_of(9.f), -1e30, log_sum(9.0, 1.0)) < key_of(-1e12f), "a large score absorbs them", 0, 0);
 }
 
 // Every continuation's place among all is another one, and the one that sorting gives.

@@ -316,7 +316,7 @@ template <class T> __device__ inline void lowest_of(const T *row, int vocab, uin
 // A row's best `want` (at most 32) keys, found by their logits, brought into the order of scores, then
 // tokens: where different logits score alike the lower tokens come first, those too that are not among
 // the best by logits.
-template <class T> __device__ inline void settle_ties(const T *row, int vocab, double cum, double lse, int want, uint64_t *top) {
+template <class T> __device__ inline void settle_ties(const T *row, int vocab, double cum, LogSum lse, int want, uint64_t *top) {
     const int lane = threadIdx.x & 63;
     const uint64_t mine = lane < want ? top[lane] : 0;
     const double s = score_of_key(uint32_t(mine >> 32), cum, lse);
@@ -408,7 +408,7 @@ template <class T, bool ONE> __global__ __launch_bounds__(512) void beam_groups_
         }
         // The blocks' sums are float32 (off by some 2^-23, each its own way), what joins them, and what
         // decides between beams, float64.
-        const double lse = open ? double(m) + log(sum) : 0.0;
+        const LogSum lse = open ? log_sum(m, log(sum)) : LogSum{0.0, 0.0};
         if (open) {
             uint32_t t = 0;
             if constexpr (ONE) {

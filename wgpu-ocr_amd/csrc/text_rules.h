@@ -116,13 +116,22 @@ OCR_HD float small_capped(const Cap &c, float s) {
 constexpr uint32_t kNothing = 0x007fffffu;
 OCR_HD float value_of(uint32_t key) { return __builtin_bit_cast(float, key ^ (key >> 31 ? 0x80000000u : 0xffffffffu)); }
 
+// A row's log-sum: its largest logit and the log of the sum of e^(x - top), and what their sum lost, which is all of
+// the second beside a large first (a row whose mask's lowest value leaves nothing).
+struct LogSum {
+    double whole, lost;
+};
+OCR_HD LogSum log_sum(double top, double rest) {
+    const double whole = top + rest, b = whole - top;
+    return {whole, (top - (whole - b)) + (rest - b)};
+}
 // A continuation's score: the beam's, and the logit of this key less the row's log-sum.
-OCR_HD double score_of_key(uint32_t key, double cum, double lse) {
-    return key > kNothing ? cum + (double(value_of(key)) - lse) : -__builtin_inf();
+OCR_HD double score_of_key(uint32_t key, double cum, LogSum lse) {
+    return key > kNothing ? cum + (double(value_of(key)) - lse.whole - lse.lost) : -__builtin_inf();
 }
 // The least key whose score is that of `key` (over minus infinity's): scores rise with the keys, but
 // not every step, since a large score absorbs logits, and a log-sum small ones.
-OCR_HD uint32_t lowest_alike(uint32_t key, double cum, double lse) {
+OCR_HD uint32_t lowest_alike(uint32_t key, double cum, LogSum lse) {
     const double s = score_of_key(key, cum, lse);
     uint32_t under = kNothing;
     while (key - under > 1) {
