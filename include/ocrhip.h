@@ -528,7 +528,8 @@ int ocr_attention_device(ocr_ctx *ctx, const ocr_attention_args *args);
 
 /* The same for the last token of every sequence of a cache (its length, lens[row], counts it; 0: it
  * sees nothing and gives zeros): q and out a row a sequence, type OCR_F16 or OCR_BF16 (a 16-bit
- * cache's own type). */
+ * cache's own type). A cached value that is not finite, within the length, makes the output so, or NaN, however
+ * little it weighs. */
 typedef struct ocr_decode_args {
     const int32_t *lens;
     const void *q;
