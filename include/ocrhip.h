@@ -581,6 +581,164 @@ int ocr_kv_fork_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_t
                        const int32_t *parents, uint32_t beams, const int32_t *spare, int32_t *table_out,
                        int32_t *lens_out, int32_t *used);
 
+/* ---- The same cache over images, over long texts, and of latent vectors ------------------------ */
+
+/* Rotary positions of several axes (time, row and column of an image's tokens): at [n][count] positions, token by
+ * token; pairs[a] pairs of a rotation go by axis a (together rot / 2), in blocks one axis after another or, with
+ * in_turn != 0, one pair of each axis in turn as long as it has some left. Pair i of the rotation turns by its axis'
+ * position times theta^(-2 i / rot), or with own_ladder != 0 theta^(-j / pairs[a]), j its place among its axis' pairs. */
+typedef struct ocr_axes {
+    const int32_t *at;
+    uint32_t count; /* 1 to 4 */
+    uint32_t pairs[4];
+    int32_t in_turn;
+    int32_t own_ladder;
+} ocr_axes;
+/* ocr_kv_append_device with the rotation by these axes; args->pos says where in the cache a token goes and no more. */
+int ocr_kv_append_axes_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_table *pages, const ocr_kv_append_args *args,
+                              const ocr_axes *axes);
+
+/* Vectors x [n][heads][dim] (tokens x_stride values apart, heads x_head; dim at most 1024) with their values first ..
+ * first + rot - 1 (rot even, at most 256) rotated by the tokens' positions, pairs as in ocr_kv_append_args, the others as they are, into
+ * out (the same type: OCR_F32, OCR_F16 or OCR_BF16). out may be x with the same strides, and must not overlap it otherwise. back != 0 turns
+ * the other way: the inverse, and the gradient. Fast where dim, first and (pairs half a rotation apart) rot are
+ * multiples of 8. */
+typedef struct ocr_rotate_args {
+    const void *x;
+    void *out;
+    int32_t type;
+    uint32_t n;
+    uint32_t heads;
+    uint32_t dim;
+    int64_t x_stride;
+    int64_t x_head;
+    int64_t out_stride;
+    int64_t out_head;
+    uint32_t first;
+    uint32_t rot;
+    double theta;
+    int32_t adjacent;
+    int32_t back;
+} ocr_rotate_args;
+int ocr_rotate_device(ocr_ctx *ctx, const ocr_rotate_args *args, const ocr_axes *axes);
+
+/* Attention that also says how much each key got. To weights (documents or sequences)[kv_heads][most] the softmax weights
+ * are added, over the query heads of each key head: for prompts (ocr_attention_device; a row a document, its keys by
+ * their place in it) over the document's queries, its last `window` (0: all); for single tokens
+ * (ocr_decode_attention_device; a row a sequence) the token's. Places from `most` on are dropped, those of no key
+ * left as they are. The sums' order is the same each time. Scores that are NaN make weights NaN. */
+int ocr_attention_weights_device(ocr_ctx *ctx, const ocr_attention_args *args, float *weights, uint32_t most, uint32_t window);
+int ocr_decode_attention_weights_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_table *pages,
+                                        const ocr_decode_args *args, float *weights, uint32_t most);
+
+/* Drops cached tokens of each sequence (its length, lens[row], within the table and `most`) until `keep` are left,
+ * each key head its own: kept are those at a position under `first`, the `recent` last positions up to newest[row],
+ * and of the others those of the largest weights, equal ones by the lower place (NaN weighs least; first + recent at
+ * most keep). Kept vectors beyond place keep - 1 move to the places of the dropped ones, the lowest to the lowest; nothing
+ * else moves, so places are no order of age: held [rows][heads][most] says which position the token at a place
+ * has, where it is negative the token is as far before newest[row] as its place is before the last. Written are lens_out,
+ * weights_out and held_out (the moved weights and positions, 0 and -1 from the new length on; they may be weights
+ * and held), also where nothing is dropped. The table stays: pages past the new length are the caller's again. A
+ * page of a sequence that is dropped from must be in no other row, nor twice in its own. Scores with slopes go by places, and so not with this. A vector whose
+ * old or new page there is not is not moved. */
+typedef struct ocr_evict_args {
+    const int32_t *lens;
+    const int32_t *newest;
+    const float *weights;
+    const int32_t *held;
+    uint32_t most;
+    uint32_t keep;
+    uint32_t first;
+    uint32_t recent;
+    float *weights_out;
+    int32_t *held_out;
+    int32_t *lens_out;
+} ocr_evict_args;
+int ocr_kv_evict_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_table *pages, const ocr_evict_args *args);
+
+/* A pool of pages of latent vectors [pages][page][rank + rot] (OCR_F16 or OCR_BF16; rank at most 512, rot even and at
+ * most 128): one a token for all heads, rank values that keys and values are made of and a rotated key of rot that all
+ * heads share. */
+typedef struct ocr_latent_cache {
+    void *data;
+    uint32_t pages;
+    uint32_t page;
+    uint32_t rank;
+    uint32_t rot;
+    int32_t type;
+} ocr_latent_cache;
+
+/* n tokens' projections x (OCR_F32, OCR_F16 or OCR_BF16, rank + rot values every `stride`): the first rank divided by
+ * sqrt(mean of squares + eps) and multiplied by norm (rank floats; NULL: neither), the others rotated by the token's
+ * position (pairs as in ocr_kv_append_args), or by the axes' where axes is not NULL; into the cache at position pos[t] of
+ * sequence seq[t], and to out [n][rank + rot] (the cache's type; may be NULL). */
+typedef struct ocr_latent_append_args {
+    const int32_t *seq;
+    const int32_t *pos;
+    const void *x;
+    int32_t type;
+    uint32_t n;
+    int64_t stride;
+    const float *norm;
+    float eps;
+    double theta;
+    int32_t adjacent;
+    void *out;
+} ocr_latent_append_args;
+int ocr_latent_append_device(ocr_ctx *ctx, const ocr_latent_cache *cache, const ocr_page_table *pages, const ocr_latent_append_args *args,
+                             const ocr_axes *axes);
+
+/* Attention of every sequence's last token over its latent vectors, as they are: queries q [rows][heads][rank + rot]
+ * that the keys' expansion has been absorbed into, scores scale q.c, out [rows][heads][rank] the weighted sum of the
+ * vectors' first rank values, for the values' expansion to follow. Types the cache's. Lengths as in
+ * ocr_decode_attention_device. Fast where rank and rot are multiples of 8, strides of 8 and addresses of 16 bytes. */
+typedef struct ocr_latent_decode_args {
+    const int32_t *lens;
+    const void *q;
+    void *out;
+    uint32_t heads;
+    int64_t q_stride;
+    int64_t out_stride;
+    float scale;
+} ocr_latent_decode_args;
+int ocr_latent_decode_device(ocr_ctx *ctx, const ocr_latent_cache *cache, const ocr_page_table *pages, const ocr_latent_decode_args *args);
+
+/* ocr_kv_fork_device over a latent cache. */
+int ocr_latent_fork_device(ocr_ctx *ctx, const ocr_latent_cache *cache, const ocr_page_table *pages, const int32_t *lens,
+                           const int32_t *parents, uint32_t beams, const int32_t *spare, int32_t *table_out, int32_t *lens_out,
+                           int32_t *used);
+
+/* Latent attention over a prompt, with keys and values expanded: q [n][heads][key + rot] every q_stride values, k
+ * [n][heads][key], tokens k_stride apart and heads k_head (so keys and values may lie beside each other), v
+ * [n][heads][value] likewise, r [n][rot] every r_stride values the key part that all heads share, out [n][heads][value].
+ * Scores scale (q[:key].k + q[key:].r). Documents, prefixes and masked values as in ocr_attention_device; key and value at
+ * most 256, rot at most 128. Fast up to keys of 128, values of 128 and rot of 64, all multiples of 8, strides of 8 and addresses of 16 bytes. */
+typedef struct ocr_latent_attention_args {
+    const void *q;
+    const void *k;
+    const void *r;
+    const void *v;
+    void *out;
+    int32_t type;
+    uint32_t n;
+    uint32_t heads;
+    uint32_t key;
+    uint32_t rot;
+    uint32_t value;
+    int64_t q_stride;
+    int64_t k_stride;
+    int64_t k_head;
+    int64_t r_stride;
+    int64_t v_stride;
+    int64_t v_head;
+    int64_t out_stride;
+    const int32_t *docs;
+    uint32_t ndocs;
+    const int32_t *prefix;
+    float scale;
+} ocr_latent_attention_args;
+int ocr_latent_attention_device(ocr_ctx *ctx, const ocr_latent_attention_args *args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -131,3 +131,83 @@ def fork(table, lens, parents, spare, page):
                 out[r, full] = spare[r]
             seen.add(p)
     return out, new, used, copies
+
+
+# ---- images' positions, eviction, latent attention ------------------------------------------------
+def pair_axes(pairs, order):
+    """(axis, place among its pairs) of each pair of a rotation."""
+    if order == "blocks":
+        return [(a, j) for a, n in enumerate(pairs) for j in range(n)]
+    return [(a, j) for j in range(max(pairs)) for a, n in enumerate(pairs) if j < n]
+
+
+def rotate_axes(x, at, first, rot, theta, pairs, axes, order, ladder, back=False):
+    """x [n][heads][dim] with rot values from `first` on rotated by positions at [n][axes]."""
+    y = np.asarray(x, np.float64).copy()
+    for i, (a, j) in enumerate(pair_axes(axes, order)):
+        c, d = (i, i + rot // 2) if pairs == "halves" else (2 * i, 2 * i + 1)
+        c, d = c + first, d + first
+        ang = at[:, a].astype(np.float64)[:, None] * theta ** -(2.0 * i / rot if ladder == "shared" else j / axes[a])
+        ang = -ang if back else ang
+        y[..., c] = x[..., c] * np.cos(ang) - x[..., d] * np.sin(ang)
+        y[..., d] = x[..., d] * np.cos(ang) + x[..., c] * np.sin(ang)
+    return y
+
+
+def prompt_weights(q, k, docs, prefix, scale, cap=0.0, slopes=None, window=None):
+    """(weights [documents][kv heads][longest], largest |score|): what each key got from its document's queries."""
+    q, k = (np.asarray(x, np.float64) for x in (q, k))
+    n, hq, hk = len(q), q.shape[1], k.shape[1]
+    docs = [0, n] if docs is None else list(docs)
+    out = np.zeros((len(docs) - 1, hk, max([b - a for a, b in zip(docs, docs[1:])] + [0])))
+    lo, hi = key_ranges(n, docs, prefix)
+    top = 0.0
+    for d, (a, b) in enumerate(zip(docs, docs[1:])):
+        for i in range(max(a, b - window if window else a), b):
+            for h in range(hq):
+                s = k[lo[i]:hi[i], h // (hq // hk)] @ q[i, h] * scale
+                bias = 0.0 if slopes is None else -float(slopes[h]) * np.abs(i - np.arange(lo[i], hi[i]))
+                out[d, h // (hq // hk), lo[i] - a: hi[i] - a] += weights(s, cap, bias)
+                top = max(top, np.abs(s[np.isfinite(s)]).max(initial=0))
+    return out, top
+
+
+def evict(weights, held, n, newest, keep, first, recent):
+    """For one sequence and head: (moves [(from, to)], weights, held) after the eviction; weights, held [places]."""
+    left = min(n, keep)
+    pos = [int(held[p]) if held[p] >= 0 else int(newest) - (n - 1 - p) for p in range(n)]
+    safe = [p < first or p > newest - recent for p in pos]
+    rank = sorted(range(n), key=lambda p: (not safe[p], np.isnan(weights[p]) and not safe[p],
+                                           0 if safe[p] or np.isnan(weights[p]) else -weights[p], p))
+    kept = set(rank[:left])
+    moves = list(zip([p for p in range(left, n) if p in kept], [p for p in range(left) if p not in kept]))
+    w, h = np.zeros_like(weights), np.full_like(held, -1)
+    w[:left], h[:left] = weights[:left], pos[:left]
+    for src, dst in moves:
+        w[dst], h[dst] = weights[src], pos[src]
+    return moves, w, h
+
+
+def latent(q, c, rank, scale):
+    """(o, sum of p |v|, largest |score|) for q [heads][rank + rot] over latent vectors c [positions][rank + rot]."""
+    if not len(c):
+        return np.zeros((len(q), rank)), np.zeros((len(q), rank)), 0.0
+    s = q @ c.T * scale
+    w = weights(s, 0.0, 0.0)
+    return w @ c[:, :rank], w @ np.abs(c[:, :rank]), np.abs(s).max()
+
+
+def latent_prompt(q, k, r, v, ranges, scale):
+    """(o, sum of p |v|, largest |score|) with keys [n][heads][key] and r [n][rot] beside them."""
+    if r is not None:
+        k = np.concatenate([k, np.repeat(r[:, None], k.shape[1], 1)], 2)
+    out, size, top = np.zeros(v.shape), np.zeros(v.shape), 0.0
+    for i in range(len(q)):
+        lo, hi = ranges[0][i], ranges[1][i]
+        for h in range(q.shape[1] if hi > lo else 0):
+            s = k[lo:hi, h] @ q[i, h] * scale
+            w = weights(s, 0.0, 0.0)
+            vv = np.where(w[:, None] > 0, v[lo:hi, h], 0)
+            out[i, h], size[i, h] = w @ vv, w @ np.abs(vv)
+            top = max(top, np.abs(s[np.isfinite(s)]).max(initial=0))
+    return out, size, top

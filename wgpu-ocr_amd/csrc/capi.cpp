@@ -1190,6 +1190,35 @@ PageTable table_of(const ocr_page_table *t) {
     need(t, "page table");
     return {t->table, t->rows, t->width};
 }
+AppendArgs append_of(const ocr_kv_cache *cache, const ocr_page_table *pages, const ocr_kv_append_args *args) {
+    need(args, "args");
+    const ocr_kv_append_args &x = *args;
+    return {cache_of(cache), table_of(pages), x.seq, x.pos, x.qkv, x.type, x.n, x.q_heads, x.stride, x.q_norm, x.k_norm,
+            x.eps, x.rot, std::log2(x.theta), x.adjacent, x.q, x.k, x.out_type};
+}
+AttentionArgs attention_of(const ocr_attention_args *args) {
+    need(args, "args");
+    const ocr_attention_args &x = *args;
+    return {x.q, x.k, x.v, x.out, x.type, x.n, x.q_heads, x.kv_heads, x.dim, x.q_stride, x.k_stride, x.v_stride,
+            x.out_stride, x.docs, x.ndocs, x.prefix, x.scale, x.cap, x.slopes};
+}
+DecodeArgs decode_of(const ocr_kv_cache *cache, const ocr_page_table *pages, const ocr_decode_args *args) {
+    need(args, "args");
+    const ocr_decode_args &x = *args;
+    return {cache_of(cache), table_of(pages), x.lens, x.q, x.out, x.type, x.q_heads, x.q_stride, x.out_stride, x.scale, x.cap, x.slopes};
+}
+// The axes' positions and what each pair goes by, for n tokens.
+template <class A> void take_axes(A &a, const ocr_axes *axes, uint32_t rot) {
+    need(axes, "axes");
+    Axes x{axes->at, axes->count, {}, axes->in_turn, axes->own_ladder};
+    for (int k = 0; k < 4; k++) x.pairs[k] = axes->pairs[k];
+    check_axes(x, rot, a.n);
+    a.at = x.at, a.axes = axis_map(x.count, x.pairs, x.in_turn, x.own);
+}
+LatentCache latent_of(const ocr_latent_cache *c) {
+    need(c, "latent cache");
+    return {c->data, c->pages, c->page, c->rank, c->rot, c->type};
+}
 
 }  // namespace
 
@@ -1198,10 +1227,7 @@ extern "C" {
 int ocr_kv_append_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_table *pages, const ocr_kv_append_args *args) {
     return guard([&] {
         need(ctx, "ctx");
-        need(args, "args");
-        const ocr_kv_append_args &x = *args;
-        const AppendArgs a{cache_of(cache), table_of(pages), x.seq, x.pos, x.qkv, x.type, x.n, x.q_heads, x.stride, x.q_norm, x.k_norm,
-                           x.eps, x.rot, std::log2(x.theta), x.adjacent, x.q, x.k, x.out_type};
+        const AppendArgs a = append_of(cache, pages, args);
         if (!check_append(a)) return;
         ctx->ctx->bind();
         launch_append(a, ctx->ctx->stream());
@@ -1222,10 +1248,7 @@ int ocr_kv_read_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_t
 int ocr_attention_device(ocr_ctx *ctx, const ocr_attention_args *args) {
     return guard([&] {
         need(ctx, "ctx");
-        need(args, "args");
-        const ocr_attention_args &x = *args;
-        const AttentionArgs a{x.q, x.k, x.v, x.out, x.type, x.n, x.q_heads, x.kv_heads, x.dim, x.q_stride, x.k_stride, x.v_stride,
-                              x.out_stride, x.docs, x.ndocs, x.prefix, x.scale, x.cap, x.slopes};
+        const AttentionArgs a = attention_of(args);
         if (!check_attention(a)) return;
         ctx->ctx->bind();
         launch_attention(a, ctx->ctx->stream());
@@ -1236,10 +1259,7 @@ int ocr_decode_attention_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const o
                                 const ocr_decode_args *args) {
     return guard([&] {
         need(ctx, "ctx");
-        need(args, "args");
-        const ocr_decode_args &x = *args;
-        const DecodeArgs a{cache_of(cache), table_of(pages), x.lens, x.q, x.out, x.type, x.q_heads, x.q_stride, x.out_stride, x.scale,
-                           x.cap, x.slopes};
+        const DecodeArgs a = decode_of(cache, pages, args);
         if (!check_decode(a)) return;
         ctx->ctx->bind();
         launch_decode(*ctx->ctx, a, ctx->ctx->stream());
@@ -1268,6 +1288,129 @@ int ocr_kv_fork_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_t
         if (!check_fork(a)) return;
         ctx->ctx->bind();
         launch_fork(a, ctx->ctx->stream());
+    });
+}
+
+int ocr_kv_append_axes_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_table *pages, const ocr_kv_append_args *args,
+                              const ocr_axes *axes) {
+    return guard([&] {
+        need(ctx, "ctx");
+        AppendArgs a = append_of(cache, pages, args);
+        const bool any = check_append(a);
+        take_axes(a, axes, a.rot);
+        if (!any) return;
+        ctx->ctx->bind();
+        launch_append(a, ctx->ctx->stream());
+    });
+}
+
+int ocr_rotate_device(ocr_ctx *ctx, const ocr_rotate_args *args, const ocr_axes *axes) {
+    return guard([&] {
+        need(ctx, "ctx");
+        need(args, "args");
+        const ocr_rotate_args &x = *args;
+        RotateArgs a{x.x, x.out, x.type, x.n, x.heads, x.dim, x.x_stride, x.x_head, x.out_stride, x.out_head, x.first, x.rot,
+                     std::log2(x.theta), x.adjacent, x.back, nullptr, {}};
+        const bool any = check_rotate(a);
+        take_axes(a, axes, a.rot);
+        if (!any) return;
+        ctx->ctx->bind();
+        launch_rotate(a, ctx->ctx->stream());
+    });
+}
+
+int ocr_attention_weights_device(ocr_ctx *ctx, const ocr_attention_args *args, float *weights, uint32_t most, uint32_t window) {
+    return guard([&] {
+        need(ctx, "ctx");
+        const AttentionArgs a = attention_of(args);
+        const Weights w{weights, most, window};
+        const bool any = check_weights(w, a.docs ? a.ndocs : 1);
+        if (!check_attention(a)) return;
+        ctx->ctx->bind();
+        if (any) launch_attention_weights(*ctx->ctx, a, w, ctx->ctx->stream());
+        else launch_attention(a, ctx->ctx->stream());
+    });
+}
+
+int ocr_decode_attention_weights_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_table *pages,
+                                        const ocr_decode_args *args, float *weights, uint32_t most) {
+    return guard([&] {
+        need(ctx, "ctx");
+        const DecodeArgs a = decode_of(cache, pages, args);
+        const Weights w{weights, most, 0};
+        const bool any = check_weights(w, a.table.rows);
+        if (!check_decode(a)) return;
+        ctx->ctx->bind();
+        if (any) launch_decode_weights(*ctx->ctx, a, w, ctx->ctx->stream());
+        else launch_decode(*ctx->ctx, a, ctx->ctx->stream());
+    });
+}
+
+int ocr_kv_evict_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_table *pages, const ocr_evict_args *args) {
+    return guard([&] {
+        need(ctx, "ctx");
+        need(args, "args");
+        const ocr_evict_args &x = *args;
+        const EvictArgs a{cache_of(cache), table_of(pages), x.lens, x.newest, x.weights, x.held, x.most, x.keep, x.first, x.recent,
+                          x.weights_out, x.held_out, x.lens_out};
+        if (!check_evict(a)) return;
+        ctx->ctx->bind();
+        launch_evict(*ctx->ctx, a, ctx->ctx->stream());
+    });
+}
+
+int ocr_latent_append_device(ocr_ctx *ctx, const ocr_latent_cache *cache, const ocr_page_table *pages, const ocr_latent_append_args *args,
+                             const ocr_axes *axes) {
+    return guard([&] {
+        need(ctx, "ctx");
+        need(args, "args");
+        const ocr_latent_append_args &x = *args;
+        LatentAppendArgs a{latent_of(cache), table_of(pages), x.seq, x.pos, x.x, x.type, x.n, x.stride, x.norm, x.eps, std::log2(x.theta),
+                           x.adjacent, x.out, nullptr, {}};
+        const bool any = check_latent_append(a);
+        if (axes) take_axes(a, axes, a.c.rot);
+        if (!any) return;
+        ctx->ctx->bind();
+        launch_latent_append(a, ctx->ctx->stream());
+    });
+}
+
+int ocr_latent_decode_device(ocr_ctx *ctx, const ocr_latent_cache *cache, const ocr_page_table *pages, const ocr_latent_decode_args *args) {
+    return guard([&] {
+        need(ctx, "ctx");
+        need(args, "args");
+        const ocr_latent_decode_args &x = *args;
+        const LatentDecodeArgs a{latent_of(cache), table_of(pages), x.lens, x.q, x.out, x.heads, x.q_stride, x.out_stride, x.scale};
+        if (!check_latent_decode(a)) return;
+        ctx->ctx->bind();
+        launch_latent_decode(*ctx->ctx, a, ctx->ctx->stream());
+    });
+}
+
+int ocr_latent_fork_device(ocr_ctx *ctx, const ocr_latent_cache *cache, const ocr_page_table *pages, const int32_t *lens,
+                           const int32_t *parents, uint32_t beams, const int32_t *spare, int32_t *table_out, int32_t *lens_out,
+                           int32_t *used) {
+    return guard([&] {
+        need(ctx, "ctx");
+        const LatentCache c = latent_of(cache);
+        const ForkArgs a{{c.p, nullptr, nullptr, nullptr, c.pages, 1, c.page, c.rank + c.rot, c.type}, table_of(pages), lens, parents, beams,
+                         spare, table_out, lens_out, used};
+        if (!check_latent_fork(c, a)) return;
+        ctx->ctx->bind();
+        launch_fork(a, ctx->ctx->stream());
+    });
+}
+
+int ocr_latent_attention_device(ocr_ctx *ctx, const ocr_latent_attention_args *args) {
+    return guard([&] {
+        need(ctx, "ctx");
+        need(args, "args");
+        const ocr_latent_attention_args &x = *args;
+        const LatentAttentionArgs a{x.q, x.k, x.r, x.v, x.out, x.type, x.n, x.heads, x.key, x.rot, x.value, x.q_stride, x.k_stride, x.k_head,
+                                    x.r_stride, x.v_stride, x.v_head, x.out_stride, x.docs, x.ndocs, x.prefix, x.scale};
+        if (!check_latent_attention(a)) return;
+        ctx->ctx->bind();
+        launch_latent_attention(a, ctx->ctx->stream());
     });
 }
 

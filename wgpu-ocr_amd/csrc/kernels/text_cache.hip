@@ -33,14 +33,6 @@ template <class C> __device__ inline float code_max_over(float m, float scale) {
     return __fmaf_rn(__fmaf_rn(-m, r, code_max<C>), r * (1.f / code_max<C>), r);
 }
 
-// The cosine and sine of pair i of rot / 2 at a position. The turns in float64: float32 angles of far
-// positions would be off by whole steps of the rotation.
-__device__ inline float2 turn_of(int pos, int i, int rot, double log2_theta) {
-    const double turns = double(pos) * (exp2(-2.0 * i / double(rot) * log2_theta) * 0.15915494309189533577);
-    float2 r;
-    sincospif(2.f * float(turns - rint(turns)), &r.y, &r.x);
-    return r;
-}
 
 // Vectors that are no whole eights, or whose rotated halves are not: one wavefront a (token, head), lane l holds values l,
 // l + 64, ... of the head's vector. 20 000 tokens of 48 heads of 64 with 36 values rotated: 324 us (all 64: 64).
@@ -73,7 +65,7 @@ template <class T, class O, class C> __global__ __launch_bounds__(64) void appen
             const int i = a.adjacent ? c >> 1 : c % half;
             const bool second = a.adjacent ? c & 1 : c >= half;
             const int other = a.adjacent ? c ^ 1 : second ? c - half : c + half;
-            const float2 r = turn_of(pos, i, a.rot, a.log2_theta);
+            const float2 r = turn_of(a, t, i, a.rot);
             const float cs = r.x, sn = r.y;
             x[u] = second ? x[u] * cs + s_x[other] * sn : x[u] * cs - s_x[other] * sn;
         }
@@ -223,7 +215,7 @@ template <class T, class O, class C, int W> __global__ __launch_bounds__(256) vo
     }
     for (int x = tid; x < n * half; x += 256) {
         const int t = x / half, i = x - t * half;
-        const float2 r = turn_of(a.pos[t0 + t], i, a.rot, a.log2_theta);
+        const float2 r = turn_of(a, t0 + t, i, a.rot);
         s_cos[t][i] = r.x, s_sin[t][i] = r.y;
     }
     if (tid < n) {
@@ -407,6 +399,10 @@ template <class P> __global__ __launch_bounds__(256) void fork_kernel(ForkArgs a
     P *kd = reinterpret_cast<P *>(static_cast<char *>(a.kv.k) + d0 * vec), *vd = reinterpret_cast<P *>(static_cast<char *>(a.kv.v) + d0 * vec);
     const uint32_t n = uint32_t(f.tail * vec / sizeof(P));
     uint32_t i = threadIdx.x;
+    if (!a.kv.v) {  // latent vectors
+        for (; i < n; i += 256) kd[i] = ks[i];
+        return;
+    }
     for (; i + 768 < n; i += 1024) {  // all on their way before the first is written
         P x[4], y[4];
 #pragma unroll
@@ -418,6 +414,30 @@ template <class P> __global__ __launch_bounds__(256) void fork_kernel(ForkArgs a
     if (coded)
         for (uint32_t e = threadIdx.x; e < f.tail; e += 256)
             a.kv.k_scale[d0 + e] = a.kv.k_scale[s0 + e], a.kv.v_scale[d0 + e] = a.kv.v_scale[s0 + e];
+}
+
+// A thread a pair, or a value that is not rotated: sizes that are no eights.
+template <class T> __global__ __launch_bounds__(256) void rotate_row_kernel(RotateArgs a) {
+    const uint32_t half = a.rot / 2, each = a.dim - half;  // a vector's items
+    const T *const x = static_cast<const T *>(a.x);
+    T *const y = static_cast<T *>(a.out);
+    const int64_t t = blockIdx.x;
+    for (uint32_t item = threadIdx.x; item < a.heads * each; item += 256) {
+        const uint32_t h = item / each, e = item - h * each;
+        const T *from = x + t * a.x_stride + h * a.x_head;
+        T *to = y + t * a.out_stride + h * a.out_head;
+        if (e >= half) {
+            const uint32_t c = e - half < a.first ? e - half : e + half;
+            if (from != to) to[c] = from[c];
+            continue;
+        }
+        const uint32_t i = a.first + (a.adjacent ? 2 * e : e), j = i + (a.adjacent ? 1 : half);
+        float2 r = turned(double(a.at[t * a.axes.count + a.axes.axis[e]]) * turns_a_step(a, e, a.rot));
+        if (a.back) r.y = -r.y;
+        const float p = to_f32(from[i]), q = to_f32(from[j]);
+        to[i] = T(p * r.x - q * r.y);
+        to[j] = T(q * r.x + p * r.y);
+    }
 }
 
 // f(lanes of a vector): the power of two that holds its eights.
@@ -453,6 +473,13 @@ void launch_append(const AppendArgs &a, hipStream_t s) {
             });
         });
     });
+    OCR_HIP(hipGetLastError());
+}
+
+void launch_rotate(const RotateArgs &a, hipStream_t s) {
+    const double values = double(a.n) * a.heads * a.dim;
+    ProbeScope probe("text_rotate", s, 3 * values, 2 * values * type_bytes(a.type), "text_rotate_row");
+    with_type(a.type, [&](auto t) { hipLaunchKernelGGL((rotate_row_kernel<decltype(t)>), dim3(a.n), dim3(256), 0, s, a); });
     OCR_HIP(hipGetLastError());
 }
 

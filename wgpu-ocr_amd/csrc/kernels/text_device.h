@@ -130,6 +130,24 @@ template <class C> constexpr float code_max = std::is_same_v<C, int8_t> ? 127.f 
 // Vectors whose largest value is under this are held as zeros: 448 over it still is a float.
 constexpr float kTinyMax = 1e-30f;
 
+// The cosine and sine of pair i of a rotation of rot values at a token's position, or its position on the pair's axis
+// (A: arguments with log2_theta, at, axes). The turns in float64: float32 angles of far positions would
+// be off by whole steps of the rotation.
+template <class A> __device__ inline double turns_a_step(const A &a, int i, int rot) {
+    const bool own = a.axes.count && a.axes.own;
+    const double over = own ? double(a.axes.pairs[a.axes.axis[i]]) : double(rot), part = own ? double(a.axes.place[i]) : 2.0 * i;
+    return exp2(-part / over * a.log2_theta) * 0.15915494309189533577;
+}
+__device__ inline float2 turned(double turns) {
+    float2 r;
+    sincospif(2.f * float(turns - rint(turns)), &r.y, &r.x);
+    return r;
+}
+template <class A> __device__ inline float2 turn_of(const A &a, int64_t t, int i, int rot) {
+    const int pos = a.axes.count ? a.at[t * a.axes.count + a.axes.axis[i]] : a.pos[t];
+    return turned(double(pos) * turns_a_step(a, i, rot));
+}
+
 // Over a wavefront, without LDS: each row of 16 lanes, then the rows in order; the last lane has the
 // result.
 template <int Ctrl, int Rows, class V> __device__ inline V dpp(V old, V v) {
@@ -171,10 +189,11 @@ __device__ inline int wave_min_i(int v) { return -1 - wave_max_i(-1 - v); }
 // One query's attention over keys [lo, hi) by one wavefront, by the formula: the scores' maximum
 // first, then exp(s - max) and the value sums, all in float32. q: the query's dim values in LDS,
 // scaled; kv.k(j, c) and kv.v(j, c): value c of key and value vector j. Scores of minus infinity
-// weigh nothing, a query that sees nothing gives zeros. done(c, value) gets each of the outputs.
+// weigh nothing, a query that sees nothing gives zeros. done(c, value) gets each of the outputs. values: how many a
+// value vector has (at most 256), if not as many as a key.
 template <class KV, class Done>
-__device__ inline void attend_row(const KV &kv, const float *q, int dim, int lo, int hi, int pos, float cap, float slope, Done &&done) {
-    const int lane = threadIdx.x & 63;
+__device__ inline void attend_row(const KV &kv, const float *q, int dim, int lo, int hi, int pos, float cap, float slope, Done &&done, int values = 0) {
+    const int lane = threadIdx.x & 63, outs = values ? values : dim;
     const Cap most = cap_of(cap, 1.f);
     auto score = [&](int j) {
         float s = 0.f;
@@ -200,12 +219,12 @@ __device__ inline void attend_row(const KV &kv, const float *q, int dim, int lo,
             if (w == 0.f) continue;
 #pragma unroll
             for (int u = 0; u < 4; u++)
-                if (lane + 64 * u < dim) o[u] = __fmaf_rn(w, kv.v(j0 + t, lane + 64 * u), o[u]);
+                if (lane + 64 * u < outs) o[u] = __fmaf_rn(w, kv.v(j0 + t, lane + 64 * u), o[u]);
         }
     }
     l = wave_sum(l);
     for (int u = 0; u < 4; u++)
-        if (lane + 64 * u < dim) done(lane + 64 * u, l == 0.f ? 0.f : o[u] / l);
+        if (lane + 64 * u < outs) done(lane + 64 * u, l == 0.f ? 0.f : o[u] / l);
 }
 
 }  // namespace ocr

@@ -51,7 +51,96 @@ struct AppendArgs {
     int adjacent;
     void *q, *k;
     int out_type;
+    const int32_t *at = nullptr;  // with axes: [n][axes.count] positions that the rotation goes by
+    AxisMap axes{};
 };
+
+// Positions of several axes, as in the C ABI (ocr_axes).
+struct Axes {
+    const int32_t *at;
+    uint32_t count;
+    uint32_t pairs[4];
+    int in_turn, own;
+};
+
+struct RotateArgs {
+    const void *x;
+    void *out;
+    int type;
+    uint32_t n, heads, dim;
+    int64_t x_stride, x_head, out_stride, out_head;
+    uint32_t first, rot;
+    double log2_theta;
+    int adjacent, back;
+    const int32_t *at;
+    AxisMap axes;
+};
+
+// What attention adds up: weights [sequences or documents][key heads][most]; window: a document's last queries that
+// count (0: all of them).
+struct Weights {
+    float *p;
+    uint32_t most, window;
+};
+
+struct EvictArgs {
+    KvCache kv;
+    PageTable table;
+    const int32_t *lens, *newest;
+    const float *weights;
+    const int32_t *held;
+    uint32_t most, keep, first, recent;
+    float *weights_out;
+    int32_t *held_out, *lens_out;
+};
+
+// A pool of latent vectors [pages][page][rank + rot].
+struct LatentCache {
+    void *p;
+    uint32_t pages, page, rank, rot;
+    int type;
+};
+
+struct LatentAppendArgs {
+    LatentCache c;
+    PageTable table;
+    const int32_t *seq, *pos;
+    const void *x;
+    int type;
+    uint32_t n;
+    int64_t stride;
+    const float *norm;
+    float eps;
+    double log2_theta;
+    int adjacent;
+    void *out;
+    const int32_t *at;
+    AxisMap axes;
+};
+
+struct LatentDecodeArgs {
+    LatentCache c;
+    PageTable table;
+    const int32_t *lens;
+    const void *q;
+    void *out;
+    uint32_t heads;
+    int64_t q_stride, out_stride;
+    float scale;
+};
+
+struct LatentAttentionArgs {
+    const void *q, *k, *r, *v;
+    void *out;
+    int type;
+    uint32_t n, heads, key, rot, value;
+    int64_t q_stride, k_stride, k_head, r_stride, v_stride, v_head, out_stride;
+    const int32_t *docs;
+    uint32_t ndocs;
+    const int32_t *prefix;
+    float scale;
+};
+constexpr uint32_t kMostRank = 512, kMostLatentRot = 128;
 
 struct ReadArgs {
     KvCache kv;
@@ -117,12 +206,27 @@ bool check_attention(const AttentionArgs &a);
 bool check_decode(const DecodeArgs &a);
 bool check_fork(const ForkArgs &a);
 bool check_beam(const BeamArgs &a);
+void check_axes(const Axes &x, uint32_t rot, uint32_t n);
+bool check_rotate(const RotateArgs &a);
+bool check_weights(const Weights &w, uint32_t rows);
+bool check_evict(const EvictArgs &a);
+bool check_latent_append(const LatentAppendArgs &a);
+bool check_latent_decode(const LatentDecodeArgs &a);
+bool check_latent_fork(const LatentCache &c, const ForkArgs &a);
+bool check_latent_attention(const LatentAttentionArgs &a);
 
 // The launches (arguments checked), queued on s.
 void launch_append(const AppendArgs &a, hipStream_t s);
 void launch_read(const ReadArgs &a, hipStream_t s);
+void launch_rotate(const RotateArgs &a, hipStream_t s);
 void launch_attention(const AttentionArgs &a, hipStream_t s);
+void launch_attention_weights(Ctx &c, const AttentionArgs &a, const Weights &w, hipStream_t s);
 void launch_decode(Ctx &c, const DecodeArgs &a, hipStream_t s);
+void launch_decode_weights(Ctx &c, const DecodeArgs &a, const Weights &w, hipStream_t s);
+void launch_evict(Ctx &c, const EvictArgs &a, hipStream_t s);
+void launch_latent_append(const LatentAppendArgs &a, hipStream_t s);
+void launch_latent_decode(Ctx &c, const LatentDecodeArgs &a, hipStream_t s);
+void launch_latent_attention(const LatentAttentionArgs &a, hipStream_t s);
 void launch_fork(const ForkArgs &a, hipStream_t s);
 void launch_beam(Ctx &c, const BeamArgs &a, hipStream_t s);
 

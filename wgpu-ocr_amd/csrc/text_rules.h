@@ -66,6 +66,31 @@ OCR_HD KeyRange key_range(int i, int n, const int32_t *docs, int ndocs, const in
     return {a, top < b ? top : b};
 }
 
+// The queries [lo, hi) of a packed row that see key j: those of its document from itself on, all of them where the
+// document's prefix holds it; with `window` > 0 only the document's last `window` of them. doc, place: the
+// key's document and its place in it (doc -1: in none, which nothing sees).
+struct QueryRange {
+    int lo, hi, doc, place;
+};
+OCR_HD QueryRange query_range(int j, int n, const int32_t *docs, int ndocs, const int32_t *prefix, int window) {
+    int a = 0, b = n, d = 0;
+    if (docs) {
+        int lo = 0, hi = ndocs;  // the last document that starts at or before j
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (docs[mid] <= j) lo = mid + 1;
+            else hi = mid;
+        }
+        if (lo == 0 || docs[lo] <= j) return {0, 0, -1, 0};
+        d = lo - 1;
+        a = docs[d] < 0 ? 0 : docs[d];
+        b = docs[lo] > n ? n : docs[lo];
+    }
+    int first = prefix && j - a < prefix[d] ? a : j;
+    if (window > 0 && b - window > first) first = b - window;
+    return {first, b, d, j - a};
+}
+
 // A row of a reordered table: what beam w of a group takes from its parent. len: the parent's
 // length; full pages are shared, a part-filled last page goes to the first child and is copied for
 // the others.
@@ -85,6 +110,43 @@ OCR_HD Fork fork_of(const int32_t *parents, uint32_t beams, uint32_t w, const in
     for (uint32_t e = 0; e < w; e++) first = first && parents[e] != p;
     f.copy = f.tail > 0 && !first;
     return f;
+}
+
+// The axis of each of a rotation's pairs, its place among that axis' pairs, and how many those are: `pairs`
+// of each of `count` axes in blocks, or of one axis after another in turn as long as each has some.
+struct AxisMap {
+    uint8_t axis[128], place[128];
+    uint8_t pairs[4];
+    uint8_t count, own;  // no axes: 0; own: each axis has the whole range of frequencies
+};
+OCR_HD AxisMap axis_map(uint32_t count, const uint32_t *pairs, bool in_turn, bool own) {
+    AxisMap m{};
+    m.count = uint8_t(count), m.own = own;
+    int at = 0;
+    for (uint32_t k = 0; k < count; k++) m.pairs[k] = uint8_t(pairs[k]);
+    for (uint32_t round = 0; round < (in_turn ? 128u : count); round++)
+        for (uint32_t x = 0; x < (in_turn ? count : pairs[round]); x++) {
+            const uint32_t a = in_turn ? x : round, place = in_turn ? round : x;
+            if (place >= pairs[a] || at >= 128) continue;
+            m.axis[at] = uint8_t(a), m.place[at] = uint8_t(place);
+            at++;
+        }
+    return m;
+}
+
+// What an eviction orders a cached token by, the largest first: protected ones, then the others by their
+// weight (as floats order, the zeros alike), NaN last. Equal ones go by their place, the lowest first.
+constexpr uint32_t kProtected = 0xffffffffu;
+OCR_HD uint32_t weight_key(float w) {
+    if (w != w) return 0;
+    const uint32_t u = __builtin_bit_cast(uint32_t, w == 0.f ? 0.f : w);
+    return u >> 31 ? ~u : u | 0x80000000u;  // minus infinity's is 0x007fffff, infinity's 0xff800000
+}
+// The position of the token at place p of n: what is held, or, where that is negative, as far before the
+// newest as its place is before the last.
+OCR_HD int64_t held_position(int32_t held, int p, int n, int32_t newest) { return held >= 0 ? held : int64_t(newest) - (n - 1 - p); }
+OCR_HD bool is_protected(int64_t pos, int32_t newest, uint32_t first, uint32_t recent) {
+    return pos < int64_t(first) || pos > int64_t(newest) - int64_t(recent);
 }
 
 // tanh(y) / y by powers of u = y^2, interpolated at the Chebyshev points of [0, 0.35^2]: up to there off by

@@ -116,6 +116,15 @@ SIGNATURES = {
     "ocr_attention_device": (ctypes.c_int, [P, P]),
     "ocr_decode_attention_device": (ctypes.c_int, [P, P, P, P]),
     "ocr_beam_select_device": (ctypes.c_int, [P, P]),
+    "ocr_kv_append_axes_device": (ctypes.c_int, [P, P, P, P, P]),
+    "ocr_rotate_device": (ctypes.c_int, [P, P, P]),
+    "ocr_attention_weights_device": (ctypes.c_int, [P, P, P, U32, U32]),
+    "ocr_decode_attention_weights_device": (ctypes.c_int, [P, P, P, P, P, U32]),
+    "ocr_kv_evict_device": (ctypes.c_int, [P, P, P, P]),
+    "ocr_latent_append_device": (ctypes.c_int, [P, P, P, P, P]),
+    "ocr_latent_decode_device": (ctypes.c_int, [P, P, P, P]),
+    "ocr_latent_fork_device": (ctypes.c_int, [P, P, P, P, P, U32, P, P, P, P]),
+    "ocr_latent_attention_device": (ctypes.c_int, [P, P]),
     "ocr_kv_fork_device": (ctypes.c_int, [P, P, P, P, P, U32, P, P, P, P]),
 }
 
@@ -578,6 +587,7 @@ ND_FAMILIES = ("conv3x3_dma", "gemm_dma", "conv_narrow", "conv_igemm", "conv_mfm
                "nd_reduce", "nd_layer_norm", "nd_softmax", "nd_argmax", "nd_pool", "nd_resize", "nd_det_prep",
                "nd_threshold")
 TEXT_FAMILIES = ("text_append", "text_read", "text_attention", "text_decode", "text_fork", "beam_select")
+MORE_TEXT_FAMILIES = ("text_rotate", "text_weights", "text_evict", "latent_append", "latent_decode", "latent_attention")
 
 
 def probe_start(family: str):
@@ -882,4 +892,4 @@ def pp_line_images(ctx: Context, rgb: np.ndarray, lines, wb: int) -> np.ndarray:
     return out
 
 
-from .text import DeviceArray, KvCache, attention, beam_select  # noqa: E402,F401
+from .text import DeviceArray, KvCache, LatentCache, attention, beam_select, latent_attention, rotate  # noqa: E402,F401

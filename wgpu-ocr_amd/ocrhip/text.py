@@ -1,5 +1,6 @@
 """A text decoder's operators (include/ocrhip.h): a paged cache of keys and values, attention over
-prompts and of single tokens over the cache, beam search.
+prompts and of single tokens over the cache, beam search; rotary positions of several axes, eviction
+from the cache by the attention weight that its keys got, latent attention.
 
 Arrays are device memory: torch tensors on the context's device, or DeviceArray over a
 DeviceBuffer. A head's values, and the heads of a token, lie one after another; tokens may lie
@@ -48,6 +49,39 @@ class ocr_decode_args(ctypes.Structure):
 class ocr_beam_args(ctypes.Structure):
     _fields_ = [("logits", P), ("type", I32), ("groups", U32), ("beams", U32), ("vocab", U32), ("stride", I64), ("scores", P),
                 ("finished", P), ("eos", I32), ("out_scores", P), ("parents", P), ("tokens", P), ("out_finished", P)]
+
+
+class ocr_axes(ctypes.Structure):
+    _fields_ = [("at", P), ("count", U32), ("pairs", U32 * 4), ("in_turn", I32), ("own_ladder", I32)]
+
+
+class ocr_rotate_args(ctypes.Structure):
+    _fields_ = [("x", P), ("out", P), ("type", I32), ("n", U32), ("heads", U32), ("dim", U32), ("x_stride", I64), ("x_head", I64),
+                ("out_stride", I64), ("out_head", I64), ("first", U32), ("rot", U32), ("theta", F64), ("adjacent", I32), ("back", I32)]
+
+
+class ocr_evict_args(ctypes.Structure):
+    _fields_ = [("lens", P), ("newest", P), ("weights", P), ("held", P), ("most", U32), ("keep", U32), ("first", U32), ("recent", U32),
+                ("weights_out", P), ("held_out", P), ("lens_out", P)]
+
+
+class ocr_latent_cache(ctypes.Structure):
+    _fields_ = [("data", P), ("pages", U32), ("page", U32), ("rank", U32), ("rot", U32), ("type", I32)]
+
+
+class ocr_latent_append_args(ctypes.Structure):
+    _fields_ = [("seq", P), ("pos", P), ("x", P), ("type", I32), ("n", U32), ("stride", I64), ("norm", P), ("eps", F32), ("theta", F64),
+                ("adjacent", I32), ("out", P)]
+
+
+class ocr_latent_decode_args(ctypes.Structure):
+    _fields_ = [("lens", P), ("q", P), ("out", P), ("heads", U32), ("q_stride", I64), ("out_stride", I64), ("scale", F32)]
+
+
+class ocr_latent_attention_args(ctypes.Structure):
+    _fields_ = [("q", P), ("k", P), ("r", P), ("v", P), ("out", P), ("type", I32), ("n", U32), ("heads", U32), ("key", U32), ("rot", U32),
+                ("value", U32), ("q_stride", I64), ("k_stride", I64), ("k_head", I64), ("r_stride", I64), ("v_stride", I64),
+                ("v_head", I64), ("out_stride", I64), ("docs", P), ("ndocs", U32), ("prefix", P), ("scale", F32)]
 
 
 class DeviceArray:
@@ -111,7 +145,9 @@ def _native(name, ctx, *args):
             return False
         lib = _root().lib()
         module.bind(*[ctypes.cast(getattr(lib, f"ocr_{f}_device"), ctypes.c_void_p).value
-                      for f in ("kv_append", "kv_read", "attention", "decode_attention", "beam_select", "kv_fork")])
+                      for f in ("kv_append", "kv_read", "attention", "decode_attention", "beam_select", "kv_fork", "kv_append_axes", "rotate",
+                                "attention_weights", "decode_attention_weights", "kv_evict", "latent_append", "latent_decode",
+                                "latent_attention")])
         _tensors = module
     rc = getattr(_tensors, name)(ctx.handle, ctx.device, *args)
     if rc > 0 or rc == -1:
@@ -178,8 +214,65 @@ def _tokens(ctx, x, what, types, n=None, heads=None, dim=None):
     return x.data_ptr() or None, n, heads, dim, strides[0] if n > 1 else row
 
 
+def _heads(ctx, x, what, types, n=None, heads=None, dim=None):
+    """(address, tokens, heads, dim, stride, head stride) of x [tokens][heads][dim], whose tokens and heads may lie apart."""
+    _device(ctx, x, what)
+    if _code(x, what) not in types:
+        raise _error(f"{what}: {' or '.join(_NAMES[t] for t in types)} is wanted, not {x.dtype}")
+    shape, strides = x.shape, x.stride()
+    if len(shape) != 3 or any(w is not None and w != v for w, v in zip((n, heads, dim), shape)):
+        want = tuple("any" if v is None else v for v in (n, heads, dim))
+        raise _error(f"{what}: shape {want} is wanted, not {tuple(shape)}")
+    n, heads, dim = shape
+    if n and dim > 1 and strides[2] != 1:
+        raise _error(f"{what}: a head's values do not lie one after another")
+    head = strides[1] if heads > 1 else dim
+    return x.data_ptr() or None, n, heads, dim, strides[0] if n > 1 else max((heads - 1) * head + dim, 0), head
+
+
 _I32, _F32, _F16, _ANY = (5,), (0,), (1, 2), (0, 1, 2)
 _PAIRS = {"halves": False, "adjacent": True}
+_ORDERS, _LADDERS = {"blocks": False, "turns": True}, {"shared": False, "own": True}
+
+
+def _places(x, what):
+    if len(x.shape) != 3:
+        raise _error(f"{what}: three dimensions are wanted, not {tuple(x.shape)}")
+    return tuple(x.shape)
+
+
+def _pairs_of(axes, count, rot):
+    """How many pairs of a rotation each axis has: the caller's, or as many each."""
+    if axes is None:
+        if count < 1 or rot // 2 % count:
+            raise _error(f"axes: a rotation of {rot} values in {count} equal parts")
+        return (rot // 2 // count,) * count
+    axes = tuple(axes)
+    if not 1 <= len(axes) <= 4 or any(not 0 <= v < 2 ** 32 for v in axes):
+        raise _error(f"axes: 1 to 4 numbers of pairs are wanted, not {axes}")
+    if count != len(axes):
+        raise _error(f"positions of {count} axes, and pairs of {len(axes)}")
+    return axes
+
+
+def _axes(ctx, at, axes, order, ladder, rot, n):
+    """The C ABI's axes of positions at [n][axes], or [n] for one."""
+    if order not in _ORDERS or ladder not in _LADDERS:
+        raise _error(f'axes in "blocks" or in "turns", a "shared" or an "own" ladder are wanted, not {order!r} and {ladder!r}')
+    if len(at.shape) not in (1, 2):
+        raise _error(f"positions: shape [{n}][axes] is wanted, not {tuple(at.shape)}")
+    count = at.shape[1] if len(at.shape) == 2 else 1
+    pairs = _pairs_of(axes, count, rot)
+    shape = (n, count) if len(at.shape) == 2 else (n,)
+    return ocr_axes(_array(ctx, at, "positions", _I32, shape), count, (U32 * 4)(*pairs), _ORDERS[order], _LADDERS[ladder])
+
+
+def _turn(pairs, theta, rot):
+    if pairs not in _PAIRS:
+        raise _error(f'pairs: "halves" or "adjacent" is wanted, not {pairs!r}')
+    if theta <= 0 or not 0 <= rot < 2 ** 32:
+        raise _error(f"a rotation of {rot} values to the base {theta}")
+    return _PAIRS[pairs]
 
 
 class KvCache:
@@ -221,14 +314,23 @@ class KvCache:
         return ocr_page_table(_array(self.ctx, table, "page table", _I32, (rows, width)), rows, width)
 
     def append(self, table, seq, pos, qkv, q, k=None, q_norm=None, k_norm=None, eps: float = 1e-6, rot: int | None = None,
-               theta: float = 1e4, pairs: str = "halves"):
+               theta: float = 1e4, pairs: str = "halves", at=None, axes=None, order: str = "blocks", ladder: str = "shared"):
         """Projections qkv [n][(q_heads + 2 heads) * dim] of the tokens at positions pos [n] of sequences seq [n]:
         queries and keys normed (q_norm, k_norm [dim] float32, or None) and rotated (the first rot
         values, all of them by default; pairs "halves" or "adjacent"); queries into q [n][q_heads][dim], keys and values
-        into the cache, keys into k [n][heads][dim] too if given (ocr_kv_append_device)."""
+        into the cache, keys into k [n][heads][dim] too if given (ocr_kv_append_device). With at [n][axes]
+        (int32) the rotation goes by those positions instead, as rotate() does with axes, order and ladder
+        (ocr_kv_append_axes_device)."""
         ctx, types = self.ctx, _F16
         rot = self.dim if rot is None else rot
-        if pairs in _PAIRS and _native("append", ctx, self._at, table, seq, pos, qkv, q, k, q_norm, k_norm, eps, rot, theta, _PAIRS[pairs]):
+        if at is not None:
+            if pairs in _PAIRS and order in _ORDERS and ladder in _LADDERS and _native(
+                    "append_axes", ctx, self._at, table, seq, pos, qkv, q, k, q_norm, k_norm, eps, rot, theta, _PAIRS[pairs], at, axes,
+                    _ORDERS[order], _LADDERS[ladder]):
+                return
+        elif axes is not None:
+            raise _error("axes without positions (at)")
+        elif pairs in _PAIRS and _native("append", ctx, self._at, table, seq, pos, qkv, q, k, q_norm, k_norm, eps, rot, theta, _PAIRS[pairs]):
             return
         qp, n, q_heads, dim, stride = _tokens(ctx, q, "queries", types, dim=self.dim)
         if stride != q_heads * dim:
@@ -238,16 +340,17 @@ class KvCache:
         code = _code(qkv, "projections")
         if code not in _ANY or tuple(qkv.shape) != (n, width) or (n and qkv.stride()[1] != 1):
             raise _error(f"projections: rows [{n}][{width}] of f32, f16 or bf16 are wanted, not {tuple(qkv.shape)} of {qkv.dtype}")
-        if pairs not in _PAIRS:
-            raise _error(f'pairs: "halves" or "adjacent" is wanted, not {pairs!r}')
-        if theta <= 0 or not 0 <= rot < 2 ** 32:
-            raise _error(f"a rotation of {rot} values to the base {theta}")
+        adjacent = _turn(pairs, theta, rot)
         out = _code(q, "queries")
         args = ocr_kv_append_args(_array(ctx, seq, "sequence numbers", _I32, (n,)), _array(ctx, pos, "positions", _I32, (n,)),
                                   qkv.data_ptr() or None, code, n, q_heads, qkv.stride()[0] if n > 1 else width,
                                   _array(ctx, q_norm, "q_norm", _F32, (dim,)), _array(ctx, k_norm, "k_norm", _F32, (dim,)), eps, rot,
-                                  theta, _PAIRS[pairs], qp, _array(ctx, k, "keys", (out,), (n, self.heads, dim)), out)
-        _call("ocr_kv_append_device", ctx.handle, ctypes.byref(self._c), ctypes.byref(self._table(table)), ctypes.byref(args))
+                                  theta, adjacent, qp, _array(ctx, k, "keys", (out,), (n, self.heads, dim)), out)
+        where = ctypes.byref(self._c), ctypes.byref(self._table(table)), ctypes.byref(args)
+        if at is None:
+            _call("ocr_kv_append_device", ctx.handle, *where)
+        else:
+            _call("ocr_kv_append_axes_device", ctx.handle, *where, ctypes.byref(_axes(ctx, at, axes, order, ladder, rot, n)))
 
     def read(self, table, lens, k, v):
         """The cached keys and values of every sequence's first positions into k and v
@@ -264,12 +367,14 @@ class KvCache:
         _call("ocr_kv_read_device", self.ctx.handle, ctypes.byref(self._c), ctypes.byref(t),
               _array(self.ctx, lens, "lengths", _I32, (t.rows,)), shape[1], code, kp, _array(self.ctx, v, "values", (code,), shape))
 
-    def attend(self, table, lens, q, out, scale: float | None = None, cap: float = 0.0, slopes=None):
+    def attend(self, table, lens, q, out, scale: float | None = None, cap: float = 0.0, slopes=None, weights=None):
         """Attention of every sequence's last token (lens [sequences] counts it) over its cached
-        vectors: q, out [sequences][q_heads][dim] (ocr_decode_attention_device)."""
+        vectors: q, out [sequences][q_heads][dim] (ocr_decode_attention_device). What each key got is
+        added to weights [sequences][heads][places] float32 if given, its query heads together
+        (ocr_decode_attention_weights_device)."""
         ctx = self.ctx
         scale = self.dim ** -0.5 if scale is None else scale
-        if _native("attend", ctx, self._at, table, lens, q, out, scale, cap, slopes):
+        if _native("attend", ctx, self._at, table, lens, q, out, scale, cap, slopes, weights):
             return
         t = self._table(table)
         qp, n, q_heads, dim, qs = _tokens(ctx, q, "queries", _F16, n=t.rows, dim=self.dim)
@@ -277,7 +382,35 @@ class KvCache:
         op, _, _, _, os = _tokens(ctx, out, "outputs", (code,), n, q_heads, dim)
         args = ocr_decode_args(_array(ctx, lens, "lengths", _I32, (n,)), qp, op, code, q_heads, qs, os,
                                scale, cap, _array(ctx, slopes, "slopes", _F32, (q_heads,)))
-        _call("ocr_decode_attention_device", ctx.handle, ctypes.byref(self._c), ctypes.byref(t), ctypes.byref(args))
+        if weights is None:
+            _call("ocr_decode_attention_device", ctx.handle, ctypes.byref(self._c), ctypes.byref(t), ctypes.byref(args))
+            return
+        most = _places(weights, "weights")[2]
+        _call("ocr_decode_attention_weights_device", ctx.handle, ctypes.byref(self._c), ctypes.byref(t), ctypes.byref(args),
+              _array(ctx, weights, "weights", _F32, (n, self.heads, most)), most)
+
+    def evict(self, table, lens, newest, weights, held, keep: int, lens_out, first: int = 0, recent: int = 0, weights_out=None,
+              held_out=None):
+        """Drops cached tokens until `keep` of a sequence's (lens [sequences]) are left, each head its own: the
+        least of weights [sequences][heads][places] (float32, what attend() and attention() add up), but none at a position
+        under `first` and none of the `recent` last up to newest [sequences], the position of its newest token. held, as
+        weights but int32, says which position the token at a place has, or less than 0 as long as no
+        eviction has said so. New lengths into lens_out, weights and positions into weights_out and held_out, by default
+        over the old ones; the kept vectors are in places 0 to the new length (ocr_kv_evict_device)."""
+        ctx = self.ctx
+        weights_out, held_out = weights if weights_out is None else weights_out, held if held_out is None else held_out
+        if _native("evict", ctx, self._at, table, lens, newest, weights, held, keep, lens_out, first, recent, weights_out, held_out):
+            return
+        t = self._table(table)
+        most = _places(weights, "weights")[2]
+        if any(not 0 <= v < 2 ** 32 for v in (keep, first, recent)):
+            raise _error(f"eviction: {keep} tokens to keep, {first} first and {recent} recent ones")
+        row = lambda x, what: _array(ctx, x, what, _I32, (t.rows,))  # noqa: E731
+        cell = lambda x, what, types: _array(ctx, x, what, types, (t.rows, self.heads, most))  # noqa: E731
+        args = ocr_evict_args(row(lens, "lengths"), row(newest, "newest positions"), cell(weights, "weights", _F32), cell(held, "positions", _I32),
+                              most, keep, first, recent, cell(weights_out, "new weights", _F32), cell(held_out, "new positions", _I32),
+                              row(lens_out, "the new lengths"))
+        _call("ocr_kv_evict_device", ctx.handle, ctypes.byref(self._c), ctypes.byref(t), ctypes.byref(args))
 
     def fork(self, table, lens, parents, spare, table_out, lens_out, used):
         """The tables and lengths of every group's beams after a step that continued `parents`
@@ -294,30 +427,160 @@ class KvCache:
               _array(ctx, table_out, "the new table", _I32, (t.rows, t.width)), one(lens_out, "the new lengths"), one(used, "used"))
 
 
-def attention(ctx, q, k, v, out, docs=None, prefix=None, scale: float | None = None, cap: float = 0.0, slopes=None):
+class LatentCache:
+    """A paged cache of latent vectors: pages of `page` positions that hold rank + rot values a token of type "f16" or
+    "bf16" (ocr_latent_cache). memory: the caller's [pages][page][rank + rot]; without it the cache allocates its
+    own. Tables as a KvCache's."""
+
+    _table = KvCache._table
+
+    def __init__(self, ctx, pages: int, page: int, rank: int, rot: int, dtype: str = "bf16", memory=None):
+        if dtype not in ("f16", "bf16"):
+            raise _error(f"latent cache: f16 or bf16 is wanted, not {dtype!r}")
+        if min(pages, page, rank) < 1 or rot < 0:
+            raise _error("latent cache: empty")
+        if max(pages, page, rank, rot) >= 2 ** 32:
+            raise _error(f"latent cache: sizes {(pages, page, rank, rot)} are past 32 bits")
+        self.ctx, self.pages, self.page, self.rank, self.rot, self.dtype = ctx, pages, page, rank, rot, dtype
+        shape, code = (pages, page, rank + rot), _SHORT[dtype]
+        self.data = DeviceArray(ctx.alloc(pages * page * (rank + rot) * 2), shape, dtype) if memory is None else memory
+        self._c = ocr_latent_cache(_array(ctx, self.data, "latent cache", (code,), shape), pages, page, rank, rot, code)
+        self._at = ctypes.addressof(self._c)
+
+    def append(self, table, seq, pos, x, out=None, norm=None, eps: float = 1e-6, theta: float = 1e4, pairs: str = "halves", at=None,
+               axes=None, order: str = "blocks", ladder: str = "shared"):
+        """Projections x [n][rank + rot] of the tokens at positions pos [n] of sequences seq [n]: the first rank values normed
+        (norm [rank] float32, or None), the others rotated by pos, or by at [n][axes] as rotate() does; into the
+        cache, and into out [n][rank + rot] of its type if given (ocr_latent_append_device)."""
+        ctx = self.ctx
+        if at is None and axes is not None:
+            raise _error("axes without positions (at)")
+        if pairs in _PAIRS and order in _ORDERS and ladder in _LADDERS and _native(
+                "latent_append", ctx, self._at, table, seq, pos, x, out, norm, eps, theta, _PAIRS[pairs], at, axes, _ORDERS[order],
+                _LADDERS[ladder]):
+            return
+        width = self.rank + self.rot
+        _device(ctx, x, "projections")
+        code = _code(x, "projections")
+        if code not in _ANY or len(x.shape) != 2 or x.shape[1] != width or (x.shape[0] and width > 1 and x.stride()[1] != 1):
+            raise _error(f"projections: rows [tokens][{width}] of f32, f16 or bf16 are wanted, not {tuple(x.shape)} of {x.dtype}")
+        n = x.shape[0]
+        adjacent = _turn(pairs, theta, self.rot)
+        args = ocr_latent_append_args(_array(ctx, seq, "sequence numbers", _I32, (n,)), _array(ctx, pos, "positions", _I32, (n,)),
+                                      x.data_ptr() or None, code, n, x.stride()[0] if n > 1 else width,
+                                      _array(ctx, norm, "norm", _F32, (self.rank,)), eps, theta, adjacent,
+                                      _array(ctx, out, "outputs", (self._c.type,), (n, width)))
+        turn = None if at is None else ctypes.byref(_axes(ctx, at, axes, order, ladder, self.rot, n))
+        _call("ocr_latent_append_device", ctx.handle, ctypes.byref(self._c), ctypes.byref(self._table(table)), ctypes.byref(args), turn)
+
+    def attend(self, table, lens, q, out, scale: float):
+        """Attention of every sequence's last token (lens [sequences] counts it) over its latent vectors: q
+        [sequences][heads][rank + rot] with the keys' expansion absorbed, out [sequences][heads][rank], the values' expansion to
+        follow (ocr_latent_decode_device)."""
+        ctx = self.ctx
+        if _native("latent_attend", ctx, self._at, table, lens, q, out, scale):
+            return
+        t, code = self._table(table), self._c.type
+        qp, n, heads, _, qs = _tokens(ctx, q, "queries", (code,), n=t.rows, dim=self.rank + self.rot)
+        op, _, _, _, os = _tokens(ctx, out, "outputs", (code,), n, heads, self.rank)
+        args = ocr_latent_decode_args(_array(ctx, lens, "lengths", _I32, (n,)), qp, op, heads, qs, os, scale)
+        _call("ocr_latent_decode_device", ctx.handle, ctypes.byref(self._c), ctypes.byref(t), ctypes.byref(args))
+
+    def fork(self, table, lens, parents, spare, table_out, lens_out, used):
+        """As KvCache.fork (ocr_latent_fork_device)."""
+        ctx, t = self.ctx, self._table(table)
+        if len(parents.shape) != 2 or parents.shape[0] * parents.shape[1] != t.rows:
+            raise _error(f"parents: shape [groups][beams] of {t.rows} sequences is wanted, not {tuple(parents.shape)}")
+        one = lambda x, what: _array(ctx, x, what, _I32, (t.rows,))  # noqa: E731
+        _call("ocr_latent_fork_device", ctx.handle, ctypes.byref(self._c), ctypes.byref(t), one(lens, "lengths"),
+              _array(ctx, parents, "parents", _I32, tuple(parents.shape)), parents.shape[1], one(spare, "spare pages"),
+              _array(ctx, table_out, "the new table", _I32, (t.rows, t.width)), one(lens_out, "the new lengths"), one(used, "used"))
+
+
+def rotate(ctx, x, at, out=None, first: int = 0, rot: int | None = None, theta: float = 1e4, pairs: str = "halves", axes=None,
+           order: str = "blocks", ladder: str = "shared", back: bool = False):
+    """Rotary positions of one or several axes (ocr_rotate_device): x [n][heads][dim] with its values from `first` on, rot of them (all by
+    default), rotated by positions at [n][axes] (int32; [n] for one axis) into out, or in place. axes: how many pairs each
+    axis has (as many each by default), in "blocks" or one after another in "turns"; the frequencies fall over all pairs
+    ("shared") or over each axis' own ("own"). back: the other way, which is also the gradient."""
+    out = x if out is None else out
+    rot = (x.shape[2] if len(x.shape) == 3 else 0) - first if rot is None else rot
+    if pairs in _PAIRS and order in _ORDERS and ladder in _LADDERS and _native("rotate", ctx, x, at, out, first, rot, theta, _PAIRS[pairs],
+                                                                               axes, _ORDERS[order], _LADDERS[ladder], bool(back)):
+        return
+    xp, n, heads, dim, xs, xh = _heads(ctx, x, "inputs", _ANY)
+    code = _code(x, "inputs")
+    op, _, _, _, os, oh = _heads(ctx, out, "outputs", (code,), n, heads, dim)
+    adjacent = _turn(pairs, theta, rot)
+    if not 0 <= first < 2 ** 32:
+        raise _error(f"a rotation from value {first} on")
+    args = ocr_rotate_args(xp, op, code, n, heads, dim, xs, xh, os, oh, first, rot, theta, adjacent, bool(back))
+    _call("ocr_rotate_device", ctx.handle, ctypes.byref(args), ctypes.byref(_axes(ctx, at, axes, order, ladder, rot, n)))
+
+
+def _documents(ctx, docs, prefix):
+    """The C ABI's documents: offsets, how many, prefixes."""
+    ndocs = 1
+    if docs is not None:
+        if len(docs.shape) != 1 or docs.shape[0] < 1:
+            raise _error(f"documents: offsets [documents + 1] are wanted, not {tuple(docs.shape)}")
+        ndocs = docs.shape[0] - 1
+    return None if docs is None else _array(ctx, docs, "documents", _I32, (ndocs + 1,)), ndocs, _array(ctx, prefix, "prefix", _I32, (ndocs,))
+
+
+def latent_attention(ctx, q, k, r, v, out, docs=None, prefix=None, scale: float | None = None):
+    """Latent attention over packed documents with expanded keys and values (ocr_latent_attention_device): q
+    [n][heads][key + rot], k [n][heads][key] and r [n][rot] that all heads share (None: no such part), v, out [n][heads][value];
+    k and v may lie beside each other, r beside the latent vectors. Documents as in attention()."""
+    if scale is None:
+        scale = q.shape[2] ** -0.5 if len(q.shape) == 3 and q.shape[2] else 1.0
+    if _native("latent_attention", ctx, q, k, r, v, out, docs, prefix, scale):
+        return
+    qp, n, heads, width, qs = _tokens(ctx, q, "queries", _F16)
+    code = _code(q, "queries")
+    kp, _, _, key, ks, kh = _heads(ctx, k, "keys", (code,), n, heads)
+    vp, _, _, value, vs, vh = _heads(ctx, v, "values", (code,), n, heads)
+    op, _, _, _, os = _tokens(ctx, out, "outputs", (code,), n, heads, value)
+    rp, rot, rs = None, width - key, 0
+    if r is not None:
+        _device(ctx, r, "shared keys")
+        if _code(r, "shared keys") != code or tuple(r.shape) != (n, rot) or (n and rot > 1 and r.stride()[1] != 1):
+            raise _error(f"shared keys: rows [{n}][{rot}] of {_NAMES[code]} are wanted, not {tuple(r.shape)} of {r.dtype}")
+        rp, rs = r.data_ptr() or None, r.stride()[0] if n > 1 else rot
+    elif rot:
+        raise _error(f"queries of {width} values over keys of {key}, and no shared keys")
+    args = ocr_latent_attention_args(qp, kp, rp, vp, op, code, n, heads, key, rot, value, qs, ks, kh, rs, vs, vh, os,
+                                     *_documents(ctx, docs, prefix), scale)
+    _call("ocr_latent_attention_device", ctx.handle, ctypes.byref(args))
+
+
+def attention(ctx, q, k, v, out, docs=None, prefix=None, scale: float | None = None, cap: float = 0.0, slopes=None, weights=None,
+              window: int | None = None):
     """Attention over packed documents (ocr_attention_device): q, out [n][q_heads][dim], k, v
     [n][kv_heads][dim], docs [documents + 1] rising offsets (None: one document), prefix
     [documents] tokens at each one's start that all of it sees, slopes [q_heads] of the distance
-    bias, cap of the scores' tanh (0: none)."""
+    bias, cap of the scores' tanh (0: none). What each key got from its document's queries (the last `window` of
+    them; None: all) is added to weights [documents][kv_heads][places] float32 if given (ocr_attention_weights_device)."""
     if scale is None:
         scale = q.shape[2] ** -0.5 if len(q.shape) == 3 and q.shape[2] else 1.0
-    if _native("attention", ctx, q, k, v, out, docs, prefix, scale, cap, slopes):
+    if window is not None and (weights is None or not 1 <= window < 2 ** 31):
+        raise _error(f"a window of {window} queries without weights" if weights is None else f"a window of {window} queries")
+    if _native("attention", ctx, q, k, v, out, docs, prefix, scale, cap, slopes, weights, 0 if window is None else window):
         return
     qp, n, q_heads, dim, qs = _tokens(ctx, q, "queries", _F16)
     code = _code(q, "queries")
     kp, _, kv_heads, _, ks = _tokens(ctx, k, "keys", (code,), n, dim=dim)
     vp, _, _, _, vs = _tokens(ctx, v, "values", (code,), n, kv_heads, dim)
     op, _, _, _, os = _tokens(ctx, out, "outputs", (code,), n, q_heads, dim)
-    ndocs = 1
-    if docs is not None:
-        if len(docs.shape) != 1 or docs.shape[0] < 1:
-            raise _error(f"documents: offsets [documents + 1] are wanted, not {tuple(docs.shape)}")
-        ndocs = docs.shape[0] - 1
-    args = ocr_attention_args(qp, kp, vp, op, code, n, q_heads, kv_heads, dim, qs, ks, vs, os,
-                              None if docs is None else _array(ctx, docs, "documents", _I32, (ndocs + 1,)), ndocs,
-                              _array(ctx, prefix, "prefix", _I32, (ndocs,)), scale, cap,
+    documents = _documents(ctx, docs, prefix)
+    args = ocr_attention_args(qp, kp, vp, op, code, n, q_heads, kv_heads, dim, qs, ks, vs, os, *documents, scale, cap,
                               _array(ctx, slopes, "slopes", _F32, (q_heads,)))
-    _call("ocr_attention_device", ctx.handle, ctypes.byref(args))
+    if weights is None:
+        _call("ocr_attention_device", ctx.handle, ctypes.byref(args))
+        return
+    most = _places(weights, "weights")[2]
+    _call("ocr_attention_weights_device", ctx.handle, ctypes.byref(args),
+          _array(ctx, weights, "weights", _F32, (documents[1], kv_heads, most)), most, window or 0)
 
 
 def beam_select(ctx, logits, scores, finished, eos: int | None, out_scores, parents, tokens, out_finished=None):
