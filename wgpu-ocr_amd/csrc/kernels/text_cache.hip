@@ -152,7 +152,10 @@ template <class T, int N> __device__ inline float value_at(const Some<T, N> &r, 
 // Values rounded to T (codes: already divided by the vector's scale).
 template <class T, int N> __device__ inline Some<T, N> some_of(const float *x) {
     Some<T, N> r;
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int k = 0; k < N; k++) r.x[k] = __float_as_uint(x[k]);
+    } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int k = 0; k < N / 2; k++)
             r.x[k] = uint32_t(__builtin_bit_cast(uint16_t, T(x[2 * k]))) | uint32_t(__builtin_bit_cast(uint16_t, T(x[2 * k + 1]))) << 16;
@@ -416,6 +419,99 @@ template <class P> __global__ __launch_bounds__(256) void fork_kernel(ForkArgs a
             a.kv.k_scale[d0 + e] = a.kv.k_scale[s0 + e], a.kv.v_scale[d0 + e] = a.kv.v_scale[s0 + e];
 }
 
+// `each` tokens a workgroup: their turns are looked up once for all heads, then a thread takes two fours of a vector at a
+// time, the two that turn with each other where pairs are halves apart, or two neighbours; in place only those that turn.
+// The next kBatch are on their way.
+constexpr int kRotateTokens = 8, kRotateBatch = 4;
+template <class T> __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a, int each, bool in_place, bool past) {
+    __shared__ __align__(16) float s_cos[kRotateTokens][128], s_sin[kRotateTokens][128];
+    __shared__ double s_step[128];
+    const int tid = threadIdx.x, half = a.rot / 2, turning = a.rot / 8, lanes = in_place ? turning : a.dim / 8;
+    const int64_t t0 = int64_t(blockIdx.x) * each;
+    const int n = int(min<int64_t>(each, a.n - t0)), heads = a.heads;
+    const int items = n * heads * lanes;
+    struct Item {
+        int t, h, c;
+    };
+    auto item_at = [&](int x) {
+        const int v = x / lanes, t = v / heads;
+        return Item{t, v - t * heads, x - v * lanes};
+    };
+    const Item step = item_at(256);
+    auto after = [&](Item i) {
+        i.t += step.t, i.h += step.h, i.c += step.c;
+        if (i.c >= lanes) i.c -= lanes, i.h++;
+        if (i.h >= heads) i.h -= heads, i.t++;
+        return i;
+    };
+    // An item's two fours.
+    auto places = [&](Item i, int *at) {
+        if (i.c < turning) {
+            at[0] = a.first + (a.adjacent ? 8 : 4) * i.c;
+            at[1] = a.adjacent ? at[0] + 4 : at[0] + half;
+        } else {
+            const int c = 8 * (i.c - turning);
+            at[0] = c < int(a.first) ? c : c + int(a.rot);
+            at[1] = at[0] + 4;
+        }
+    };
+    const T *const x0 = static_cast<const T *>(a.x) + t0 * a.x_stride;
+    T *const y0 = static_cast<T *>(a.out) + t0 * a.out_stride;
+    struct Vec {
+        Some<T, 4> x[2];
+    };
+    auto load = [&](Item i) {
+        if (i.t >= n) i = Item{0, 0, 0};
+        int at[2];
+        places(i, at);
+        const T *src = x0 + i.t * a.x_stride + i.h * a.x_head;
+        return Vec{load_some<T, 4, true>(src + at[0]), load_some<T, 4, true>(src + at[1])};
+    };
+    Item item = item_at(tid);
+    Vec next[kRotateBatch];
+    auto load_batch = [&](Item i) {
+#pragma unroll
+        for (int u = 0; u < kRotateBatch; u++) next[u] = load(i), i = after(i);
+    };
+    load_batch(item);
+    for (int i = tid; i < half; i += 256) s_step[i] = turns_a_step(a, i, a.rot);
+    __syncthreads();
+    for (int x = tid; x < n * half; x += 256) {
+        const int t = x / half, i = x - t * half;
+        const float2 r = turned(double(a.at[(t0 + t) * a.axes.count + a.axes.axis[i]]) * s_step[i]);
+        s_cos[t][i] = r.x, s_sin[t][i] = a.back ? -r.y : r.y;
+    }
+    __syncthreads();
+    for (int done = tid; done < items; done += 256 * kRotateBatch) {
+#pragma unroll
+        for (int u = 0; u < kRotateBatch; u++, item = after(item)) {
+            if (item.t >= n) break;
+            int at[2];
+            places(item, at);
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) x[k] = value_at(next[u].x[k / 4], k % 4);
+            if (item.c < turning) {
+                const f32x4 cs = *reinterpret_cast<const f32x4 *>(&s_cos[item.t][4 * item.c]), sn = *reinterpret_cast<const f32x4 *>(&s_sin[item.t][4 * item.c]);
+                auto turn = [](float &p, float &q, float c, float s) {
+                    const float y = p;
+                    p = y * c - q * s;
+                    q = q * c + y * s;
+                };
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    if (!a.adjacent) turn(x[k], x[4 + k], cs[k], sn[k]);
+                    else turn(x[2 * k], x[2 * k + 1], cs[k], sn[k]);
+                }
+            }
+            T *dst = y0 + item.t * a.out_stride + item.h * a.out_head;
+            store_some(dst + at[0], some_of<T, 4>(x), past);
+            store_some(dst + at[1], some_of<T, 4>(x + 4), past);
+        }
+        if (done + 256 * kRotateBatch < items) load_batch(item);
+    }
+}
+
 // A thread a pair, or a value that is not rotated: sizes that are no eights.
 template <class T> __global__ __launch_bounds__(256) void rotate_row_kernel(RotateArgs a) {
     const uint32_t half = a.rot / 2, each = a.dim - half;  // a vector's items
@@ -478,8 +574,17 @@ void launch_append(const AppendArgs &a, hipStream_t s) {
 
 void launch_rotate(const RotateArgs &a, hipStream_t s) {
     const double values = double(a.n) * a.heads * a.dim;
-    ProbeScope probe("text_rotate", s, 3 * values, 2 * values * type_bytes(a.type), "text_rotate_row");
-    with_type(a.type, [&](auto t) { hipLaunchKernelGGL((rotate_row_kernel<decltype(t)>), dim3(a.n), dim3(256), 0, s, a); });
+    const bool in_place = a.x == a.out, eights = a.dim % 8 == 0 && a.first % 8 == 0 && a.rot % 8 == 0 && a.x_stride < 1 << 30 && a.out_stride < 1 << 30;
+    ProbeScope probe("text_rotate", s, 3 * values, 2 * values * type_bytes(a.type), eights ? "text_rotate_eights" : "text_rotate_row");
+    const uint32_t lanes = in_place ? a.rot / 8 : a.dim / 8;
+    if (eights && lanes == 0) return;  // in place, and nothing turns
+    const int each = a.n >= 2048 ? int(std::min<uint32_t>(kRotateTokens, std::max<uint32_t>(1, 2048 / (a.heads * lanes)))) : 1;
+    const bool past = (in_place ? values * a.rot / a.dim : values) * type_bytes(a.type) > kHeld;
+    with_type(a.type, [&](auto t) {
+        using T = decltype(t);
+        if (eights) hipLaunchKernelGGL((rotate_kernel<T>), dim3((a.n + each - 1) / each), dim3(256), 0, s, a, each, in_place, past);
+        else hipLaunchKernelGGL((rotate_row_kernel<T>), dim3(a.n), dim3(256), 0, s, a);
+    });
     OCR_HIP(hipGetLastError());
 }
 
