@@ -89,30 +89,6 @@ template <class T> __global__ __launch_bounds__(64) void latent_row_kernel(Laten
         if (lane + 64 * u < rank) out[lane + 64 * u] = T(l == 0.f ? 0.f : o[u] / l);
 }
 
-// A key of its own part and the part that all heads share.
-template <class T> struct SharedKv {
-    const T *kp, *rp, *vp;
-    int64_t ks, rs, vs;
-    int key;
-    __device__ float k(int j, int c) const { return to_f32(c < key ? kp[j * ks + c] : rp[j * rs + c - key]); }
-    __device__ float v(int j, int c) const { return to_f32(vp[j * vs + c]); }
-};
-
-// A prompt's token and head by the formula, one wavefront.
-template <class T> __global__ __launch_bounds__(64) void expanded_row_kernel(LatentAttentionArgs a) {
-    __shared__ float s_q[256 + kMostLatentRot];
-    const int64_t i = blockIdx.x;
-    const int h = blockIdx.y, width = a.key + a.rot;
-    const T *q = static_cast<const T *>(a.q) + i * a.q_stride + int64_t(h) * width;
-    for (int c = threadIdx.x; c < width; c += 64) s_q[c] = to_f32(q[c]) * a.scale;
-    __syncthreads();
-    const KeyRange r = key_range(int(i), int(a.n), a.docs, int(a.ndocs), a.prefix);
-    const SharedKv<T> kv{static_cast<const T *>(a.k) + h * a.k_head, static_cast<const T *>(a.r), static_cast<const T *>(a.v) + h * a.v_head,
-                         a.k_stride, a.r_stride, a.v_stride, int(a.key)};
-    T *out = static_cast<T *>(a.out) + i * a.out_stride + int64_t(h) * a.value;
-    attend_row(kv, s_q, width, r.lo, r.hi, int(i), 0.f, 0.f, [&](int c, float o) { out[c] = T(o); }, int(a.value));
-}
-
 }  // namespace
 
 void launch_latent_append(const LatentAppendArgs &a, hipStream_t s) {
@@ -128,13 +104,6 @@ void launch_latent_decode(Ctx &, const LatentDecodeArgs &a, hipStream_t s) {
     const double vecs = double(a.table.rows) * a.table.width * a.c.page;
     ProbeScope probe("latent_decode", s, 2.0 * vecs * a.heads * (2 * a.c.rank + a.c.rot), 2.0 * vecs * (a.c.rank + a.c.rot), "latent_decode_row");
     with_type16(a.c.type, [&](auto t) { hipLaunchKernelGGL((latent_row_kernel<decltype(t)>), dim3(a.table.rows, a.heads), dim3(64), 0, s, a); });
-    OCR_HIP(hipGetLastError());
-}
-
-void launch_latent_attention(const LatentAttentionArgs &a, hipStream_t s) {
-    const double n = a.n;
-    ProbeScope probe("latent_attention", s, n * n * a.heads * (a.key + a.rot + a.value), 4.0 * n * a.heads * (a.key + a.value), "latent_attention_row");
-    with_type16(a.type, [&](auto t) { hipLaunchKernelGGL((expanded_row_kernel<decltype(t)>), dim3(a.n, a.heads), dim3(64), 0, s, a); });
     OCR_HIP(hipGetLastError());
 }
 

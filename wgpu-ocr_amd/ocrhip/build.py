@@ -19,7 +19,7 @@ ARCH = "gfx950"
 DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # Matrix products whose sums stay in ordinary registers: softmax kernels read and rescale them all
 # the time, and each move to and from the accumulation registers is an instruction.
-FILE_FLAGS = {f"text_{n}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"] for n in ("attn", "decode")}
+FILE_FLAGS = {f"text_{n}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"] for n in ("attn", "decode", "expanded", "latent", "weights")}
 COMMON = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function"]
 
 
