@@ -62,10 +62,8 @@ struct DecodePlan {
     Cap cap;  // in units of log2
 };
 
-// Parts of a sequence joined: part [row][head][parts] holds dim normalised values, then log2 of the
-// sum of weights.
-constexpr int kPartTail = 4;  // keeps the rows' 16-byte alignment
-
+// part, where a sequence is cut: [row][head][parts], each dim normalised values, then log2 of the sum of weights (join_parts).
+//
 // T: the queries' type, C: the cache's; products of 8-bit caches in float16, which holds their codes
 // exactly.
 template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void decode_kernel(DecodeArgs a, DecodePlan plan, float *part) {
@@ -388,42 +386,16 @@ template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 
     }
 }
 
-// One workgroup a (sequence, head): four values a thread, the parts side by side.
+// One workgroup a (sequence, head).
 template <int N> __global__ __launch_bounds__(N) void decode_join_kernel(DecodeArgs a, uint32_t parts, const float *part) {
-    __shared__ __align__(16) float s_o[N * 4];
-    __shared__ float s_l[N];
     const int64_t r = blockIdx.x;
-    const int h = blockIdx.y, dim = a.kv.dim, tid = threadIdx.x;
+    const int h = blockIdx.y, dim = a.kv.dim, pitch = dim + kPartTail;
     const int len = clamp_len(a.lens[r], a.table.width, a.kv.page), count = parts_of(len, parts).count;
-    const int pitch = dim + kPartTail, lanes = dim / 4, side = N / lanes, c = tid % lanes, k = tid / lanes;
     const float *src = part + (r * a.q_heads + h) * parts * pitch;
-    // Each thread's parts are k, k + side, ...: a running maximum over them, then over the threads.
-    f32x4 o{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
-    if (k < side) {
-#pragma unroll 4
-        for (int i = k; i < count; i += side) {
-            const float lse = src[i * pitch + dim];
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(src + i * pitch + 4 * c);
-            const float mn = fmaxf(m, lse), f = mn == -INFINITY ? 0.f : exp2_f32(m - mn), w = lse == -INFINITY ? 0.f : exp2_f32(lse - mn);
-            o = o * f + x * w;
-            l = l * f + w, m = mn;
-        }
-    }
-    s_l[tid] = m;
-    __syncthreads();
-    float top = -INFINITY;
-    for (int i = 0; i < side; i++) top = fmaxf(top, s_l[c + i * lanes]);
-    __syncthreads();
-    const float f = top == -INFINITY ? 0.f : exp2_f32(m - top);
-    s_l[tid] = l * f;
-    *reinterpret_cast<f32x4 *>(&s_o[tid * 4]) = o * f;
-    __syncthreads();
-    if (k != 0) return;
-    o = f32x4{0.f, 0.f, 0.f, 0.f}, l = 0.f;
-    for (int i = 0; i < side; i++) o += *reinterpret_cast<const f32x4 *>(&s_o[(c + i * lanes) * 4]), l += s_l[c + i * lanes];
-    const int64_t at = r * a.out_stride + int64_t(h) * dim + 4 * c;
-    for (int i = 0; i < 4; i++) store16(a.out, a.type, at + i, l == 0.f ? 0.f : o[i] / l);
+    const int64_t at = r * a.out_stride + int64_t(h) * dim;
+    join_parts<N>(count, dim, [&](int i) { return src + i * pitch; }, [&](int c, f32x4 o) {
+        for (int i = 0; i < 4; i++) store16(a.out, a.type, at + c + i, o[i]);
+    });
 }
 
 template <class T, class C> void launch_tiles(const DecodeArgs &a, uint32_t parts, float *part, hipStream_t s) {

@@ -227,4 +227,43 @@ __device__ inline void attend_row(const KV &kv, const float *q, int dim, int lo,
         if (lane + 64 * u < outs) done(lane + 64 * u, l == 0.f ? 0.f : o[u] / l);
 }
 
+// Parts of one query's attention joined by a workgroup of N threads, four of its dim values a thread and the parts side by
+// side. part(i): part i's dim normalised values, then log2 of its sum of weights; done(c, four) gets each four.
+template <int N, class Part, class Done> __device__ inline void join_parts(int count, int dim, Part &&part, Done &&done) {
+    __shared__ __align__(16) float s_o[N * 4];
+    __shared__ float s_l[N];
+    const int tid = threadIdx.x, lanes = dim / 4, side = N / lanes, c = tid % lanes, k = tid / lanes;
+    // Each thread's parts are k, k + side, ...: a running maximum over them, then over the threads.
+    f32x4 o{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    if (k < side) {
+#pragma unroll 4
+        for (int i = k; i < count; i += side) {
+            const float *src = part(i);
+            const float lse = src[dim];
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(src + 4 * c);
+            const float mn = fmaxf(m, lse), f = mn == -INFINITY ? 0.f : exp2_f32(m - mn), w = lse == -INFINITY ? 0.f : exp2_f32(lse - mn);
+            o = o * f + x * w;
+            l = l * f + w, m = mn;
+        }
+    }
+    s_l[tid] = m;
+    __syncthreads();
+    float top = -INFINITY;
+    for (int i = 0; i < side; i++) top = fmaxf(top, s_l[c + i * lanes]);
+    __syncthreads();
+    const float f = top == -INFINITY ? 0.f : exp2_f32(m - top);
+    s_l[tid] = l * f;
+    *reinterpret_cast<f32x4 *>(&s_o[tid * 4]) = o * f;
+    __syncthreads();
+    if (k != 0) return;
+    o = f32x4{0.f, 0.f, 0.f, 0.f}, l = 0.f;
+    for (int i = 0; i < side; i++) o += *reinterpret_cast<const f32x4 *>(&s_o[(c + i * lanes) * 4]), l += s_l[c + i * lanes];
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = l == 0.f ? 0.f : o[i] / l;
+    done(4 * c, o);
+}
+// Parts end in four floats, which keeps their 16-byte alignment.
+constexpr int kPartTail = 4;
+
 }  // namespace ocr

@@ -230,6 +230,23 @@ OCR_HD Parts parts_of(int len, uint32_t parts) {
     return parts == 1 ? Parts{1, len} : Parts{int((uint32_t(len) + uint32_t(each) - 1) / uint32_t(each)), each};
 }
 
+// How single-token attention over latent vectors is cut: all sequences' tiles of kLatentTile positions one after
+// another, in equal runs, so that sequences of unlike lengths leave no workgroup idle. A run ends in the middle of at most two
+// sequences, so it has two places for parts: 0 for a sequence that an earlier run began, 1 for one that goes on after it.
+constexpr int kLatentTile = 32, kLeastRun = 2;
+OCR_HD int latent_tiles(int len) { return int((uint32_t(len) + kLatentTile - 1) / kLatentTile); }
+OCR_HD int64_t latent_run(int64_t total, int runs) {
+    const int64_t each = (total + runs - 1) / runs;
+    return each < kLeastRun ? kLeastRun : each;
+}
+// Runs [first, last] that have tiles of a sequence whose first tile is `start`.
+struct Runs {
+    int64_t first, last;
+};
+OCR_HD Runs runs_of(int64_t start, int tiles, int64_t each) { return {start / each, (start + tiles - 1) / each}; }
+// The place of run g's part of it.
+OCR_HD int64_t part_place(int64_t g, int64_t start, int64_t each) { return 2 * g + (start >= g * each ? 1 : 0); }
+
 // The power of two over a positive number, at most 2^126.
 OCR_HD float over_pow2(float x) {
     const uint32_t u = (__builtin_bit_cast(uint32_t, x) & 0x7f800000u) + 0x00800000u;
