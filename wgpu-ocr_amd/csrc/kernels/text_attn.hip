@@ -59,26 +59,6 @@ template <class T> __global__ __launch_bounds__(64) void attention_row_kernel(At
 // is fine (kFineCap). Score by score it costs more: a page of 2929 tokens with scores past the cap: 104 us, so 135.
 enum Scores { kPlain, kCapped, kBias, kAny };
 
-// cap tanh(s / cap) of unscaled scores as s times a polynomial of their squares (tanh_ratio, its powers
-// of scale / cap in the factors), which lasts to 0.35 of the cap. In units of log2; the exponential's and the reciprocal's way takes half again as long.
-struct SmallCap {
-    float k[4], most;
-    __device__ SmallCap(float scale, float cap) {
-        const float y = scale / cap, t = y * y;
-        k[0] = scale * 1.4426950408889634f;
-        float power = k[0];
-#pragma unroll
-        for (int e = 1; e < 4; e++) power *= t, k[e] = kTanhPart[e] * power;
-        // Where the powers leave float32: as far as those that are left reach (the fourth power's part under 2^-25 of
-        // the score, the square's), and no score's square is infinite.
-        most = y >= 1e3f ? -1.f : fabsf(k[3]) >= 1e-36f ? kSmallTanh / y : fminf((fabsf(k[1]) >= 1e-36f ? 0.02f : 3e-4f) / y, 1e18f);
-    }
-    __device__ float factor(float s) const {
-        const float t = s * s;
-        return __fmaf_rn(__fmaf_rn(__fmaf_rn(k[3], t, k[2]), t, k[1]), t, k[0]);
-    }
-};
-
 // 32 queries of one head a wavefront over tiles of KT keys that come into LDS by DMA while the tile
 // before is worked on. DP: the head's values rounded up to 32. QW: of the four wavefronts, those with
 // queries of their own; where it is two, the other two take the same queries over the other half of
@@ -298,6 +278,7 @@ template <class T, int DP, Scores KIND, int QW> __global__ __launch_bounds__(256
             const float m2 = s_o[64 * 16 * NB], l2 = s_o[64 * (16 * NB + 1)], mn = fmaxf(m, m2);
             const float f = mn == -INFINITY ? 1.f : exp2_f32(m - mn), f2 = mn == -INFINITY ? 1.f : exp2_f32(m2 - mn);
             l = l * f + l2 * f2;
+            m = mn;
 #pragma unroll
             for (int e = 0; e < 16 * NB; e++) o[e / 16][e % 16] = o[e / 16][e % 16] * f + s_o[64 * e] * f2;
         }
@@ -311,6 +292,11 @@ template <class T, int DP, Scores KIND, int QW> __global__ __launch_bounds__(256
         for (int e = 0; e < 16; e++) bad += o[b][e] * 0.f;
     const unsigned long long spoilt = wave < QW ? __ballot(sees && !(bad == 0.f)) : 0;
     const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (a.sums && wave < QW && half == 0 && i < int(a.n)) {  // weights are e^(score - the one) times the other, in units of log2
+        float *const sums = a.sums + 2 * int64_t(h) * sums_pitch(a.n) + i;
+        sums[0] = m == -INFINITY ? 0.f : m - lift<T>;
+        sums[sums_pitch(a.n)] = inv;
+    }
     if (wave < QW && i < int(a.n) && !((spoilt >> (lane & 31) | spoilt >> ((lane & 31) + 32)) & 1)) {
         T *out = static_cast<T *>(a.out) + int64_t(i) * a.out_stride + int64_t(h) * dim;
 #pragma unroll
@@ -350,11 +336,16 @@ template <class T, Scores KIND> void launch_dims(const AttentionArgs &a, bool fe
 
 }  // namespace
 
-void launch_attention(const AttentionArgs &a, hipStream_t s) {
-    // Whole 16-byte pieces, and rows of a tile within 32 bits of each other.
+// Whole 16-byte pieces, and rows of a tile within 32 bits of each other.
+bool attention_tiles(const AttentionArgs &a) {
     bool pieces = a.dim % 8 == 0 && head_blocks((a.n + 63) / 64, a.q_heads, a.kv_heads) < 1 << 24;
     for (const void *p : {a.q, a.k, a.v, static_cast<const void *>(a.out)}) pieces = pieces && reinterpret_cast<uintptr_t>(p) % 16 == 0;
     for (int64_t st : {a.q_stride, a.k_stride, a.v_stride, a.out_stride}) pieces = pieces && st % 8 == 0 && st < 1 << 24;
+    return pieces;
+}
+
+void launch_attention(const AttentionArgs &a, hipStream_t s) {
+    const bool pieces = attention_tiles(a);
     const bool few = few_tiles(a);
     ProbeScope probe("text_attention", s, 2.0 * a.n * a.n * a.q_heads * a.dim, 4.0 * a.n * (a.q_heads + a.kv_heads) * a.dim,
                      !pieces ? "text_attention_row" : few ? "text_attention_64" : "text_attention_128");

@@ -64,9 +64,18 @@ struct DecodePlan {
 
 // part, where a sequence is cut: [row][head][parts], each dim normalised values, then log2 of the sum of weights (join_parts).
 //
+// What is kept for the weights of the keys (KEEP): every query head's scores in units of log2, [row][q_heads][pitch], and
+// each part's reference and sum of weights, [row][q_heads][parts]. Scores of 4 query heads are an eighth of the bytes of an 8-bit
+// key and value of 128: keeping them costs less than reading the keys again.
+struct Kept {
+    float *scores;
+    float2 *sums;
+    uint32_t pitch;
+};
+
 // T: the queries' type, C: the cache's; products of 8-bit caches in float16, which holds their codes
 // exactly.
-template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void decode_kernel(DecodeArgs a, DecodePlan plan, float *part) {
+template <class T, class C, int DP, bool KEEP> __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void decode_kernel(DecodeArgs a, DecodePlan plan, float *part, Kept kept) {
     using M = std::conditional_t<scaled<C>, f16, C>;
     typedef M mvec __attribute__((ext_vector_type(8)));
     constexpr int NU = DP * int(sizeof(C)) / 64;    // 16-byte pieces of a vector that a lane holds
@@ -268,6 +277,13 @@ template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 
                     for (int i = 0; i < 4; i++)
                         if (t0 + 16 * t + 4 * g4 + i >= cn) sc[t][i] = -INFINITY;
             }
+            if constexpr (KEEP) {
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    const uint32_t at = uint32_t(c0 + t0 + 16 * t + 4 * g4);  // the parts start at whole tiles
+                    if (real && at < kept.pitch) *reinterpret_cast<f32x4 *>(kept.scores + (r * a.q_heads + h) * kept.pitch + at) = f32x4{sc[t][0], sc[t][1], sc[t][2], sc[t][3]};
+                }
+            }
             float top = -INFINITY;
 #pragma unroll
             for (int t = 0; t < 2; t++)
@@ -371,6 +387,7 @@ template <class T, class C, int DP> __global__ __launch_bounds__(256, DP <= 128 
     }
     if (wave != 0 || !real) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (KEEP && g4 == 0) kept.sums[(r * a.q_heads + h) * parts + blockIdx.z] = {m + kSlack, l};  // l is 2^-kSlack of the sum relative to m
     if (part) {
         float *dst = part + ((r * a.q_heads + h) * parts + blockIdx.z) * (dim + kPartTail);
 #pragma unroll
@@ -398,14 +415,52 @@ template <int N> __global__ __launch_bounds__(N) void decode_join_kernel(DecodeA
     });
 }
 
-template <class T, class C> void launch_tiles(const DecodeArgs &a, uint32_t parts, float *part, hipStream_t s) {
+// What single tokens' keys got: the weights that the kept scores stand for, over a key head's query heads, added to w.
+// Four positions a thread; every workgroup joins the parts' sums for its query heads.
+constexpr int kWeighPositions = 1024;
+__global__ __launch_bounds__(256) void decode_weights_kernel(DecodeArgs a, Weights w, uint32_t parts, Kept kept) {
+    __shared__ float2 s_sums[1024];  // a query head's reference and one over its sum
+    const int64_t r = blockIdx.x;
+    const int hk = blockIdx.y, group = int(a.q_heads / a.kv.heads), tid = threadIdx.x;
+    const int len = clamp_len(a.lens[r], a.table.width, a.kv.page), end = int(min(uint32_t(len), w.most));
+    const int p = int(blockIdx.z) * kWeighPositions + 4 * tid;
+    if (int(blockIdx.z) * kWeighPositions >= end) return;
+    const int count = parts_of(len, parts).count;
+    const int64_t q0 = r * a.q_heads + int64_t(hk) * group;
+    for (int g = tid; g < group; g += 256) {
+        const float2 *from = kept.sums + (q0 + g) * parts;
+        float m = -INFINITY, l = 0.f;
+        for (int i = 0; i < count; i++) m = fmaxf(m, from[i].x);
+        for (int i = 0; i < count; i++) l += from[i].x == -INFINITY ? 0.f * from[i].y : from[i].y * exp2_f32(from[i].x - m);
+        s_sums[g] = {m == -INFINITY ? 0.f : m, l == 0.f ? 0.f : 1.f / l};
+    }
+    __syncthreads();
+    if (p >= end) return;
+    f32x4 sum{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int g = 0; g < group; g++) {
+        const f32x4 s = *reinterpret_cast<const f32x4 *>(kept.scores + (q0 + g) * kept.pitch + p);
+#pragma unroll
+        for (int i = 0; i < 4; i++) sum[i] = __fmaf_rn(exp2_f32(s[i] - s_sums[g].x), s_sums[g].y, sum[i]);
+    }
+    float *out = w.p + (r * a.kv.heads + hk) * w.most + p;
+    typedef float loose __attribute__((ext_vector_type(4), aligned(4)));
+    if (p + 4 <= end) {
+        *reinterpret_cast<loose *>(out) += sum;
+    } else {
+        for (int i = 0; i < 4; i++)
+            if (p + i < end) out[i] += sum[i];
+    }
+}
+
+template <class T, class C, bool KEEP> void launch_tiles(const DecodeArgs &a, uint32_t parts, float *part, const Kept &kept, hipStream_t s) {
     const int group = int(a.q_heads / a.kv.heads);
     const DecodePlan plan{parts, group, (group + 15) / 16, a.kv.page & (a.kv.page - 1) ? -1 : __builtin_ctz(a.kv.page),
                           reinterpret_cast<uintptr_t>(a.q) % 16 == 0 && a.q_stride % 8 == 0, cap_of(a.cap, 1.4426950408889634f)};
     const dim3 grid(a.table.rows, a.kv.heads * plan.blocks, parts);
-    if (a.kv.dim <= 64) hipLaunchKernelGGL((decode_kernel<T, C, 64>), grid, dim3(256), 0, s, a, plan, part);
-    else if (a.kv.dim <= 128) hipLaunchKernelGGL((decode_kernel<T, C, 128>), grid, dim3(256), 0, s, a, plan, part);
-    else hipLaunchKernelGGL((decode_kernel<T, C, 256>), grid, dim3(256), 0, s, a, plan, part);
+    if (a.kv.dim <= 64) hipLaunchKernelGGL((decode_kernel<T, C, 64, KEEP>), grid, dim3(256), 0, s, a, plan, part, kept);
+    else if (a.kv.dim <= 128) hipLaunchKernelGGL((decode_kernel<T, C, 128, KEEP>), grid, dim3(256), 0, s, a, plan, part, kept);
+    else hipLaunchKernelGGL((decode_kernel<T, C, 256, KEEP>), grid, dim3(256), 0, s, a, plan, part, kept);
     OCR_HIP(hipGetLastError());
 }
 
@@ -420,7 +475,10 @@ template <class F> void with_pair(const DecodeArgs &a, F &&f) {
 
 }  // namespace
 
-void launch_decode(Ctx &c, const DecodeArgs &a, hipStream_t s) {
+namespace {
+
+// The sequences' parts, and w's weights where it is given.
+void launch(Ctx &c, const DecodeArgs &a, const Weights *w, hipStream_t s) {
     const bool pieces = whole_pieces(a.kv);
     // Parts until there are two workgroups for every compute unit; a sequence has as many as its own
     // length gives work to. 4 sequences of 131 072: 256 workgroups 194 us, 384 204, 512 179, 1024
@@ -439,15 +497,38 @@ void launch_decode(Ctx &c, const DecodeArgs &a, hipStream_t s) {
         OCR_HIP(hipGetLastError());
         return;
     }
-    DBuf part;
-    if (parts > 1) part = DBuf(&c, size_t(a.table.rows) * a.q_heads * parts * (a.kv.dim + kPartTail) * 4, s);
-    with_pair(a, [&](auto t, auto k) { launch_tiles<decltype(t), decltype(k)>(a, parts, part.as<float>(), s); });
+    DBuf part, scores, sums;
+    const size_t rows = size_t(a.table.rows) * a.q_heads;
+    if (parts > 1) part = DBuf(&c, rows * parts * (a.kv.dim + kPartTail) * 4, s);
+    if (w) {
+        Kept kept{nullptr, nullptr, uint32_t((std::min<uint64_t>(w->most, most) + 3) & ~3ull)};
+        scores = DBuf(&c, rows * kept.pitch * 4, s), sums = DBuf(&c, rows * parts * sizeof(float2), s);
+        kept.scores = scores.as<float>(), kept.sums = sums.as<float2>();
+        with_pair(a, [&](auto t, auto k) { launch_tiles<decltype(t), decltype(k), true>(a, parts, part.as<float>(), kept, s); });
+        const ProbeScope weigh("text_weights", s, 2.0 * rows * kept.pitch, 4.0 * rows * kept.pitch + 8.0 * a.table.rows * a.kv.heads * kept.pitch, "text_weights_single");
+        hipLaunchKernelGGL(decode_weights_kernel, dim3(a.table.rows, a.kv.heads, (kept.pitch + kWeighPositions - 1) / kWeighPositions), dim3(256), 0, s, a, *w, parts, kept);
+    } else {
+        with_pair(a, [&](auto t, auto k) { launch_tiles<decltype(t), decltype(k), false>(a, parts, part.as<float>(), {}, s); });
+    }
     if (parts > 1) {
         const dim3 grid(a.table.rows, a.q_heads);
         if (parts <= 8) hipLaunchKernelGGL(decode_join_kernel<64>, grid, dim3(64), 0, s, a, parts, part.as<float>());
         else hipLaunchKernelGGL(decode_join_kernel<256>, grid, dim3(256), 0, s, a, parts, part.as<float>());
         OCR_HIP(hipGetLastError());
     }
+}
+
+}  // namespace
+
+void launch_decode(Ctx &c, const DecodeArgs &a, hipStream_t s) { launch(c, a, nullptr, s); }
+
+void launch_decode_weights(Ctx &c, const DecodeArgs &a, const Weights &w, hipStream_t s) {
+    if (whole_pieces(a.kv) && (uint64_t(a.table.width) * a.kv.page + kWeighPositions - 1) / kWeighPositions < 65536) {
+        launch(c, a, &w, s);
+        return;
+    }
+    launch_decode(c, a, s);
+    launch_single_weights_row(a, w, s);
 }
 
 }  // namespace ocr

@@ -120,6 +120,26 @@ __device__ inline float large_capped(const Cap &c, float s) {
 }
 __device__ inline float capped(const Cap &c, float s) { return fabsf(s) <= c.small ? small_capped(c, s) : large_capped(c, s); }
 
+// cap tanh(s / cap) of unscaled scores as s times a polynomial of their squares (tanh_ratio, its powers
+// of scale / cap in the factors), which lasts to 0.35 of the cap. In units of log2; the exponential's and the reciprocal's way takes half again as long.
+struct SmallCap {
+    float k[4], most;
+    __device__ SmallCap(float scale, float cap) {
+        const float y = scale / cap, t = y * y;
+        k[0] = scale * 1.4426950408889634f;
+        float power = k[0];
+#pragma unroll
+        for (int e = 1; e < 4; e++) power *= t, k[e] = kTanhPart[e] * power;
+        // Where the powers leave float32: as far as those that are left reach (the fourth power's part under 2^-25 of
+        // the score, the square's), and no score's square is infinite.
+        most = y >= 1e3f ? -1.f : fabsf(k[3]) >= 1e-36f ? kSmallTanh / y : fminf((fabsf(k[1]) >= 1e-36f ? 0.02f : 3e-4f) / y, 1e18f);
+    }
+    __device__ float factor(float s) const {
+        const float t = s * s;
+        return __fmaf_rn(__fmaf_rn(__fmaf_rn(k[3], t, k[2]), t, k[1]), t, k[0]);
+    }
+};
+
 // The code of a value already divided by its vector's scale (rounded to nearest, ties to even).
 template <class C> __device__ inline C code_of(float v) {
     if constexpr (std::is_same_v<C, int8_t>) return int8_t(rintf(v));

@@ -1,10 +1,15 @@
-// How much of the attention each key got, added up: of a prompt's queries and of single tokens.
+// How much of the attention each key got from a prompt's queries, added up (single tokens': text_decode.hip).
+//
+// The attention itself leaves every query's reference and one over its sum, so a weight is e^(s - reference) times that:
+// the scores are made a second time, S = Q K^T with the queries as rows, so that a lane has one key and sums its
+// column in a register, without maximum, rescaling or atomics.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 
 #include "../runtime.h"
 #include "text_device.h"
+#include "text_tile.h"
 
 namespace ocr {
 
@@ -130,12 +135,175 @@ template <class T, class C> __global__ __launch_bounds__(64) void single_weights
     }
 }
 
+// 32 keys a wavefront, held in registers, over tiles of 64 queries of one head that come into LDS by DMA while the tile
+// before is worked on. A workgroup's 128 keys of a key head; slice: one of its query heads, and one of `cuts` parts of the queries.
+// part [slice][kv_heads][n]. CAPPED: with a cap or slopes.
+template <class T, int DP, bool CAPPED> __global__ __launch_bounds__(256) void prompt_weights_kernel(AttentionArgs a, int window, int tiles, int cuts, float *part) {
+    typedef T tvec __attribute__((ext_vector_type(8)));
+    constexpr int PW = DP <= 64 ? 64 : DP <= 128 ? 128 : 256, QT = PW == 256 ? 32 : 64, KS = DP / 16;
+    using TQ = Tile<PW, QT>;
+    constexpr int BUF = TQ::BYTES + 2 * 256;  // the queries, their references and their sums' inverses
+    __shared__ __align__(16) char s_q[2 * BUF];
+    __shared__ int s_lo[4], s_hi[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+    const int group = int(a.q_heads / a.kv_heads), slices = group * cuts;
+    // Dies take key heads in turn; a die's workgroups go through a head's keys before the next slice, whose queries stay in its level-two cache.
+    const int hk = int(blockIdx.x % a.kv_heads), rest = int(blockIdx.x / a.kv_heads), tile = rest % tiles, slice = rest / tiles;
+    const int h = hk * group + slice / cuts, cut = slice % cuts, dim = a.dim, pieces = dim / 8;
+    if (slice >= slices) return;
+    const int j = tile * 128 + 32 * wave + (lane & 31);
+    QueryRange r{0, 0, -1, 0};
+    if (j < int(a.n)) r = query_range(j, int(a.n), a.docs, int(a.ndocs), a.prefix, window);
+    const bool seen = r.lo < r.hi;
+    const int wlo = wave_min_i(seen ? r.lo : 0x7fffffff), whi = wave_max_i(seen ? r.hi : 0);
+    const int flo = wave_max_i(seen ? r.lo : 0x7fffffff), fhi = wave_min_i(seen ? r.hi : 0);  // all keys are seen by those in [flo, fhi)
+    if (lane == 0) s_lo[wave] = wlo, s_hi[wave] = whi;
+    tvec kf[KS];
+    {
+        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0;
+        const char *k = static_cast<const char *>(a.k) + (int64_t(min(j, int(a.n) - 1)) * a.k_stride + int64_t(hk) * dim) * 2;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            u32x4 x{0, 0, 0, 0};
+            if (2 * s + half < pieces) x = *reinterpret_cast<const u32x4 *>(k + 16 * (2 * s + half));
+            kf[s] = __builtin_bit_cast(tvec, x ^ flip);
+        }
+    }
+    const TQ tq(a.q_stride, pieces);
+    if (pieces < TQ::PP) {  // pieces that no copy writes count nothing
+        for (int x = tid; x < 2 * BUF / 16; x += 256) *reinterpret_cast<u32x4 *>(s_q + 16 * x) = u32x4{0, 0, 0, 0};
+    }
+    __syncthreads();
+    int qlo = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3])), qhi = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
+    qlo = __builtin_amdgcn_readfirstlane(qlo), qhi = __builtin_amdgcn_readfirstlane(qhi);
+    float sum = 0.f;
+    if (qlo < qhi) {
+        // This part's tiles of queries.
+        const int t0 = qlo / QT, t1 = (qhi + QT - 1) / QT, each = (t1 - t0 + cuts - 1) / cuts;
+        const int i0 = (t0 + cut * each) * QT, i1 = min(qhi, (t0 + (cut + 1) * each) * QT);
+        const char *const qbase = static_cast<const char *>(a.q) + int64_t(h) * dim * 2;
+        const float *const sums = a.sums + 2 * int64_t(h) * sums_pitch(a.n);
+        const unsigned lds0 = lds_addr(s_q);
+        auto copy = [&](int i, int buf) {
+            tq.copy(qbase + int64_t(i) * tq.step, lds0 + buf * BUF + wave * 1024, int(a.n) - i);
+            // Sixteen lanes for the references, sixteen for the inverses.
+            if (wave == 0 && lane < 32)
+                dma16s_to(sums + i, unsigned(((lane >> 4) * sums_pitch(a.n) + 4 * (lane & 15) % QT) * 4), lds0 + buf * BUF + TQ::BYTES);
+        };
+        int qoff[KS];
+#pragma unroll
+        for (int s = 0; s < KS; s++) qoff[s] = (lane & 31) * PW * 2 + ((2 * s + half) ^ TQ::swap_of(lane & 15)) * 16;
+        const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);
+        const float slope = CAPPED && a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.f;
+        const SmallCap small(fabsf(a.scale), CAPPED && a.cap > 0.f ? a.cap : 1.f);
+        const Cap cap = cap_of(a.cap, 1.4426950408889634f);
+        // 32 queries from i on.
+        auto turn = [&](int i, const char *s_b, int u) __attribute__((always_inline)) {
+            if (i >= whi || i + 32 <= wlo) return;
+            f32x16 s;
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[e] = 0.f;
+#pragma unroll
+            for (int st = 0; st < KS; st++) s = mfma32(*reinterpret_cast<const tvec *>(s_b + qoff[st] + u * 32 * PW * 2), kf[st], s);
+            if constexpr (CAPPED) {
+                float top = 0.f;
+                if (a.cap > 0.f) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) top = fmaxf(top, fabsf(s[e]));
+                }
+                if (a.cap > 0.f && __any(top > small.most)) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) s[e] = capped(cap, s[e] * c);
+                } else if (a.cap > 0.f) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) s[e] *= small.factor(s[e]);
+                } else {
+                    s *= c;
+                }
+                if (a.slopes) {
+                    const float d = float(i + 4 * half - j);
+#pragma unroll
+                    for (int e = 0; e < 16; e++) s[e] -= slope * fabsf(d + float(8 * (e / 4) + e % 4));
+                }
+            }
+            const bool whole = i >= flo && i + 32 <= fhi;
+            const unsigned first = unsigned(i + 4 * half - r.lo), count = seen ? unsigned(r.hi - r.lo) : 0;
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const f32x4 ref = *reinterpret_cast<const f32x4 *>(s_b + TQ::BYTES + (32 * u + 2 * e + 4 * half) * 4);
+                const f32x4 inv = *reinterpret_cast<const f32x4 *>(s_b + TQ::BYTES + 256 + (32 * u + 2 * e + 4 * half) * 4);
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const float p = exp2_f32(CAPPED ? s[e + x] - ref[x] : __fmaf_rn(s[e + x], c, -ref[x]));
+                    // What is not seen may be anything, and so may its query's sum.
+                    if (whole) sum = __fmaf_rn(p, inv[x], sum);
+                    else sum += first + unsigned(2 * e + x) < count ? p * inv[x] : 0.f;
+                }
+            }
+        };
+        auto step = [&](int i, auto which) __attribute__((always_inline)) {
+            constexpr int buf = decltype(which)::value;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            lds_barrier();  // the tile is there, and all have left the other buffer
+            if (i + QT < i1) copy(i + QT, buf ^ 1);
+#pragma unroll
+            for (int u = 0; u < QT / 32; u++) turn(i + 32 * u, s_q + buf * BUF, u);
+        };
+        if (i0 < i1) copy(i0, 0);
+        for (int i = i0; i < i1; i += 2 * QT) {
+            step(i, std::integral_constant<int, 0>{});
+            if (i + QT < i1) step(i + QT, std::integral_constant<int, 1>{});
+        }
+    }
+    sum += __shfl_xor(sum, 32);
+    if (half == 0 && j < int(a.n)) part[(int64_t(slice) * a.kv_heads + hk) * a.n + j] = sum;
+}
+
+// The slices' sums of every key, in order, to its place.
+__global__ __launch_bounds__(256) void prompt_weights_join_kernel(AttentionArgs a, Weights w, int slices, const float *part) {
+    const int j = int(blockIdx.x * 256 + threadIdx.x), hk = blockIdx.y;
+    if (j >= int(a.n)) return;
+    const QueryRange r = query_range(j, int(a.n), a.docs, int(a.ndocs), a.prefix, int(w.window));
+    if (r.doc < 0 || uint32_t(r.place) >= w.most) return;
+    float sum = 0.f;
+#pragma unroll 4
+    for (int x = 0; x < slices; x++) sum += part[(int64_t(x) * a.kv_heads + hk) * a.n + j];
+    w.p[(int64_t(r.doc) * a.kv_heads + hk) * w.most + r.place] += sum;
+}
+
+template <class T, bool CAPPED> void launch_dims(const AttentionArgs &a, int window, int tiles, int cuts, float *part, hipStream_t s) {
+    const dim3 grid(unsigned(tiles) * a.q_heads * unsigned(cuts));
+    if (a.dim <= 32) hipLaunchKernelGGL((prompt_weights_kernel<T, 32, CAPPED>), grid, dim3(256), 0, s, a, window, tiles, cuts, part);
+    else if (a.dim <= 64) hipLaunchKernelGGL((prompt_weights_kernel<T, 64, CAPPED>), grid, dim3(256), 0, s, a, window, tiles, cuts, part);
+    else if (a.dim <= 96) hipLaunchKernelGGL((prompt_weights_kernel<T, 96, CAPPED>), grid, dim3(256), 0, s, a, window, tiles, cuts, part);
+    else if (a.dim <= 128) hipLaunchKernelGGL((prompt_weights_kernel<T, 128, CAPPED>), grid, dim3(256), 0, s, a, window, tiles, cuts, part);
+    else hipLaunchKernelGGL((prompt_weights_kernel<T, 256, CAPPED>), grid, dim3(256), 0, s, a, window, tiles, cuts, part);
+}
+
 }  // namespace
 
-void launch_attention_weights(Ctx &c, const AttentionArgs &a, const Weights &w, hipStream_t s) {
+void launch_attention_weights(Ctx &c, const AttentionArgs &args, const Weights &w, hipStream_t s) {
+    AttentionArgs a = args;
+    const bool pieces = attention_tiles(a);
+    DBuf sums(&c, pieces ? 2 * size_t(a.q_heads) * sums_pitch(a.n) * 4 : size_t(a.n) * a.q_heads * sizeof(float2), s);
+    if (pieces) a.sums = sums.as<float>();
     launch_attention(a, s);
-    ProbeScope probe("text_weights", s, 2.0 * a.n * a.n * a.q_heads * a.dim, 2.0 * a.n * (a.q_heads + a.kv_heads) * a.dim, "text_weights_row");
-    DBuf sums(&c, size_t(a.n) * a.q_heads * sizeof(float2), s);
+    ProbeScope probe("text_weights", s, 2.0 * a.n * a.n * a.q_heads * a.dim, 2.0 * a.n * (a.q_heads + a.kv_heads) * a.dim,
+                     pieces ? "text_weights_tiles" : "text_weights_row");
+    if (pieces) {
+        // The queries cut until every compute unit has four workgroups.
+        const int tiles = int((a.n + 127) / 128), group = int(a.q_heads / a.kv_heads);
+        const int64_t mine = int64_t(tiles) * a.q_heads, most = (a.n + 255) / 256;
+        const int cuts = int(std::max<int64_t>(1, std::min<int64_t>({16, (1024 + mine - 1) / mine, most})));
+        DBuf part(&c, size_t(group) * cuts * a.kv_heads * a.n * 4, s);
+        with_type16(a.type, [&](auto t) {
+            if (a.cap > 0.f || a.slopes) launch_dims<decltype(t), true>(a, int(w.window), tiles, cuts, part.as<float>(), s);
+            else launch_dims<decltype(t), false>(a, int(w.window), tiles, cuts, part.as<float>(), s);
+        });
+        hipLaunchKernelGGL(prompt_weights_join_kernel, dim3((a.n + 255) / 256, a.kv_heads), dim3(256), 0, s, a, w, group * cuts, part.as<float>());
+        OCR_HIP(hipGetLastError());
+        return;
+    }
     with_type16(a.type, [&](auto t) {
         using T = decltype(t);
         hipLaunchKernelGGL((row_sums_kernel<T>), dim3(a.n, a.q_heads), dim3(64), 0, s, a, sums.as<float2>());
@@ -144,8 +312,7 @@ void launch_attention_weights(Ctx &c, const AttentionArgs &a, const Weights &w, 
     OCR_HIP(hipGetLastError());
 }
 
-void launch_decode_weights(Ctx &c, const DecodeArgs &a, const Weights &w, hipStream_t s) {
-    launch_decode(c, a, s);
+void launch_single_weights_row(const DecodeArgs &a, const Weights &w, hipStream_t s) {
     ProbeScope probe("text_weights", s, 2.0 * a.table.rows * w.most * a.q_heads * a.kv.dim, 8.0 * a.table.rows * w.most * a.kv.heads, "text_weights_row");
     with_type16(a.type, [&](auto t) {
         with_cache(a.kv.type, [&](auto k) {

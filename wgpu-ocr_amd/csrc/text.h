@@ -162,7 +162,9 @@ struct AttentionArgs {
     const int32_t *prefix;
     float scale, cap;
     const float *slopes;
+    float *sums = nullptr;  // the tiles' kernels: every query's reference and one over its sum of weights, [q_heads][2][sums_pitch(n)]
 };
+OCR_HD int64_t sums_pitch(uint32_t n) { return (int64_t(n) + 63) / 64 * 64; }
 
 struct DecodeArgs {
     KvCache kv;
@@ -220,9 +222,11 @@ void launch_append(const AppendArgs &a, hipStream_t s);
 void launch_read(const ReadArgs &a, hipStream_t s);
 void launch_rotate(const RotateArgs &a, hipStream_t s);
 void launch_attention(const AttentionArgs &a, hipStream_t s);
+bool attention_tiles(const AttentionArgs &a);  // whether launch_attention takes the tiles' kernels
 void launch_attention_weights(Ctx &c, const AttentionArgs &a, const Weights &w, hipStream_t s);
 void launch_decode(Ctx &c, const DecodeArgs &a, hipStream_t s);
 void launch_decode_weights(Ctx &c, const DecodeArgs &a, const Weights &w, hipStream_t s);
+void launch_single_weights_row(const DecodeArgs &a, const Weights &w, hipStream_t s);  // the weights alone, by the formula
 void launch_evict(Ctx &c, const EvictArgs &a, hipStream_t s);
 void launch_latent_append(const LatentAppendArgs &a, hipStream_t s);
 void launch_latent_decode(Ctx &c, const LatentDecodeArgs &a, hipStream_t s);
