@@ -135,10 +135,10 @@ template <class T, class C> __global__ __launch_bounds__(64) void single_weights
     }
 }
 
-// 32 keys a wavefront, held in registers, over tiles of 64 queries of one head that come into LDS by DMA while the tile
-// before is worked on. A workgroup's 128 keys of a key head; slice: one of its query heads, and one of `cuts` parts of the queries.
+// 32 KB keys a wavefront, held in registers, over tiles of 64 queries of one head that come into LDS by DMA while the tile
+// before is worked on. A workgroup's 128 KB keys of a key head; slice: one of its query heads, and one of `cuts` parts of the queries.
 // part [slice][kv_heads][n]. CAPPED: with a cap or slopes.
-template <class T, int DP, bool CAPPED> __global__ __launch_bounds__(256) void prompt_weights_kernel(AttentionArgs a, int window, int tiles, int cuts, float *part) {
+template <class T, int DP, bool CAPPED, int KB> __global__ __launch_bounds__(256) void prompt_weights_kernel(AttentionArgs a, int window, int tiles, int cuts, float *part) {
     typedef T tvec __attribute__((ext_vector_type(8)));
     constexpr int PW = DP <= 64 ? 64 : DP <= 128 ? 128 : 256, QT = PW == 256 ? 32 : 64, KS = DP / 16;
     using TQ = Tile<PW, QT>;
@@ -151,22 +151,32 @@ template <class T, int DP, bool CAPPED> __global__ __launch_bounds__(256) void p
     const int hk = int(blockIdx.x % a.kv_heads), rest = int(blockIdx.x / a.kv_heads), tile = rest % tiles, slice = rest / tiles;
     const int h = hk * group + slice / cuts, cut = slice % cuts, dim = a.dim, pieces = dim / 8;
     if (slice >= slices) return;
-    const int j = tile * 128 + 32 * wave + (lane & 31);
-    QueryRange r{0, 0, -1, 0};
-    if (j < int(a.n)) r = query_range(j, int(a.n), a.docs, int(a.ndocs), a.prefix, window);
-    const bool seen = r.lo < r.hi;
-    const int wlo = wave_min_i(seen ? r.lo : 0x7fffffff), whi = wave_max_i(seen ? r.hi : 0);
-    const int flo = wave_max_i(seen ? r.lo : 0x7fffffff), fhi = wave_min_i(seen ? r.hi : 0);  // all keys are seen by those in [flo, fhi)
+    int j[KB], lo[KB], hi[KB];  // the lane's keys, and the queries that see them
+    int wlo = 0x7fffffff, whi = 0, flo = 0, fhi = 0x7fffffff;  // some key is seen by those in [wlo, whi), all by those in [flo, fhi)
+#pragma unroll
+    for (int t = 0; t < KB; t++) {
+        j[t] = tile * (128 * KB) + 32 * (KB * wave + t) + (lane & 31);
+        QueryRange r{0, 0, -1, 0};
+        if (j[t] < int(a.n)) r = query_range(j[t], int(a.n), a.docs, int(a.ndocs), a.prefix, window);
+        const bool seen = r.lo < r.hi;
+        lo[t] = seen ? r.lo : 0, hi[t] = seen ? r.hi : 0;
+        wlo = min(wlo, seen ? r.lo : 0x7fffffff), whi = max(whi, hi[t]);
+        flo = max(flo, lo[t]), fhi = min(fhi, hi[t]);
+    }
+    wlo = wave_min_i(wlo), whi = wave_max_i(whi), flo = wave_max_i(flo), fhi = wave_min_i(fhi);
     if (lane == 0) s_lo[wave] = wlo, s_hi[wave] = whi;
-    tvec kf[KS];
+    tvec kf[KB][KS];
     {
         const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0;
-        const char *k = static_cast<const char *>(a.k) + (int64_t(min(j, int(a.n) - 1)) * a.k_stride + int64_t(hk) * dim) * 2;
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
-            u32x4 x{0, 0, 0, 0};
-            if (2 * s + half < pieces) x = *reinterpret_cast<const u32x4 *>(k + 16 * (2 * s + half));
-            kf[s] = __builtin_bit_cast(tvec, x ^ flip);
+        for (int t = 0; t < KB; t++) {
+            const char *k = static_cast<const char *>(a.k) + (int64_t(min(j[t], int(a.n) - 1)) * a.k_stride + int64_t(hk) * dim) * 2;
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                u32x4 x{0, 0, 0, 0};
+                if (2 * s + half < pieces) x = *reinterpret_cast<const u32x4 *>(k + 16 * (2 * s + half));
+                kf[t][s] = __builtin_bit_cast(tvec, x ^ flip);
+            }
         }
     }
     const TQ tq(a.q_stride, pieces);
@@ -176,7 +186,7 @@ template <class T, int DP, bool CAPPED> __global__ __launch_bounds__(256) void p
     __syncthreads();
     int qlo = min(min(s_lo[0], s_lo[1]), min(s_lo[2], s_lo[3])), qhi = max(max(s_hi[0], s_hi[1]), max(s_hi[2], s_hi[3]));
     qlo = __builtin_amdgcn_readfirstlane(qlo), qhi = __builtin_amdgcn_readfirstlane(qhi);
-    float sum = 0.f;
+    float sum[KB][4] = {};
     if (qlo < qhi) {
         // This part's tiles of queries.
         const int t0 = qlo / QT, t1 = (qhi + QT - 1) / QT, each = (t1 - t0 + cuts - 1) / cuts;
@@ -200,46 +210,62 @@ template <class T, int DP, bool CAPPED> __global__ __launch_bounds__(256) void p
         // 32 queries from i on.
         auto turn = [&](int i, const char *s_b, int u) __attribute__((always_inline)) {
             if (i >= whi || i + 32 <= wlo) return;
-            f32x16 s;
+            f32x16 s[KB];
 #pragma unroll
-            for (int e = 0; e < 16; e++) s[e] = 0.f;
+            for (int t = 0; t < KB; t++)
 #pragma unroll
-            for (int st = 0; st < KS; st++) s = mfma32(*reinterpret_cast<const tvec *>(s_b + qoff[st] + u * 32 * PW * 2), kf[st], s);
+                for (int e = 0; e < 16; e++) s[t][e] = 0.f;
+#pragma unroll
+            for (int st = 0; st < KS; st++) {
+                const tvec q = *reinterpret_cast<const tvec *>(s_b + qoff[st] + u * 32 * PW * 2);
+#pragma unroll
+                for (int t = 0; t < KB; t++) s[t] = mfma32(q, kf[t][st], s[t]);
+            }
             if constexpr (CAPPED) {
                 float top = 0.f;
                 if (a.cap > 0.f) {
 #pragma unroll
-                    for (int e = 0; e < 16; e++) top = fmaxf(top, fabsf(s[e]));
+                    for (int t = 0; t < KB; t++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) top = fmaxf(top, fabsf(s[t][e]));
                 }
-                if (a.cap > 0.f && __any(top > small.most)) {
+                const bool large = a.cap > 0.f && __any(top > small.most);
 #pragma unroll
-                    for (int e = 0; e < 16; e++) s[e] = capped(cap, s[e] * c);
-                } else if (a.cap > 0.f) {
+                for (int t = 0; t < KB; t++) {
+                    if (large) {
 #pragma unroll
-                    for (int e = 0; e < 16; e++) s[e] *= small.factor(s[e]);
-                } else {
-                    s *= c;
-                }
-                if (a.slopes) {
-                    const float d = float(i + 4 * half - j);
+                        for (int e = 0; e < 16; e++) s[t][e] = capped(cap, s[t][e] * c);
+                    } else if (a.cap > 0.f) {
 #pragma unroll
-                    for (int e = 0; e < 16; e++) s[e] -= slope * fabsf(d + float(8 * (e / 4) + e % 4));
-                }
-            }
-            const bool whole = i >= flo && i + 32 <= fhi;
-            const unsigned first = unsigned(i + 4 * half - r.lo), count = seen ? unsigned(r.hi - r.lo) : 0;
+                        for (int e = 0; e < 16; e++) s[t][e] *= small.factor(s[t][e]);
+                    } else {
+                        s[t] *= c;
+                    }
+                    if (a.slopes) {
+                        const float d = float(i + 4 * half - j[t]);
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const f32x4 ref = *reinterpret_cast<const f32x4 *>(s_b + TQ::BYTES + (32 * u + 2 * e + 4 * half) * 4);
-                const f32x4 inv = *reinterpret_cast<const f32x4 *>(s_b + TQ::BYTES + 256 + (32 * u + 2 * e + 4 * half) * 4);
-#pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    const float p = exp2_f32(CAPPED ? s[e + x] - ref[x] : __fmaf_rn(s[e + x], c, -ref[x]));
-                    // What is not seen may be anything, and so may its query's sum.
-                    if (whole) sum = __fmaf_rn(p, inv[x], sum);
-                    else sum += first + unsigned(2 * e + x) < count ? p * inv[x] : 0.f;
+                        for (int e = 0; e < 16; e++) s[t][e] -= slope * fabsf(d + float(8 * (e / 4) + e % 4));
+                    }
                 }
             }
+            auto add = [&](auto whole) __attribute__((always_inline)) {
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const f32x4 ref = *reinterpret_cast<const f32x4 *>(s_b + TQ::BYTES + (32 * u + 2 * e + 4 * half) * 4);
+                    const f32x4 inv = *reinterpret_cast<const f32x4 *>(s_b + TQ::BYTES + 256 + (32 * u + 2 * e + 4 * half) * 4);
+#pragma unroll
+                    for (int t = 0; t < KB; t++)
+#pragma unroll
+                        for (int x = 0; x < 4; x++) {
+                            const float p = exp2_f32(CAPPED ? s[t][e + x] - ref[x] : __fmaf_rn(s[t][e + x], c, -ref[x]));
+                            // What is not seen may be anything, and so may its query's sum.
+                            if constexpr (decltype(whole)::value) sum[t][x] = __fmaf_rn(p, inv[x], sum[t][x]);
+                            else sum[t][x] += unsigned(i + 4 * half + 2 * e + x - lo[t]) < unsigned(hi[t] - lo[t]) ? p * inv[x] : 0.f;
+                        }
+                }
+            };
+            if (i >= flo && i + 32 <= fhi) add(std::true_type{});
+            else add(std::false_type{});
         };
         auto step = [&](int i, auto which) __attribute__((always_inline)) {
             constexpr int buf = decltype(which)::value;
@@ -255,8 +281,12 @@ template <class T, int DP, bool CAPPED> __global__ __launch_bounds__(256) void p
             if (i + QT < i1) step(i + QT, std::integral_constant<int, 1>{});
         }
     }
-    sum += __shfl_xor(sum, 32);
-    if (half == 0 && j < int(a.n)) part[(int64_t(slice) * a.kv_heads + hk) * a.n + j] = sum;
+#pragma unroll
+    for (int t = 0; t < KB; t++) {
+        float all = (sum[t][0] + sum[t][1]) + (sum[t][2] + sum[t][3]);
+        all += __shfl_xor(all, 32);
+        if (half == 0 && j[t] < int(a.n)) part[(int64_t(slice) * a.kv_heads + hk) * a.n + j[t]] = all;
+    }
 }
 
 // The slices' sums of every key, in order, to its place.
@@ -271,13 +301,17 @@ __global__ __launch_bounds__(256) void prompt_weights_join_kernel(AttentionArgs 
     w.p[(int64_t(r.doc) * a.kv_heads + hk) * w.most + r.place] += sum;
 }
 
-template <class T, bool CAPPED> void launch_dims(const AttentionArgs &a, int window, int tiles, int cuts, float *part, hipStream_t s) {
+template <class T, int DP, bool CAPPED> void launch_keys(const AttentionArgs &a, int window, int tiles, int cuts, bool many, float *part, hipStream_t s) {
     const dim3 grid(unsigned(tiles) * a.q_heads * unsigned(cuts));
-    if (a.dim <= 32) hipLaunchKernelGGL((prompt_weights_kernel<T, 32, CAPPED>), grid, dim3(256), 0, s, a, window, tiles, cuts, part);
-    else if (a.dim <= 64) hipLaunchKernelGGL((prompt_weights_kernel<T, 64, CAPPED>), grid, dim3(256), 0, s, a, window, tiles, cuts, part);
-    else if (a.dim <= 96) hipLaunchKernelGGL((prompt_weights_kernel<T, 96, CAPPED>), grid, dim3(256), 0, s, a, window, tiles, cuts, part);
-    else if (a.dim <= 128) hipLaunchKernelGGL((prompt_weights_kernel<T, 128, CAPPED>), grid, dim3(256), 0, s, a, window, tiles, cuts, part);
-    else hipLaunchKernelGGL((prompt_weights_kernel<T, 256, CAPPED>), grid, dim3(256), 0, s, a, window, tiles, cuts, part);
+    if (many && DP <= 128) hipLaunchKernelGGL((prompt_weights_kernel<T, DP, CAPPED, DP <= 128 ? 2 : 1>), grid, dim3(256), 0, s, a, window, tiles, cuts, part);
+    else hipLaunchKernelGGL((prompt_weights_kernel<T, DP, CAPPED, 1>), grid, dim3(256), 0, s, a, window, tiles, cuts, part);
+}
+template <class T, bool CAPPED> void launch_dims(const AttentionArgs &a, int window, int tiles, int cuts, bool many, float *part, hipStream_t s) {
+    if (a.dim <= 32) launch_keys<T, 32, CAPPED>(a, window, tiles, cuts, many, part, s);
+    else if (a.dim <= 64) launch_keys<T, 64, CAPPED>(a, window, tiles, cuts, many, part, s);
+    else if (a.dim <= 96) launch_keys<T, 96, CAPPED>(a, window, tiles, cuts, many, part, s);
+    else if (a.dim <= 128) launch_keys<T, 128, CAPPED>(a, window, tiles, cuts, many, part, s);
+    else launch_keys<T, 256, CAPPED>(a, window, tiles, cuts, many, part, s);
 }
 
 }  // namespace
@@ -292,13 +326,14 @@ void launch_attention_weights(Ctx &c, const AttentionArgs &args, const Weights &
                      pieces ? "text_weights_tiles" : "text_weights_row");
     if (pieces) {
         // The queries cut until every compute unit has four workgroups.
-        const int tiles = int((a.n + 127) / 128), group = int(a.q_heads / a.kv_heads);
+        const bool many = a.dim <= 128 && int64_t((a.n + 255) / 256) * a.q_heads >= 512;  // 64 keys a wavefront
+        const int keys = many ? 256 : 128, tiles = int((a.n + keys - 1) / keys), group = int(a.q_heads / a.kv_heads);
         const int64_t mine = int64_t(tiles) * a.q_heads, most = (a.n + 255) / 256;
         const int cuts = int(std::max<int64_t>(1, std::min<int64_t>({16, (1024 + mine - 1) / mine, most})));
         DBuf part(&c, size_t(group) * cuts * a.kv_heads * a.n * 4, s);
         with_type16(a.type, [&](auto t) {
-            if (a.cap > 0.f || a.slopes) launch_dims<decltype(t), true>(a, int(w.window), tiles, cuts, part.as<float>(), s);
-            else launch_dims<decltype(t), false>(a, int(w.window), tiles, cuts, part.as<float>(), s);
+            if (a.cap > 0.f || a.slopes) launch_dims<decltype(t), true>(a, int(w.window), tiles, cuts, many, part.as<float>(), s);
+            else launch_dims<decltype(t), false>(a, int(w.window), tiles, cuts, many, part.as<float>(), s);
         });
         hipLaunchKernelGGL(prompt_weights_join_kernel, dim3((a.n + 255) / 256, a.kv_heads), dim3(256), 0, s, a, w, group * cuts, part.as<float>());
         OCR_HIP(hipGetLastError());
