@@ -95,6 +95,10 @@ struct LatentPlan {
     int runs;    // workgroups that share the tiles
     int groups;  // of 16 heads
 };
+// A lane's value for all, in a scalar register.
+__device__ inline int64_t lane_value(int64_t v, int lane) {
+    return int64_t(uint64_t(uint32_t(__builtin_amdgcn_readlane(int(v >> 32), lane))) << 32 | uint32_t(__builtin_amdgcn_readlane(int(v), lane)));
+}
 // f(first sequence of a 64, its lane's tiles, tiles before the lane's sequence) until it answers true; the tiles of all.
 template <class F> __device__ inline int64_t scan_tiles(const LatentDecodeArgs &a, F &&f) {
     const int lane = threadIdx.x & 63;
@@ -108,32 +112,42 @@ template <class F> __device__ inline int64_t scan_tiles(const LatentDecodeArgs &
             if (lane >= d) upto += x;
         }
         if (f(r0, mine, before + upto - mine)) break;
-        before += __shfl(upto, 63);
+        before += lane_value(upto, 63);
     }
     return before;
 }
 
-// 16 heads a wavefront, HB wavefronts over the same tiles of 32 positions, whose vectors come into LDS by DMA, SLOTS - 1
-// tiles ahead. RC: the rank rounded up (the rotated part to 64). Each run of tiles goes through its sequences one after another.
+// One run of tiles by W wavefronts of 16 heads each over the same tiles of 32 positions, whose vectors come into LDS by
+// DMA, up to three tiles ahead. RC: the rank rounded up (the rotated part to 64). Each run goes through its sequences
+// one after another.
 //
 // S^T = C Q^T, O^T = C^T P^T: the vectors are keys, row by row, and values, through the transposing reads, from one
-// copy in LDS. A row's pieces are exchanged so that the reads of 16 rows touch every bank.
-template <class T, int RC, int HB, int SLOTS> __global__ __launch_bounds__(64 * HB, HB < 4 ? 1 : 2) void latent_tile_kernel(LatentDecodeArgs a, LatentPlan plan, float *part) {
+// copy in LDS, rows of an odd number of 128 bytes whose pieces of 16 are exchanged by the row's last three bits: 16 rows' reads touch
+// every bank both ways. Every product's LDS read is asked for PF products before it, in an order that is kept: left to
+// itself the compiler reads, waits and multiplies one after another (163 us where this takes 147). The exponentials go among
+// the next tile's first products, the copies among the second ones. A wavefront of rank 512 has a SIMD's registers for itself:
+// 128 for sums, 72 for the query. 64 sequences of 2048 to 8191 positions, 128 heads, rank
+// 512 + 64, bf16 (377 MB, 91 GFLOP): 118 us without the copies, 128 without the second products.
+template <class T, int RC, int W> __global__ __launch_bounds__(64 * W, 1) void latent_tile_kernel(LatentDecodeArgs a, LatentPlan plan, float *part) {
     typedef T tvec __attribute__((ext_vector_type(8)));
-    constexpr int DP = RC + 64, PP = DP / 8, PB = DP * 2, TILE = kLatentTile * PB;
-    constexpr int NS = DP / 32, NB = RC / 16;
-    constexpr int PER = PP / 8;  // copies of a wavefront for eight rows
-    constexpr int CH = HB == 8 ? 1024 : 512;  // positions looked up at a time
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    constexpr int DP = RC + 64, PP = DP / 8, PB = DP * 2, TILE = kLatentTile * PB, SLOTS = 4;
+    constexpr int NS = DP / 32, NB = RC / 16, PF = 4;
+    constexpr int MINE = kLatentTile * PP / 64 / W;  // a wavefront's copies of a tile
+    static_assert(kLatentTile * PP % (64 * W) == 0, "whole copies");
+    constexpr int CH = 2048;  // positions looked up at a time
     __shared__ __align__(16) char s_c[SLOTS * TILE];
-    __shared__ int64_t s_at[CH];  // a position's vector in the pool, in bytes; negative: none
+    __shared__ int32_t s_at[CH];  // a position's vector in the pool, negative: none
     __shared__ int s_gaps;        // whether some of them are none
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g4 = lane >> 4;
     const int rank = a.c.rank, width = rank + int(a.c.rot), pieces = width / 8;
-    const int h = (int(blockIdx.y) * HB + wave) * 16 + n;
+    // Workgroups of the same run and other heads are eight apart: on one die, whose level-two cache then reads the tiles once.
+    const int shares = (plan.groups + W - 1) / W, share = int(blockIdx.x / 8 % shares);
+    const int h = (share * W + wave) * 16 + n;
     const bool real = h < int(a.heads);
     const int64_t total = scan_tiles(a, [](uint32_t, int, int64_t) { return false; });
-    const int64_t each = latent_run(total, plan.runs), g = blockIdx.x;
-    int64_t x = g * each;
+    const int64_t each = latent_run(total, plan.runs), run = blockIdx.x / (8 * shares) * 8 + blockIdx.x % 8;
+    int64_t x = run * each;
     const int64_t x1 = min(total, x + each);
     if (x >= x1) return;
     // The sequence of tile x, and its own first tile.
@@ -142,62 +156,47 @@ template <class T, int RC, int HB, int SLOTS> __global__ __launch_bounds__(64 * 
         const unsigned long long here = __ballot(before <= x && x < before + mine);
         if (!here) return false;
         const int at = __builtin_ctzll(here);
-        r = r0 + at, start = __shfl(before, at);
+        r = r0 + at, start = lane_value(before, at);
         return true;
     });
 
+    // Copies: the wavefront's j-th of a tile takes 64 of its pieces. Where its lane's row lies is looked up AHEAD copies before.
     const unsigned lds0 = lds_addr(s_c);
-    // Eight rows' (group 0 .. 3) copy k of the tile at position t0 of the lookup.
-    auto copy_one = [&](int t0, int slot, int group, int k, int from) __attribute__((always_inline)) {
-        const int row = (64 * k + from) / PP, piece = (64 * k + from) % PP ^ (row >> 1);
-        int64_t at = s_at[t0 + 8 * group + row];
-        at = at < 0 ? 0 : at;
-        const int p = min(piece ^ (group & 1) * 4, pieces - 1);
-        dma16_to(static_cast<const char *>(a.c.p) + at + 16 * p, lds0 + slot * TILE + group * 8 * PB + k * 1024);
+    constexpr int AHEAD = std::min(MINE, 6);
+    struct Rows {
+        int at[AHEAD];
     };
-    auto copy = [&](int t0, int slot) __attribute__((always_inline)) {
-        int from = lane;  // rows and pieces are worked out each time: held, they would push the sums out of the registers
-        asm volatile("" : "+v"(from));
-        if constexpr (HB == 8) {  // two wavefronts share eight rows
-            constexpr int FIRST = (PER + 1) / 2;
-            if (wave & 1) {
+    auto row_at = [&](int t, int j) __attribute__((always_inline)) { return s_at[t * kLatentTile + (64 * (wave + W * j) + lane) / PP]; };
+    auto look = [&](int t) __attribute__((always_inline)) {
+        Rows r;
 #pragma unroll
-                for (int k = FIRST; k < PER; k++) copy_one(t0, slot, wave >> 1, k, from);
-            } else {
-#pragma unroll
-                for (int k = 0; k < FIRST; k++) copy_one(t0, slot, wave >> 1, k, from);
-            }
-        } else {
-#pragma unroll
-            for (int y = 0; y < 4 / HB; y++)
-#pragma unroll
-                for (int k = 0; k < PER; k++) copy_one(t0, slot, wave * (4 / HB) + y, k, from);
-        }
+        for (int j = 0; j < AHEAD; j++) r.at[j] = row_at(t, j);
+        return r;
     };
-    // Waits until all but the copies of `ahead` tiles are there.
-    auto arrived = [&](bool ahead) __attribute__((always_inline)) {
-        if (!ahead || SLOTS == 2) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        } else if constexpr (HB == 8) {
-            constexpr int FIRST = (PER + 1) / 2;
-            if (wave & 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((SLOTS - 2) * (PER - FIRST)) : "memory");
-            else asm volatile("s_waitcnt vmcnt(%0)" ::"n"((SLOTS - 2) * FIRST) : "memory");
-        } else {
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((SLOTS - 2) * PER * 4 / HB) : "memory");
-        }
+    auto copy = [&](int t, int j, Rows &rows) __attribute__((always_inline)) {
+        int from = 64 * (wave + W * j) + lane;
+        asm volatile("" : "+v"(from));  // worked out each time: held, they would take as many registers as there are copies
+        const int row = from / PP, piece = min((from - row * PP) ^ (row & 7), pieces - 1);
+        dma16_to(static_cast<const char *>(a.c.p) + uint64_t(uint32_t(max(rows.at[j % AHEAD], 0))) * uint32_t(width * 2) + uint32_t(16 * piece),
+                 lds0 + t % SLOTS * TILE + (wave + W * j) * 1024);
+        if (j + AHEAD < MINE) rows.at[j % AHEAD] = row_at(t, j + AHEAD);
     };
-    // Reads: piece 4 st + g4 of row 16 t + n, values 16 b on of rows 4 g4 .. and 16 + 4 g4 ...
-    const int kat[2] = {n * PB + (g4 ^ (n >> 1)) * 16, n * PB + ((4 + g4) ^ (n >> 1)) * 16};
+    // Waits until at most `tiles` tiles' copies are on their way (40 at most: the wait's number has six bits).
+    auto wait_for = [&](auto tiles) __attribute__((always_inline)) {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(decltype(tiles)::value * MINE) : "memory");
+    };
+    // Reads. Keys: rows n and 16 + n, piece 4 st + g4; values: columns 16 b on, of the rows whose scores the lane has.
+    const int kat[2] = {n * PB + (g4 ^ (n & 7)) * 16, n * PB + ((4 + g4) ^ (n & 7)) * 16};
     int vat[4];
     {
-        const int row = 4 * g4 + ((lane & 15) >> 2);
+        const int row = 4 * g4 + (n >> 2);
 #pragma unroll
-        for (int b = 0; b < 4; b++) vat[b] = row * PB + ((2 * b + ((lane & 3) >> 1)) ^ (row >> 1)) * 16 + 8 * (lane & 1);
+        for (int b = 0; b < 4; b++) vat[b] = row * PB + ((2 * b + (n >> 1 & 1)) ^ (row & 7)) * 16 + 8 * (n & 1);
     }
     const float c = a.scale * 1.4426950408889634f;
 
     for (; x < x1; r++) {
-        const int len = clamp_len(a.lens[r], a.table.width, a.c.page), tiles = latent_tiles(len);
+        const int len = __builtin_amdgcn_readfirstlane(clamp_len(a.lens[r], a.table.width, a.c.page)), tiles = latent_tiles(len);
         if (tiles == 0) continue;
         const int64_t first = x - start, count = min(int64_t(tiles) - first, x1 - x);
         const int lo = int(first) * kLatentTile, hi = int(min(int64_t(len), (first + count) * kLatentTile));
@@ -213,87 +212,142 @@ template <class T, int RC, int HB, int SLOTS> __global__ __launch_bounds__(64 * 
 #pragma unroll
         for (int b = 0; b < NB; b++) o[b] = f32x4{0.f, 0.f, 0.f, 0.f};
         float m = -INFINITY, l = 0.f;
+        struct Scores {
+            f32x4 s[2];
+        };
+        // f(i): other work among the products.
+        auto scores = [&](const char *s_t, auto &&f) __attribute__((always_inline)) {
+            Scores z{};
+            auto read = [&](int i) { return *reinterpret_cast<const tvec *>(s_t + kat[i / 2 & 1] + i / 4 * 128 + i % 2 * 16 * PB); };
+            tvec k[PF];
+#pragma unroll
+            for (int i = 0; i < PF; i++) k[i] = read(i);
+#pragma unroll
+            for (int i = 0; i < 2 * NS; i++) {
+                z.s[i % 2] = mfma16(k[i % PF], qf[i / 2], z.s[i % 2]);
+                if (i + PF < 2 * NS) k[i % PF] = read(i + PF);
+                f(i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            asm volatile("" : "+v"(z.s[0]), "+v"(z.s[1]));  // here, and not where they are used, with all that was read held until then
+            return z;
+        };
+        // Adds tile t by its scores z, which it makes the next one's (NEXT: there is one; else only `left` positions of this one may
+        // be there). MORE: and tile t + 3 is asked for.
+        auto turn = [&](Scores &z, int t, int left, auto next_, auto more_) __attribute__((always_inline)) {
+            constexpr bool NEXT = decltype(next_)::value, MORE = decltype(more_)::value;
+            const char *const s_t = s_c + t % SLOTS * TILE;
+            Rows rows;
+            if constexpr (MORE) rows = look(t + 3);
+            float sc[8];  // in units of log2
+#pragma unroll
+            for (int i = 0; i < 8; i++) sc[i] = z.s[i / 4][i % 4] * c;
+            if (!NEXT && left < kLatentTile) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (16 * (i / 4) + 4 * g4 + i % 4 >= left) sc[i] = -INFINITY;
+            }
+            float top = sc[0];
+#pragma unroll
+            for (int i = 1; i < 8; i++) top = fmaxf(top, sc[i]);
+            if (__any(top > m + kSlack)) {
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : exp2_f32(m - mn);
+                l *= f;
+#pragma unroll
+                for (int b = 0; b < NB; b++) o[b] *= f;
+                m = mn;
+            }
+            const float ref = m == -INFINITY ? 0.f : m - lift<T>;
+            tvec p;
+            auto weight = [&](int i) __attribute__((always_inline)) {
+                if (i >= 8) return;
+                const float w = exp2_f32(sc[i] - ref);
+                l += w;
+                p[i] = T(w);
+            };
+            if constexpr (NEXT) {
+                z = scores(s_c + (t + 1) % SLOTS * TILE, weight);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) weight(i);
+            }
+            auto read = [&](int b) __attribute__((always_inline)) {
+                const char *const at = s_t + vat[b % 4] + b / 4 * 128;
+                const u32x2 y = lds_read_tr16(at), v = lds_read_tr16(at + 16 * PB);
+                return __builtin_bit_cast(tvec, u32x4{y[0], y[1], v[0], v[1]});
+            };
+            tvec v[PF];
+#pragma unroll
+            for (int i = 0; i < PF; i++) v[i] = read(i);
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                o[i] = mfma16(v[i % PF], p, o[i]);
+                if (i + PF < NB) v[i % PF] = read(i + PF);
+                if constexpr (MORE) {
+#pragma unroll
+                    for (int j = 0; j < MINE; j++)
+                        if (j * NB / MINE == i) copy(t + 3, j, rows);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
         for (int c0 = lo; c0 < hi; c0 += CH) {
             const int cn = min(CH, hi - c0), nt = latent_tiles(cn);
             __syncthreads();  // all have left the lookup and the tiles
             if (tid == 0) s_gaps = 0;
             __syncthreads();
-            for (int i = tid; i < nt * kLatentTile; i += 64 * HB) {
+            for (int i = tid; i < nt * kLatentTile; i += 64 * W) {
                 const int pos = c0 + min(i, cn - 1);  // past the last: that again, which is finite if it is
                 const int32_t p = page_of(a.table.p + r * a.table.width, a.table.width, a.c.page, a.c.pages, pos);
-                s_at[i] = p < 0 ? -1 : (int64_t(p) * a.c.page + uint32_t(pos) % a.c.page) * width * 2;
+                s_at[i] = p < 0 ? -1 : int32_t(p * a.c.page + uint32_t(pos) % a.c.page);
                 if (p < 0) s_gaps = 1;
             }
             __syncthreads();
-            const bool gaps = s_gaps;
-            for (int t = 0; t < SLOTS - 1 && t < nt; t++) copy(t * kLatentTile, t);
-            int slot = 0;
-            for (int t = 0; t < nt; t++) {
-                arrived(t + SLOTS - 2 < nt);
-                lds_barrier();  // the tile is there, and all have left the one before
-                if (gaps) {     // no page: zeros
-                    for (int i = tid; i < kLatentTile * PP; i += 64 * HB)
-                        if (s_at[t * kLatentTile + i / PP] < 0) *reinterpret_cast<u32x4 *>(s_c + slot * TILE + 16 * i) = u32x4{0, 0, 0, 0};
-                    lds_barrier();
-                }
-                if (t + SLOTS - 1 < nt) copy((t + SLOTS - 1) * kLatentTile, slot == 0 ? SLOTS - 1 : slot - 1);
-                const char *const s_t = s_c + slot * TILE;
-                slot = slot == SLOTS - 1 ? 0 : slot + 1;
-                f32x4 s[2];
+            const bool gaps = __builtin_amdgcn_readfirstlane(s_gaps);
+            // After a wait for tile t: all wavefronts' pieces are there, and all have left tile t - 2.
+            auto arrived = [&](int t) __attribute__((always_inline)) {
+                lds_barrier();
+                if (!gaps) return;
+                char *const s_t = s_c + t % SLOTS * TILE;  // no page: zeros
+                for (int i = tid; i < kLatentTile * PP; i += 64 * W)
+                    if (s_at[t * kLatentTile + i / PP] < 0) *reinterpret_cast<u32x4 *>(s_t + 16 * i) = u32x4{0, 0, 0, 0};
+                lds_barrier();
+            };
+            for (int t = 0; t < 3 && t < nt; t++) {
+                Rows rows = look(t);
 #pragma unroll
-                for (int u = 0; u < 2; u++) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int st = 0; st < NS; st++)
-#pragma unroll
-                    for (int u = 0; u < 2; u++)
-                        s[u] = mfma16(*reinterpret_cast<const tvec *>(s_t + kat[st & 1] + (st / 2) * 128 + u * 16 * PB), qf[st], s[u]);
-                float sc[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) sc[i] = s[i >> 2][i & 3] * c;  // in units of log2
-                if ((t + 1) * kLatentTile > cn) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        if (t * kLatentTile + 16 * (i >> 2) + 4 * g4 + (i & 3) >= cn) sc[i] = -INFINITY;
-                }
-                float top = sc[0];
-#pragma unroll
-                for (int i = 1; i < 8; i++) top = fmaxf(top, sc[i]);
-                if (__any(top > m + kSlack)) {
-                    top = fmaxf(top, __shfl_xor(top, 16));
-                    top = fmaxf(top, __shfl_xor(top, 32));
-                    const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : exp2_f32(m - mn);
-                    l *= f;
-#pragma unroll
-                    for (int b = 0; b < NB; b++) o[b] *= f;
-                    m = mn;
-                }
-                const float ref = m == -INFINITY ? 0.f : m - lift<T>;
-                tvec p;
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float w = exp2_f32(sc[i] - ref);
-                    l += w;
-                    p[i] = T(w);
-                }
-#pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    const u32x2 y = lds_read_tr16(s_t + vat[b & 3] + (b / 4) * 128), z = lds_read_tr16(s_t + vat[b & 3] + (b / 4) * 128 + 16 * PB);
-                    o[b] = mfma16(__builtin_bit_cast(tvec, u32x4{y[0], y[1], z[0], z[1]}), p, o[b]);
-                }
+                for (int j = 0; j < MINE; j++) copy(t, j, rows);
             }
+            if (nt >= 3) wait_for(std::integral_constant<int, 2>{});
+            else wait_for(std::integral_constant<int, 0>{});
+            arrived(0);
+            Scores z = scores(s_c, [](int) {});
+            int t = 0;
+            for (; t + 3 < nt; t++) {
+                wait_for(std::integral_constant<int, 1>{});  // tiles t + 1 and t + 2 are on their way
+                arrived(t + 1);
+                turn(z, t, kLatentTile, std::true_type{}, std::true_type{});
+            }
+            for (; t + 1 < nt; t++) {
+                wait_for(std::integral_constant<int, 0>{});
+                arrived(t + 1);
+                turn(z, t, kLatentTile, std::true_type{}, std::false_type{});
+            }
+            turn(z, t, cn - t * kLatentTile, std::false_type{}, std::false_type{});
         }
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
         const float inv = l == 0.f ? 0.f : 1.f / l;
         if (real && count == tiles) {
             T *out = static_cast<T *>(a.out) + r * a.out_stride + int64_t(h) * rank;
-            typedef T t4 __attribute__((ext_vector_type(4)));
 #pragma unroll
             for (int b = 0; b < NB; b++)
                 if (16 * b + 4 * g4 < rank)
                     *reinterpret_cast<t4 *>(out + 16 * b + 4 * g4) = t4{T(o[b][0] * inv), T(o[b][1] * inv), T(o[b][2] * inv), T(o[b][3] * inv)};
         } else if (real) {
-            float *dst = part + (part_place(g, start, each) * a.heads + h) * (rank + kPartTail);
+            float *dst = part + (part_place(run, start, each) * a.heads + h) * (rank + kPartTail);
 #pragma unroll
             for (int b = 0; b < NB; b++)
                 if (16 * b + 4 * g4 < rank) *reinterpret_cast<f32x4 *>(dst + 16 * b + 4 * g4) = o[b] * inv;
@@ -310,7 +364,7 @@ template <class T> __global__ __launch_bounds__(256) void latent_join_kernel(Lat
     const int h = blockIdx.y, rank = a.c.rank, tiles = latent_tiles(clamp_len(a.lens[r], a.table.width, a.c.page));
     int64_t start = 0;
     const int64_t total = scan_tiles(a, [&](uint32_t r0, int, int64_t before) {
-        if (r - r0 < 64) start = __shfl(before, int(r - r0) & 63);
+        if (r - r0 < 64) start = lane_value(before, int(r - r0) & 63);
         return false;
     });
     const int64_t each = latent_run(total, plan.runs);
@@ -323,15 +377,16 @@ template <class T> __global__ __launch_bounds__(256) void latent_join_kernel(Lat
     });
 }
 
-template <class T, int RC, int HB, int SLOTS> void launch_tiles(const LatentDecodeArgs &a, const LatentPlan &plan, float *part, hipStream_t s) {
-    hipLaunchKernelGGL((latent_tile_kernel<T, RC, HB, SLOTS>), dim3(plan.runs, (plan.groups + HB - 1) / HB), dim3(64 * HB), 0, s, a, plan, part);
+template <class T, int RC, int W> void launch_tiles(const LatentDecodeArgs &a, const LatentPlan &plan, float *part, hipStream_t s) {
+    const unsigned shares = (plan.groups + W - 1) / W;
+    hipLaunchKernelGGL((latent_tile_kernel<T, RC, W>), dim3((plan.runs + 7) / 8 * 8 * shares), dim3(64 * W), 0, s, a, plan, part);
 }
-// f(rank class, wavefronts): the least that hold the rank and the heads.
-template <class T> void launch_heads(const LatentDecodeArgs &a, const LatentPlan &plan, float *part, hipStream_t s) {
-    const int gr = plan.groups;
-    if (a.c.rank <= 128) gr <= 1 ? launch_tiles<T, 128, 1, 4>(a, plan, part, s) : gr <= 2 ? launch_tiles<T, 128, 2, 4>(a, plan, part, s) : gr <= 4 ? launch_tiles<T, 128, 4, 4>(a, plan, part, s) : launch_tiles<T, 128, 8, 4>(a, plan, part, s);
-    else if (a.c.rank <= 256) gr <= 1 ? launch_tiles<T, 256, 1, 3>(a, plan, part, s) : gr <= 2 ? launch_tiles<T, 256, 2, 3>(a, plan, part, s) : gr <= 4 ? launch_tiles<T, 256, 4, 3>(a, plan, part, s) : launch_tiles<T, 256, 8, 4>(a, plan, part, s);
-    else gr <= 1 ? launch_tiles<T, 512, 1, 2>(a, plan, part, s) : gr <= 2 ? launch_tiles<T, 512, 2, 2>(a, plan, part, s) : gr <= 4 ? launch_tiles<T, 512, 4, 2>(a, plan, part, s) : launch_tiles<T, 512, 8, 4>(a, plan, part, s);
+// The wavefronts that hold the heads, up to 64 of them.
+template <class T, int RC> void launch_heads(const LatentDecodeArgs &a, const LatentPlan &plan, float *part, hipStream_t s) {
+    // One wavefront has not the registers for a whole tile of rank 512's copies: of two the second has no heads.
+    if (RC < 512 && plan.groups <= 1) launch_tiles<T, RC, RC < 512 ? 1 : 2>(a, plan, part, s);
+    else if (plan.groups <= 2) launch_tiles<T, RC, 2>(a, plan, part, s);
+    else launch_tiles<T, RC, 4>(a, plan, part, s);
 }
 
 }  // namespace
@@ -347,7 +402,8 @@ void launch_latent_append(const LatentAppendArgs &a, hipStream_t s) {
 
 void launch_latent_decode(Ctx &c, const LatentDecodeArgs &a, hipStream_t s) {
     const double vecs = double(a.table.rows) * a.table.width * a.c.page;
-    bool pieces = a.c.rank % 8 == 0 && a.c.rot % 8 == 0 && a.c.rot <= 64 && a.q_stride % 8 == 0 && a.out_stride % 8 == 0;
+    bool pieces = a.c.rank % 8 == 0 && a.c.rot % 8 == 0 && a.c.rot <= 64 && a.q_stride % 8 == 0 && a.out_stride % 8 == 0 &&
+                  uint64_t(a.c.pages) * a.c.page < 0x80000000u;
     for (const void *p : {static_cast<const void *>(a.c.p), a.q, static_cast<const void *>(a.out)}) pieces = pieces && reinterpret_cast<uintptr_t>(p) % 16 == 0;
     ProbeScope probe("latent_decode", s, 2.0 * vecs * a.heads * (2 * a.c.rank + a.c.rot), 2.0 * vecs * (a.c.rank + a.c.rot),
                      pieces ? "latent_decode_runs" : "latent_decode_row");
@@ -356,15 +412,16 @@ void launch_latent_decode(Ctx &c, const LatentDecodeArgs &a, hipStream_t s) {
         OCR_HIP(hipGetLastError());
         return;
     }
-    // A workgroup of 128 heads fills a compute unit, of fewer two do.
+    // Four tiles of rank 512 fill a compute unit's LDS.
     LatentPlan plan{0, int((a.heads + 15) / 16)};
-    const int64_t most = int64_t(a.table.rows) * latent_tiles(int(a.table.width * a.c.page));
-    const int64_t units = plan.groups > 4 ? 256 : 512;
-    plan.runs = int(std::max<int64_t>(1, std::min<int64_t>(units / ((plan.groups + 7) / 8), (most + kLeastRun - 1) / kLeastRun)));
+    const int64_t most = int64_t(a.table.rows) * latent_tiles(int(a.table.width * a.c.page)), units = a.c.rank > 256 ? 256 : 512;
+    plan.runs = int(std::max<int64_t>(1, std::min<int64_t>(units / ((plan.groups + 3) / 4), (most + kLeastRun - 1) / kLeastRun)));
     DBuf part(&c, size_t(2) * plan.runs * a.heads * (a.c.rank + kPartTail) * 4, s);
     with_type16(a.c.type, [&](auto t) {
         using T = decltype(t);
-        launch_heads<T>(a, plan, part.as<float>(), s);
+        if (a.c.rank <= 128) launch_heads<T, 128>(a, plan, part.as<float>(), s);
+        else if (a.c.rank <= 256) launch_heads<T, 256>(a, plan, part.as<float>(), s);
+        else launch_heads<T, 512>(a, plan, part.as<float>(), s);
         hipLaunchKernelGGL((latent_join_kernel<T>), dim3(a.table.rows, a.heads), dim3(256), 0, s, a, plan, part.as<float>());
     });
     OCR_HIP(hipGetLastError());
