@@ -247,6 +247,11 @@ __device__ inline void attend_row(const KV &kv, const float *q, int dim, int lo,
         if (lane + 64 * u < outs) done(lane + 64 * u, l == 0.f ? 0.f : o[u] / l);
 }
 
+// A lane's value for all, in a scalar register.
+__device__ inline int64_t lane_value(int64_t v, int lane) {
+    return int64_t(uint64_t(uint32_t(__builtin_amdgcn_readlane(int(v >> 32), lane))) << 32 | uint32_t(__builtin_amdgcn_readlane(int(v), lane)));
+}
+
 // Parts of one query's attention joined by a workgroup of N threads, four of its dim values a thread and the parts side by
 // side. part(i): part i's dim normalised values, then log2 of its sum of weights; done(c, four) gets each four.
 template <int N, class Part, class Done> __device__ inline void join_parts(int count, int dim, Part &&part, Done &&done) {

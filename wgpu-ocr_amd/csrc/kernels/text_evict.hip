@@ -61,54 +61,87 @@ template <class P> __device__ inline void move_vectors(const EvictArgs &a, int64
     }
 }
 
+constexpr int kMostMovesHere = 1024;
+
 // One workgroup of N threads a (sequence, head): which stay, the lists of moves, the weights and positions. KEYS: how many
-// places' keys fit in LDS (0: they are made again each time). P: the vectors' pieces if they are moved here too.
-template <int N, int KEYS, class P> __global__ __launch_bounds__(N) void evict_kernel(EvictArgs a, Move *moves_all, int32_t *counts, int cap, bool move_here) {
-    constexpr int W = N / 64;
+// places' keys fit in LDS (0: they are made again each time). HERE: the vectors are moved as well, in pieces P.
+template <int N, int KEYS, bool HERE, class P> __global__ __launch_bounds__(N) void evict_kernel(EvictArgs a, Move *moves_all, int32_t *counts, int cap) {
+    constexpr int W = N / 64, U = 4, COPIES = 8;
+    constexpr int RUNS = KEYS && KEYS < 32768 ? KEYS / 64 : 512;  // of 64 places, numbered at a time
     __shared__ uint32_t s_key[KEYS ? KEYS : 1];
-    __shared__ int s_bins[256];
-    __shared__ int s_count[3][W];  // the wavefronts' equal keys, free places, moved vectors
+    __shared__ __align__(16) int s_bins[256 * COPIES];
+    __shared__ unsigned long long s_stay[RUNS], s_same[RUNS];
+    __shared__ int s_to[RUNS], s_from[RUNS];
+    __shared__ Move s_moves[HERE ? kMostMovesHere : 1];
     __shared__ uint32_t s_prefix;
-    __shared__ int s_want, s_over;
+    __shared__ int s_want, s_over, s_moved;
     const uint32_t heads = a.kv.heads, h = blockIdx.x % heads;
     const int64_t r = blockIdx.x / heads, base = int64_t(blockIdx.x) * a.most;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int n = min(clamp_len(a.lens[r], a.table.width, a.kv.page), int(a.most)), left = min(n, int(a.keep)), newest = a.newest[r];
-    auto position = [&](int p) { return held_position(a.held[base + p], p, n, newest); };
-    auto make = [&](int p) { return is_protected(position(p), newest, a.first, a.recent) ? kProtected : weight_key(a.weights[base + p]); };
-    auto key = [&](int p) { return KEYS ? s_key[p] : make(p); };
+    auto position_of = [&](int p, int32_t held) { return held_position(held, p, n, newest); };
+    auto key_of = [&](int p, int32_t held, float w) { return is_protected(position_of(p, held), newest, a.first, a.recent) ? kProtected : weight_key(w); };
+    auto place = [&](int to, int from) {  // the weight and position of one place at another
+        const float w = a.weights[base + from];
+        const int32_t pos = int32_t(position_of(from, a.held[base + from]));
+        a.weights_out[base + to] = w, a.held_out[base + to] = pos;
+    };
+    // f(u, p, key) over every N-th place from tid on, U at a time with their loads together; FIRST: the keys are made and kept.
+    auto keys = [&](int p0, int p1, int step, auto first_, auto &&f) __attribute__((always_inline)) {
+        constexpr bool MAKE = decltype(first_)::value || KEYS == 0;
+        for (; p0 < p1; p0 += U * step) {
+            uint32_t k[U];
+            if constexpr (MAKE) {
+                int32_t held[U];
+                float w[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int p = min(p0 + u * step + lane, n - 1);
+                    held[u] = a.held[base + p], w[u] = a.weights[base + p];
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int p = min(p0 + u * step + lane, n - 1);
+                    k[u] = key_of(p, held[u], w[u]);
+                    if (KEYS) s_key[p] = k[u];
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < U; u++) k[u] = s_key[min(p0 + u * step + lane, n - 1)];
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (p0 + u * step < p1) f(p0 + u * step, k[u]);
+        }
+    };
     if (h == 0 && tid == 0) a.lens_out[r] = left;
+    Move *const moves = HERE ? s_moves : moves_all + int64_t(blockIdx.x) * cap;
     int moved = 0;
-    Move *const moves = moves_all + int64_t(blockIdx.x) * cap;
-    if (n > left) {
-        if (KEYS)
-            for (int p = tid; p < n; p += N) s_key[p] = make(p);
+    if (n <= left) {
+        for (int p = tid; p < n; p += N) place(p, p);
+    } else {
         // The least key that stays: `prefix` above the bits that are still open, of whose places `want` stay.
         uint32_t prefix = 0;
         int want = left, shift = 24;
         bool all = false;  // every key of the prefix stays
         for (;; shift -= 8) {
-            for (int b = tid; b < 256; b += N) s_bins[b] = 0;
+            for (int i = tid; i < 64 * COPIES; i += N) reinterpret_cast<u32x4 *>(s_bins)[i] = u32x4{0, 0, 0, 0};
             __syncthreads();
-            for (int p0 = wave * 64; p0 < n; p0 += N) {
-                const int p = p0 + lane;
-                const uint32_t k = p < n ? key(p) : 0;
-                const bool in = p < n && (shift == 24 || k >> ((shift + 8) & 31) == prefix);
-                const uint32_t bin = k >> shift & 255;
-                const unsigned long long some = __ballot(in);
-                if (!some) continue;
-                // Keys of one bin (protected places, weights of zero) are added at once.
-                const int first = __builtin_ctzll(some);
-                const uint32_t common = __builtin_amdgcn_readlane(bin, first);
-                const unsigned long long alike = __ballot(in && bin == common);
-                if (lane == first) atomicAdd(&s_bins[common], __popcll(alike));
-                if (in && bin != common) atomicAdd(&s_bins[bin], 1);
-            }
+            auto count = [&](int p0, uint32_t k) __attribute__((always_inline)) {
+                if (p0 + lane < n && (shift == 24 || k >> ((shift + 8) & 31) == prefix)) atomicAdd(&s_bins[(k >> shift & 255) * COPIES + lane % COPIES], 1);
+            };
+            if (shift == 24) keys(wave * 64, n, N, std::true_type{}, count);
+            else keys(wave * 64, n, N, std::false_type{}, count);
             __syncthreads();
             if (wave == 0) {  // lane l has the bins 255 - 4 l down to 252 - 4 l
                 int c[4], sum = 0;
 #pragma unroll
-                for (int u = 0; u < 4; u++) c[u] = s_bins[255 - 4 * lane - u], sum += c[u];
+                for (int u = 0; u < 4; u++) {
+                    c[u] = 0;
+#pragma unroll
+                    for (int i = 0; i < COPIES; i++) c[u] += s_bins[(255 - 4 * lane - u) * COPIES + i];
+                    sum += c[u];
+                }
                 int upto = sum;
 #pragma unroll
                 for (int d = 1; d < 64; d *= 2) {
@@ -129,72 +162,66 @@ template <int N, int KEYS, class P> __global__ __launch_bounds__(N) void evict_k
             if (shift == 0 || all) break;
         }
         const uint32_t least = prefix << shift;
-        // Runs of 64 places a wavefront; keys over the least stay, and of the equal ones the first `want`.
-        const int runs = (n + 63) / 64, each = (runs + W - 1) / W, r0 = min(wave * each, runs), r1 = min(r0 + each, runs);
-        int equal = 0;  // before this wavefront's
-        if (!all) {
-            int mine = 0;
-            for (int x = r0; x < r1; x++) {
-                const int p = 64 * x + lane;
-                mine += __popcll(__ballot(p < n && key(p) == least));
-            }
-            if (lane == 0) s_count[0][wave] = mine;
+        // Masks of the places over and at the least key, then wavefront 0 numbers their runs: keys over it stay, and of the
+        // equal ones the first `want` (`all`: every key of the prefix counts as over).
+        int ties = 0, past = 0;
+        for (int x0 = 0; x0 * 64 < n; x0 += RUNS) {
+            const int runs = min(RUNS, (n + 63) / 64 - x0);
+            keys(64 * (x0 + wave), 64 * (x0 + runs), N, std::false_type{}, [&](int p0, uint32_t k) __attribute__((always_inline)) {
+                const bool in = p0 + lane < n;
+                const unsigned long long over = __ballot(in && (k > least || (all && k == least))), same = __ballot(in && !all && k == least);
+                if (lane == 0) s_stay[p0 / 64 - x0] = over, s_same[p0 / 64 - x0] = same;
+            });
             __syncthreads();
-            for (int w = 0; w < wave; w++) equal += s_count[0][w];
-        }
-        // f(run, mask of the places that stay)
-        auto sweep = [&](auto &&f) {
-            int ties = equal;
-            for (int x = r0; x < r1; x++) {
-                const int p = 64 * x + lane;
-                const uint32_t k = p < n ? key(p) : 0;
-                unsigned long long stay;
-                if (all) {
-                    stay = __ballot(p < n && k >= least);
-                } else {
-                    const unsigned long long same = __ballot(p < n && k == least);
-                    const int tie = ties + __popcll(same & ((1ull << lane) - 1));
-                    stay = __ballot(p < n && (k > least || (k == least && tie < want)));
-                    ties += __popcll(same);
+            // Of the places of run x, those under the new length.
+            auto under = [&](int x) { return 64 * x >= left ? 0ull : left - 64 * x >= 64 ? ~0ull : (1ull << (left - 64 * x)) - 1; };
+            if (wave == 0)
+                for (int x = 0; x < runs; x += 64) {
+                    const bool in = x + lane < runs;
+                    unsigned long long same = in ? s_same[x + lane] : 0, stay = in ? s_stay[x + lane] : 0;
+                    auto before = [&](int mine, int &sum) {  // of this lane, and the sum goes up by all
+                        int upto = mine;
+#pragma unroll
+                        for (int d = 1; d < 64; d *= 2) {
+                            const int y = __shfl_up(upto, d);
+                            if (lane >= d) upto += y;
+                        }
+                        const int at = sum + upto - mine;
+                        sum += __builtin_amdgcn_readlane(upto, 63);
+                        return at;
+                    };
+                    const int open = want - before(__popcll(same), ties);  // of the equal ones, these stay
+                    const unsigned long long some = __ballot(open > 0 && __popcll(same) > open);  // one run at most
+                    if (some) {
+                        const int l = __builtin_ctzll(some), first = __builtin_amdgcn_readlane(open, l);
+                        const unsigned long long m = lane_value(same, l), kept = __ballot(m >> lane & 1 && __popcll(m & ((1ull << lane) - 1)) < first);
+                        if (lane == l) same = kept;
+                    }
+                    if (open > 0) stay |= same;
+                    const unsigned long long u = under(x0 + x + lane);
+                    const int to = before(in ? __popcll(u & ~stay) : 0, moved), from = before(in ? __popcll(stay & ~u) : 0, past);
+                    if (in) s_stay[x + lane] = stay, s_to[x + lane] = to, s_from[x + lane] = from;
                 }
-                f(x, stay);
+            __syncthreads();
+            for (int x = wave; x < runs; x += W) {
+                const unsigned long long stay = s_stay[x], u = under(x0 + x), gaps = u & ~stay, out = stay & ~u, below = (1ull << lane) - 1;
+                const int p = 64 * (x0 + x) + lane;
+                if (gaps >> lane & 1) moves[s_to[x] + __popcll(gaps & below)].to = p;
+                if (out >> lane & 1) moves[s_from[x] + __popcll(out & below)].from = p;
+                if (u & stay & 1ull << lane) place(p, p);
             }
-        };
-        // Of the places of run x, those under the new length.
-        auto under = [&](int x) { return 64 * x >= left ? 0ull : left - 64 * x >= 64 ? ~0ull : (1ull << (left - 64 * x)) - 1; };
-        int free_places = 0, past = 0;
-        sweep([&](int x, unsigned long long stay) { free_places += __popcll(under(x) & ~stay), past += __popcll(stay & ~under(x)); });
-        if (lane == 0) s_count[1][wave] = free_places, s_count[2][wave] = past;
-        __syncthreads();
-        int to = 0, from = 0;
-        for (int w = 0; w < W; w++) {
-            if (w < wave) to += s_count[1][w], from += s_count[2][w];
-            moved += s_count[1][w];
+            __syncthreads();
         }
-        sweep([&](int x, unsigned long long stay) {
-            const unsigned long long below = (1ull << lane) - 1, gaps = under(x) & ~stay, out = stay & ~under(x);
-            if (gaps >> lane & 1) moves[to + __popcll(gaps & below)].to = 64 * x + lane;
-            if (out >> lane & 1) moves[from + __popcll(out & below)].from = 64 * x + lane;
-            to += __popcll(gaps), from += __popcll(out);
-        });
+        if (tid == 0) s_moved = moved;
+        __syncthreads();
+        moved = s_moved;
     }
-    if (tid == 0) counts[blockIdx.x] = moved;
-    // In this order they may be the old arrays: what stays, what moves (read from past the new length), what is left.
-    for (int p = tid; p < left; p += N) {
-        const float w = a.weights[base + p];
-        const int32_t pos = int32_t(position(p));
-        a.weights_out[base + p] = w, a.held_out[base + p] = pos;
-    }
-    __syncthreads();
-    for (int i = tid; i < moved; i += N) {
-        const Move m = moves[i];
-        const float w = a.weights[base + m.from];
-        const int32_t pos = int32_t(position(m.from));
-        a.weights_out[base + m.to] = w, a.held_out[base + m.to] = pos;
-    }
-    if (move_here) move_vectors<P>(a, r, h, moves, moved, tid, N);
+    if (!HERE && tid == 0) counts[blockIdx.x] = moved;
+    // The arrays may be the old ones: what moved is read from past the new length, what is left there is cleared after.
+    for (int i = tid; i < moved; i += N) place(moves[i].to, moves[i].from);
     __syncthreads();
     for (int p = left + tid; p < int(a.most); p += N) a.weights_out[base + p] = 0.f, a.held_out[base + p] = -1;
+    if (HERE) move_vectors<P>(a, r, h, moves, moved, tid, N);
 }
 
 // The moves of blockIdx.x's (sequence, head), shared by the workgroups of blockIdx.y.
@@ -210,22 +237,27 @@ void launch_evict(Ctx &c, const EvictArgs &a, hipStream_t s) {
     const uint64_t places = std::min<uint64_t>(a.most, uint64_t(a.table.width) * a.kv.page);
     const uint64_t cap = std::max<uint64_t>(1, std::min<uint64_t>(a.keep, places > a.keep ? places - a.keep : 0));  // moves of one of them, at most
     const size_t vec = size_t(a.kv.dim) * type_bytes(a.kv.type);
-    const bool pieces = whole_pieces(a.kv), move_here = cap * vec <= 32768;
-    ProbeScope probe("text_evict", s, 4.0 * pairs * places, 16.0 * pairs * places, move_here ? "text_evict_one" : "text_evict_two");
-    DBuf moves(&c, size_t(pairs) * cap * sizeof(Move), s), counts(&c, size_t(pairs) * 4, s);
+    const bool pieces = whole_pieces(a.kv), here = cap * vec <= 32768 && cap <= kMostMovesHere;
+    ProbeScope probe("text_evict", s, 4.0 * pairs * places, 16.0 * pairs * places, here ? "text_evict_one" : "text_evict_two");
+    DBuf moves(&c, here ? 16 : size_t(pairs) * cap * sizeof(Move), s), counts(&c, size_t(pairs) * 4, s);
     Move *const list = moves.as<Move>();
     int32_t *const count = counts.as<int32_t>();
-    auto with = [&](auto piece) {
+    auto with = [&](auto here_, auto piece) {
         using P = decltype(piece);
-        if (places <= 4096) hipLaunchKernelGGL((evict_kernel<256, 4096, P>), dim3(pairs), dim3(256), 0, s, a, list, count, int(cap), move_here);
-        else if (places <= 32768) hipLaunchKernelGGL((evict_kernel<1024, 32768, P>), dim3(pairs), dim3(1024), 0, s, a, list, count, int(cap), move_here);
-        else hipLaunchKernelGGL((evict_kernel<1024, 0, P>), dim3(pairs), dim3(1024), 0, s, a, list, count, int(cap), move_here);
-        if (!move_here)
-            hipLaunchKernelGGL((evict_move_kernel<P>), dim3(pairs, unsigned(std::min<uint64_t>(1024, (cap * vec + 32767) / 32768))), dim3(256), 0, s, a,
-                               list, count, int(cap));
+        constexpr bool HERE = decltype(here_)::value;
+        if (places <= 4096) hipLaunchKernelGGL((evict_kernel<256, 4096, HERE, P>), dim3(pairs), dim3(256), 0, s, a, list, count, int(cap));
+        else if (places <= 32768 - 4096) hipLaunchKernelGGL((evict_kernel<1024, 32768 - 4096, HERE, P>), dim3(pairs), dim3(1024), 0, s, a, list, count, int(cap));
+        else hipLaunchKernelGGL((evict_kernel<1024, 0, HERE, P>), dim3(pairs), dim3(1024), 0, s, a, list, count, int(cap));
     };
-    if (pieces) with(u32x4{});
-    else with(uint8_t{});
+    if (here) {
+        if (pieces) with(std::true_type{}, u32x4{});
+        else with(std::true_type{}, uint8_t{});
+    } else {
+        with(std::false_type{}, u32x4{});
+        const dim3 grid(pairs, unsigned(std::min<uint64_t>(1024, (cap * vec + 32767) / 32768)));
+        if (pieces) hipLaunchKernelGGL((evict_move_kernel<u32x4>), grid, dim3(256), 0, s, a, list, count, int(cap));
+        else hipLaunchKernelGGL((evict_move_kernel<uint8_t>), grid, dim3(256), 0, s, a, list, count, int(cap));
+    }
     OCR_HIP(hipGetLastError());
 }
 

@@ -95,10 +95,6 @@ struct LatentPlan {
     int runs;    // workgroups that share the tiles
     int groups;  // of 16 heads
 };
-// A lane's value for all, in a scalar register.
-__device__ inline int64_t lane_value(int64_t v, int lane) {
-    return int64_t(uint64_t(uint32_t(__builtin_amdgcn_readlane(int(v >> 32), lane))) << 32 | uint32_t(__builtin_amdgcn_readlane(int(v), lane)));
-}
 // f(first sequence of a 64, its lane's tiles, tiles before the lane's sequence) until it answers true; the tiles of all.
 template <class F> __device__ inline int64_t scan_tiles(const LatentDecodeArgs &a, F &&f) {
     const int lane = threadIdx.x & 63;
