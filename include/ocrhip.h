@@ -193,12 +193,15 @@ int ocr_recognize_device(ocr_recognizer *rec, const ocr_batch *d_batches, uint32
  * without its waits): between start and stop, every launch of the kernel family (process-wide:
  * "conv_mfma", "gru", "conv_transpose", "conv_direct", "conv_generic", "maxpool", "mask_up",
  * "grey_resize", "line_crop", "avgpool_t", "argmax", "copy", "text_append", "text_read",
- * "text_attention", "text_decode", "text_fork", "beam_select") is bracketed by HIP events on its
+ * "text_attention", "text_decode", "text_fork", "beam_select", "text_rotate", "text_weights",
+ * "text_evict", "latent_append", "latent_decode", "latent_attention") is bracketed by HIP events on its
  * own stream. stop waits for them and returns the launches, their summed duration in ms and
  * their summed algorithmic FLOPs and bytes. Where a family has several kernels that a rule on
  * sizes picks from, each is a name of its own as well ("gemm_thin" of "gemm_dma"; "text_append_eights" and "_row",
  * "text_read_eights" and "_row", "text_attention_64", "_128" and "_row", "text_decode_whole", "_parts" and "_row",
- * "text_fork_pieces" and "_bytes", "beam_select_one" and "_two"). */
+ * "text_fork_pieces" and "_bytes", "beam_select_one" and "_two", "text_rotate_eights" and "_row",
+ * "text_weights_tiles", "_single" and "_row", "text_evict_one" and "_two", "latent_decode_runs" and "_row",
+ * "latent_attention_64", "_128" and "_row"). */
 int ocr_probe_start(const char *family);
 int ocr_probe_stop(const char *family, uint32_t *calls, double *ms, double *flops, double *bytes);
 
@@ -601,8 +604,7 @@ int ocr_kv_append_axes_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr
 /* Vectors x [n][heads][dim] (tokens x_stride values apart, heads x_head; dim at most 1024) with their values first ..
  * first + rot - 1 (rot even, at most 256) rotated by the tokens' positions, pairs as in ocr_kv_append_args, the others as they are, into
  * out (the same type: OCR_F32, OCR_F16 or OCR_BF16). out may be x with the same strides, and must not overlap it otherwise. back != 0 turns
- * the other way: the inverse, and the gradient. Fast where dim, first and (pairs half a rotation apart) rot are
- * multiples of 8. */
+ * the other way: the inverse, and the gradient. Fast where dim, first and rot are multiples of 8. */
 typedef struct ocr_rotate_args {
     const void *x;
     void *out;
@@ -626,7 +628,9 @@ int ocr_rotate_device(ocr_ctx *ctx, const ocr_rotate_args *args, const ocr_axes 
  * are added, over the query heads of each key head: for prompts (ocr_attention_device; a row a document, its keys by
  * their place in it) over the document's queries, its last `window` (0: all); for single tokens
  * (ocr_decode_attention_device; a row a sequence) the token's. Places from `most` on are dropped, those of no key
- * left as they are. The sums' order is the same each time. Scores that are NaN make weights NaN. */
+ * left as they are. The sums' order is the same each time. Scores that are NaN make weights NaN. Weights and what else
+ * the call reads or writes must not overlap. Single tokens' scores are kept in the context's memory meanwhile, 4 bytes for each
+ * query head and place. */
 int ocr_attention_weights_device(ocr_ctx *ctx, const ocr_attention_args *args, float *weights, uint32_t most, uint32_t window);
 int ocr_decode_attention_weights_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_table *pages,
                                         const ocr_decode_args *args, float *weights, uint32_t most);

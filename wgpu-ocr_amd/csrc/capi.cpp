@@ -1326,6 +1326,7 @@ int ocr_attention_weights_device(ocr_ctx *ctx, const ocr_attention_args *args, f
         const Weights w{weights, most, window};
         const bool any = check_weights(w, a.docs ? a.ndocs : 1);
         if (!check_attention(a)) return;
+        if (any) check_apart(w, a);
         ctx->ctx->bind();
         if (any) launch_attention_weights(*ctx->ctx, a, w, ctx->ctx->stream());
         else launch_attention(a, ctx->ctx->stream());
@@ -1340,6 +1341,7 @@ int ocr_decode_attention_weights_device(ocr_ctx *ctx, const ocr_kv_cache *cache,
         const Weights w{weights, most, 0};
         const bool any = check_weights(w, a.table.rows);
         if (!check_decode(a)) return;
+        if (any) check_apart(w, a);
         ctx->ctx->bind();
         if (any) launch_decode_weights(*ctx->ctx, a, w, ctx->ctx->stream());
         else launch_decode(*ctx->ctx, a, ctx->ctx->stream());

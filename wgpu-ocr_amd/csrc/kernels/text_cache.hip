@@ -526,22 +526,23 @@ template <class T> __global__ __launch_bounds__(256) void rotate_row_kernel(Rota
     const uint32_t half = a.rot / 2, each = a.dim - half;  // a vector's items
     const T *const x = static_cast<const T *>(a.x);
     T *const y = static_cast<T *>(a.out);
-    const int64_t t = blockIdx.x;
-    for (uint32_t item = threadIdx.x; item < a.heads * each; item += 256) {
-        const uint32_t h = item / each, e = item - h * each;
-        const T *from = x + t * a.x_stride + h * a.x_head;
-        T *to = y + t * a.out_stride + h * a.out_head;
-        if (e >= half) {
-            const uint32_t c = e - half < a.first ? e - half : e + half;
-            if (from != to) to[c] = from[c];
-            continue;
+    for (int64_t t = blockIdx.x; t < a.n; t += gridDim.x) {
+        for (uint32_t item = threadIdx.x; item < a.heads * each; item += 256) {
+            const uint32_t h = item / each, e = item - h * each;
+            const T *from = x + t * a.x_stride + h * a.x_head;
+            T *to = y + t * a.out_stride + h * a.out_head;
+            if (e >= half) {
+                const uint32_t c = e - half < a.first ? e - half : e + half;
+                if (from != to) to[c] = from[c];
+                continue;
+            }
+            const uint32_t i = a.first + (a.adjacent ? 2 * e : e), j = i + (a.adjacent ? 1 : half);
+            float2 r = turned(double(a.at[t * a.axes.count + a.axes.axis[e]]) * turns_a_step(a, e, a.rot));
+            if (a.back) r.y = -r.y;
+            const float p = to_f32(from[i]), q = to_f32(from[j]);
+            to[i] = T(p * r.x - q * r.y);
+            to[j] = T(q * r.x + p * r.y);
         }
-        const uint32_t i = a.first + (a.adjacent ? 2 * e : e), j = i + (a.adjacent ? 1 : half);
-        float2 r = turned(double(a.at[t * a.axes.count + a.axes.axis[e]]) * turns_a_step(a, e, a.rot));
-        if (a.back) r.y = -r.y;
-        const float p = to_f32(from[i]), q = to_f32(from[j]);
-        to[i] = T(p * r.x - q * r.y);
-        to[j] = T(q * r.x + p * r.y);
     }
 }
 
@@ -591,7 +592,7 @@ void launch_rotate(const RotateArgs &a, hipStream_t s) {
     with_type(a.type, [&](auto t) {
         using T = decltype(t);
         if (eights) hipLaunchKernelGGL((rotate_kernel<T>), dim3((a.n + each - 1) / each), dim3(256), 0, s, a, each, in_place);
-        else hipLaunchKernelGGL((rotate_row_kernel<T>), dim3(a.n), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((rotate_row_kernel<T>), dim3(std::min<uint32_t>(a.n, 1 << 22)), dim3(256), 0, s, a);
     });
     OCR_HIP(hipGetLastError());
 }

@@ -211,6 +211,9 @@ bool check_beam(const BeamArgs &a);
 void check_axes(const Axes &x, uint32_t rot, uint32_t n);
 bool check_rotate(const RotateArgs &a);
 bool check_weights(const Weights &w, uint32_t rows);
+// That weights to be added to lie beside what the (checked) attention reads and writes.
+void check_apart(const Weights &w, const AttentionArgs &a);
+void check_apart(const Weights &w, const DecodeArgs &a);
 bool check_evict(const EvictArgs &a);
 bool check_latent_append(const LatentAppendArgs &a);
 bool check_latent_decode(const LatentDecodeArgs &a);

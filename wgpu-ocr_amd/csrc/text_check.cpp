@@ -263,6 +263,19 @@ bool check_weights(const Weights &w, uint32_t rows) {
     return true;
 }
 
+void check_apart(const Weights &w, const AttentionArgs &a) {
+    const size_t n1 = a.n - 1, size = size_t(a.docs ? a.ndocs : 1) * a.kv_heads * w.most * 4, q = size_t(a.q_heads) * a.dim, k = size_t(a.kv_heads) * a.dim;
+    if (overlap(w.p, size, a.out, (n1 * a.out_stride + q) * 2) || overlap(w.p, size, a.q, (n1 * a.q_stride + q) * 2) ||
+        overlap(w.p, size, a.k, (n1 * a.k_stride + k) * 2) || overlap(w.p, size, a.v, (n1 * a.v_stride + k) * 2))
+        fail("the weights overlap the queries, keys, values or outputs");
+}
+void check_apart(const Weights &w, const DecodeArgs &a) {
+    const size_t n1 = a.table.rows - 1, size = size_t(a.table.rows) * a.kv.heads * w.most * 4, q = size_t(a.q_heads) * a.kv.dim;
+    if (overlap(w.p, size, a.out, (n1 * a.out_stride + q) * 2) || overlap(w.p, size, a.q, (n1 * a.q_stride + q) * 2) ||
+        overlap(w.p, size, a.lens, size_t(a.table.rows) * 4))
+        fail("the weights overlap the queries, outputs or lengths");
+}
+
 bool check_evict(const EvictArgs &a) {
     check_cache(a.kv);
     check_table(a.table, a.kv.page);
