@@ -360,7 +360,7 @@ template <class T> __global__ __launch_bounds__(256) void latent_join_kernel(Lat
     const int h = blockIdx.y, rank = a.c.rank, tiles = latent_tiles(clamp_len(a.lens[r], a.table.width, a.c.page));
     int64_t start = 0;
     const int64_t total = scan_tiles(a, [&](uint32_t r0, int, int64_t before) {
-        if (r - r0 < 64) start = lane_value(before, int(r - r0) & 63);
+        if (r >= r0 && r - r0 < 64) start = lane_value(before, int(r - r0));
         return false;
     });
     const int64_t each = latent_run(total, plan.runs);
