@@ -71,7 +71,27 @@ struct Kept {
     float *scores;
     float2 *sums;
     uint32_t pitch;
+    Weights w;  // where a workgroup has all of a key head's scores it adds them up itself: else p is null
 };
+
+// What four keys got from a key head's query heads (rows q0 on), added to out; sums(g): a query head's reference and one over its sum.
+template <class F> __device__ inline void add_weights(const Kept &kept, int64_t q0, int group, int p, int end, float *out, F &&sums) {
+    f32x4 sum{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int g = 0; g < group; g++) {
+        const f32x4 s = *reinterpret_cast<const f32x4 *>(kept.scores + (q0 + g) * kept.pitch + p);
+        const float2 x = sums(g);
+#pragma unroll
+        for (int i = 0; i < 4; i++) sum[i] = __fmaf_rn(exp2_f32(s[i] - x.x), x.y, sum[i]);
+    }
+    typedef float loose __attribute__((ext_vector_type(4), aligned(4)));
+    if (p + 4 <= end) {
+        *reinterpret_cast<loose *>(out + p) += sum;
+    } else {
+        for (int i = 0; i < 4; i++)
+            if (p + i < end) out[p + i] += sum[i];
+    }
+}
 
 // T: the queries' type, C: the cache's; products of 8-bit caches in float16, which holds their codes
 // exactly.
@@ -385,21 +405,33 @@ template <class T, class C, int DP, bool KEEP> __global__ __launch_bounds__(256,
             m = mn;
         }
     }
-    if (wave != 0 || !real) return;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (KEEP && g4 == 0) kept.sums[(r * a.q_heads + h) * parts + blockIdx.z] = {m + kSlack, l};  // l is 2^-kSlack of the sum relative to m
-    if (part) {
-        float *dst = part + ((r * a.q_heads + h) * parts + blockIdx.z) * (dim + kPartTail);
+    if (wave == 0 && real) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (KEEP && g4 == 0) {  // l is 2^-kSlack of the sum relative to m
+            if (kept.w.p) s_ml[0][0][n] = m == -INFINITY ? 0.f : m + kSlack, s_ml[0][1][n] = inv;
+            else kept.sums[(r * a.q_heads + h) * parts + blockIdx.z] = {m + kSlack, l};
+        }
+        if (part) {
+            float *dst = part + ((r * a.q_heads + h) * parts + blockIdx.z) * (dim + kPartTail);
 #pragma unroll
-        for (int b = 0; b < NB; b++)
-            if (16 * b + 4 * g4 < dim) *reinterpret_cast<f32x4 *>(dst + 16 * b + 4 * g4) = o[b] * inv;
-        if (g4 == 0) dst[dim] = l == 0.f ? -INFINITY : m + log2f(l);
-    } else {
-        const int64_t at = r * a.out_stride + int64_t(h) * dim;
+            for (int b = 0; b < NB; b++)
+                if (16 * b + 4 * g4 < dim) *reinterpret_cast<f32x4 *>(dst + 16 * b + 4 * g4) = o[b] * inv;
+            if (g4 == 0) dst[dim] = l == 0.f ? -INFINITY : m + log2f(l);
+        } else {
+            const int64_t at = r * a.out_stride + int64_t(h) * dim;
 #pragma unroll
-        for (int b = 0; b < NB; b++)
-            for (int i = 0; i < 4; i++)
-                if (16 * b + 4 * g4 < dim) store16(a.out, a.type, at + 16 * b + 4 * g4 + i, o[b][i] * inv);
+            for (int b = 0; b < NB; b++)
+                for (int i = 0; i < 4; i++)
+                    if (16 * b + 4 * g4 < dim) store16(a.out, a.type, at + 16 * b + 4 * g4 + i, o[b][i] * inv);
+        }
+    }
+    if constexpr (KEEP) {
+        if (!kept.w.p) return;
+        __syncthreads();
+        const int end = int(min(uint32_t(len), kept.w.most));
+        for (int p = 4 * tid; p < end; p += 1024)
+            add_weights(kept, r * a.q_heads + int64_t(hk) * group, group, p, end, kept.w.p + (r * a.kv.heads + hk) * kept.w.most,
+                        [&](int g) { return float2{s_ml[0][0][g], s_ml[0][1][g]}; });
     }
 }
 
@@ -435,22 +467,7 @@ __global__ __launch_bounds__(256) void decode_weights_kernel(DecodeArgs a, Weigh
         s_sums[g] = {m == -INFINITY ? 0.f : m, l == 0.f ? 0.f : 1.f / l};
     }
     __syncthreads();
-    if (p >= end) return;
-    f32x4 sum{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int g = 0; g < group; g++) {
-        const f32x4 s = *reinterpret_cast<const f32x4 *>(kept.scores + (q0 + g) * kept.pitch + p);
-#pragma unroll
-        for (int i = 0; i < 4; i++) sum[i] = __fmaf_rn(exp2_f32(s[i] - s_sums[g].x), s_sums[g].y, sum[i]);
-    }
-    float *out = w.p + (r * a.kv.heads + hk) * w.most + p;
-    typedef float loose __attribute__((ext_vector_type(4), aligned(4)));
-    if (p + 4 <= end) {
-        *reinterpret_cast<loose *>(out) += sum;
-    } else {
-        for (int i = 0; i < 4; i++)
-            if (p + i < end) out[i] += sum[i];
-    }
+    if (p < end) add_weights(kept, q0, group, p, end, w.p + (r * a.kv.heads + hk) * w.most, [&](int g) { return s_sums[g]; });
 }
 
 template <class T, class C, bool KEEP> void launch_tiles(const DecodeArgs &a, uint32_t parts, float *part, const Kept &kept, hipStream_t s) {
@@ -501,12 +518,15 @@ void launch(Ctx &c, const DecodeArgs &a, const Weights *w, hipStream_t s) {
     const size_t rows = size_t(a.table.rows) * a.q_heads;
     if (parts > 1) part = DBuf(&c, rows * parts * (a.kv.dim + kPartTail) * 4, s);
     if (w) {
-        Kept kept{nullptr, nullptr, uint32_t((std::min<uint64_t>(w->most, most) + 3) & ~3ull)};
+        Kept kept{nullptr, nullptr, uint32_t((std::min<uint64_t>(w->most, most) + 3) & ~3ull), {}};
+        if (parts == 1 && a.q_heads / a.kv.heads <= 16) kept.w = *w;
         scores = DBuf(&c, rows * kept.pitch * 4, s), sums = DBuf(&c, rows * parts * sizeof(float2), s);
         kept.scores = scores.as<float>(), kept.sums = sums.as<float2>();
         with_pair(a, [&](auto t, auto k) { launch_tiles<decltype(t), decltype(k), true>(a, parts, part.as<float>(), kept, s); });
-        const ProbeScope weigh("text_weights", s, 2.0 * rows * kept.pitch, 4.0 * rows * kept.pitch + 8.0 * a.table.rows * a.kv.heads * kept.pitch, "text_weights_single");
-        hipLaunchKernelGGL(decode_weights_kernel, dim3(a.table.rows, a.kv.heads, (kept.pitch + kWeighPositions - 1) / kWeighPositions), dim3(256), 0, s, a, *w, parts, kept);
+        if (!kept.w.p) {
+            const ProbeScope weigh("text_weights", s, 2.0 * rows * kept.pitch, 4.0 * rows * kept.pitch + 8.0 * a.table.rows * a.kv.heads * kept.pitch, "text_weights_single");
+            hipLaunchKernelGGL(decode_weights_kernel, dim3(a.table.rows, a.kv.heads, (kept.pitch + kWeighPositions - 1) / kWeighPositions), dim3(256), 0, s, a, *w, parts, kept);
+        }
     } else {
         with_pair(a, [&](auto t, auto k) { launch_tiles<decltype(t), decltype(k), false>(a, parts, part.as<float>(), {}, s); });
     }

@@ -135,6 +135,15 @@ template <class T, class C> __global__ __launch_bounds__(64) void single_weights
     }
 }
 
+// The documents' offsets, few ones in LDS: the search for a key's document is six loads one after another for 36 of them.
+constexpr int kFewDocs = 256;
+__device__ inline const int32_t *offsets_here(const AttentionArgs &a, int32_t *s_docs) {
+    if (!a.docs || a.ndocs >= kFewDocs) return a.docs;
+    for (uint32_t i = threadIdx.x; i <= a.ndocs; i += blockDim.x) s_docs[i] = a.docs[i];
+    __syncthreads();
+    return s_docs;
+}
+
 // 32 KB keys a wavefront, held in registers, over tiles of 64 queries of one head that come into LDS by DMA while the tile
 // before is worked on. A workgroup's 128 KB keys of a key head; slice: one of its query heads, and one of `cuts` parts of the queries.
 // part [slice][kv_heads][n]. CAPPED: with a cap or slopes.
@@ -145,6 +154,7 @@ template <class T, int DP, bool CAPPED, int KB> __global__ __launch_bounds__(256
     constexpr int BUF = TQ::BYTES + 2 * 256;  // the queries, their references and their sums' inverses
     __shared__ __align__(16) char s_q[2 * BUF];
     __shared__ int s_lo[4], s_hi[4];
+    __shared__ int32_t s_docs[kFewDocs];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     const int group = int(a.q_heads / a.kv_heads), slices = group * cuts;
     // Dies take key heads in turn; a die's workgroups go through a head's keys before the next slice, whose queries stay in its level-two cache.
@@ -152,19 +162,8 @@ template <class T, int DP, bool CAPPED, int KB> __global__ __launch_bounds__(256
     const int h = hk * group + slice / cuts, cut = slice % cuts, dim = a.dim, pieces = dim / 8;
     if (slice >= slices) return;
     int j[KB], lo[KB], hi[KB];  // the lane's keys, and the queries that see them
-    int wlo = 0x7fffffff, whi = 0, flo = 0, fhi = 0x7fffffff;  // some key is seen by those in [wlo, whi), all by those in [flo, fhi)
 #pragma unroll
-    for (int t = 0; t < KB; t++) {
-        j[t] = tile * (128 * KB) + 32 * (KB * wave + t) + (lane & 31);
-        QueryRange r{0, 0, -1, 0};
-        if (j[t] < int(a.n)) r = query_range(j[t], int(a.n), a.docs, int(a.ndocs), a.prefix, window);
-        const bool seen = r.lo < r.hi;
-        lo[t] = seen ? r.lo : 0, hi[t] = seen ? r.hi : 0;
-        wlo = min(wlo, seen ? r.lo : 0x7fffffff), whi = max(whi, hi[t]);
-        flo = max(flo, lo[t]), fhi = min(fhi, hi[t]);
-    }
-    wlo = wave_min_i(wlo), whi = wave_max_i(whi), flo = wave_max_i(flo), fhi = wave_min_i(fhi);
-    if (lane == 0) s_lo[wave] = wlo, s_hi[wave] = whi;
+    for (int t = 0; t < KB; t++) j[t] = tile * (128 * KB) + 32 * (KB * wave + t) + (lane & 31);
     tvec kf[KB][KS];
     {
         const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0;
@@ -179,6 +178,19 @@ template <class T, int DP, bool CAPPED, int KB> __global__ __launch_bounds__(256
             }
         }
     }
+    const int32_t *const docs = offsets_here(a, s_docs);
+    int wlo = 0x7fffffff, whi = 0, flo = 0, fhi = 0x7fffffff;  // some key is seen by those in [wlo, whi), all by those in [flo, fhi)
+#pragma unroll
+    for (int t = 0; t < KB; t++) {
+        QueryRange r{0, 0, -1, 0};
+        if (j[t] < int(a.n)) r = query_range(j[t], int(a.n), docs, int(a.ndocs), a.prefix, window);
+        const bool seen = r.lo < r.hi;
+        lo[t] = seen ? r.lo : 0, hi[t] = seen ? r.hi : 0;
+        wlo = min(wlo, seen ? r.lo : 0x7fffffff), whi = max(whi, hi[t]);
+        flo = max(flo, lo[t]), fhi = min(fhi, hi[t]);
+    }
+    wlo = wave_min_i(wlo), whi = wave_max_i(whi), flo = wave_max_i(flo), fhi = wave_min_i(fhi);
+    if (lane == 0) s_lo[wave] = wlo, s_hi[wave] = whi;
     const TQ tq(a.q_stride, pieces);
     if (pieces < TQ::PP) {  // pieces that no copy writes count nothing
         for (int x = tid; x < 2 * BUF / 16; x += 256) *reinterpret_cast<u32x4 *>(s_q + 16 * x) = u32x4{0, 0, 0, 0};
@@ -291,13 +303,17 @@ template <class T, int DP, bool CAPPED, int KB> __global__ __launch_bounds__(256
 
 // The slices' sums of every key, in order, to its place.
 __global__ __launch_bounds__(256) void prompt_weights_join_kernel(AttentionArgs a, Weights w, int slices, const float *part) {
+    __shared__ int32_t s_docs[kFewDocs];
     const int j = int(blockIdx.x * 256 + threadIdx.x), hk = blockIdx.y;
-    if (j >= int(a.n)) return;
-    const QueryRange r = query_range(j, int(a.n), a.docs, int(a.ndocs), a.prefix, int(w.window));
-    if (r.doc < 0 || uint32_t(r.place) >= w.most) return;
     float sum = 0.f;
+    if (j < int(a.n)) {
 #pragma unroll 4
-    for (int x = 0; x < slices; x++) sum += part[(int64_t(x) * a.kv_heads + hk) * a.n + j];
+        for (int x = 0; x < slices; x++) sum += part[(int64_t(x) * a.kv_heads + hk) * a.n + j];
+    }
+    const int32_t *const docs = offsets_here(a, s_docs);
+    if (j >= int(a.n)) return;
+    const QueryRange r = query_range(j, int(a.n), docs, int(a.ndocs), a.prefix, int(w.window));
+    if (r.doc < 0 || uint32_t(r.place) >= w.most) return;
     w.p[(int64_t(r.doc) * a.kv_heads + hk) * w.most + r.place] += sum;
 }
 
