@@ -127,6 +127,9 @@ template <class T, int DK, int DR, int DV, int QW> __global__ __launch_bounds__(
     float m = -INFINITY, l = 0.f;
     const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);  // not 0: masked scores stay minus infinity
 
+    // Every product's LDS read is asked for four products before it, in an order that is kept: left to itself the compiler reads,
+    // waits and multiplies one after another (364 us where this takes 341, two ahead 343).
+    constexpr int kAhead = 4;
     // 32 KB keys from jw on; s: the buffer, at the wavefront's part of it.
     auto turn = [&](int jw, const char *s_b) __attribute__((always_inline)) {
         if (jw >= whi || jw + 32 * KB <= wlo) return;
@@ -135,12 +138,21 @@ template <class T, int DK, int DR, int DV, int QW> __global__ __launch_bounds__(
         for (int t = 0; t < KB; t++) {
 #pragma unroll
             for (int e = 0; e < 16; e++) s[t][e] = 0.f;
+        }
+        auto key_read = [&](int x) __attribute__((always_inline)) {
+            const int t = x / (KS + RS), st = x % (KS + RS);
+            return *reinterpret_cast<const tvec *>(st < KS ? s_b + koff[st < KS ? st : 0] + (part + t * 32) * DK * 2 : s_b + roff[st < KS ? 0 : st - KS] + (part + t * 32) * 128);
+        };
+        {
+            tvec k[kAhead];
 #pragma unroll
-            for (int st = 0; st < KS; st++)
-                s[t] = mfma32(*reinterpret_cast<const tvec *>(s_b + koff[st] + (part + t * 32) * DK * 2), qf[st], s[t]);
+            for (int x = 0; x < kAhead; x++) k[x] = key_read(x);
 #pragma unroll
-            for (int st = 0; st < RS; st++)
-                s[t] = mfma32(*reinterpret_cast<const tvec *>(s_b + roff[st] + (part + t * 32) * 128), qf[KS + st], s[t]);
+            for (int x = 0; x < KB * (KS + RS); x++) {
+                s[x / (KS + RS)] = mfma32(k[x % kAhead], qf[x % (KS + RS)], s[x / (KS + RS)]);
+                if (x + kAhead < KB * (KS + RS)) k[x % kAhead] = key_read(x + kAhead);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
         if (jw < flo || jw + 32 * KB > fhi) {
             const unsigned first = unsigned(jw + 4 * half - r.lo), count = unsigned(r.hi - r.lo);
@@ -173,16 +185,21 @@ template <class T, int DK, int DR, int DV, int QW> __global__ __launch_bounds__(
                 l += x;
                 p[t][e / 8][e % 8] = T(x);
             }
+        auto value_read = [&](int x) __attribute__((always_inline)) {
+            const int t = x / (2 * NB), u = x / NB % 2, b = x % NB;
+            const u32x2 y = lds_read_tr16(s_b + voff[b][0] + (part + 32 * t + 16 * u) * DV * 2);
+            const u32x2 z = lds_read_tr16(s_b + voff[b][1] + (part + 32 * t + 16 * u) * DV * 2);
+            return __builtin_bit_cast(tvec, u32x4{y[0], y[1], z[0], z[1]});
+        };
+        tvec v[kAhead];
 #pragma unroll
-        for (int t = 0; t < KB; t++)
+        for (int x = 0; x < kAhead; x++) v[x] = value_read(x);
 #pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    const u32x2 x = lds_read_tr16(s_b + voff[b][0] + (part + 32 * t + 16 * u) * DV * 2);
-                    const u32x2 y = lds_read_tr16(s_b + voff[b][1] + (part + 32 * t + 16 * u) * DV * 2);
-                    o[b] = mfma32(__builtin_bit_cast(tvec, u32x4{x[0], x[1], y[0], y[1]}), p[t][u], o[b]);
-                }
+        for (int x = 0; x < KB * 2 * NB; x++) {
+            o[x % NB] = mfma32(v[x % kAhead], p[x / (2 * NB)][x / NB % 2], o[x % NB]);
+            if (x + kAhead < KB * 2 * NB) v[x % kAhead] = value_read(x + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
     auto step = [&](int j0, auto which) __attribute__((always_inline)) {
         constexpr int buf = decltype(which)::value;

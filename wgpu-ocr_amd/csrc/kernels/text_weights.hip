@@ -341,11 +341,12 @@ void launch_attention_weights(Ctx &c, const AttentionArgs &args, const Weights &
     ProbeScope probe("text_weights", s, 2.0 * a.n * a.n * a.q_heads * a.dim, 2.0 * a.n * (a.q_heads + a.kv_heads) * a.dim,
                      pieces ? "text_weights_tiles" : "text_weights_row");
     if (pieces) {
-        // The queries cut until every compute unit has four workgroups.
+        // The queries cut until every compute unit has two workgroups: 36 documents of up to 130, 4 key heads of 4, 11.0 us with the
+        // join; four workgroups 13.2, one 12.1.
         const bool many = a.dim <= 128 && int64_t((a.n + 255) / 256) * a.q_heads >= 512;  // 64 keys a wavefront
         const int keys = many ? 256 : 128, tiles = int((a.n + keys - 1) / keys), group = int(a.q_heads / a.kv_heads);
         const int64_t mine = int64_t(tiles) * a.q_heads, most = (a.n + 255) / 256;
-        const int cuts = int(std::max<int64_t>(1, std::min<int64_t>({16, (1024 + mine - 1) / mine, most})));
+        const int cuts = int(std::max<int64_t>(1, std::min<int64_t>({16, (512 + mine - 1) / mine, most})));
         DBuf part(&c, size_t(group) * cuts * a.kv_heads * a.n * 4, s);
         with_type16(a.type, [&](auto t) {
             if (a.cap > 0.f || a.slopes) launch_dims<decltype(t), true>(a, int(w.window), tiles, cuts, many, part.as<float>(), s);
