@@ -10,6 +10,7 @@
 #include <algorithm>
 
 #include "../runtime.h"
+#include "lds_dma.h"
 #include "text_device.h"
 
 namespace ocr {
@@ -70,6 +71,7 @@ template <int N, int KEYS, bool HERE, class P> __global__ __launch_bounds__(N) v
     constexpr int RUNS = KEYS && KEYS < 32768 ? KEYS / 64 : 512;  // of 64 places, numbered at a time
     __shared__ uint32_t s_key[KEYS ? KEYS : 1];
     __shared__ __align__(16) int s_bins[256 * COPIES];
+    __shared__ __align__(16) int s_sum[256];
     __shared__ unsigned long long s_stay[RUNS], s_same[RUNS];
     __shared__ int s_to[RUNS], s_from[RUNS];
     __shared__ Move s_moves[HERE ? kMostMovesHere : 1];
@@ -133,15 +135,15 @@ template <int N, int KEYS, bool HERE, class P> __global__ __launch_bounds__(N) v
             if (shift == 24) keys(wave * 64, n, N, std::true_type{}, count);
             else keys(wave * 64, n, N, std::false_type{}, count);
             __syncthreads();
+            if (tid < 256) {
+                const u32x4 *const copies = reinterpret_cast<const u32x4 *>(s_bins + tid * COPIES);
+                const u32x4 x = copies[0] + copies[1];
+                s_sum[255 - tid] = int((x[0] + x[1]) + (x[2] + x[3]));
+            }
+            lds_barrier();
             if (wave == 0) {  // lane l has the bins 255 - 4 l down to 252 - 4 l
-                int c[4], sum = 0;
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    c[u] = 0;
-#pragma unroll
-                    for (int i = 0; i < COPIES; i++) c[u] += s_bins[(255 - 4 * lane - u) * COPIES + i];
-                    sum += c[u];
-                }
+                const u32x4 c = *reinterpret_cast<const u32x4 *>(s_sum + 4 * lane);
+                const int sum = int((c[0] + c[1]) + (c[2] + c[3]));
                 int upto = sum;
 #pragma unroll
                 for (int d = 1; d < 64; d *= 2) {
@@ -150,11 +152,13 @@ template <int N, int KEYS, bool HERE, class P> __global__ __launch_bounds__(N) v
                 }
                 int before = upto - sum;
                 if (before < want && want <= upto) {
-                    int u = 0;
-                    while (before + c[u] < want) before += c[u++];
+                    int u = 0, here = int(c[0]);
+#pragma unroll
+                    for (int x = 1; x < 4; x++)
+                        if (before + here < want) before += here, here = int(c[x]), u = x;
                     s_prefix = prefix << 8 | uint32_t(255 - 4 * lane - u);
                     s_want = want - before;
-                    s_over = c[u] == want - before;
+                    s_over = here == want - before;
                 }
             }
             __syncthreads();
