@@ -67,6 +67,7 @@ struct DecodePlan {
 // What is kept for the weights of the keys (KEEP): every query head's scores in units of log2, [row][q_heads][pitch], and
 // each part's reference and sum of weights, [row][q_heads][parts]. Scores of 4 query heads are an eighth of the bytes of an 8-bit
 // key and value of 128: keeping them costs less than reading the keys again.
+// 16 sequences of up to 30 011, 32 heads over 8 of 128, e4m3: 175 us (151 without the stores), and 17 for the weights.
 struct Kept {
     float *scores;
     float2 *sums;

@@ -49,6 +49,8 @@ template <class T> __global__ __launch_bounds__(64) void expanded_row_kernel(Lat
 // 32 queries of one head a wavefront over tiles of 64 keys that come into LDS by DMA while the tile before is worked
 // on. DK, DR, DV: the key's own and shared values and the value's, rounded up. QW: of the four wavefronts, those with queries of
 // their own; where it is two, the other two take the same queries over the other half of each tile's keys.
+// Two documents of up to 5000, 32 heads of 128 + 64 and 128, bf16 (292 GFLOP): 329 to 343 us, 850 to 890 TFLOP/s, where a large product
+// reaches 1213: matrix cores and exponentials take turns. 36 documents of up to 130, 12 heads of 64 + 32: 11 us, half of it before the first products.
 template <class T, int DK, int DR, int DV, int QW> __global__ __launch_bounds__(256, 2) void expanded_tile_kernel(LatentAttentionArgs a, int tiles) {
     typedef T tvec __attribute__((ext_vector_type(8)));
     constexpr int KT = 64, KB = KT / 32 * QW / 4;

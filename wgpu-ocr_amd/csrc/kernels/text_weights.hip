@@ -147,6 +147,8 @@ __device__ inline const int32_t *offsets_here(const AttentionArgs &a, int32_t *s
 // 32 KB keys a wavefront, held in registers, over tiles of 64 queries of one head that come into LDS by DMA while the tile
 // before is worked on. A workgroup's 128 KB keys of a key head; slice: one of its query heads, and one of `cuts` parts of the queries.
 // part [slice][kv_heads][n]. CAPPED: with a cap or slopes.
+// Two documents of up to 5000, 32 query heads over 8 of 128, bf16: 165 us, the matrix cores busy a quarter of it; an exponential, two
+// fused products and a wait for LDS a score are some 24 cycles of a wavefront. 32 keys a wavefront 239 us.
 template <class T, int DP, bool CAPPED, int KB> __global__ __launch_bounds__(256) void prompt_weights_kernel(AttentionArgs a, int window, int tiles, int cuts, float *part) {
     typedef T tvec __attribute__((ext_vector_type(8)));
     constexpr int PW = DP <= 64 ? 64 : DP <= 128 ? 128 : 256, QT = PW == 256 ? 32 : 64, KS = DP / 16;
