@@ -635,7 +635,7 @@ int ocr_attention_weights_device(ocr_ctx *ctx, const ocr_attention_args *args, f
 int ocr_decode_attention_weights_device(ocr_ctx *ctx, const ocr_kv_cache *cache, const ocr_page_table *pages,
                                         const ocr_decode_args *args, float *weights, uint32_t most);
 
-/* Drops cached tokens of each sequence (its length, lens[row], within the table and `most`) until `keep` are left,
+/* Drops cached tokens of each sequence (its length, lens[row], within the table and `most`, at most 2^30) until `keep` are left,
  * each key head its own: kept are those at a position under `first`, the `recent` last positions up to newest[row],
  * and of the others those of the largest weights, equal ones by the lower place (NaN weighs least; first + recent at
  * most keep). Kept vectors beyond place keep - 1 move to the places of the dropped ones, the lowest to the lowest; nothing
@@ -695,7 +695,7 @@ int ocr_latent_append_device(ocr_ctx *ctx, const ocr_latent_cache *cache, const 
 /* Attention of every sequence's last token over its latent vectors, as they are: queries q [rows][heads][rank + rot]
  * that the keys' expansion has been absorbed into, scores scale q.c, out [rows][heads][rank] the weighted sum of the
  * vectors' first rank values, for the values' expansion to follow. Types the cache's. Lengths as in
- * ocr_decode_attention_device. Fast where rank and rot are multiples of 8, strides of 8 and addresses of 16 bytes. */
+ * ocr_decode_attention_device, tables of at most 2^30 positions. Fast where rank and rot (at most 64) are multiples of 8, strides of 8 and addresses of 16 bytes. */
 typedef struct ocr_latent_decode_args {
     const int32_t *lens;
     const void *q;

@@ -208,6 +208,7 @@ static void refusals() {
     e("table", [](EvictArgs &a) { a.table.p = nullptr; });
     e("no places", [](EvictArgs &a) { a.most = 0; });
     e("too many places", [](EvictArgs &a) { a.most = 0x80000000u; });
+    e("places that a step past the last would leave 32 bits", [](EvictArgs &a) { a.most = 0x7ffffff0u; });
     e("nothing to keep", [](EvictArgs &a) { a.keep = a.first = a.recent = 0; });
     e("too many to keep", [](EvictArgs &a) { a.keep = 0x80000000u; });
     e("more protected than kept", [](EvictArgs &a) { a.recent = 37; });
@@ -269,6 +270,7 @@ static void refusals() {
     check(check_latent_decode(ld), "latent attention of single tokens");
     Refusals<LatentDecodeArgs, bool (*)(const LatentDecodeArgs &)> d{ld, check_latent_decode};
     d("cache", [](LatentDecodeArgs &a) { a.c.p = nullptr; });
+    d("positions that a step past the last would leave 32 bits", [](LatentDecodeArgs &a) { a.table.width = 0x7ffffffu; });
     d("no heads", [](LatentDecodeArgs &a) { a.heads = 0; });
     d("many heads", [](LatentDecodeArgs &a) { a.heads = 1025, a.q_stride = 1025 * 32, a.out_stride = 1025 * 24; });
     d("scale", [](LatentDecodeArgs &a) { a.scale = NAN; });

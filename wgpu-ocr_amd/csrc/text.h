@@ -141,6 +141,8 @@ struct LatentAttentionArgs {
     float scale;
 };
 constexpr uint32_t kMostRank = 512, kMostLatentRot = 128;
+// Of a sequence, where kernels count on past the last one in 32 bits.
+constexpr uint32_t kMostPlaces = 1u << 30;
 
 struct ReadArgs {
     KvCache kv;

@@ -279,7 +279,7 @@ void check_apart(const Weights &w, const DecodeArgs &a) {
 bool check_evict(const EvictArgs &a) {
     check_cache(a.kv);
     check_table(a.table, a.kv.page);
-    if (a.most == 0 || a.most > 0x7fffffffu) fail("eviction: " + std::to_string(a.most) + " places");
+    if (a.most == 0 || a.most > kMostPlaces) fail("eviction: " + std::to_string(a.most) + " places");
     if (a.keep == 0 || a.keep > 0x7fffffffu) fail("eviction: " + std::to_string(a.keep) + " tokens to keep");
     if (uint64_t(a.first) + a.recent > a.keep)
         fail("eviction: " + std::to_string(a.first) + " first and " + std::to_string(a.recent) + " recent tokens of " + std::to_string(a.keep) + " to keep");
@@ -327,6 +327,7 @@ bool check_latent_append(const LatentAppendArgs &a) {
 bool check_latent_decode(const LatentDecodeArgs &a) {
     check_latent(a.c);
     check_table(a.table, a.c.page);
+    if (uint64_t(a.table.width) * a.c.page > kMostPlaces) fail("latent attention: a table of " + std::to_string(uint64_t(a.table.width) * a.c.page) + " positions");
     if (a.heads == 0 || a.heads > 1024) fail(std::to_string(a.heads) + " query heads (1 to 1024)");
     check_scores(a.scale, 0);
     check_stride(a.q_stride, int64_t(a.heads) * (a.c.rank + a.c.rot), "queries");
