@@ -285,6 +285,8 @@ void launch_latent_attention(const LatentAttentionArgs &a, hipStream_t s) {
                   head_blocks((a.n + 63) / 64, a.heads, a.heads) < 1 << 24;
     for (const void *p : {a.q, a.k, a.r, a.v, static_cast<const void *>(a.out)}) pieces = pieces && reinterpret_cast<uintptr_t>(p) % 16 == 0;
     for (int64_t st : {a.q_stride, a.k_stride, a.k_head, a.rot ? a.r_stride : 0, a.v_stride, a.v_head, a.out_stride}) pieces = pieces && st % 8 == 0 && st < 1 << 24;
+    // Until every compute unit has a workgroup of 128 queries, 64 a workgroup: 36 documents of up to 130 11.6 us and 12.1, two of up
+    // to 5000 425 and 375.
     const bool few = int64_t((a.n + 127) / 128) * a.heads <= 256;
     ProbeScope probe("latent_attention", s, n * n * a.heads * (a.key + a.rot + a.value), 4.0 * n * a.heads * (a.key + a.value),
                      !pieces ? "latent_attention_row" : few ? "latent_attention_64" : "latent_attention_128");
