@@ -414,9 +414,10 @@ void launch_latent_decode(Ctx &c, const LatentDecodeArgs &a, hipStream_t s) {
         OCR_HIP(hipGetLastError());
         return;
     }
-    // Four tiles of rank 512 fill a compute unit's LDS.
+    // A workgroup for every compute unit, whose LDS four tiles of rank 512 or 256 fill. Two: 24 sequences of up to 4000, 64 heads of rank 256
+    // 42 us for 32; of up to 6000 of rank 128, which leave room for it, 29 for 27, and 3 of up to 20 000 with 16 heads 20 for 21.
     LatentPlan plan{0, int((a.heads + 15) / 16)};
-    const int64_t most = int64_t(a.table.rows) * latent_tiles(int(a.table.width * a.c.page)), units = a.c.rank > 256 ? 256 : 512;
+    const int64_t most = int64_t(a.table.rows) * latent_tiles(int(a.table.width * a.c.page)), units = 256;
     plan.runs = int(std::max<int64_t>(1, std::min<int64_t>(units / ((plan.groups + 3) / 4), (most + kLeastRun - 1) / kLeastRun)));
     DBuf part(&c, size_t(2) * plan.runs * a.heads * (a.c.rank + kPartTail) * 4, s);
     const int each = int(std::max<int64_t>(1, std::min<int64_t>(4, int64_t(a.table.rows) * a.heads / 1024)));  // heads of a workgroup that joins
